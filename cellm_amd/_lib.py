@@ -101,6 +101,17 @@ SIGNATURES = {
                                                     _i64, _i64, _i64, C.c_float, C.c_float, _i64, _vp, _vp]),
     "cellm_hip_attention_gqa_f16kv_noalloc": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64,
                                                      _i64, _i64, _i64, C.c_float, C.c_float, _vp, _vp]),
+    "cellm_hip_kv_write_q8": (_i32, [_vp] * 3 + [_i64] * 4 + [_vp] * 6 + [_i64] * 5 + [_vp]),
+    "cellm_hip_rope_kv_write_q8": (_i32, [_vp] * 5 + [_i64] * 5 + [_vp] * 3 + [_i64] + [_vp] * 5 + [_i64] * 5 + [_vp]),
+    "cellm_hip_kv_read_q8": (_i32, [_vp] * 6 + [_i64] * 2 + [_vp] + [_i64] * 7 + [_i32] + [_vp] * 3),
+    "cellm_hip_attention_gqa_q8kv": (_i32, [_vp] * 7 + [_i64] * 2 + [_vp] + [_i64] * 8 +
+                                     [C.c_float, C.c_float, _i64, _vp, _vp]),
+    "cellm_hip_attention_tree_f16kv": (_i32, [_vp] * 5 + [_i64] * 2 + [_vp] * 2 + [_i64] * 8 +
+                                       [C.c_float, C.c_float, _i64, _vp, _vp]),
+    "cellm_hip_attention_tree_q8kv": (_i32, [_vp] * 7 + [_i64] * 2 + [_vp] * 2 + [_i64] * 8 +
+                                      [C.c_float, C.c_float, _i64, _vp, _vp]),
+    "cellm_hip_kv_accept_f16": (_i32, [_vp] * 4 + [_i64] * 2 + [_vp] * 2 + [_i64] * 7 + [_vp]),
+    "cellm_hip_kv_accept_q8": (_i32, [_vp] * 6 + [_i64] * 2 + [_vp] * 2 + [_i64] * 7 + [_vp]),
     "cellm_hip_silu_mul_f32": (_i32, [_vp, _vp, _vp, _i64, _vp]),
     "cellm_hip_gelu_tanh_mul_f32": (_i32, [_vp, _vp, _vp, _i64, _vp]),
     "cellm_hip_add_f32_inplace": (_i32, [_vp, _vp, _vp, _i64, _vp]),

@@ -1763,3 +1763,291 @@ int32_t cellm_hip_argmax_f32_keys(cellm_hip_ctx_t* ctx, const float* logits, int
 }
 
 }  // extern "C"
+
+// ---- the 8-bit paged cache and drafted trees (kv_cache.hip, attention_paged.hip) ----
+
+namespace {
+
+// What every call on a paged cache checks; `rows` rows, `per` to a row of the block tables.
+int32_t check_kv(int64_t rows, int64_t per, int64_t n_kv_heads, int64_t head_dim, int64_t max_blocks,
+                 int64_t total_blocks, int64_t n_layers, int64_t tpb, int64_t layer)
+{
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return set_error(CELLM_HIP_ERR_UNSUPPORTED, "head_dim %lld: 64, 128 or 256", (long long)head_dim);
+    if (rows < 0 || rows > (1 << 20) || per < 1 || rows % per != 0)
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "rows=%lld (up to 2^20) must be a multiple of the %lld that share a table",
+                         (long long)rows, (long long)per);
+    // vectors of one array are numbered in 32 bits, positions with room for a step past the last
+    if (n_kv_heads < 1 || n_kv_heads > 4096 || max_blocks < 1 || total_blocks < 1 || n_layers < 1 || tpb < 1 || layer < 0 ||
+        layer >= n_layers || max_blocks > (1 << 30) || tpb > (1 << 30) || max_blocks * tpb > (1 << 30) ||
+        total_blocks > INT32_MAX || n_layers > INT32_MAX || n_layers * n_kv_heads > INT32_MAX ||
+        n_layers * n_kv_heads * tpb > (int64_t)UINT32_MAX / total_blocks)
+        return set_error(CELLM_HIP_ERR_INVALID_ARG,
+                         "bad paged-cache geometry max_blocks=%lld total_blocks=%lld layers=%lld tpb=%lld layer=%lld kv "
+                         "heads=%lld (at most 2^30 positions of a table, fewer than 2^32 vectors)",
+                         (long long)max_blocks, (long long)total_blocks, (long long)n_layers, (long long)tpb, (long long)layer,
+                         (long long)n_kv_heads);
+    return CELLM_HIP_OK;
+}
+
+KvGeom kv_geom(const uint32_t* bt, int64_t max_blocks, int64_t total_blocks, int64_t n_layers, int64_t n_kv_heads,
+               int64_t tpb, int64_t layer)
+{
+    return KvGeom{bt, (int)max_blocks, (int)total_blocks, (int)n_layers, (int)n_kv_heads, (int)tpb, (int)layer};
+}
+
+int32_t kv_write_q8_impl(cellm_hip_ctx* ctx, const float* q, const float* k, const float* v, int64_t rows, int64_t per,
+                         int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, const int32_t* positions,
+                         const int32_t* slots, const float* cos_sin, int64_t table_positions, float* q_out, int8_t* kcodes,
+                         float* kscales, int8_t* vcodes, float* vscales, const uint32_t* block_tables, int64_t max_blocks,
+                         int64_t total_blocks, int64_t n_layers, int64_t tpb, int64_t layer, void* stream)
+{
+    if (int32_t rc = check_kv(rows, per, n_kv_heads, head_dim, max_blocks, total_blocks, n_layers, tpb, layer)) return rc;
+    if (n_heads < 0 || n_heads > 4096 || (cos_sin && (table_positions < 1 || table_positions > INT32_MAX)))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "bad heads %lld or table_positions %lld", (long long)n_heads,
+                         (long long)table_positions);
+    if (rows == 0) return CELLM_HIP_OK;
+    if (!k || !v || !positions || !kcodes || !kscales || !vcodes || !vscales || !block_tables)
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(cos_sin) || !aligned16(kcodes) ||
+        !aligned16(vcodes))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "q, k, v, cos_sin and the codes must be 16-byte aligned");
+    DeviceGuard g(ctx->device);
+    HIP_TRY(launch_kv_write_q8(q, k, v, q_out, (int)rows, (int)per, (int)n_heads, (int)head_dim, positions, slots, cos_sin,
+                               (int)table_positions, ctx->rope_interleaved.load(), kcodes, kscales, vcodes, vscales,
+                               kv_geom(block_tables, max_blocks, total_blocks, n_layers, n_kv_heads, tpb, layer),
+                               pick_stream(ctx, stream)),
+            "kv_write_q8 launch");
+    return CELLM_HIP_OK;
+}
+
+int32_t attention_paged_impl(cellm_hip_ctx* ctx, const PagedAttnArgs& in, int64_t rows, int64_t per, int64_t n_heads,
+                             int64_t n_kv_heads, int64_t head_dim, int64_t max_blocks, int64_t total_blocks, int64_t n_layers,
+                             int64_t tpb, int64_t layer, int64_t window, void* stream)
+{
+    if (int32_t rc = check_kv(rows, per, n_kv_heads, head_dim, max_blocks, total_blocks, n_layers, tpb, layer)) return rc;
+    if (n_heads < 1 || n_heads > 4096 || n_heads % n_kv_heads != 0 || rows * n_heads > (1 << 28))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "bad heads %lld / %lld over %lld rows", (long long)n_heads,
+                         (long long)n_kv_heads, (long long)rows);
+    if (window < 0 || window > (1 << 30)) return set_error(CELLM_HIP_ERR_INVALID_ARG, "bad window %lld", (long long)window);
+    if (!(in.scale >= 0.0f) || !(in.cap >= 0.0f) || std::isinf(in.scale) || std::isinf(in.cap))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "attn_scale and soft_cap must be finite and >= 0 (0 = none)");
+    if (rows == 0) return CELLM_HIP_OK;
+    if (!in.q || !in.kc || !in.vc || !in.g.bt || !in.pos || !in.out) return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
+    if (!aligned16(in.q) || !aligned16(in.kc) || !aligned16(in.vc) || !aligned16(in.out))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "q, K, V and out must be 16-byte aligned");
+    PagedAttnArgs a = in;
+    a.g = kv_geom(in.g.bt, max_blocks, total_blocks, n_layers, n_kv_heads, tpb, layer);
+    a.rows = (int)rows;
+    a.per = (int)per;
+    a.n_heads = (int)n_heads;
+    a.head_dim = (int)head_dim;
+    a.window = (int)window;
+    if (!(a.scale > 0.0f)) a.scale = 1.0f / std::sqrt((float)head_dim);
+    DeviceGuard g(ctx->device);
+    HIP_TRY(launch_attention_paged(a, pick_stream(ctx, stream)), "attention launch");
+    return CELLM_HIP_OK;
+}
+
+int32_t attention_tree_impl(cellm_hip_ctx* ctx, PagedAttnArgs& a, const uint64_t* masks, int64_t tables, int64_t tree,
+                            int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int64_t max_blocks, int64_t total_blocks,
+                            int64_t n_layers, int64_t tpb, int64_t layer, int64_t window, void* stream)
+{
+    if (tree < 1 || tree > kMaxTree || tables < 0 || tables > (1 << 20))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "tables=%lld of trees of %lld nodes (1 to %d)", (long long)tables,
+                         (long long)tree, kMaxTree);
+    if (window > 0 && window < tree)  // a drafted ancestor is never outside the window
+        return set_error(CELLM_HIP_ERR_UNSUPPORTED, "window %lld is shorter than the tree's %lld nodes", (long long)window,
+                         (long long)tree);
+    if (tables > 0 && !masks) return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
+    a.masks = masks;
+    a.words = (int)((tree + 63) / 64);
+    return attention_paged_impl(ctx, a, tables * tree, tree, n_heads, n_kv_heads, head_dim, max_blocks, total_blocks,
+                                n_layers, tpb, layer, window, stream);
+}
+
+int32_t kv_accept_impl(cellm_hip_ctx* ctx, void* kc, float* ks, void* vc, float* vs, bool q8, const uint32_t* block_tables,
+                       int64_t max_blocks, int64_t total_blocks, const int32_t* context_lens, const int32_t* accepted,
+                       int64_t max_accept, int64_t tables, int64_t tree, int64_t n_kv_heads, int64_t head_dim,
+                       int64_t n_layers, int64_t tpb, void* stream)
+{
+    if (int32_t rc = check_kv(tables, 1, n_kv_heads, head_dim, max_blocks, total_blocks, n_layers, tpb, 0)) return rc;
+    if (tree < 1 || tree > kMaxTree || max_accept < 1 || max_accept > tree || tables > 65535)
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "paths of up to %lld of %lld nodes (at most %d), %lld tables (at most 65535)",
+                         (long long)max_accept, (long long)tree, kMaxTree, (long long)tables);
+    if (tables == 0) return CELLM_HIP_OK;
+    if (!kc || !vc || (q8 && (!ks || !vs)) || !block_tables || !context_lens || !accepted)
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
+    if (!aligned16(kc) || !aligned16(vc)) return set_error(CELLM_HIP_ERR_INVALID_ARG, "K and V must be 16-byte aligned");
+    const int64_t units = q8 ? n_layers * n_kv_heads : n_layers, row = q8 ? head_dim : 2 * n_kv_heads * head_dim;
+    if (units * (row / 16) > INT32_MAX) return set_error(CELLM_HIP_ERR_INVALID_ARG, "too many layers and heads for one call");
+    DeviceGuard g(ctx->device);
+    HIP_TRY(launch_kv_accept(kc, ks, vc, vs, (int)units, (int)row, (int)tables, context_lens, accepted, (int)max_accept,
+                             (int)tree, (int)tpb, (int)max_blocks, (int)total_blocks, block_tables, pick_stream(ctx, stream)),
+            "kv_accept launch");
+    return CELLM_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t cellm_hip_kv_write_q8(cellm_hip_ctx_t* ctx, const float* k, const float* v, int64_t rows, int64_t rows_per_table,
+                              int64_t n_kv_heads, int64_t head_dim, const int32_t* positions, int8_t* kcodes, float* kscales,
+                              int8_t* vcodes, float* vscales, const uint32_t* block_tables, int64_t max_blocks,
+                              int64_t total_blocks, int64_t n_layers, int64_t tokens_per_block, int64_t layer, void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    return kv_write_q8_impl(ctx, nullptr, k, v, rows, rows_per_table, 0, n_kv_heads, head_dim, positions, nullptr, nullptr, 0,
+                            nullptr, kcodes, kscales, vcodes, vscales, block_tables, max_blocks, total_blocks, n_layers,
+                            tokens_per_block, layer, stream);
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_rope_kv_write_q8(cellm_hip_ctx_t* ctx, const float* q, const float* k, const float* v, float* q_out,
+                                   int64_t rows, int64_t rows_per_table, int64_t n_heads, int64_t n_kv_heads,
+                                   int64_t head_dim, const int32_t* positions, const int32_t* slots, const float* cos_sin,
+                                   int64_t table_positions, int8_t* kcodes, float* kscales, int8_t* vcodes, float* vscales,
+                                   const uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks, int64_t n_layers,
+                                   int64_t tokens_per_block, int64_t layer, void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    if (n_heads < 1) return set_error(CELLM_HIP_ERR_INVALID_ARG, "bad heads %lld", (long long)n_heads);
+    if (rows > 0 && (!q || !q_out || !cos_sin)) return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
+    return kv_write_q8_impl(ctx, q, k, v, rows, rows_per_table, n_heads, n_kv_heads, head_dim, positions, slots, cos_sin,
+                            table_positions, q_out, kcodes, kscales, vcodes, vscales, block_tables, max_blocks, total_blocks,
+                            n_layers, tokens_per_block, layer, stream);
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_kv_read_q8(cellm_hip_ctx_t* ctx, const int8_t* kcodes, const float* kscales, const int8_t* vcodes,
+                             const float* vscales, const uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks,
+                             const int32_t* positions, int64_t rows, int64_t rows_per_table, int64_t n_kv_heads,
+                             int64_t head_dim, int64_t n_layers, int64_t tokens_per_block, int64_t layer, int32_t out_dtype,
+                             void* k_out, void* v_out, void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    if (int32_t rc = check_kv(rows, rows_per_table, n_kv_heads, head_dim, max_blocks, total_blocks, n_layers,
+                              tokens_per_block, layer))
+        return rc;
+    if (!valid_dtype(out_dtype)) return set_error(CELLM_HIP_ERR_INVALID_ARG, "bad dtype");
+    if (rows == 0) return CELLM_HIP_OK;
+    if (!kcodes || !kscales || !vcodes || !vscales || !block_tables || !positions || !k_out || !v_out)
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
+    if (!aligned16(kcodes) || !aligned16(vcodes) || !aligned16(k_out) || !aligned16(v_out))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "the codes and outputs must be 16-byte aligned");
+    DeviceGuard g(ctx->device);
+    HIP_TRY(launch_kv_read_q8(kcodes, kscales, vcodes, vscales, positions, (int)rows, (int)rows_per_table, (int)head_dim,
+                              kv_geom(block_tables, max_blocks, total_blocks, n_layers, n_kv_heads, tokens_per_block, layer),
+                              k_out, v_out, out_dtype, pick_stream(ctx, stream)),
+            "kv_read_q8 launch");
+    return CELLM_HIP_OK;
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_attention_gqa_q8kv(cellm_hip_ctx_t* ctx, const float* q, const int8_t* kcodes, const float* kscales,
+                                     const int8_t* vcodes, const float* vscales, const uint32_t* block_tables,
+                                     int64_t max_blocks, int64_t total_blocks, const int32_t* positions, int64_t rows,
+                                     int64_t rows_per_table, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                     int64_t n_layers, int64_t tokens_per_block, int64_t layer, float attn_scale,
+                                     float soft_cap, int64_t window, float* out, void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    if (rows > 0 && (!kscales || !vscales)) return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
+    PagedAttnArgs a{};
+    a.q = q;
+    a.kc = kcodes;
+    a.ks = kscales;
+    a.vc = vcodes;
+    a.vs = vscales;
+    a.g.bt = block_tables;
+    a.pos = positions;
+    a.scale = attn_scale;
+    a.cap = soft_cap;
+    a.out = out;
+    return attention_paged_impl(ctx, a, rows, rows_per_table, n_heads, n_kv_heads, head_dim, max_blocks, total_blocks,
+                                n_layers, tokens_per_block, layer, window, stream);
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_attention_tree_q8kv(cellm_hip_ctx_t* ctx, const float* q, const int8_t* kcodes, const float* kscales,
+                                      const int8_t* vcodes, const float* vscales, const uint32_t* block_tables,
+                                      int64_t max_blocks, int64_t total_blocks, const int32_t* context_lens,
+                                      const uint64_t* masks, int64_t tables, int64_t tree, int64_t n_heads,
+                                      int64_t n_kv_heads, int64_t head_dim, int64_t n_layers, int64_t tokens_per_block,
+                                      int64_t layer, float attn_scale, float soft_cap, int64_t window, float* out,
+                                      void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    if (tables > 0 && (!kscales || !vscales)) return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
+    PagedAttnArgs a{};
+    a.q = q;
+    a.kc = kcodes;
+    a.ks = kscales;
+    a.vc = vcodes;
+    a.vs = vscales;
+    a.g.bt = block_tables;
+    a.pos = context_lens;
+    a.scale = attn_scale;
+    a.cap = soft_cap;
+    a.out = out;
+    return attention_tree_impl(ctx, a, masks, tables, tree, n_heads, n_kv_heads, head_dim, max_blocks, total_blocks, n_layers,
+                               tokens_per_block, layer, window, stream);
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_attention_tree_f16kv(cellm_hip_ctx_t* ctx, const float* q, const uint16_t* kcache, const uint16_t* vcache,
+                                       const uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks,
+                                       const int32_t* context_lens, const uint64_t* masks, int64_t tables, int64_t tree,
+                                       int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int64_t n_layers,
+                                       int64_t tokens_per_block, int64_t layer, float attn_scale, float soft_cap,
+                                       int64_t window, float* out, void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    PagedAttnArgs a{};
+    a.q = q;
+    a.kc = kcache;
+    a.vc = vcache;
+    a.g.bt = block_tables;
+    a.pos = context_lens;
+    a.scale = attn_scale;
+    a.cap = soft_cap;
+    a.out = out;
+    return attention_tree_impl(ctx, a, masks, tables, tree, n_heads, n_kv_heads, head_dim, max_blocks, total_blocks, n_layers,
+                               tokens_per_block, layer, window, stream);
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_kv_accept_f16(cellm_hip_ctx_t* ctx, uint16_t* kcache, uint16_t* vcache, const uint32_t* block_tables,
+                                int64_t max_blocks, int64_t total_blocks, const int32_t* context_lens,
+                                const int32_t* accepted, int64_t max_accept, int64_t tables, int64_t tree,
+                                int64_t n_kv_heads, int64_t head_dim, int64_t n_layers, int64_t tokens_per_block,
+                                void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    return kv_accept_impl(ctx, kcache, nullptr, vcache, nullptr, false, block_tables, max_blocks, total_blocks, context_lens,
+                          accepted, max_accept, tables, tree, n_kv_heads, head_dim, n_layers, tokens_per_block, stream);
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_kv_accept_q8(cellm_hip_ctx_t* ctx, int8_t* kcodes, float* kscales, int8_t* vcodes, float* vscales,
+                               const uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks,
+                               const int32_t* context_lens, const int32_t* accepted, int64_t max_accept, int64_t tables,
+                               int64_t tree, int64_t n_kv_heads, int64_t head_dim, int64_t n_layers,
+                               int64_t tokens_per_block, void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    return kv_accept_impl(ctx, kcodes, kscales, vcodes, vscales, true, block_tables, max_blocks, total_blocks, context_lens,
+                          accepted, max_accept, tables, tree, n_kv_heads, head_dim, n_layers, tokens_per_block, stream);
+    CELLM_API_END(report_exception)
+}
+
+}  // extern "C"

@@ -184,6 +184,41 @@ hipError_t launch_attention_mma(const float* q, const uint16_t* kcache, const ui
                                 int rows, int n_heads, int n_kv_heads, int head_dim, int n_layers, int tokens_per_block,
                                 int layer, float scale, float soft_cap, int window, int max_splits, float* part,
                                 uint32_t* counters, float* out, hipStream_t st);
+// The 8-bit paged cache (kv_cache.hip).  `per` consecutive rows share a row of the block tables.
+struct KvGeom {
+    const uint32_t* bt;  // [rows / per][max_blocks]
+    int max_blocks, total_blocks, n_layers, n_kv, tpb, layer;
+};
+hipError_t launch_kv_write_q8(const float* q, const float* k, const float* v, float* q_out, int rows, int per, int n_heads,
+                              int head_dim, const int32_t* pos, const int32_t* slots, const float* cos_sin,
+                              int table_positions, int interleaved, int8_t* kc, float* ks, int8_t* vc, float* vs,
+                              const KvGeom& g, hipStream_t st);  // q null: K and V only; cos_sin null: no rotation
+hipError_t launch_kv_read_q8(const int8_t* kc, const float* ks, const int8_t* vc, const float* vs, const int32_t* pos,
+                             int rows, int per, int head_dim, const KvGeom& g, void* k_out, void* v_out, int out_dtype,
+                             hipStream_t st);
+// K and V as `units` rows of row_bytes per slot, ((block * units + unit) * tpb + slot) * row_bytes; ks, vs null for f16
+hipError_t launch_kv_accept(void* kc, float* ks, void* vc, float* vs, int units, int row_bytes, int tables,
+                            const int32_t* ctx, const int32_t* accepted, int most, int tree, int tpb, int max_blocks,
+                            int total_blocks, const uint32_t* bt, hipStream_t st);
+// Attention over pages that `per` consecutive rows share (attention_paged.hip): of 8-bit pages (ks, vs) or f16
+// ones (null), up to each row's position, or (masks) of the nodes of trees drafted behind ctx positions.
+struct PagedAttnArgs {
+    const float* q;
+    const void* kc;
+    const float* ks;
+    const void* vc;
+    const float* vs;
+    KvGeom g;
+    const int32_t* pos;      // [rows]; with masks the contexts, [rows / per]
+    const uint64_t* masks;   // [rows][words], or null
+    int words, rows, per, n_heads, head_dim;
+    float scale, cap;
+    int window;
+    float* out;
+};
+constexpr int kMaxTree = 256;  // nodes of a drafted tree
+hipError_t launch_attention_paged(const PagedAttnArgs& a, hipStream_t st);
+
 // First maximum per row (non-finite -> -inf): chunk blocks of 4096 elements in one launch; rows past
 // one chunk need scratch of argmax_scratch_bytes whose first argmax_counter_bytes (the per-row
 // counters) are zero before the first call and are left at zero by every call.

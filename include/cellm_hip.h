@@ -547,6 +547,118 @@ int32_t cellm_hip_attention_gqa_f16kv_noalloc(cellm_hip_ctx_t* ctx, const float*
                                               int64_t n_layers, int64_t tokens_per_block, int64_t layer,
                                               float attn_scale, float soft_cap, float* out, void* stream);
 
+/* ---- the 8-bit paged cache ----------------------------------------------------
+ * K and V as int8 codes with one f32 scale per (token, kv head): a head vector
+ * x[head_dim] is held as s = max|x| / 127 (an f32 quotient; 0, and the codes 0,
+ * where it is below the smallest normal f32; at most the largest f32
+ * of which 127 are finite) and c = x / s rounded to the nearest
+ * (halves to even) and held to +-127, and stands for c * s.  A vector with an
+ * infinity or a NaN gets the scale NaN and reads as NaN.  Vector (block, layer,
+ * kv head h, slot) is number
+ *   ((block * n_layers + layer) * n_kv_heads + h) * tokens_per_block + slot
+ * of the codes (int8 [head_dim] each, 16-byte aligned array) and of the scales.
+ * The counterpart of the reference's int8 cache (crates/cellm-cache/src/kvcache.rs:48-556,
+ * attention :1441-1514), with scales per head and a layout of this library's own.
+ *
+ * In these calls rows_per_table consecutive rows share one row of block_tables
+ * ([rows / rows_per_table][max_blocks]; rows a multiple of it): 1 for one token per
+ * session, the number of its tokens for a prompt.  Pages with block >= total_blocks
+ * are missing: nothing is written to them and they read as zeros.  A row of position
+ * < 0 is skipped, and its output left as it was (the padding of a batch of prompts).
+ * head_dim 64, 128 or 256 (else CELLM_HIP_ERR_UNSUPPORTED), up to 2^20 rows, tables of
+ * up to 2^30 positions, arrays of fewer than 2^32 vectors. */
+
+/* K and V [rows][n_kv_heads][head_dim] f32 into the pages of `layer` at each row's
+ * position, as cellm_hip_kv_write_f16 does for f16.  The rows of one call go to
+ * different slots. */
+int32_t cellm_hip_kv_write_q8(cellm_hip_ctx_t* ctx, const float* k, const float* v, int64_t rows, int64_t rows_per_table,
+                              int64_t n_kv_heads, int64_t head_dim, const int32_t* positions, int8_t* kcodes, float* kscales,
+                              int8_t* vcodes, float* vscales, const uint32_t* block_tables, int64_t max_blocks,
+                              int64_t total_blocks, int64_t n_layers, int64_t tokens_per_block, int64_t layer, void* stream);
+
+/* RoPE on q and k by each row's position and the K/V write in one launch, as
+ * cellm_hip_rope_kv_write_f16 (the same rotation, pairs and table): q_out = RoPE(q)
+ * (q_out may be q itself, and overlaps it in no other way), RoPE(k) and v quantised
+ * into the pages; k is left as it was.  slots [rows], or NULL for the positions, are
+ * the cache positions of the rows: drafted tokens stand in slots of their own behind
+ * the context and are rotated by their depth.  A slot < 0 or past the table writes no
+ * K and V. */
+int32_t cellm_hip_rope_kv_write_q8(cellm_hip_ctx_t* ctx, const float* q, const float* k, const float* v, float* q_out,
+                                   int64_t rows, int64_t rows_per_table, int64_t n_heads, int64_t n_kv_heads,
+                                   int64_t head_dim, const int32_t* positions, const int32_t* slots, const float* cos_sin,
+                                   int64_t table_positions, int8_t* kcodes, float* kscales, int8_t* vcodes, float* vscales,
+                                   const uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks, int64_t n_layers,
+                                   int64_t tokens_per_block, int64_t layer, void* stream);
+
+/* The values that the codes at each row's position stand for, k_out and v_out
+ * [rows][n_kv_heads][head_dim] in out_dtype: the f32 product c * s, rounded once more
+ * to f16 or bf16.  A missing page or a position past the table reads as zeros. */
+int32_t cellm_hip_kv_read_q8(cellm_hip_ctx_t* ctx, const int8_t* kcodes, const float* kscales, const int8_t* vcodes,
+                             const float* vscales, const uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks,
+                             const int32_t* positions, int64_t rows, int64_t rows_per_table, int64_t n_kv_heads,
+                             int64_t head_dim, int64_t n_layers, int64_t tokens_per_block, int64_t layer, int32_t out_dtype,
+                             void* k_out, void* v_out, void* stream);
+
+/* cellm_hip_attention_gqa_f16kv_window over 8-bit pages: q and out
+ * [rows][n_heads][head_dim] f32, row r attends to the positions up to its own of its
+ * table (the table's last at most), the last `window` of them with a window > 0;
+ * attn_scale and soft_cap as there.  Any number of query heads per kv head.
+ * Positions may differ from row to row of a table in any way.  A q vector with an
+ * infinity or a NaN gives a row of NaN, and so does an attended vector of scale NaN;
+ * what a row does not attend to never reaches it. */
+int32_t cellm_hip_attention_gqa_q8kv(cellm_hip_ctx_t* ctx, const float* q, const int8_t* kcodes, const float* kscales,
+                                     const int8_t* vcodes, const float* vscales, const uint32_t* block_tables,
+                                     int64_t max_blocks, int64_t total_blocks, const int32_t* positions, int64_t rows,
+                                     int64_t rows_per_table, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                     int64_t n_layers, int64_t tokens_per_block, int64_t layer, float attn_scale,
+                                     float soft_cap, int64_t window, float* out, void* stream);
+
+/* ---- trees of drafted tokens -----------------------------------------------------
+ * The check of drafted continuations in one pass: the `tree` nodes (1 to 256) of each
+ * of `tables` sessions stand in the slots context_lens[t] + 0 .. tree - 1 of their
+ * session's pages, behind context_lens[t] positions of context (cellm_hip_kv_write_f16 or
+ * cellm_hip_rope_kv_write_q8 puts them there).  masks [tables][tree][ceil(tree / 64)]
+ * uint64: bit i of node j's words is set where j sees node i (its ancestors and itself;
+ * bits from `tree` on are ignored).  q and out [tables][tree][n_heads][head_dim]: node j
+ * attends to the context and to the drafted slots of its mask.  With a window > 0 (at
+ * least `tree`) it sees the context's positions above context_lens[t] + n - 1 - window
+ * for a mask of n nodes, the last of which is its own.  A node with an empty mask, and a
+ * session with a context < 0, is skipped and its output left as it was; context
+ * positions and slots past the table are not there, and a node that sees none gets
+ * zeros.  Otherwise as cellm_hip_attention_gqa_q8kv, and over f16 pages
+ * (cellm_hip_attention_gqa_f16kv's) for head_dim 64, 128 and 256. */
+int32_t cellm_hip_attention_tree_f16kv(cellm_hip_ctx_t* ctx, const float* q, const uint16_t* kcache, const uint16_t* vcache,
+                                       const uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks,
+                                       const int32_t* context_lens, const uint64_t* masks, int64_t tables, int64_t tree,
+                                       int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int64_t n_layers,
+                                       int64_t tokens_per_block, int64_t layer, float attn_scale, float soft_cap,
+                                       int64_t window, float* out, void* stream);
+int32_t cellm_hip_attention_tree_q8kv(cellm_hip_ctx_t* ctx, const float* q, const int8_t* kcodes, const float* kscales,
+                                      const int8_t* vcodes, const float* vscales, const uint32_t* block_tables,
+                                      int64_t max_blocks, int64_t total_blocks, const int32_t* context_lens,
+                                      const uint64_t* masks, int64_t tables, int64_t tree, int64_t n_heads,
+                                      int64_t n_kv_heads, int64_t head_dim, int64_t n_layers, int64_t tokens_per_block,
+                                      int64_t layer, float attn_scale, float soft_cap, int64_t window, float* out,
+                                      void* stream);
+
+/* Keeps the accepted path of each tree: for i = 0, 1, ... the K and V of slot
+ * context_lens[t] + accepted[t][i] go to slot context_lens[t] + i, in every layer of the
+ * cache, so that the context grows by the path.  accepted [tables][max_accept] holds
+ * rising node numbers (a parent comes before its child) below `tree`; a row ends at its
+ * first entry that is negative, too large or not above the one before.  Sessions with a
+ * context < 0 are skipped, and so are tokens whose page is missing.  Different tables
+ * hold different pages here.  At most 65535 tables. */
+int32_t cellm_hip_kv_accept_f16(cellm_hip_ctx_t* ctx, uint16_t* kcache, uint16_t* vcache, const uint32_t* block_tables,
+                                int64_t max_blocks, int64_t total_blocks, const int32_t* context_lens,
+                                const int32_t* accepted, int64_t max_accept, int64_t tables, int64_t tree,
+                                int64_t n_kv_heads, int64_t head_dim, int64_t n_layers, int64_t tokens_per_block,
+                                void* stream);
+int32_t cellm_hip_kv_accept_q8(cellm_hip_ctx_t* ctx, int8_t* kcodes, float* kscales, int8_t* vcodes, float* vscales,
+                               const uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks,
+                               const int32_t* context_lens, const int32_t* accepted, int64_t max_accept, int64_t tables,
+                               int64_t tree, int64_t n_kv_heads, int64_t head_dim, int64_t n_layers,
+                               int64_t tokens_per_block, void* stream);
+
 /* MetalOps::encode_silu_mul_f32_inplace (metal.rs:232-243, the CPU loop of
  * llama.rs:477-484): gate[i] = silu(gate[i]) * up[i], silu(g) = g / (1 + exp(-g)),
  * in place on gate. */
