@@ -7,6 +7,29 @@
 // (trees) the context and, behind it, the drafted slots whose bit its mask has.  A missing
 // page counts as zero keys and values.  8-bit keys and values are c * s with one scale per
 // (token, kv head), which leaves both sums: q . k = s_k (q . c_k), and s_v joins the weight.
+//
+// The (row, query head) pairs of a table that read one kv head are its columns; a block
+// computes 16 of them over a range of positions, so each K and V element is fetched once for
+// all.  Its four waves take chunks of CH positions in turn and meet in LDS at the end:
+//   S^T [CH][16 columns] = K . Q^T       O^T [HD][16 columns] += V^T . P^T
+// Row m of a K tile is position 4 (m % 4) + m / 4 of its 16, which leaves lane (column c,
+// group g) of S^T with positions 4 j + g, j = 0, 1, ...: the k order of the second product is
+// free as long as V^T and P^T agree, so those weights are its B operand as they are, and the
+// four groups of a V load read four neighbouring positions.  V^T needs a lane's row to be a
+// dim: row c of tile e is dim c * HD / 16 + e, so lane c reads HD / 16 neighbouring dims of
+// its positions and no V goes through LDS.
+//
+// 8-bit pages: q is held as integers of 2^-22 of its head's largest |q| (rounded to the
+// nearest), as three signed 8-bit digits, and q . c_k is three exact sums on
+// v_mfma_i32_16x16x64_i8 with the codes as they are.  f16 pages: q as two f16 parts, hi =
+// RNE_f16(q') and lo = RNE_f16(q' - hi) of q scaled by a power of two (23 bits of an element,
+// 2^-38 of the largest).  The weights (times s_v) are two such parts too, scaled so that the
+// largest that the column has met lies in [2^13, 2^14), over the codes as exact f16 integers
+// or f16 values.  Scores, exponentials, maxima and sums are f32.
+//
+// The positions of a set of columns are split over blocks by a rule on the device (plan()),
+// which knows how long every context is; the last block of a set to finish adds the others'
+// sums in split order.
 #include <algorithm>
 #include <cmath>
 
@@ -19,7 +42,44 @@ namespace cellm {
 
 namespace {
 
-constexpr int kThreads = 256;
+typedef float f2_t __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4, kThreads = kWaves * 64, kCols = 16;
+constexpr int kMaxSplits = 64;   // of a set's positions
+constexpr int kPlanSets = 512;   // sets that plan() looks at, 8 a lane; more run unsplit
+constexpr int kPlanBlocks = 768; // blocks that it aims at: three on each of 256 CUs
+
+struct MmaArgs {
+    PagedAttnArgs a;
+    int group, tiles, sets;  // heads per kv head; sets of 16 columns of a table, and of all tables
+    int cap, tpb_shift;      // positions of a table; log2(tpb), or -1
+    int want;                // blocks per kv head that plan() aims at; 0: one block per set
+    uint32_t* counters;      // [set][kv head]: splits done, zero between calls
+    float* part;             // [work][kv head][16][HD + 2]
+};
+
+__device__ __forceinline__ bool finite_f32(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) != 0x7F800000u; }
+__device__ __forceinline__ void st_agent(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float ld_agent(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ f2_t ld_agent2(const float* p)  // 8-byte aligned
+{
+    return __builtin_bit_cast(f2_t, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+// LDS of one wave, written and read across its lanes: the wave's LDS operations run in order, and the
+// compiler moves none across this
+__device__ __forceinline__ void wave_lds_fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ int rfl(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// e^x for x <= 0 to the accuracy of the hardware exponential: x log2(e) in two parts, the second folded in
+// to first order.  -inf gives NaN (callers select masked positions away).
+__device__ __forceinline__ float exp_neg(float x)
+{
+    const float kLog2e = 1.4426950216293335f, kLog2eLo = 1.9259629911266175e-8f, kLn2 = 0.6931471805599453f;
+    const float h = x * kLog2e;
+    const float r = __builtin_fmaf(x, kLog2eLo, __builtin_fmaf(x, kLog2e, -h));
+    const float e = __builtin_amdgcn_exp2f(h);
+    return __builtin_fmaf(e, r * kLn2, e);
+}
 
 // What a row sees: positions start..ctx - 1, then (masks) those of ctx..end - 1 whose bit is set.
 struct Sight {
@@ -31,10 +91,15 @@ struct Sight {
     }
 };
 
-// false: the row has no position, or its mask no node, and its output is left as it was
-__device__ __forceinline__ bool sight_of(const PagedAttnArgs& a, int row, Sight& s)
+__device__ __forceinline__ uint64_t tree_word(const PagedAttnArgs& a, const uint64_t* bits, int w)
 {
-    const int cap = a.g.max_blocks * a.g.tpb;
+    const int left = a.per - 64 * w;
+    return bits[w] & (left >= 64 ? ~0ull : (1ull << left) - 1);
+}
+
+// false: the row has no position, or its mask no node, and its output is left as it was
+__device__ __forceinline__ bool sight_of(const PagedAttnArgs& a, int cap, int table, int row, Sight& s)
+{
     if (!a.masks) {
         const int p = a.pos[row];
         s.end = s.ctx = min(p, cap - 1) + 1;
@@ -42,14 +107,10 @@ __device__ __forceinline__ bool sight_of(const PagedAttnArgs& a, int row, Sight&
         s.bits = nullptr;
         return p >= 0;
     }
-    const int c = a.pos[row / a.per];
+    const int c = a.pos[table];
     int nodes = 0;
     s.bits = a.masks + (size_t)row * a.words;
-    for (int w = 0; w < a.words; ++w) {
-        const int left = a.per - 64 * w;
-        const uint64_t m = left >= 64 ? ~0ull : (1ull << left) - 1;
-        nodes += __popcll(s.bits[w] & m);
-    }
+    for (int w = 0; w < a.words; ++w) nodes += __popcll(tree_word(a, s.bits, w));
     s.ctx = min(c, cap);
     s.end = min(s.ctx + a.per, cap);
     // the node stands at position ctx + nodes - 1 (its ancestors and itself)
@@ -57,8 +118,22 @@ __device__ __forceinline__ bool sight_of(const PagedAttnArgs& a, int row, Sight&
     return c >= 0 && nodes > 0;
 }
 
-// element offset of head kvh's vector of position p, or -1 where its page is missing; and its number
-template <bool Q8, int HD>
+// Bit b: whether the row sees position p0 + b.
+__device__ __forceinline__ uint64_t visible(const PagedAttnArgs& a, const Sight& s, int p0)
+{
+    const auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };  // bits 0..n - 1
+    uint64_t v = below(s.ctx - p0);
+    if (a.masks && p0 + 64 > s.ctx && p0 < s.end) {  // not for a column that is none: it has no bits
+        const int at = p0 - s.ctx, w = at >> 6, sh = at & 63;  // drafted slot of bit 0, perhaps negative
+        const uint64_t lo = w >= 0 && w < a.words ? tree_word(a, s.bits, w) : 0;
+        const uint64_t hi = w + 1 >= 0 && w + 1 < a.words ? tree_word(a, s.bits, w + 1) : 0;
+        v |= sh ? lo >> sh | hi << (64 - sh) : lo;
+    }
+    return v & below(s.end - p0) & ~below(s.start - p0);
+}
+
+// vector number of head kvh at position p, or -1 where its page is missing
+template <bool Q8>
 __device__ __forceinline__ long long vector_at(const KvGeom& g, int table, int p, int kvh)
 {
     const int b = p / g.tpb;
@@ -69,41 +144,36 @@ __device__ __forceinline__ long long vector_at(const KvGeom& g, int table, int p
     else return (page * g.tpb + (p - b * g.tpb)) * g.n_kv + kvh;
 }
 
-// One block per (row, query head): 256 positions at a time, a score per thread, then HD
-// threads per position.
-template <bool Q8, int HD>
-__global__ __launch_bounds__(kThreads) void attn_paged_plain_kernel(const PagedAttnArgs a)
+__device__ __forceinline__ float capped(const PagedAttnArgs& a, float s)
 {
-    __shared__ float qs[HD], ws[kThreads], red[kThreads];
-    __shared__ long long vec[kThreads];
-    const int row = blockIdx.x / a.n_heads, head = blockIdx.x % a.n_heads, kvh = head / (a.n_heads / a.g.n_kv);
-    const int t = threadIdx.x, table = row / a.per;
-    Sight si;
-    if (!sight_of(a, row, si)) return;  // the same for the whole block
-    if (t < HD) qs[t] = a.q[((size_t)row * a.n_heads + head) * HD + t];
-    __syncthreads();
-    const auto score = [&](int p, long long v) {
+    return a.cap > 0.0f ? tanhf(s / a.cap) * a.cap : s;
+}
+
+// Positions lo..up - 1 of one (row, head) over f16 pages by plain f32 sums, the whole block: maximum m, sum l of
+// e^(score - m) and, in threads below HD, the weighted sum of V (returned).  256 positions at a time: a score per
+// thread, then HD threads per position.  For columns whose sums in f16 parts are not finite: inf * lo may be NaN where
+// inf * v is not, and so is the 0 * inf of a position that the column does not see.
+template <int HD>
+__device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table, int row, int head, int lo, int up,
+                             bool part, unsigned char* lds, float& m, float& l)
+{
+    long long* const vec = reinterpret_cast<long long*>(lds);
+    float* const red = reinterpret_cast<float*>(vec + kThreads);
+    float* const ws = red + kThreads;
+    const int t = threadIdx.x, kvh = head / (a.n_heads / a.g.n_kv);
+    const float* qr = a.q + ((size_t)row * a.n_heads + head) * HD;
+    const auto score = [&](long long v) {
         float d = 0.0f;
         if (v >= 0) {
-            if constexpr (Q8) {
-                const u4_t* src = reinterpret_cast<const u4_t*>(static_cast<const int8_t*>(a.kc) + v * HD);
-                for (int i = 0; i < HD / 16; ++i) {
-                    const u4_t w = src[i];
+            const u4_t* src = reinterpret_cast<const u4_t*>(static_cast<const uint16_t*>(a.kc) + v * HD);
+#pragma unroll 1
+            for (int i = 0; i < HD / 8; ++i) {
+                const h8_t w = __builtin_bit_cast(h8_t, src[i]);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) d = d + qs[16 * i + j] * (float)(int8_t)(w[j >> 2] >> (8 * (j & 3)));
-                }
-                d = d * a.ks[v];
-            } else {
-                const u4_t* src = reinterpret_cast<const u4_t*>(static_cast<const uint16_t*>(a.kc) + v * HD);
-                for (int i = 0; i < HD / 8; ++i) {
-                    const h8_t w = __builtin_bit_cast(h8_t, src[i]);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) d = d + qs[8 * i + j] * (float)w[j];
-                }
+                for (int j = 0; j < 8; ++j) d = d + qr[8 * i + j] * (float)w[j];
             }
         }
-        d = d * a.scale;
-        return a.cap > 0.0f ? tanhf(d / a.cap) * a.cap : d;
+        return capped(a, d * a.scale);
     };
     const auto reduce = [&](float v, auto op) {
         __syncthreads();
@@ -115,54 +185,664 @@ __global__ __launch_bounds__(kThreads) void attn_paged_plain_kernel(const PagedA
         }
         return red[0];
     };
-    float m = -INFINITY;
-    for (int p = si.start + t; p < si.end; p += kThreads)
-        if (si.sees(p)) m = fmaxf(m, score(p, vector_at<Q8, HD>(a.g, table, p, kvh)));
-    m = reduce(m, [](float x, float y) { return fmaxf(x, y); });
+    float mt = -INFINITY;
+#pragma unroll 1
+    for (int p = lo + t; p < up; p += kThreads)
+        if (si.sees(p)) mt = fmaxf(mt, score(vector_at<false>(a.g, table, p, kvh)));
+    m = reduce(mt, [](float x, float y) { return fmaxf(x, y); });
     constexpr int NP = kThreads / HD;
     const int d = t % HD;
-    float l = 0.0f, o = 0.0f;
-    for (int p0 = si.start; p0 < si.end; p0 += kThreads) {
+    float lt = 0.0f, o = 0.0f;
+#pragma unroll 1
+    for (int p0 = lo; p0 < up; p0 += kThreads) {
         const int p = p0 + t;
         long long v = -1;
         float w = 0.0f;
-        if (p < si.end && si.sees(p)) {
-            v = vector_at<Q8, HD>(a.g, table, p, kvh);
-            w = expf(score(p, v) - m);
-            l = l + w;
-            if constexpr (Q8) w = v >= 0 ? w * a.vs[v] : 0.0f;
+        if (p < up && si.sees(p)) {
+            v = vector_at<false>(a.g, table, p, kvh);
+            const float s = score(v);
+            // a range whose scores are all -inf weighs nothing beside others, and its l = NaN says that there were some
+            w = expf(s - m);
+            lt = lt + w;
+            if (part && m == -INFINITY) w = 0.0f;
         }
         __syncthreads();
         vec[t] = v;
         ws[t] = w;
         __syncthreads();
-        for (int j = t / HD; j < min(kThreads, si.end - p0); j += NP) {
-            if (vec[j] < 0) continue;
-            if constexpr (Q8) o = o + ws[j] * (float)static_cast<const int8_t*>(a.vc)[vec[j] * HD + d];
-            else o = o + ws[j] * (float)static_cast<const _Float16*>(a.vc)[vec[j] * HD + d];
-        }
+#pragma unroll 1
+        for (int j = t / HD; j < min(kThreads, up - p0); j += NP)
+            if (vec[j] >= 0) o = o + ws[j] * (float)static_cast<const _Float16*>(a.vc)[vec[j] * HD + d];
     }
-    l = reduce(l, [](float x, float y) { return x + y; });
+    l = reduce(lt, [](float x, float y) { return x + y; });
     __syncthreads();
     red[t] = o;
     __syncthreads();
-    if (t < HD) {
-        o = 0.0f;
+    o = 0.0f;
+    if (t < HD)
         for (int j = 0; j < NP; ++j) o = o + red[j * HD + t];
-        a.out[((size_t)row * a.n_heads + head) * HD + t] = l != 0.0f ? o / l : 0.0f;
+    __syncthreads();
+    return o;
+}
+
+// Positions lo..hi - 1 that the columns of a set may see; false: none of its rows has a position.
+__device__ __forceinline__ bool set_range(const MmaArgs& A, int set, int& lo, int& hi)
+{
+    const PagedAttnArgs& a = A.a;
+    const int table = set / A.tiles, c0 = (set - table * A.tiles) * kCols;
+    lo = A.cap;
+    hi = 0;
+    if (a.masks) {
+        const int c = a.pos[table], ctx = min(c, A.cap);
+        if (c < 0) return false;
+        hi = min(ctx + a.per, A.cap);
+        lo = a.window > 0 ? min(max(ctx + 1 - a.window, 0), hi - 1) : 0;  // a position at least: rows that see none get zeros
+        return true;
     }
+    const int j1 = min(a.per - 1, (c0 + kCols - 1) / A.group);
+    for (int j = c0 / A.group; j <= j1; ++j) {
+        const int p = a.pos[table * a.per + j];
+        if (p < 0) continue;
+        const int end = min(p, A.cap - 1) + 1;
+        hi = max(hi, end);
+        lo = min(lo, a.window > 0 ? max(end - a.window, 0) : 0);
+    }
+    return hi > 0;
+}
+
+struct Work {
+    int set, lo, hi, split, splits, slot0;  // positions of this block; slot0: work number of the set's split 0
+};
+
+// Work number w of a kv head.  Every wave looks at all sets (64 lanes, up to 8 sets each): their positions in units of
+// UNIT add up to the work, each set gets as many splits as units, in shares of the same size for all (so that
+// contexts of different lengths end together) and at most kMaxSplits, and the splits are numbered through.
+template <int UNIT>
+__device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
+{
+    const int lane = threadIdx.x & 63;
+    if (A.want == 0) {
+        k = Work{A.sets - 1 - w, 0, 0, 0, 1, 0};  // a prompt's last rows, which see the most, first
+        if (!set_range(A, k.set, k.lo, k.hi)) return false;
+        k.lo = rfl(k.lo) & ~63;
+        k.hi = rfl(k.hi);
+        return true;
+    }
+    constexpr int N = kPlanSets / 64;
+    int units[N], from[N], to[N], total = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        units[i] = from[i] = to[i] = 0;
+        if (64 * i >= A.sets) continue;  // the same for the whole wave
+        const int e = lane + 64 * i;
+        if (e < A.sets && set_range(A, e, from[i], to[i])) {
+            from[i] &= ~63;
+            units[i] = (to[i] - from[i] + UNIT - 1) / UNIT;
+        }
+        total += units[i];
+    }
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
+    const int share = max(1, (total + A.want - 1) / A.want);
+    int base = 0;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (64 * i >= A.sets || found) continue;
+        int n = min(kMaxSplits, (units[i] + share - 1) / share);
+        const int each = n > 0 ? (units[i] + n - 1) / n : 1;
+        n = (units[i] + each - 1) / each;
+        int up = n;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(up, o);
+            if (lane >= o) up += v;
+        }
+        const int first = base + up - n;
+        const unsigned long long hit = __ballot(w >= first && w < first + n);
+        if (hit) {  // one lane
+            const int src = __builtin_ctzll(hit);
+            found = true;
+            k.set = src + 64 * i;
+            k.splits = __builtin_amdgcn_readlane(n, src);
+            k.slot0 = __builtin_amdgcn_readlane(first, src);
+            k.split = w - k.slot0;
+            const int step = __builtin_amdgcn_readlane(each, src) * UNIT;
+            k.lo = __builtin_amdgcn_readlane(from[i], src) + k.split * step;
+            k.hi = min(__builtin_amdgcn_readlane(to[i], src), k.lo + step);
+        }
+        base += __builtin_amdgcn_readlane(up, 63);
+    }
+    return found;
+}
+
+template <bool Q8, int HD>
+struct Shape {
+    static constexpr int CH = Q8 ? (HD <= 128 ? 64 : 32) : (HD <= 64 ? 64 : 32);  // positions of a chunk
+    static constexpr int UNIT = kWaves * CH;
+    static constexpr int ES = Q8 ? 1 : 2;                    // bytes of an element of K and V
+    static constexpr int QS = Q8 ? HD + 16 : 2 * HD + 16;    // bytes between the columns of a q part in LDS
+    static constexpr int QP = Q8 ? 3 : 2;                    // parts of q
+    static constexpr int NR = HD / 4 < 32 ? HD / 4 : 32;     // registers of O^T that the waves add at a time
+};
+
+// codes of four dims at positions j (a) and j + 1 (b) as exact f16 pairs by dim: 0x6400 | (c + 128) is 1152 + c
+__device__ __forceinline__ void pairs_of_codes(uint32_t a, uint32_t b, uint32_t (&o)[4])
+{
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    const uint32_t s01 = __builtin_amdgcn_perm(b, a, 0x05010400u), s23 = __builtin_amdgcn_perm(b, a, 0x07030602u);
+    const h2_t bias = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    o[0] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, s01, 0x04010400u)) + bias);
+    o[1] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, s01, 0x04030402u)) + bias);
+    o[2] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, s23, 0x04010400u)) + bias);
+    o[3] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, s23, 0x04030402u)) + bias);
+}
+
+template <bool Q8, int HD, bool CAP>
+__global__ __launch_bounds__(kThreads) void attn_paged_kernel(const MmaArgs A)
+{
+    using S = Shape<Q8, HD>;
+    constexpr int CH = S::CH, NT = CH / 16, NP = CH / 4, KS = CH / 32;  // K tiles; positions of a lane; k steps of V
+    constexpr int KK = Q8 ? HD / 64 : HD / 32;                          // k steps of a K tile
+    constexpr int DT = HD / 16, VW = DT * S::ES / 4;                    // tiles of O^T; words of V per lane and position
+    constexpr int kMergeBytes = kWaves * S::NR * 64 * 4;
+    __shared__ __align__(16) unsigned char merge[kMergeBytes > 16384 ? kMergeBytes : 16384];
+    __shared__ __align__(16) unsigned char qs[S::QP * kCols * S::QS];
+    __shared__ float qscale[kCols];
+    __shared__ __align__(16) uint32_t kidx[kWaves][CH], vidx[kWaves][CH];  // [c][tile], [g][j]
+    __shared__ __align__(16) float kscl[kWaves][Q8 ? CH : 1], vscl[kWaves][Q8 ? CH : 1];
+    __shared__ float ml[kWaves][2][kCols];
+    __shared__ uint32_t flags;
+    __shared__ int last;
+
+    const PagedAttnArgs& a = A.a;
+    const int t = threadIdx.x, lane = t & 63, wave = rfl(t >> 6);
+    const int c = lane & 15, g4 = lane >> 4;
+    const int kvh = blockIdx.x % a.g.n_kv;
+    Work k;
+    if (!plan<S::UNIT>(A, blockIdx.x / a.g.n_kv, k)) return;  // the same for the whole block
+    const int table = k.set / A.tiles, col0 = (k.set - table * A.tiles) * kCols;
+    const auto row_of = [&](int col) { return table * a.per + (col0 + col) / A.group; };
+    const auto head_of = [&](int col) { return kvh * A.group + (col0 + col) % A.group; };
+    const int n_cols = a.per * A.group - col0;  // columns from n_cols on are none
+
+    // ---- the first chunk's page entries
+    const auto block_of = [&](int p) { return A.tpb_shift >= 0 ? p >> A.tpb_shift : p / a.g.tpb; };
+    const uint32_t* const bt = a.g.bt + (size_t)table * a.g.max_blocks;
+    int b_next = block_of(k.lo + wave * CH + (lane & (CH - 1)));
+    uint32_t blk_next = bt[min(b_next, a.g.max_blocks - 1)];
+
+    // ---- what column c sees
+    Sight si{0, 0, 0, a.masks};
+    const bool has = c < n_cols && sight_of(a, A.cap, table, row_of(min(c, n_cols - 1)), si);
+    if (!has) si.start = si.ctx = si.end = 0;
+    const uint32_t present = (uint32_t)__ballot(has) & 0xFFFFu;
+
+    // ---- q in LDS: 16 threads per column, HD / 16 elements each
+    {
+        constexpr int NE = HD / 16;
+        const int col = t >> 4, part = t & 15;
+        float x[NE];
+        if (present >> col & 1) {
+            const f4_t* src = reinterpret_cast<const f4_t*>(a.q + ((size_t)row_of(col) * a.n_heads + head_of(col)) * HD + part * NE);
+#pragma unroll
+            for (int i = 0; i < NE / 4; ++i) {
+                const f4_t v = src[i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[4 * i + j] = v[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NE; ++i) x[i] = 0.0f;
+        }
+        uint32_t mx = 0;  // |x| in the order of its bits; f16 pages: of the finite ones
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            const uint32_t b = __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu;
+            mx = max(mx, Q8 || b < 0x7F800000u ? b : 0u);
+        }
+        mx = team_max_u32<16>(mx);
+        const int top = max((int)(mx >> 23), 1) - 127;
+        unsigned char* dst = qs + col * S::QS + part * NE * S::ES;
+        if constexpr (Q8) {
+            const bool bad = mx >= 0x7F800000u;
+            const int e = mx > 0 && !bad ? 21 - top : 0;
+            uint32_t y[NE];
+#pragma unroll
+            for (int i = 0; i < NE; ++i) y[i] = (uint32_t)(int)rintf(bad ? 0.0f : ldexpf(x[i], e)) + 0x00808080u;
+#pragma unroll
+            for (int i = 0; i < NE / 4; ++i) {  // the three low bytes less 128 are the balanced digits
+                const uint32_t* w = y + 4 * i;
+                const uint32_t a01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), a23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+                const uint32_t b01 = __builtin_amdgcn_perm(w[1], w[0], 0x0C0C0602u), b23 = __builtin_amdgcn_perm(w[3], w[2], 0x0C0C0602u);
+                const uint32_t d[3] = {__builtin_amdgcn_perm(a23, a01, 0x05040100u), __builtin_amdgcn_perm(a23, a01, 0x07060302u),
+                                       __builtin_amdgcn_perm(b23, b01, 0x05040100u)};
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    *reinterpret_cast<uint32_t*>(dst + p * kCols * S::QS + 4 * i) = d[p] ^ 0x80808080u;
+            }
+            if (part == 0) qscale[col] = bad ? __builtin_nanf("") : ldexpf(a.scale, -e);
+        } else {
+            const int e = mx > 0 ? 13 - top : 0;
+#pragma unroll
+            for (int i = 0; i < NE; i += 2) {
+                h2_t hi, lo;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float v = ldexpf(x[i + j], e);
+                    hi[j] = (_Float16)v;
+                    lo[j] = finite_f32(v) ? (_Float16)(v - (float)hi[j]) : (_Float16)0.0f;
+                }
+                *reinterpret_cast<uint32_t*>(dst + 2 * i) = as_u32(hi);
+                *reinterpret_cast<uint32_t*>(dst + kCols * S::QS + 2 * i) = as_u32(lo);
+            }
+            if (part == 0) qscale[col] = ldexpf(a.scale, -e);
+        }
+        if (t == 0) flags = 0;
+    }
+    __syncthreads();
+    const float qsc = qscale[c];
+
+    f4_t o[DT];
+#pragma unroll
+    for (int e = 0; e < DT; ++e) o[e] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    // maximum of the scores, sum of the weights, and the scale of O: O^T is o * unit, unit a power of two that puts the
+    // largest weight * s_v so far into [2^13, 2^14) (8-bit pages; `top_w`, that weight, moves with the maximum)
+    float m = -INFINITY, l = 0.0f, unit = Q8 ? 0.0f : 0x1p-13f, top_w = 0.0f;
+    const unsigned char* const kbase = static_cast<const unsigned char*>(a.kc) + 16 * g4;
+    const unsigned char* const vbase = static_cast<const unsigned char*>(a.vc) + DT * S::ES * c;
+
+    for (int p0 = k.lo + wave * CH; p0 < k.hi; p0 += kWaves * CH) {
+        unsigned long long miss;
+        float ks_own = 0.0f, vs_own = 0.0f;
+        {
+            const int pp = p0 + (lane & (CH - 1));
+            const bool ok = pp < k.hi && b_next < a.g.max_blocks && blk_next < (uint32_t)a.g.total_blocks;
+            const uint32_t page = blk_next * (uint32_t)a.g.n_layers + (uint32_t)a.g.layer, off = (uint32_t)(pp - b_next * a.g.tpb);
+            const uint32_t vn = !ok ? 0u : Q8 ? (page * (uint32_t)a.g.n_kv + (uint32_t)kvh) * (uint32_t)a.g.tpb + off
+                                              : (page * (uint32_t)a.g.tpb + off) * (uint32_t)a.g.n_kv + (uint32_t)kvh;
+            if constexpr (Q8) {
+                ks_own = a.ks[vn];
+                vs_own = a.vs[vn];
+            }
+            miss = __ballot(!ok);
+            wave_lds_fence();
+            if (lane < CH) {  // position 16 tile + 4 i + g
+                const int tile = lane >> 4, i = lane >> 2 & 3, g = lane & 3;
+                kidx[wave][(4 * g + i) * NT + tile] = vn;
+                vidx[wave][g * NP + 4 * tile + i] = vn;
+            }
+            wave_lds_fence();
+        }
+        b_next = block_of(p0 + kWaves * CH + (lane & (CH - 1)));
+        blk_next = bt[min(b_next, a.g.max_blocks - 1)];
+        u4_t kr[NT][KK];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const unsigned char* src = kbase + (size_t)kidx[wave][c * NT + i] * (HD * S::ES);
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) kr[i][kk] = *reinterpret_cast<const u4_t*>(src + 64 * kk);
+        }
+        uint32_t vr[NP][VW];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const unsigned char* src = vbase + (size_t)vidx[wave][g4 * NP + j] * (HD * S::ES);
+            if constexpr (VW == 1) vr[j][0] = *reinterpret_cast<const uint32_t*>(src);
+            else if constexpr (VW == 2) {
+                const u2_t v = *reinterpret_cast<const u2_t*>(src);
+                vr[j][0] = v[0];
+                vr[j][1] = v[1];
+            } else {
+#pragma unroll
+                for (int w = 0; w < VW / 4; ++w) {
+                    const u4_t v = *reinterpret_cast<const u4_t*>(src + 16 * w);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) vr[j][4 * w + x] = v[x];
+                }
+            }
+        }
+        asm volatile("" ::: "memory");  // every load issued before any is used
+        if constexpr (Q8) {
+            if (lane < CH) {
+                const int tile = lane >> 4, i = lane >> 2 & 3, g = lane & 3;
+                const bool gone = miss >> lane & 1;  // a missing page counts as zeros
+                kscl[wave][g * NP + 4 * tile + i] = gone ? 0.0f : ks_own;
+                vscl[wave][g * NP + 4 * tile + i] = gone ? 0.0f : vs_own;
+            }
+            wave_lds_fence();
+        } else if (miss) {  // a missing page counts as zeros, and so do the positions past the range
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const bool gone = miss >> (16 * i + 4 * (c & 3) + (c >> 2)) & 1;
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) kr[i][kk] = gone ? u4_t{0, 0, 0, 0} : kr[i][kk];
+            }
+        }
+        // ---- scores of positions p0 + 4 j + g4
+        const uint64_t vis = visible(a, si, p0) >> g4;  // bit 4 j: position j of this lane
+        constexpr uint64_t kAll = CH == 64 ? ~0ull : (1ull << CH) - 1;
+        const bool partial = __ballot(has && ((vis << g4 | ((1ull << g4) - 1)) & kAll) != kAll) != 0;
+        float s[NP];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            if constexpr (Q8) {
+                i4_t d[3] = {};
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) {
+                        const i4_t qv = *reinterpret_cast<const i4_t*>(qs + (p * kCols + c) * S::QS + 64 * kk + 16 * g4);
+                        d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4_t, kr[i][kk]), qv, d[p], 0, 0, 0);
+                    }
+                const f4_t ksv = *reinterpret_cast<const f4_t*>(&kscl[wave][g4 * NP + 4 * i]);
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    s[4 * i + x] = __builtin_fmaf((float)d[2][x], 65536.0f, (float)(d[1][x] * 256 + d[0][x])) * qsc * ksv[x];
+            } else {
+                f4_t d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int p = 1; p >= 0; --p)  // the low parts first
+#pragma unroll
+                    for (int kk = 0; kk < KK; ++kk) {
+                        const h8_t qv = *reinterpret_cast<const h8_t*>(qs + (p * kCols + c) * S::QS + 64 * kk + 16 * g4);
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, kr[i][kk]), qv, d, 0, 0, 0);
+                    }
+#pragma unroll
+                for (int x = 0; x < 4; ++x) s[4 * i + x] = d[x] * qsc;
+            }
+        }
+        float mc = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            if constexpr (CAP) s[j] = capped(a, s[j]);
+            if (partial) s[j] = vis >> (4 * j) & 1 ? s[j] : -INFINITY;
+            mc = fmaxf(mc, s[j]);
+        }
+        mc = fmaxf(mc, lane_xor<16>(mc, 64));
+        mc = fmaxf(mc, lane_xor<32>(mc, 64));
+        // ---- weights
+        const float mn = fmaxf(m, mc);
+        const float shrink = mn > m && m > -INFINITY ? exp_neg(m - mn) : 1.0f;  // from -inf: l and O are 0
+        m = mn;
+        float lc = 0.0f, wc = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            float w = exp_neg(s[j] - mn);
+            if (partial) w = vis >> (4 * j) & 1 ? w : 0.0f;
+            lc = lc + w;
+            if constexpr (Q8) {
+                w = w * vscl[wave][g4 * NP + j];
+                if (partial) w = vis >> (4 * j) & 1 ? w : 0.0f;  // a scale there may be anything
+                wc = fmaxf(wc, w);
+            }
+            s[j] = w;
+        }
+        l = l * shrink + lc;
+        float ratio = shrink, factor = 0x1p13f;
+        if constexpr (Q8) {
+            wc = fmaxf(wc, lane_xor<16>(wc, 64));
+            wc = fmaxf(wc, lane_xor<32>(wc, 64));
+            top_w = fmaxf(top_w * shrink, wc);
+            // unit = 2^(E - 13) for top_w in [2^E, 2^(E + 1)), within f32
+            const uint32_t ex = min(max(__builtin_bit_cast(uint32_t, top_w) >> 23, 14u), 254u);
+            const float un = __builtin_bit_cast(float, (ex - 13u) << 23);
+            factor = __builtin_bit_cast(float, (267u - ex) << 23);
+            ratio = shrink * (unit * factor);  // the old unit over the new one
+            unit = un;
+        }
+        if (__ballot(ratio != 1.0f)) {
+#pragma unroll
+            for (int e = 0; e < DT; ++e) o[e] = o[e] * ratio;
+        }
+        h8_t ph[KS], pl[KS];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const float w = s[j] * factor;
+            const _Float16 h = (_Float16)w;
+            ph[j >> 3][j & 7] = h;
+            pl[j >> 3][j & 7] = (_Float16)(w - (float)h);
+        }
+        // ---- O^T += V^T . P^T
+        if constexpr (Q8) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    u4_t vt[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t x[4];
+                        pairs_of_codes(vr[8 * ks + 2 * i][w], vr[8 * ks + 2 * i + 1][w], x);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) vt[e][i] = x[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const h8_t v = __builtin_bit_cast(h8_t, vt[e]);
+                        o[4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ks], o[4 * w + e], 0, 0, 0);
+                        o[4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ks], o[4 * w + e], 0, 0, 0);
+                    }
+                }
+        } else {
+            if (miss) {
+#pragma unroll
+                for (int j = 0; j < NP; ++j)
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) vr[j][w] = miss >> (4 * j + g4) & 1 ? 0u : vr[j][w];
+            }
+#pragma unroll
+            for (int w = 0; w < VW; ++w)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        u4_t vt;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            vt[i] = __builtin_amdgcn_perm(vr[8 * ks + 2 * i + 1][w], vr[8 * ks + 2 * i][w], e ? 0x07060302u : 0x05040100u);
+                        const h8_t v = __builtin_bit_cast(h8_t, vt);
+                        o[2 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ks], o[2 * w + e], 0, 0, 0);
+                        o[2 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ks], o[2 * w + e], 0, 0, 0);
+                    }
+        }
+    }
+    l = l + lane_xor<16>(l, 64);
+    l = l + lane_xor<32>(l, 64);
+
+    // ---- the waves meet: lane (c, g) holds dims g HD / 4 + r of its column, r = 0..HD / 4 - 1, in register (r % DT, r / DT)
+    if (g4 == 0) {
+        ml[wave][0][c] = m;
+        ml[wave][1][c] = l;
+    }
+    const bool split = k.splits > 1;
+    const auto part_of = [&](int col, int sp) {
+        return A.part + (((size_t)(k.slot0 + sp) * a.g.n_kv + kvh) * kCols + col) * (HD + 2);
+    };
+    const auto out_of = [&](int col) { return a.out + ((size_t)row_of(col) * a.n_heads + head_of(col)) * HD; };
+    float* const mine = reinterpret_cast<float*>(merge) + lane;
+    bool odd = false;  // a sum that is not finite
+#pragma unroll
+    for (int rd = 0; rd < HD / 4 / S::NR; ++rd) {
+        if (rd) __syncthreads();
+#pragma unroll
+        for (int r = 0; r < S::NR; ++r) {
+            const int x = rd * S::NR + r;
+            mine[(wave * S::NR + r) * 64] = o[x % DT][x / DT] * unit;
+        }
+        __syncthreads();
+        float mm = ml[0][0][c], ll = 0.0f, acc[S::NR / 4];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, ml[w][0][c]);
+#pragma unroll
+        for (int r = 0; r < S::NR / 4; ++r) acc[r] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float ew = ml[w][0][c] > -INFINITY ? expf(ml[w][0][c] - mm) : ml[w][1][c];  // no weight: l is 0 (or NaN)
+            ll = ll + ml[w][1][c] * ew;
+#pragma unroll
+            for (int r = 0; r < S::NR / 4; ++r) acc[r] = acc[r] + mine[(w * S::NR + wave * (S::NR / 4) + r) * 64] * ew;
+        }
+        if (has) {
+            const int d0 = g4 * (HD / 4) + rd * S::NR + wave * (S::NR / 4);
+            if (split) {
+                float* p = part_of(c, k.split);
+#pragma unroll
+                for (int r = 0; r < S::NR / 4; ++r) st_agent(p + d0 + r, acc[r]);
+                if (rd == 0 && wave == 0 && g4 == 0) {
+                    st_agent(p + HD, mm);
+                    st_agent(p + HD + 1, ll);
+                }
+            } else {
+                const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+#pragma unroll
+                for (int r = 0; r < S::NR / 4; r += 4)
+                    *reinterpret_cast<f4_t*>(out_of(c) + d0 + r) = f4_t{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]} * inv;
+            }
+            if constexpr (!Q8) {
+#pragma unroll
+                for (int r = 0; r < S::NR / 4; ++r) odd |= !finite_f32(acc[r]);
+                odd |= !finite_f32(ll);
+            }
+        }
+    }
+    if constexpr (!Q8) {
+        if (odd) atomicOr(&flags, 1u << c);
+        __syncthreads();
+        const uint32_t again = flags;
+        if (again) {  // rare: columns that are not finite over this block's positions
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // their first values are written
+            __syncthreads();
+#pragma unroll 1
+            for (int col = 0; col < kCols; ++col) {
+                if (!(again >> col & 1)) continue;
+                Sight sc;
+                sight_of(a, A.cap, table, row_of(col), sc);
+                float mm, ll;
+                const float v = plain_range<HD>(a, sc, table, row_of(col), head_of(col), max(k.lo, sc.start), min(k.hi, sc.end),
+                                                split, merge, mm, ll);
+                if (split) {
+                    float* p = part_of(col, k.split);
+                    if (t < HD) st_agent(p + t, v);
+                    if (t == 0) {
+                        st_agent(p + HD, mm);
+                        st_agent(p + HD + 1, ll);
+                    }
+                } else if (t < HD) {
+                    out_of(col)[t] = ll != 0.0f ? v / ll : 0.0f;
+                }
+            }
+        }
+    }
+    if (!split) return;
+    // ---- this block's partials are performed at the coherence point before it counts itself
+    uint32_t* const counter = A.counters + (size_t)k.set * a.g.n_kv + kvh;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t == 0)
+        last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(k.splits - 1);
+    __syncthreads();
+    if (!last) return;
+    // split maxima and sums to LDS, then weights e^(m_k - M), then two dims a thread, eight loads at a time
+    const int n = k.splits;
+    float* const mk = reinterpret_cast<float*>(merge);  // [column][split], then the weights
+    float* const lk = mk + kCols * kMaxSplits;
+    for (int i = t; i < kCols * n; i += kThreads) {
+        const int col = i / n, sp = i - col * n;
+        if (!(present >> col & 1)) continue;
+        const float* p = part_of(col, sp) + HD;
+        mk[i] = ld_agent(p);
+        lk[i] = ld_agent(p + 1);
+    }
+    __syncthreads();
+    for (int col = wave; col < kCols; col += kWaves) {
+        if (!(present >> col & 1)) continue;
+        const float mv = lane < n ? mk[col * n + lane] : -INFINITY, lv = lane < n ? lk[col * n + lane] : 0.0f;
+        const float mm = group_max<64>(mv);
+        // a split without a score above -inf weighs nothing beside others; where all are so, its l is 0 (nothing
+        // seen: zeros) or NaN
+        const float ew = mv > -INFINITY ? expf(mv - mm) : mm > -INFINITY ? 0.0f : 1.0f;
+        const float ll = group_sum<64>(mv > -INFINITY || !(mm > -INFINITY) ? lv * ew : 0.0f);
+        if (lane < n) mk[col * n + lane] = ew;
+        if (lane == 0) ml[0][0][col] = ll;
+    }
+    __syncthreads();
+    for (int i = t; i < kCols * (HD / 2); i += kThreads) {
+        const int col = i / (HD / 2), d = 2 * (i % (HD / 2));
+        if (!(present >> col & 1)) continue;
+        f2_t acc = {0.0f, 0.0f};
+        for (int sp = 0; sp < n; sp += 8) {
+            f2_t v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = ld_agent2(part_of(col, min(sp + j, n - 1)) + d);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (sp + j < n) acc = acc + v[j] * mk[col * n + sp + j];
+        }
+        const float ll = ml[0][0][col];
+        *reinterpret_cast<f2_t*>(out_of(col) + d) = acc * (ll != 0.0f ? 1.0f / ll : 0.0f);
+    }
+    if (t == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <typename F>
+void by_shape(bool q8, int head_dim, F&& f)
+{
+    const auto with = [&](auto q) {
+        if (head_dim == 64) f(q, std::integral_constant<int, 64>{});
+        else if (head_dim == 128) f(q, std::integral_constant<int, 128>{});
+        else f(q, std::integral_constant<int, 256>{});
+    };
+    q8 ? with(std::true_type{}) : with(std::false_type{});
+}
+
+struct Layout {
+    int group, tiles, sets, want;
+    long long works;  // per kv head
+};
+
+Layout layout_of(const PagedAttnArgs& a)
+{
+    Layout y{};
+    y.group = a.n_heads / a.g.n_kv;
+    y.tiles = (a.per * y.group + kCols - 1) / kCols;
+    y.sets = a.rows / a.per * y.tiles;
+    const long long cap = (long long)a.g.max_blocks * a.g.tpb;
+    int unit = 0;
+    by_shape(a.ks != nullptr, a.head_dim, [&](auto q, auto hd) { unit = Shape<decltype(q)::value, decltype(hd)::value>::UNIT; });
+    const long long units = (cap + unit - 1) / unit;
+    if (y.sets <= kPlanSets && (long long)y.sets * a.g.n_kv < kPlanBlocks && units > 1) y.want = std::max(1, kPlanBlocks / a.g.n_kv);
+    // each set's last split may be short
+    y.works = y.want ? std::min<long long>(y.want + y.sets, y.sets * std::min<long long>(kMaxSplits, units)) : y.sets;
+    return y;
 }
 
 }  // namespace
 
-hipError_t launch_attention_paged(const PagedAttnArgs& a, hipStream_t st)
+size_t attention_paged_workspace_bytes(const PagedAttnArgs& a)
 {
-    const dim3 grid((unsigned)a.rows * (unsigned)a.n_heads);
-    const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, st, a); };
-    const bool q8 = a.ks != nullptr;
-    if (a.head_dim == 64) q8 ? go(attn_paged_plain_kernel<true, 64>) : go(attn_paged_plain_kernel<false, 64>);
-    else if (a.head_dim == 128) q8 ? go(attn_paged_plain_kernel<true, 128>) : go(attn_paged_plain_kernel<false, 128>);
-    else q8 ? go(attn_paged_plain_kernel<true, 256>) : go(attn_paged_plain_kernel<false, 256>);
+    const Layout y = layout_of(a);
+    return y.want ? attention_counter_bytes() + (size_t)y.works * a.g.n_kv * kCols * (a.head_dim + 2) * sizeof(float) : 0;
+}
+
+hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipStream_t st)
+{
+    const Layout y = layout_of(a);
+    MmaArgs A{};
+    A.a = a;
+    A.group = y.group;
+    A.tiles = y.tiles;
+    A.sets = y.sets;
+    A.want = y.want;
+    A.cap = a.g.max_blocks * a.g.tpb;
+    A.tpb_shift = (a.g.tpb & (a.g.tpb - 1)) == 0 ? __builtin_ctz((unsigned)a.g.tpb) : -1;
+    A.counters = reinterpret_cast<uint32_t*>(workspace);
+    A.part = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + attention_counter_bytes());
+    const dim3 grid((unsigned)(y.works * a.g.n_kv));
+    by_shape(a.ks != nullptr, a.head_dim, [&](auto q, auto hd) {
+        constexpr bool Q8 = decltype(q)::value;
+        constexpr int HD = decltype(hd)::value;
+        if (a.cap > 0.0f) hipLaunchKernelGGL((attn_paged_kernel<Q8, HD, true>), grid, dim3(kThreads), 0, st, A);
+        else hipLaunchKernelGGL((attn_paged_kernel<Q8, HD, false>), grid, dim3(kThreads), 0, st, A);
+    });
     return hipGetLastError();
 }
 

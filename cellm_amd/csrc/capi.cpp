@@ -13,9 +13,11 @@
 #include <cstdio>
 #include <cstring>
 #include <atomic>
+#include <map>
 #include <mutex>
 #include <string>
 #include <unordered_map>
+#include <utility>
 #include <vector>
 
 #include "../../include/cellm_hip.h"
@@ -103,6 +105,7 @@ struct cellm_hip_ctx {
     std::unordered_map<hipStream_t, DeviceBuffer> aux;         // unfused gate/up: the up rows, one per stream
     std::unordered_map<hipStream_t, DeviceBuffer> attn;        // split-sequence attention partials, one per stream
     std::unordered_map<hipStream_t, DeviceBuffer> argmax;      // argmax row counters + chunk partials, one per stream
+    std::map<std::pair<unsigned long long, hipStream_t>, DeviceBuffer> graph_scratch;  // one per capture and stream
     std::vector<void*> retired;                                // outgrown scratch that captured graphs still write to
     float* attn_static = nullptr;  // this device's static attention scratch (cellm_hip_attention_gqa_f16kv_noalloc)
     std::atomic<int> rope_interleaved{0};  // RoPE pairs of the fused decode ops (cellm_hip_set_rope_interleaved)
@@ -702,6 +705,8 @@ void cellm_hip_destroy(cellm_hip_ctx_t* ctx)
             (void)hipStreamSynchronize(kv.first);
             if (kv.second.ptr) (void)hipFree(kv.second.ptr);
         }
+    for (auto& kv : ctx->graph_scratch)
+        if (kv.second.ptr) (void)hipFree(kv.second.ptr);
     for (void* p : ctx->retired) (void)hipFree(p);
     for (auto& kv : ctx->weights)
         if (kv.second.ptr) (void)hipFree(kv.second.ptr);
@@ -1768,6 +1773,46 @@ int32_t cellm_hip_argmax_f32_keys(cellm_hip_ctx_t* ctx, const float* logits, int
 
 namespace {
 
+// Scratch of a call that its kernel leaves as it found it in its first zero_prefix bytes (zero): the stream's
+// attention scratch, or, under a capture, scratch of that graph's own, so that graphs captured on one stream may
+// run at once and beside eager calls.  It lasts as long as the context, as the graph may.  The caller holds ctx->mu
+// until the kernel is enqueued.
+int32_t get_graph_safe_scratch(cellm_hip_ctx* ctx, hipStream_t st, size_t need, float** out, size_t zero_prefix)
+{
+    *out = nullptr;
+    if (need == 0) return CELLM_HIP_OK;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    HIP_TRY(hipStreamGetCaptureInfo(st, &status, &id), "hipStreamGetCaptureInfo");
+    if (status == hipStreamCaptureStatusNone) return get_stream_buffer(ctx, ctx->attn, st, need, out, zero_prefix);
+    if (status != hipStreamCaptureStatusActive) return set_error(CELLM_HIP_ERR_DEVICE, "the stream's capture is invalid");
+    DeviceBuffer& b = ctx->graph_scratch[{id, st}];
+    if (b.bytes < need) {
+        const RelaxedCapture relaxed;
+        if (b.ptr) ctx->retired.push_back(b.ptr);  // earlier nodes of the graph use it
+        b = DeviceBuffer{};
+        void* p = nullptr;
+        HIP_TRY(hipMalloc(&p, need), "hipMalloc(graph scratch)");
+        // cleared now, by a kernel on a stream that no capture holds: the graph's own replays find zeros
+        hipStream_t tmp = nullptr;
+        hipError_t e = hipStreamCreateWithFlags(&tmp, hipStreamNonBlocking);
+        if (e == hipSuccess) {
+            e = launch_fill_f32(static_cast<float*>(p), 0.0f, std::min(zero_prefix, need) / sizeof(float), tmp);
+            const hipError_t e2 = hipStreamSynchronize(tmp);
+            if (e == hipSuccess) e = e2;
+            (void)hipStreamDestroy(tmp);
+        }
+        if (e != hipSuccess) {
+            (void)hipFree(p);
+            return hip_error(e, "clearing graph scratch");
+        }
+        b.ptr = p;
+        b.bytes = need;
+    }
+    *out = static_cast<float*>(b.ptr);
+    return CELLM_HIP_OK;
+}
+
 // What every call on a paged cache checks; `rows` rows, `per` to a row of the block tables.
 int32_t check_kv(int64_t rows, int64_t per, int64_t n_kv_heads, int64_t head_dim, int64_t max_blocks,
                  int64_t total_blocks, int64_t n_layers, int64_t tpb, int64_t layer)
@@ -1845,7 +1890,12 @@ int32_t attention_paged_impl(cellm_hip_ctx* ctx, const PagedAttnArgs& in, int64_
     a.window = (int)window;
     if (!(a.scale > 0.0f)) a.scale = 1.0f / std::sqrt((float)head_dim);
     DeviceGuard g(ctx->device);
-    HIP_TRY(launch_attention_paged(a, pick_stream(ctx, stream)), "attention launch");
+    const std::lock_guard<std::recursive_mutex> lk(ctx->mu);  // held until the scratch user is enqueued
+    const hipStream_t st = pick_stream(ctx, stream);
+    float* ws = nullptr;
+    if (int32_t rc = get_graph_safe_scratch(ctx, st, attention_paged_workspace_bytes(a), &ws, attention_counter_bytes()))
+        return rc;
+    HIP_TRY(launch_attention_paged(a, ws, st), "attention launch");
     return CELLM_HIP_OK;
 }
 

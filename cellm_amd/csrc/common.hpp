@@ -150,6 +150,17 @@ __device__ __forceinline__ float group_max(float v)
     if constexpr (W >= 2) v = fmaxf(v, lane_xor<1>(v, W));
     return v;
 }
+// Maximum of unsigned words over aligned teams of W lanes (a power of two <= 32).
+template <int W>
+__device__ __forceinline__ uint32_t team_max_u32(uint32_t v)
+{
+    if constexpr (W >= 32) v = max(v, __builtin_bit_cast(uint32_t, lane_xor<16>(__builtin_bit_cast(float, v), 64)));
+    if constexpr (W >= 16) v = max(v, __builtin_bit_cast(uint32_t, lane_xor<8>(__builtin_bit_cast(float, v), 64)));
+    if constexpr (W >= 8) v = max(v, __builtin_bit_cast(uint32_t, lane_xor<4>(__builtin_bit_cast(float, v), 64)));
+    if constexpr (W >= 4) v = max(v, __builtin_bit_cast(uint32_t, lane_xor<2>(__builtin_bit_cast(float, v), 64)));
+    if constexpr (W >= 2) v = max(v, __builtin_bit_cast(uint32_t, lane_xor<1>(__builtin_bit_cast(float, v), 64)));
+    return v;
+}
 // Sums of V values over aligned teams of W lanes, transposed (V <= W, both powers
 // of two): log2(V) halving steps, each at offset O = W/2, W/4, ..., leave every
 // lane with one value, and plain butterfly steps finish the sum over the team.

@@ -217,7 +217,10 @@ struct PagedAttnArgs {
     float* out;
 };
 constexpr int kMaxTree = 256;  // nodes of a drafted tree
-hipError_t launch_attention_paged(const PagedAttnArgs& a, hipStream_t st);
+// Scratch of one call, 0 for none: attention_counter_bytes() of counters, zero before the first call and after
+// every one, then the splits' sums.
+size_t attention_paged_workspace_bytes(const PagedAttnArgs& a);
+hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipStream_t st);
 
 // First maximum per row (non-finite -> -inf): chunk blocks of 4096 elements in one launch; rows past
 // one chunk need scratch of argmax_scratch_bytes whose first argmax_counter_bytes (the per-row

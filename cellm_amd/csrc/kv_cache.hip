@@ -36,22 +36,6 @@ __device__ __forceinline__ long long vector_of(const KvGeom& g, int table, int s
     return ((long long)blk * g.n_layers + g.layer) * g.n_kv * (long long)g.tpb + (slot - b * g.tpb);
 }
 
-// maximum over aligned teams of W lanes, of unsigned words
-template <int W>
-__device__ __forceinline__ uint32_t team_max_u32(uint32_t v)
-{
-    const auto step = [&](auto off) {
-        constexpr int O = decltype(off)::value;
-        if constexpr (W > O) v = max(v, __builtin_bit_cast(uint32_t, lane_xor<O>(__builtin_bit_cast(float, v), 64)));
-    };
-    step(std::integral_constant<int, 1>{});
-    step(std::integral_constant<int, 2>{});
-    step(std::integral_constant<int, 4>{});
-    step(std::integral_constant<int, 8>{});
-    step(std::integral_constant<int, 16>{});
-    return v;
-}
-
 struct WriteArgs {
     const float* q;       // nullptr: no q
     const float* k;
