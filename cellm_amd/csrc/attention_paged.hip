@@ -23,9 +23,15 @@
 // nearest), as three signed 8-bit digits, and q . c_k is three exact sums on
 // v_mfma_i32_16x16x64_i8 with the codes as they are.  f16 pages: q as two f16 parts, hi =
 // RNE_f16(q') and lo = RNE_f16(q' - hi) of q scaled by a power of two (23 bits of an element,
-// 2^-38 of the largest).  The weights (times s_v) are two such parts too, scaled so that the
-// largest that the column has met lies in [2^13, 2^14), over the codes as exact f16 integers
-// or f16 values.  Scores, exponentials, maxima and sums are f32.
+// 2^-38 of the largest).  Scores, exponentials and sums are f32.
+//
+// Weights are powers of two, w = 2^(c s - R) (c s rounded by itself, so that scores too large for
+// the difference to have bits still compare) with c = log2(e) times what of the score's scale
+// is left out of s, against a reference R of each column that stands in for the maximum: l and
+// O hold sums of w and of w s_v v, so any R gives the same quotient.  The products w s_v are
+// two f16 parts like q's, over the codes as exact f16 integers or f16 values, and R is raised
+// (and l and O with it) only where one of them passes 2^15, to leave the largest at 2^13: a
+// test of the lanes' own values, where a maximum of each chunk would be sums over lanes.
 //
 // The positions of a set of columns are split over blocks by a rule on the device (plan()),
 // which knows how long every context is; the last block of a set to finish adds the others'
@@ -42,44 +48,54 @@ namespace cellm {
 
 namespace {
 
-typedef float f2_t __attribute__((ext_vector_type(2)));
-
 constexpr int kWaves = 4, kThreads = kWaves * 64, kCols = 16;
 constexpr int kMaxSplits = 64;   // of a set's positions
 constexpr int kPlanSets = 512;   // sets that plan() looks at, 8 a lane; more run unsplit
-constexpr int kPlanBlocks = 768; // blocks that it aims at: three on each of 256 CUs
+#ifndef PB
+#define PB 512
+#endif
+#ifndef CTMIN
+#define CTMIN 16
+#endif
+#ifndef MINSHARE
+#define MINSHARE 1
+#endif
+constexpr int kPlanBlocks = PB;
 
 struct MmaArgs {
     PagedAttnArgs a;
-    int group, tiles, sets;  // heads per kv head; sets of 16 columns of a table, and of all tables
+    int group, cols, tiles, sets;  // heads per kv head; columns of a set; sets of a table, and of all tables
     int cap, tpb_shift;      // positions of a table; log2(tpb), or -1
     int want;                // blocks per kv head that plan() aims at; 0: one block per set
     uint32_t* counters;      // [set][kv head]: splits done, zero between calls
-    float* part;             // [work][kv head][16][HD + 2]
+    float* part;             // [work][kv head]: [cols][HD] sums, [cols] references, [cols] sums of weights
+    uint32_t part_bytes;
 };
 
 __device__ __forceinline__ bool finite_f32(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) != 0x7F800000u; }
-__device__ __forceinline__ void st_agent(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float ld_agent(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ f2_t ld_agent2(const float* p)  // 8-byte aligned
+// Agent-coherent (sc1) stores and loads of a split's sums, 16 bytes at a time; offsets in floats.
+constexpr int kSc1 = 16;
+__device__ __forceinline__ void st_agent4(__amdgpu_buffer_rsrc_t r, uint32_t off, f4_t v)
 {
-    return __builtin_bit_cast(f2_t, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, v), r, (int)(4u * off), 0, kSc1);
+}
+__device__ __forceinline__ f4_t ld_agent4(__amdgpu_buffer_rsrc_t r, uint32_t off)
+{
+    return __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(4u * off), 0, kSc1));
+}
+__device__ __forceinline__ void st_agent(__amdgpu_buffer_rsrc_t r, uint32_t off, float v)
+{
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), r, (int)(4u * off), 0, kSc1);
+}
+__device__ __forceinline__ float ld_agent(__amdgpu_buffer_rsrc_t r, uint32_t off)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)(4u * off), 0, kSc1));
 }
 // LDS of one wave, written and read across its lanes: the wave's LDS operations run in order, and the
 // compiler moves none across this
 __device__ __forceinline__ void wave_lds_fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ int rfl(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// e^x for x <= 0 to the accuracy of the hardware exponential: x log2(e) in two parts, the second folded in
-// to first order.  -inf gives NaN (callers select masked positions away).
-__device__ __forceinline__ float exp_neg(float x)
-{
-    const float kLog2e = 1.4426950216293335f, kLog2eLo = 1.9259629911266175e-8f, kLn2 = 0.6931471805599453f;
-    const float h = x * kLog2e;
-    const float r = __builtin_fmaf(x, kLog2eLo, __builtin_fmaf(x, kLog2e, -h));
-    const float e = __builtin_amdgcn_exp2f(h);
-    return __builtin_fmaf(e, r * kLn2, e);
-}
 
 // What a row sees: positions start..ctx - 1, then (masks) those of ctx..end - 1 whose bit is set.
 struct Sight {
@@ -149,13 +165,13 @@ __device__ __forceinline__ float capped(const PagedAttnArgs& a, float s)
     return a.cap > 0.0f ? tanhf(s / a.cap) * a.cap : s;
 }
 
-// Positions lo..up - 1 of one (row, head) over f16 pages by plain f32 sums, the whole block: maximum m, sum l of
-// e^(score - m) and, in threads below HD, the weighted sum of V (returned).  256 positions at a time: a score per
-// thread, then HD threads per position.  For columns whose sums in f16 parts are not finite: inf * lo may be NaN where
+// The units of positions lo, lo + step, ... below up of one (row, head) over f16 pages by plain f32 sums, the whole block: reference R, log2(e) times
+// the largest score, sum l of the weights and, in threads below HD, the weighted sum of V (returned).  A unit at a time: a score
+// per thread, then HD threads per position.  For columns whose sums in f16 parts are not finite: inf * lo may be NaN where
 // inf * v is not, and so is the 0 * inf of a position that the column does not see.
-template <int HD>
-__device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table, int row, int head, int lo, int up,
-                             bool part, unsigned char* lds, float& m, float& l)
+template <int HD, int UNIT>
+__device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table, int row, int head, int lo, int up, int step,
+                             bool part, unsigned char* lds, float& R, float& l)
 {
     long long* const vec = reinterpret_cast<long long*>(lds);
     float* const red = reinterpret_cast<float*>(vec + kThreads);
@@ -187,22 +203,23 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
     };
     float mt = -INFINITY;
 #pragma unroll 1
-    for (int p = lo + t; p < up; p += kThreads)
-        if (si.sees(p)) mt = fmaxf(mt, score(vector_at<false>(a.g, table, p, kvh)));
-    m = reduce(mt, [](float x, float y) { return fmaxf(x, y); });
+    for (int p = lo + t; p < up; p += step)
+        if (t < UNIT && si.sees(p)) mt = fmaxf(mt, score(vector_at<false>(a.g, table, p, kvh)));
+    const float m = reduce(mt, [](float x, float y) { return fmaxf(x, y); });
+    R = m * kLog2e;
     constexpr int NP = kThreads / HD;
     const int d = t % HD;
     float lt = 0.0f, o = 0.0f;
 #pragma unroll 1
-    for (int p0 = lo; p0 < up; p0 += kThreads) {
+    for (int p0 = lo; p0 < up; p0 += step) {
         const int p = p0 + t;
         long long v = -1;
         float w = 0.0f;
-        if (p < up && si.sees(p)) {
+        if (t < UNIT && p < up && si.sees(p)) {
             v = vector_at<false>(a.g, table, p, kvh);
             const float s = score(v);
             // a range whose scores are all -inf weighs nothing beside others, and its l = NaN says that there were some
-            w = expf(s - m);
+            w = exp2f(__builtin_fmaf(s, kLog2e, -R));
             lt = lt + w;
             if (part && m == -INFINITY) w = 0.0f;
         }
@@ -211,7 +228,7 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
         ws[t] = w;
         __syncthreads();
 #pragma unroll 1
-        for (int j = t / HD; j < min(kThreads, up - p0); j += NP)
+        for (int j = t / HD; j < min(UNIT, up - p0); j += NP)
             if (vec[j] >= 0) o = o + ws[j] * (float)static_cast<const _Float16*>(a.vc)[vec[j] * HD + d];
     }
     l = reduce(lt, [](float x, float y) { return x + y; });
@@ -229,7 +246,7 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
 __device__ __forceinline__ bool set_range(const MmaArgs& A, int set, int& lo, int& hi)
 {
     const PagedAttnArgs& a = A.a;
-    const int table = set / A.tiles, c0 = (set - table * A.tiles) * kCols;
+    const int table = set / A.tiles, c0 = (set - table * A.tiles) * A.cols;
     lo = A.cap;
     hi = 0;
     if (a.masks) {
@@ -239,7 +256,7 @@ __device__ __forceinline__ bool set_range(const MmaArgs& A, int set, int& lo, in
         lo = a.window > 0 ? min(max(ctx + 1 - a.window, 0), hi - 1) : 0;  // a position at least: rows that see none get zeros
         return true;
     }
-    const int j1 = min(a.per - 1, (c0 + kCols - 1) / A.group);
+    const int j1 = min(a.per - 1, (c0 + A.cols - 1) / A.group);
     for (int j = c0 / A.group; j <= j1; ++j) {
         const int p = a.pos[table * a.per + j];
         if (p < 0) continue;
@@ -251,7 +268,8 @@ __device__ __forceinline__ bool set_range(const MmaArgs& A, int set, int& lo, in
 }
 
 struct Work {
-    int set, lo, hi, split, splits, slot0;  // positions of this block; slot0: work number of the set's split 0
+    int set, lo, hi, step;      // units of positions lo, lo + step, ... below hi
+    int split, splits, slot0;   // slot0: work number of the set's split 0
 };
 
 // Work number w of a kv head.  Every wave looks at all sets (64 lanes, up to 8 sets each): their positions in units of
@@ -262,7 +280,7 @@ __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
 {
     const int lane = threadIdx.x & 63;
     if (A.want == 0) {
-        k = Work{A.sets - 1 - w, 0, 0, 0, 1, 0};  // a prompt's last rows, which see the most, first
+        k = Work{A.sets - 1 - w, 0, 0, UNIT, 0, 1, 0};  // a prompt's last rows, which see the most, first
         if (!set_range(A, k.set, k.lo, k.hi)) return false;
         k.lo = rfl(k.lo) & ~63;
         k.hi = rfl(k.hi);
@@ -282,7 +300,7 @@ __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
         total += units[i];
     }
     for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-    const int share = max(1, (total + A.want - 1) / A.want);
+    const int share = max(MINSHARE, (total + A.want - 1) / A.want);
     int base = 0;
     bool found = false;
 #pragma unroll
@@ -305,9 +323,9 @@ __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
             k.splits = __builtin_amdgcn_readlane(n, src);
             k.slot0 = __builtin_amdgcn_readlane(first, src);
             k.split = w - k.slot0;
-            const int step = __builtin_amdgcn_readlane(each, src) * UNIT;
-            k.lo = __builtin_amdgcn_readlane(from[i], src) + k.split * step;
-            k.hi = min(__builtin_amdgcn_readlane(to[i], src), k.lo + step);
+            k.lo = __builtin_amdgcn_readlane(from[i], src) + k.split * UNIT;
+            k.hi = __builtin_amdgcn_readlane(to[i], src);
+            k.step = k.splits * UNIT;
         }
         base += __builtin_amdgcn_readlane(up, 63);
     }
@@ -337,20 +355,22 @@ __device__ __forceinline__ void pairs_of_codes(uint32_t a, uint32_t b, uint32_t 
     o[3] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, s23, 0x04030402u)) + bias);
 }
 
-template <bool Q8, int HD, bool CAP>
-__global__ __launch_bounds__(kThreads) void attn_paged_kernel(const MmaArgs A)
+template <bool Q8, int HD, int CT, bool CAP>
+__global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A)
 {
     using S = Shape<Q8, HD>;
     constexpr int CH = S::CH, NT = CH / 16, NP = CH / 4, KS = CH / 32;  // K tiles; positions of a lane; k steps of V
     constexpr int KK = Q8 ? HD / 64 : HD / 32;                          // k steps of a K tile
     constexpr int DT = HD / 16, VW = DT * S::ES / 4;                    // tiles of O^T; words of V per lane and position
+    constexpr int COLS = kCols * CT;
     constexpr int kMergeBytes = kWaves * S::NR * 64 * 4;
-    __shared__ __align__(16) unsigned char merge[kMergeBytes > 16384 ? kMergeBytes : 16384];
-    __shared__ __align__(16) unsigned char qs[S::QP * kCols * S::QS];
-    __shared__ float qscale[kCols];
+    static_assert(kMergeBytes >= COLS * kMaxSplits * 8 && kMergeBytes >= kThreads * 16, "LDS of the later steps");
+    __shared__ __align__(16) unsigned char merge[kMergeBytes];
+    __shared__ __align__(16) unsigned char qs[S::QP * COLS * S::QS];
+    __shared__ float qscale[COLS];
     __shared__ __align__(16) uint32_t kidx[kWaves][CH], vidx[kWaves][CH];  // [c][tile], [g][j]
-    __shared__ __align__(16) float kscl[kWaves][Q8 ? CH : 1], vscl[kWaves][Q8 ? CH : 1];
-    __shared__ float ml[kWaves][2][kCols];
+    __shared__ __align__(16) float kscl[kWaves][Q8 ? CH : 4], vscl[kWaves][Q8 ? CH : 4];
+    __shared__ float ml[kWaves][2][COLS];
     __shared__ uint32_t flags;
     __shared__ int last;
 
@@ -360,7 +380,7 @@ __global__ __launch_bounds__(kThreads) void attn_paged_kernel(const MmaArgs A)
     const int kvh = blockIdx.x % a.g.n_kv;
     Work k;
     if (!plan<S::UNIT>(A, blockIdx.x / a.g.n_kv, k)) return;  // the same for the whole block
-    const int table = k.set / A.tiles, col0 = (k.set - table * A.tiles) * kCols;
+    const int table = k.set / A.tiles, col0 = (k.set - table * A.tiles) * COLS;
     const auto row_of = [&](int col) { return table * a.per + (col0 + col) / A.group; };
     const auto head_of = [&](int col) { return kvh * A.group + (col0 + col) % A.group; };
     const int n_cols = a.per * A.group - col0;  // columns from n_cols on are none
@@ -368,19 +388,27 @@ __global__ __launch_bounds__(kThreads) void attn_paged_kernel(const MmaArgs A)
     // ---- the first chunk's page entries
     const auto block_of = [&](int p) { return A.tpb_shift >= 0 ? p >> A.tpb_shift : p / a.g.tpb; };
     const uint32_t* const bt = a.g.bt + (size_t)table * a.g.max_blocks;
-    int b_next = block_of(k.lo + wave * CH + (lane & (CH - 1)));
-    uint32_t blk_next = bt[min(b_next, a.g.max_blocks - 1)];
+    const int b_first = block_of(k.lo + wave * CH + (lane & (CH - 1)));
+    const uint32_t blk_first = bt[min(b_first, a.g.max_blocks - 1)];
 
-    // ---- what column c sees
-    Sight si{0, 0, 0, a.masks};
-    const bool has = c < n_cols && sight_of(a, A.cap, table, row_of(min(c, n_cols - 1)), si);
-    if (!has) si.start = si.ctx = si.end = 0;
-    const uint32_t present = (uint32_t)__ballot(has) & 0xFFFFu;
+    // ---- what column 16 u + c sees
+    Sight si[CT];
+    bool has[CT];
+    uint32_t present = 0;
+#pragma unroll
+    for (int u = 0; u < CT; ++u) {
+        const int col = kCols * u + c;
+        si[u] = Sight{0, 0, 0, a.masks};
+        has[u] = col < n_cols && sight_of(a, A.cap, table, row_of(min(col, n_cols - 1)), si[u]);
+        if (!has[u]) si[u].start = si[u].ctx = si[u].end = 0;
+        present |= ((uint32_t)__ballot(has[u]) & 0xFFFFu) << (kCols * u);
+    }
 
     // ---- q in LDS: 16 threads per column, HD / 16 elements each
-    {
+#pragma unroll
+    for (int u = 0; u < CT; ++u) {
         constexpr int NE = HD / 16;
-        const int col = t >> 4, part = t & 15;
+        const int col = kCols * u + (t >> 4), part = t & 15;
         float x[NE];
         if (present >> col & 1) {
             const f4_t* src = reinterpret_cast<const f4_t*>(a.q + ((size_t)row_of(col) * a.n_heads + head_of(col)) * HD + part * NE);
@@ -418,7 +446,7 @@ __global__ __launch_bounds__(kThreads) void attn_paged_kernel(const MmaArgs A)
                                        __builtin_amdgcn_perm(b23, b01, 0x05040100u)};
 #pragma unroll
                 for (int p = 0; p < 3; ++p)
-                    *reinterpret_cast<uint32_t*>(dst + p * kCols * S::QS + 4 * i) = d[p] ^ 0x80808080u;
+                    *reinterpret_cast<uint32_t*>(dst + p * COLS * S::QS + 4 * i) = d[p] ^ 0x80808080u;
             }
             if (part == 0) qscale[col] = bad ? __builtin_nanf("") : ldexpf(a.scale, -e);
         } else {
@@ -433,56 +461,75 @@ __global__ __launch_bounds__(kThreads) void attn_paged_kernel(const MmaArgs A)
                     lo[j] = finite_f32(v) ? (_Float16)(v - (float)hi[j]) : (_Float16)0.0f;
                 }
                 *reinterpret_cast<uint32_t*>(dst + 2 * i) = as_u32(hi);
-                *reinterpret_cast<uint32_t*>(dst + kCols * S::QS + 2 * i) = as_u32(lo);
+                *reinterpret_cast<uint32_t*>(dst + COLS * S::QS + 2 * i) = as_u32(lo);
             }
             if (part == 0) qscale[col] = ldexpf(a.scale, -e);
         }
         if (t == 0) flags = 0;
     }
     __syncthreads();
-    const float qsc = qscale[c];
 
-    f4_t o[DT];
+    f4_t o[CT][DT];
+    float R[CT], l[CT], qsc[CT], cs[CT];  // reference, sum of the weights; scale of the sums and of the exponents
+    float F[CT];                          // O is in units of 1 / F
+    bool coarse = false;                  // F is not 1 somewhere
 #pragma unroll
-    for (int e = 0; e < DT; ++e) o[e] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    // maximum of the scores, sum of the weights, and the scale of O: O^T is o * unit, unit a power of two that puts the
-    // largest weight * s_v so far into [2^13, 2^14) (8-bit pages; `top_w`, that weight, moves with the maximum)
-    float m = -INFINITY, l = 0.0f, unit = Q8 ? 0.0f : 0x1p-13f, top_w = 0.0f;
+    for (int u = 0; u < CT; ++u) {
+#pragma unroll
+        for (int e = 0; e < DT; ++e) o[u][e] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        F[u] = 1.0f;
+        R[u] = -INFINITY;  // the first chunk's weights pass any bound
+        l[u] = 0.0f;
+        qsc[u] = qscale[kCols * u + c];
+        cs[u] = CAP ? kLog2e : qsc[u] * kLog2e;
+    }
     const unsigned char* const kbase = static_cast<const unsigned char*>(a.kc) + 16 * g4;
     const unsigned char* const vbase = static_cast<const unsigned char*>(a.vc) + DT * S::ES * c;
 
-    for (int p0 = k.lo + wave * CH; p0 < k.hi; p0 += kWaves * CH) {
-        unsigned long long miss;
-        float ks_own = 0.0f, vs_own = 0.0f;
-        {
-            const int pp = p0 + (lane & (CH - 1));
-            const bool ok = pp < k.hi && b_next < a.g.max_blocks && blk_next < (uint32_t)a.g.total_blocks;
-            const uint32_t page = blk_next * (uint32_t)a.g.n_layers + (uint32_t)a.g.layer, off = (uint32_t)(pp - b_next * a.g.tpb);
-            const uint32_t vn = !ok ? 0u : Q8 ? (page * (uint32_t)a.g.n_kv + (uint32_t)kvh) * (uint32_t)a.g.tpb + off
-                                              : (page * (uint32_t)a.g.tpb + off) * (uint32_t)a.g.n_kv + (uint32_t)kvh;
-            if constexpr (Q8) {
-                ks_own = a.ks[vn];
-                vs_own = a.vs[vn];
-            }
-            miss = __ballot(!ok);
-            wave_lds_fence();
-            if (lane < CH) {  // position 16 tile + 4 i + g
-                const int tile = lane >> 4, i = lane >> 2 & 3, g = lane & 3;
-                kidx[wave][(4 * g + i) * NT + tile] = vn;
-                vidx[wave][g * NP + 4 * tile + i] = vn;
-            }
-            wave_lds_fence();
+    // A chunk's loads are issued an iteration ahead, into the registers that its predecessor has just used: K and the
+    // scales after the scores, V after the weighted sums, page entries two chunks ahead.  The last iteration loads too:
+    // behind a branch every wait for V would be one for the K issued after it.
+    uint32_t blk;                       // page entry of this lane's position, of the chunk whose indexes come next
+    int b_of;                           // its place in the table
+    unsigned long long miss, miss_next; // positions without a page, or past the range
+    float ks_own = 0.0f, vs_own = 0.0f;
+    u4_t kr[NT][KK];
+    uint32_t vr[NP][VW];
+    uint32_t vn = 0;
+    const auto load_page = [&](int p0) {
+        b_of = block_of(p0 + (lane & (CH - 1)));
+        blk = bt[min(b_of, a.g.max_blocks - 1)];
+    };
+    const auto index = [&](int p0) {    // vector numbers of the chunk at p0 into LDS
+        const int pp = p0 + (lane & (CH - 1));
+        const bool ok = pp < k.hi && b_of < a.g.max_blocks && blk < (uint32_t)a.g.total_blocks;
+        const uint32_t page = blk * (uint32_t)a.g.n_layers + (uint32_t)a.g.layer, off = (uint32_t)(pp - b_of * a.g.tpb);
+        // where there is none: the last vector again, loaded but not used
+        vn = !ok ? vn : Q8 ? (page * (uint32_t)a.g.n_kv + (uint32_t)kvh) * (uint32_t)a.g.tpb + off
+                           : (page * (uint32_t)a.g.tpb + off) * (uint32_t)a.g.n_kv + (uint32_t)kvh;
+        miss_next = __ballot(!ok);
+        wave_lds_fence();
+        if (lane < CH) {  // position 16 tile + 4 i + g
+            const int tile = lane >> 4, i = lane >> 2 & 3, g = lane & 3;
+            kidx[wave][(4 * g + i) * NT + tile] = vn;
+            vidx[wave][g * NP + 4 * tile + i] = vn;
         }
-        b_next = block_of(p0 + kWaves * CH + (lane & (CH - 1)));
-        blk_next = bt[min(b_next, a.g.max_blocks - 1)];
-        u4_t kr[NT][KK];
+        wave_lds_fence();
+    };
+    const auto load_k = [&]() {
+        if constexpr (Q8) {
+            ks_own = a.ks[vn];
+            vs_own = a.vs[vn];
+        }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const unsigned char* src = kbase + (size_t)kidx[wave][c * NT + i] * (HD * S::ES);
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) kr[i][kk] = *reinterpret_cast<const u4_t*>(src + 64 * kk);
         }
-        uint32_t vr[NP][VW];
+        asm volatile("" ::: "memory");  // issued here
+    };
+    const auto load_v = [&]() {
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const unsigned char* src = vbase + (size_t)vidx[wave][g4 * NP + j] * (HD * S::ES);
@@ -500,7 +547,20 @@ __global__ __launch_bounds__(kThreads) void attn_paged_kernel(const MmaArgs A)
                 }
             }
         }
-        asm volatile("" ::: "memory");  // every load issued before any is used
+        asm volatile("" ::: "memory");
+    };
+    const int step = k.step;
+    int p0 = k.lo + wave * CH;
+    if (p0 < k.hi) {
+        b_of = b_first;
+        blk = blk_first;
+        index(p0);
+        load_page(p0 + step);
+        load_k();
+        load_v();
+    }
+    for (; p0 < k.hi; p0 += step) {
+        miss = miss_next;
         if constexpr (Q8) {
             if (lane < CH) {
                 const int tile = lane >> 4, i = lane >> 2 & 3, g = lane & 3;
@@ -508,8 +568,10 @@ __global__ __launch_bounds__(kThreads) void attn_paged_kernel(const MmaArgs A)
                 kscl[wave][g * NP + 4 * tile + i] = gone ? 0.0f : ks_own;
                 vscl[wave][g * NP + 4 * tile + i] = gone ? 0.0f : vs_own;
             }
-            wave_lds_fence();
-        } else if (miss) {  // a missing page counts as zeros, and so do the positions past the range
+        }
+        index(p0 + step);
+        load_page(p0 + 2 * step);
+        if (!Q8 && miss) {  // a missing page counts as zeros, and so do the positions past the range
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
                 const bool gone = miss >> (16 * i + 4 * (c & 3) + (c >> 2)) & 1;
@@ -517,91 +579,123 @@ __global__ __launch_bounds__(kThreads) void attn_paged_kernel(const MmaArgs A)
                 for (int kk = 0; kk < KK; ++kk) kr[i][kk] = gone ? u4_t{0, 0, 0, 0} : kr[i][kk];
             }
         }
-        // ---- scores of positions p0 + 4 j + g4
-        const uint64_t vis = visible(a, si, p0) >> g4;  // bit 4 j: position j of this lane
-        constexpr uint64_t kAll = CH == 64 ? ~0ull : (1ull << CH) - 1;
-        const bool partial = __ballot(has && ((vis << g4 | ((1ull << g4) - 1)) & kAll) != kAll) != 0;
-        float s[NP];
+        // ---- scores of positions p0 + 4 j + g4, less their scale qsc without a cap
+        h8_t ph[CT][KS], pl[CT][KS];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            if constexpr (Q8) {
-                i4_t d[3] = {};
+        for (int u = 0; u < CT; ++u) {
+            float s[NP];
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk)
+            for (int i = 0; i < NT; ++i) {
+                if constexpr (Q8) {
+                    i4_t d[3] = {};
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) {
-                        const i4_t qv = *reinterpret_cast<const i4_t*>(qs + (p * kCols + c) * S::QS + 64 * kk + 16 * g4);
-                        d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4_t, kr[i][kk]), qv, d[p], 0, 0, 0);
-                    }
-                const f4_t ksv = *reinterpret_cast<const f4_t*>(&kscl[wave][g4 * NP + 4 * i]);
+                    for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    s[4 * i + x] = __builtin_fmaf((float)d[2][x], 65536.0f, (float)(d[1][x] * 256 + d[0][x])) * qsc * ksv[x];
-            } else {
-                f4_t d = {0.0f, 0.0f, 0.0f, 0.0f};
+                        for (int p = 0; p < 3; ++p) {
+                            const i4_t qv = *reinterpret_cast<const i4_t*>(qs + (p * COLS + kCols * u + c) * S::QS + 64 * kk + 16 * g4);
+                            d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4_t, kr[i][kk]), qv, d[p], 0, 0, 0);
+                        }
+                    const f4_t ksv = *reinterpret_cast<const f4_t*>(&kscl[wave][g4 * NP + 4 * i]);
 #pragma unroll
-                for (int p = 1; p >= 0; --p)  // the low parts first
+                    for (int x = 0; x < 4; ++x)
+                        s[4 * i + x] = __builtin_fmaf((float)d[2][x], 65536.0f, (float)(d[1][x] * 256 + d[0][x])) * ksv[x];
+                } else {
+                    f4_t d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int kk = 0; kk < KK; ++kk) {
-                        const h8_t qv = *reinterpret_cast<const h8_t*>(qs + (p * kCols + c) * S::QS + 64 * kk + 16 * g4);
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, kr[i][kk]), qv, d, 0, 0, 0);
-                    }
+                    for (int p = 1; p >= 0; --p)  // the low parts first
 #pragma unroll
-                for (int x = 0; x < 4; ++x) s[4 * i + x] = d[x] * qsc;
+                        for (int kk = 0; kk < KK; ++kk) {
+                            const h8_t qv = *reinterpret_cast<const h8_t*>(qs + (p * COLS + kCols * u + c) * S::QS + 64 * kk + 16 * g4);
+                            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, kr[i][kk]), qv, d, 0, 0, 0);
+                        }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[4 * i + x] = d[x];
+                }
             }
-        }
-        float mc = -INFINITY;
+            if (u == CT - 1) load_k();
+            float vs[NP];
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            if constexpr (CAP) s[j] = capped(a, s[j]);
-            if (partial) s[j] = vis >> (4 * j) & 1 ? s[j] : -INFINITY;
-            mc = fmaxf(mc, s[j]);
-        }
-        mc = fmaxf(mc, lane_xor<16>(mc, 64));
-        mc = fmaxf(mc, lane_xor<32>(mc, 64));
-        // ---- weights
-        const float mn = fmaxf(m, mc);
-        const float shrink = mn > m && m > -INFINITY ? exp_neg(m - mn) : 1.0f;  // from -inf: l and O are 0
-        m = mn;
-        float lc = 0.0f, wc = 0.0f;
+            for (int j = 0; j < NP; ++j) vs[j] = Q8 ? vscl[wave][g4 * NP + j] : 1.0f;
+            if constexpr (CAP) {
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            float w = exp_neg(s[j] - mn);
-            if (partial) w = vis >> (4 * j) & 1 ? w : 0.0f;
-            lc = lc + w;
-            if constexpr (Q8) {
-                w = w * vscl[wave][g4 * NP + j];
-                if (partial) w = vis >> (4 * j) & 1 ? w : 0.0f;  // a scale there may be anything
-                wc = fmaxf(wc, w);
+                for (int j = 0; j < NP; ++j) s[j] = capped(a, s[j] * qsc[u]);
             }
-            s[j] = w;
-        }
-        l = l * shrink + lc;
-        float ratio = shrink, factor = 0x1p13f;
-        if constexpr (Q8) {
-            wc = fmaxf(wc, lane_xor<16>(wc, 64));
-            wc = fmaxf(wc, lane_xor<32>(wc, 64));
-            top_w = fmaxf(top_w * shrink, wc);
-            // unit = 2^(E - 13) for top_w in [2^E, 2^(E + 1)), within f32
-            const uint32_t ex = min(max(__builtin_bit_cast(uint32_t, top_w) >> 23, 14u), 254u);
-            const float un = __builtin_bit_cast(float, (ex - 13u) << 23);
-            factor = __builtin_bit_cast(float, (267u - ex) << 23);
-            ratio = shrink * (unit * factor);  // the old unit over the new one
-            unit = un;
-        }
-        if (__ballot(ratio != 1.0f)) {
+            // ---- weights; of positions that some column does not see, those are 0 whatever they hold
+            const bool partial = __ballot(has[u] && (p0 < si[u].start || p0 + CH > si[u].ctx)) != 0;
+            uint64_t vis = ~0ull;  // bit 4 j: position j of this lane
+            float w[NP], lc, mx;
+            const auto weigh = [&]() {
+                lc = mx = 0.0f;
 #pragma unroll
-            for (int e = 0; e < DT; ++e) o[e] = o[e] * ratio;
-        }
-        h8_t ph[KS], pl[KS];
+                for (int j = 0; j < NP; ++j) w[j] = __builtin_amdgcn_exp2f(s[j] * cs[u] - R[u]);
+                if (partial) {
+                    asm volatile("");  // a branch
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            const float w = s[j] * factor;
-            const _Float16 h = (_Float16)w;
-            ph[j >> 3][j & 7] = h;
-            pl[j >> 3][j & 7] = (_Float16)(w - (float)h);
+                    for (int j = 0; j < NP; ++j) w[j] = vis >> (4 * j) & 1 ? w[j] : 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    lc = lc + w[j];
+                    if constexpr (Q8) w[j] = w[j] * vs[j];
+                    mx = fmaxf(mx, w[j]);
+                }
+                if (Q8 && coarse) {
+                    asm volatile("");
+                    mx = mx * F[u];
+#pragma unroll
+                    for (int j = 0; j < NP; ++j) w[j] = w[j] * F[u];
+                }
+            };
+            if (partial) {
+                vis = visible(a, si[u], p0) >> g4;
+#pragma unroll
+                for (int j = 0; j < NP; ++j) vs[j] = vis >> (4 * j) & 1 ? vs[j] : 0.0f;
+            }
+            weigh();
+            if (__ballot(mx > 0x1p15f || lc > 0x1p100f)) {
+                // the reference that leaves the largest product at 2^13 (and weights of small s_v below 2^90)
+                float m1 = -INFINITY, m2 = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    const float h = vis >> (4 * j) & 1 ? s[j] * cs[u] : -INFINITY;
+                    m1 = fmaxf(m1, h);
+                    m2 = fmaxf(m2, Q8 ? h + __builtin_amdgcn_logf(vs[j]) : h);
+                }
+                m1 = fmaxf(m1, lane_xor<16>(m1, 64));
+                m1 = fmaxf(m1, lane_xor<32>(m1, 64));
+                m2 = fmaxf(m2, lane_xor<16>(m2, 64));
+                m2 = fmaxf(m2, lane_xor<32>(m2, 64));
+                const float up = fmaxf(R[u], fmaxf(m2 - 13.0f, m1 - 90.0f));
+                float ratio = up > R[u] ? __builtin_amdgcn_exp2f(R[u] - up) : 1.0f;  // from -inf: 0, as l and O are
+                R[u] = up;
+                l[u] = l[u] * ratio;
+                if constexpr (Q8) {
+                    // beyond 2^20 a reference has no bits for the 13: the products are scaled down instead
+                    const float over = m2 - up;
+                    const float f = over > 15.0f && over < 1000.0f ? fminf(F[u], __builtin_amdgcn_exp2f(13.0f - rintf(over))) : F[u];
+                    ratio = ratio * (f / F[u]);
+                    F[u] = f;
+                    coarse = coarse || __ballot(f != 1.0f) != 0;
+                }
+#pragma unroll
+                for (int e = 0; e < DT; ++e) o[u][e] = o[u][e] * ratio;
+                weigh();
+            }
+            l[u] = l[u] + lc;
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                const _Float16 h = (_Float16)w[j];
+                ph[u][j >> 3][j & 7] = h;
+                pl[u][j >> 3][j & 7] = (_Float16)(w[j] - (float)h);
+            }
         }
         // ---- O^T += V^T . P^T
+        if (!Q8 && miss) {
+#pragma unroll
+            for (int j = 0; j < NP; ++j)
+#pragma unroll
+                for (int w = 0; w < VW; ++w) vr[j][w] = miss >> (4 * j + g4) & 1 ? 0u : vr[j][w];
+        }
         if constexpr (Q8) {
 #pragma unroll
             for (int w = 0; w < VW; ++w)
@@ -616,19 +710,15 @@ __global__ __launch_bounds__(kThreads) void attn_paged_kernel(const MmaArgs A)
                         for (int e = 0; e < 4; ++e) vt[e][i] = x[e];
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const h8_t v = __builtin_bit_cast(h8_t, vt[e]);
-                        o[4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ks], o[4 * w + e], 0, 0, 0);
-                        o[4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ks], o[4 * w + e], 0, 0, 0);
-                    }
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int u = 0; u < CT; ++u) {
+                            const h8_t v = __builtin_bit_cast(h8_t, vt[e]);
+                            o[u][4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u][ks], o[u][4 * w + e], 0, 0, 0);
+                            o[u][4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u][ks], o[u][4 * w + e], 0, 0, 0);
+                        }
                 }
         } else {
-            if (miss) {
-#pragma unroll
-                for (int j = 0; j < NP; ++j)
-#pragma unroll
-                    for (int w = 0; w < VW; ++w) vr[j][w] = miss >> (4 * j + g4) & 1 ? 0u : vr[j][w];
-            }
 #pragma unroll
             for (int w = 0; w < VW; ++w)
 #pragma unroll
@@ -640,91 +730,110 @@ __global__ __launch_bounds__(kThreads) void attn_paged_kernel(const MmaArgs A)
                         for (int i = 0; i < 4; ++i)
                             vt[i] = __builtin_amdgcn_perm(vr[8 * ks + 2 * i + 1][w], vr[8 * ks + 2 * i][w], e ? 0x07060302u : 0x05040100u);
                         const h8_t v = __builtin_bit_cast(h8_t, vt);
-                        o[2 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ks], o[2 * w + e], 0, 0, 0);
-                        o[2 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ks], o[2 * w + e], 0, 0, 0);
+#pragma unroll
+                        for (int u = 0; u < CT; ++u) {
+                            o[u][2 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u][ks], o[u][2 * w + e], 0, 0, 0);
+                            o[u][2 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u][ks], o[u][2 * w + e], 0, 0, 0);
+                        }
                     }
         }
+        load_v();
     }
-    l = l + lane_xor<16>(l, 64);
-    l = l + lane_xor<32>(l, 64);
 
     // ---- the waves meet: lane (c, g) holds dims g HD / 4 + r of its column, r = 0..HD / 4 - 1, in register (r % DT, r / DT)
-    if (g4 == 0) {
-        ml[wave][0][c] = m;
-        ml[wave][1][c] = l;
+#pragma unroll
+    for (int u = 0; u < CT; ++u) {
+        l[u] = l[u] + lane_xor<16>(l[u], 64);
+        l[u] = l[u] + lane_xor<32>(l[u], 64);
+        if (Q8 && coarse) {
+#pragma unroll
+            for (int e = 0; e < DT; ++e) o[u][e] = o[u][e] / F[u];
+        }
+        if (g4 == 0) {
+            ml[wave][0][kCols * u + c] = R[u];
+            ml[wave][1][kCols * u + c] = l[u];
+        }
     }
     const bool split = k.splits > 1;
-    const auto part_of = [&](int col, int sp) {
-        return A.part + (((size_t)(k.slot0 + sp) * a.g.n_kv + kvh) * kCols + col) * (HD + 2);
-    };
+    const __amdgpu_buffer_rsrc_t part = buffer_rsrc(A.part, A.part_bytes);
+    constexpr uint32_t kPart = COLS * (HD + 2);  // floats of a block's sums: [COLS][HD], then R and l, [COLS] each
+    const auto part_of = [&](int sp) { return (uint32_t)((k.slot0 + sp) * a.g.n_kv + kvh) * kPart; };
     const auto out_of = [&](int col) { return a.out + ((size_t)row_of(col) * a.n_heads + head_of(col)) * HD; };
     float* const mine = reinterpret_cast<float*>(merge) + lane;
-    bool odd = false;  // a sum that is not finite
 #pragma unroll
-    for (int rd = 0; rd < HD / 4 / S::NR; ++rd) {
-        if (rd) __syncthreads();
+    for (int u = 0; u < CT; ++u) {
+        const int col = kCols * u + c;
+        bool odd = false;  // a sum that is not finite
 #pragma unroll
-        for (int r = 0; r < S::NR; ++r) {
-            const int x = rd * S::NR + r;
-            mine[(wave * S::NR + r) * 64] = o[x % DT][x / DT] * unit;
-        }
-        __syncthreads();
-        float mm = ml[0][0][c], ll = 0.0f, acc[S::NR / 4];
+        for (int rd = 0; rd < HD / 4 / S::NR; ++rd) {
+            if (u || rd) __syncthreads();
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, ml[w][0][c]);
+            for (int r = 0; r < S::NR; ++r) {
+                const int x = rd * S::NR + r;
+                mine[(wave * S::NR + r) * 64] = o[u][x % DT][x / DT];
+            }
+            __syncthreads();
+            float mm = ml[0][0][col], ll = 0.0f, acc[S::NR / 4];
 #pragma unroll
-        for (int r = 0; r < S::NR / 4; ++r) acc[r] = 0.0f;
+            for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, ml[w][0][col]);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float ew = ml[w][0][c] > -INFINITY ? expf(ml[w][0][c] - mm) : ml[w][1][c];  // no weight: l is 0 (or NaN)
-            ll = ll + ml[w][1][c] * ew;
+            for (int r = 0; r < S::NR / 4; ++r) acc[r] = 0.0f;
 #pragma unroll
-            for (int r = 0; r < S::NR / 4; ++r) acc[r] = acc[r] + mine[(w * S::NR + wave * (S::NR / 4) + r) * 64] * ew;
-        }
-        if (has) {
-            const int d0 = g4 * (HD / 4) + rd * S::NR + wave * (S::NR / 4);
-            if (split) {
-                float* p = part_of(c, k.split);
+            for (int w = 0; w < kWaves; ++w) {
+                // no weight (l is 0, or NaN)
+                const float ew = ml[w][0][col] > -INFINITY ? __builtin_amdgcn_exp2f(ml[w][0][col] - mm) : ml[w][1][col];
+                ll = ll + ml[w][1][col] * ew;
 #pragma unroll
-                for (int r = 0; r < S::NR / 4; ++r) st_agent(p + d0 + r, acc[r]);
-                if (rd == 0 && wave == 0 && g4 == 0) {
-                    st_agent(p + HD, mm);
-                    st_agent(p + HD + 1, ll);
+                for (int r = 0; r < S::NR / 4; ++r) acc[r] = acc[r] + mine[(w * S::NR + wave * (S::NR / 4) + r) * 64] * ew;
+            }
+            if (has[u]) {
+                const int d0 = g4 * (HD / 4) + rd * S::NR + wave * (S::NR / 4);
+                if (split) {
+                    const uint32_t at = part_of(k.split);
+#pragma unroll
+                    for (int r = 0; r < S::NR / 4; r += 4)
+                        st_agent4(part, at + col * HD + d0 + r, f4_t{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]});
+                    if (rd == 0 && wave == 0 && g4 == 0) {
+                        st_agent(part, at + COLS * HD + col, mm);
+                        st_agent(part, at + COLS * (HD + 1) + col, ll);
+                    }
+                } else {
+                    const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+#pragma unroll
+                    for (int r = 0; r < S::NR / 4; r += 4)
+                        *reinterpret_cast<f4_t*>(out_of(col) + d0 + r) = f4_t{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]} * inv;
                 }
-            } else {
-                const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+                if constexpr (!Q8) {
 #pragma unroll
-                for (int r = 0; r < S::NR / 4; r += 4)
-                    *reinterpret_cast<f4_t*>(out_of(c) + d0 + r) = f4_t{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]} * inv;
+                    for (int r = 0; r < S::NR / 4; ++r) odd |= !finite_f32(acc[r]);
+                    odd |= !finite_f32(ll);
+                }
             }
-            if constexpr (!Q8) {
-#pragma unroll
-                for (int r = 0; r < S::NR / 4; ++r) odd |= !finite_f32(acc[r]);
-                odd |= !finite_f32(ll);
-            }
+        }
+        if constexpr (!Q8) {
+            if (odd) atomicOr(&flags, 1u << col);
         }
     }
     if constexpr (!Q8) {
-        if (odd) atomicOr(&flags, 1u << c);
         __syncthreads();
         const uint32_t again = flags;
         if (again) {  // rare: columns that are not finite over this block's positions
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // their first values are written
             __syncthreads();
 #pragma unroll 1
-            for (int col = 0; col < kCols; ++col) {
+            for (int col = 0; col < COLS; ++col) {
                 if (!(again >> col & 1)) continue;
                 Sight sc;
                 sight_of(a, A.cap, table, row_of(col), sc);
                 float mm, ll;
-                const float v = plain_range<HD>(a, sc, table, row_of(col), head_of(col), max(k.lo, sc.start), min(k.hi, sc.end),
-                                                split, merge, mm, ll);
+                const float v = plain_range<HD, S::UNIT>(a, sc, table, row_of(col), head_of(col), k.lo, min(k.hi, sc.end), k.step,
+                                                         split, merge, mm, ll);
                 if (split) {
-                    float* p = part_of(col, k.split);
-                    if (t < HD) st_agent(p + t, v);
+                    const uint32_t at = part_of(k.split);
+                    if (t < HD) st_agent(part, at + col * HD + t, v);
                     if (t == 0) {
-                        st_agent(p + HD, mm);
-                        st_agent(p + HD + 1, ll);
+                        st_agent(part, at + COLS * HD + col, mm);
+                        st_agent(part, at + COLS * (HD + 1) + col, ll);
                     }
                 } else if (t < HD) {
                     out_of(col)[t] = ll != 0.0f ? v / ll : 0.0f;
@@ -741,44 +850,76 @@ __global__ __launch_bounds__(kThreads) void attn_paged_kernel(const MmaArgs A)
         last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(k.splits - 1);
     __syncthreads();
     if (!last) return;
-    // split maxima and sums to LDS, then weights e^(m_k - M), then two dims a thread, eight loads at a time
+    // The splits' references and sums of weights to LDS, then weights 2^(R_k - R).  The values: an item is four dims of a
+    // column that is there; few items share their splits among groups of threads, which meet in LDS.
     const int n = k.splits;
-    float* const mk = reinterpret_cast<float*>(merge);  // [column][split], then the weights
-    float* const lk = mk + kCols * kMaxSplits;
-    for (int i = t; i < kCols * n; i += kThreads) {
-        const int col = i / n, sp = i - col * n;
+    float* const mk = reinterpret_cast<float*>(merge);  // [column][kMaxSplits], then the weights
+    float* const lk = mk + COLS * kMaxSplits;
+    f4_t* const red = reinterpret_cast<f4_t*>(lk);      // once lk is read
+    const int items = __popc(present) * (HD / 4), groups = max(1, kThreads / items);
+    const auto column = [&](int i) {                    // of the i-th that is there
+        uint32_t left = present;
+        for (int x = 0; x < i; ++x) left &= left - 1;
+        return __builtin_ctz(left);
+    };
+    constexpr int U = 8;  // loads in flight
+    f4_t v[U];
+    const int group = t / items;
+    int item = t - group * items;
+    bool busy = group < groups && items > 0;
+    uint32_t at = busy ? column(item / (HD / 4)) * HD + 4 * (item % (HD / 4)) : 0u;
+    const auto load = [&](int sp) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = ld_agent4(part, part_of(min(sp + j * groups, n - 1)) + at);
+    };
+    if (busy) load(group);
+    for (int i = t; i < COLS * n; i += kThreads) {
+        const int sp = i / COLS, col = i % COLS;
         if (!(present >> col & 1)) continue;
-        const float* p = part_of(col, sp) + HD;
-        mk[i] = ld_agent(p);
-        lk[i] = ld_agent(p + 1);
+        mk[col * kMaxSplits + sp] = ld_agent(part, part_of(sp) + COLS * HD + col);
+        lk[col * kMaxSplits + sp] = ld_agent(part, part_of(sp) + COLS * (HD + 1) + col);
     }
     __syncthreads();
-    for (int col = wave; col < kCols; col += kWaves) {
+    for (int col = wave; col < COLS; col += kWaves) {
         if (!(present >> col & 1)) continue;
-        const float mv = lane < n ? mk[col * n + lane] : -INFINITY, lv = lane < n ? lk[col * n + lane] : 0.0f;
+        const float mv = lane < n ? mk[col * kMaxSplits + lane] : -INFINITY, lv = lane < n ? lk[col * kMaxSplits + lane] : 0.0f;
         const float mm = group_max<64>(mv);
         // a split without a score above -inf weighs nothing beside others; where all are so, its l is 0 (nothing
         // seen: zeros) or NaN
-        const float ew = mv > -INFINITY ? expf(mv - mm) : mm > -INFINITY ? 0.0f : 1.0f;
+        const float ew = mv > -INFINITY ? __builtin_amdgcn_exp2f(mv - mm) : mm > -INFINITY ? 0.0f : 1.0f;
         const float ll = group_sum<64>(mv > -INFINITY || !(mm > -INFINITY) ? lv * ew : 0.0f);
-        if (lane < n) mk[col * n + lane] = ew;
+        if (lane < n) mk[col * kMaxSplits + lane] = ew;
         if (lane == 0) ml[0][0][col] = ll;
     }
     __syncthreads();
-    for (int i = t; i < kCols * (HD / 2); i += kThreads) {
-        const int col = i / (HD / 2), d = 2 * (i % (HD / 2));
-        if (!(present >> col & 1)) continue;
-        f2_t acc = {0.0f, 0.0f};
-        for (int sp = 0; sp < n; sp += 8) {
-            f2_t v[8];
+    for (;;) {  // more than 256 items: again for the others, in one group
+        f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int col = (int)(at / HD);
+        if (busy) {
+            for (int sp = group; sp < n; sp += U * groups) {
+                if (sp > group) load(sp);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = ld_agent2(part_of(col, min(sp + j, n - 1)) + d);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (sp + j < n) acc = acc + v[j] * mk[col * n + sp + j];
+                for (int j = 0; j < U; ++j)
+                    if (sp + j * groups < n) acc = acc + v[j] * mk[col * kMaxSplits + sp + j * groups];
+            }
         }
-        const float ll = ml[0][0][col];
-        *reinterpret_cast<f2_t*>(out_of(col) + d) = acc * (ll != 0.0f ? 1.0f / ll : 0.0f);
+        if (groups > 1) {
+            red[t] = acc;
+            __syncthreads();
+            if (group == 0)
+                for (int x = 1; x < groups; ++x) acc = acc + red[x * items + t];
+        }
+        if (busy && group == 0) {
+            const float ll = ml[0][0][col];
+            *reinterpret_cast<f4_t*>(out_of(col) + at % HD) = acc * (ll != 0.0f ? 1.0f / ll : 0.0f);
+        }
+        item += kThreads;
+        if (groups > 1 || item - t >= items) break;
+        busy = item < items;
+        if (busy) {
+            at = column(item / (HD / 4)) * HD + 4 * (item % (HD / 4));
+            load(0);
+        }
     }
     if (t == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -795,7 +936,7 @@ void by_shape(bool q8, int head_dim, F&& f)
 }
 
 struct Layout {
-    int group, tiles, sets, want;
+    int group, ct, cols, tiles, sets, want;
     long long works;  // per kv head
 };
 
@@ -803,13 +944,16 @@ Layout layout_of(const PagedAttnArgs& a)
 {
     Layout y{};
     y.group = a.n_heads / a.g.n_kv;
-    y.tiles = (a.per * y.group + kCols - 1) / kCols;
+    const long long columns = (long long)a.per * y.group;
+    y.ct = columns > CTMIN && a.head_dim <= 128 ? 2 : 1;
+    y.cols = kCols * y.ct;
+    y.tiles = (int)((columns + y.cols - 1) / y.cols);
     y.sets = a.rows / a.per * y.tiles;
     const long long cap = (long long)a.g.max_blocks * a.g.tpb;
     int unit = 0;
     by_shape(a.ks != nullptr, a.head_dim, [&](auto q, auto hd) { unit = Shape<decltype(q)::value, decltype(hd)::value>::UNIT; });
     const long long units = (cap + unit - 1) / unit;
-    if (y.sets <= kPlanSets && (long long)y.sets * a.g.n_kv < kPlanBlocks && units > 1) y.want = std::max(1, kPlanBlocks / a.g.n_kv);
+    if (y.sets <= kPlanSets && (long long)y.sets * a.g.n_kv < kPlanBlocks && units > 1) y.want = std::max(1, std::max(kPlanBlocks / a.g.n_kv - y.sets, kPlanBlocks / 4 / a.g.n_kv));
     // each set's last split may be short
     y.works = y.want ? std::min<long long>(y.want + y.sets, y.sets * std::min<long long>(kMaxSplits, units)) : y.sets;
     return y;
@@ -820,7 +964,7 @@ Layout layout_of(const PagedAttnArgs& a)
 size_t attention_paged_workspace_bytes(const PagedAttnArgs& a)
 {
     const Layout y = layout_of(a);
-    return y.want ? attention_counter_bytes() + (size_t)y.works * a.g.n_kv * kCols * (a.head_dim + 2) * sizeof(float) : 0;
+    return y.want ? attention_counter_bytes() + (size_t)y.works * a.g.n_kv * y.cols * (a.head_dim + 2) * sizeof(float) : 0;
 }
 
 hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipStream_t st)
@@ -829,6 +973,7 @@ hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipS
     MmaArgs A{};
     A.a = a;
     A.group = y.group;
+    A.cols = y.cols;
     A.tiles = y.tiles;
     A.sets = y.sets;
     A.want = y.want;
@@ -836,12 +981,16 @@ hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipS
     A.tpb_shift = (a.g.tpb & (a.g.tpb - 1)) == 0 ? __builtin_ctz((unsigned)a.g.tpb) : -1;
     A.counters = reinterpret_cast<uint32_t*>(workspace);
     A.part = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + attention_counter_bytes());
+    A.part_bytes = (uint32_t)((size_t)y.works * a.g.n_kv * y.cols * (a.head_dim + 2) * sizeof(float));  // below 2^31: plan()'s blocks
     const dim3 grid((unsigned)(y.works * a.g.n_kv));
     by_shape(a.ks != nullptr, a.head_dim, [&](auto q, auto hd) {
         constexpr bool Q8 = decltype(q)::value;
         constexpr int HD = decltype(hd)::value;
-        if (a.cap > 0.0f) hipLaunchKernelGGL((attn_paged_kernel<Q8, HD, true>), grid, dim3(kThreads), 0, st, A);
-        else hipLaunchKernelGGL((attn_paged_kernel<Q8, HD, false>), grid, dim3(kThreads), 0, st, A);
+        const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, st, A); };
+        if constexpr (HD <= 128) {
+            if (y.ct == 2) return a.cap > 0.0f ? go(attn_paged_kernel<Q8, HD, 2, true>) : go(attn_paged_kernel<Q8, HD, 2, false>);
+        }
+        a.cap > 0.0f ? go(attn_paged_kernel<Q8, HD, 1, true>) : go(attn_paged_kernel<Q8, HD, 1, false>);
     });
     return hipGetLastError();
 }
