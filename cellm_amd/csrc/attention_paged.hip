@@ -49,16 +49,14 @@ namespace cellm {
 namespace {
 
 constexpr int kWaves = 4, kThreads = kWaves * 64, kCols = 16;
-constexpr int kMaxSplits = 64;   // of a set's positions
+constexpr int kMaxSplits = 64;    // of a set's positions
+constexpr int kWholeUnits = 3;    // sets of so many units of positions are not split
 constexpr int kPlanSets = 512;   // sets that plan() looks at, 8 a lane; more run unsplit
 #ifndef PB
 #define PB 512
 #endif
 #ifndef CTMIN
-#define CTMIN 16
-#endif
-#ifndef MINSHARE
-#define MINSHARE 1
+#define CTMIN 256
 #endif
 constexpr int kPlanBlocks = PB;
 
@@ -300,13 +298,13 @@ __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
         total += units[i];
     }
     for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-    const int share = max(MINSHARE, (total + A.want - 1) / A.want);
+    const int share = max(1, (total + A.want - 1) / A.want);
     int base = 0;
     bool found = false;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         if (64 * i >= A.sets || found) continue;
-        int n = min(kMaxSplits, (units[i] + share - 1) / share);
+        int n = units[i] <= kWholeUnits ? min(units[i], 1) : min(kMaxSplits, (units[i] + share - 1) / share);
         const int each = n > 0 ? (units[i] + n - 1) / n : 1;
         n = (units[i] + each - 1) / each;
         int up = n;
@@ -335,11 +333,11 @@ __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
 template <bool Q8, int HD>
 struct Shape {
     static constexpr int CH = Q8 ? (HD <= 128 ? 64 : 32) : (HD <= 64 ? 64 : 32);  // positions of a chunk
-    static constexpr int UNIT = kWaves * CH;
     static constexpr int ES = Q8 ? 1 : 2;                    // bytes of an element of K and V
-    static constexpr int QS = Q8 ? HD + 16 : 2 * HD + 16;    // bytes between the columns of a q part in LDS
+    static constexpr int KK = Q8 ? HD / 64 : HD / 32;        // k steps of a K tile
     static constexpr int QP = Q8 ? 3 : 2;                    // parts of q
-    static constexpr int NR = HD / 4 < 32 ? HD / 4 : 32;     // registers of O^T that the waves add at a time
+    static constexpr int NE = Q8 ? 16 : 8;                   // elements of q of a lane and k step: NE (4 kk + g) + 0, 1, ...
+    static constexpr int DT = HD / 16;                       // tiles of O^T
 };
 
 // codes of four dims at positions j (a) and j + 1 (b) as exact f16 pairs by dim: 0x6400 | (c + 128) is 1152 + c
@@ -355,23 +353,309 @@ __device__ __forceinline__ void pairs_of_codes(uint32_t a, uint32_t b, uint32_t 
     o[3] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, s23, 0x04030402u)) + bias);
 }
 
+// q's parts of the column `some`, the B operands of the scores, and the scale that is left out of them.
+template <bool Q8, int HD>
+__device__ __forceinline__ void q_parts(const PagedAttnArgs& a, const f4_t (&qf)[Shape<Q8, HD>::KK][Shape<Q8, HD>::NE / 4],
+                                        u4_t (&d)[Shape<Q8, HD>::KK][Shape<Q8, HD>::QP], float& qsc)
+{
+    using S = Shape<Q8, HD>;
+    uint32_t mx = 0;  // |q| in the order of its bits; f16 pages: of the finite ones
+#pragma unroll
+    for (int kk = 0; kk < S::KK; ++kk)
+#pragma unroll
+        for (int i = 0; i < S::NE; ++i) {
+            const float x = qf[kk][i >> 2][i & 3];  // a bit_cast of the element itself reads the vector's first
+            const uint32_t b = __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu;
+            mx = max(mx, Q8 || b < 0x7F800000u ? b : 0u);
+        }
+    mx = max(mx, __builtin_bit_cast(uint32_t, lane_xor<16>(__builtin_bit_cast(float, mx), 64)));
+    mx = max(mx, __builtin_bit_cast(uint32_t, lane_xor<32>(__builtin_bit_cast(float, mx), 64)));
+    const int top = max((int)(mx >> 23), 1) - 127;
+    const bool bad = Q8 && mx >= 0x7F800000u;
+    const int e = mx > 0 && !bad ? (Q8 ? 21 : 13) - top : 0;
+    qsc = bad ? __builtin_nanf("") : ldexpf(a.scale, -e);
+#pragma unroll
+    for (int kk = 0; kk < S::KK; ++kk) {
+        if constexpr (Q8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // the three low bytes less 128 are the balanced digits
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = (uint32_t)(int)rintf(bad ? 0.0f : ldexpf(qf[kk][i][j], e)) + 0x00808080u;
+                const uint32_t a01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), a23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+                const uint32_t b01 = __builtin_amdgcn_perm(w[1], w[0], 0x0C0C0602u), b23 = __builtin_amdgcn_perm(w[3], w[2], 0x0C0C0602u);
+                d[kk][0][i] = __builtin_amdgcn_perm(a23, a01, 0x05040100u) ^ 0x80808080u;
+                d[kk][1][i] = __builtin_amdgcn_perm(a23, a01, 0x07060302u) ^ 0x80808080u;
+                d[kk][2][i] = __builtin_amdgcn_perm(b23, b01, 0x05040100u) ^ 0x80808080u;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                h2_t hi, lo;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int x = 2 * i + j;
+                    const float v = ldexpf(qf[kk][x >> 2][x & 3], e);
+                    hi[j] = (_Float16)v;
+                    lo[j] = finite_f32(v) ? (_Float16)(v - (float)hi[j]) : (_Float16)0.0f;
+                }
+                d[kk][0][i] = as_u32(hi);
+                d[kk][1][i] = as_u32(lo);
+            }
+        }
+    }
+}
+
+// A column's sums so far: reference (the first chunk's weights pass any bound), sum of the weights, O^T in units of 1 / F.
+template <int DT>
+struct Sums {
+    float R, l, F;
+    f4_t o[DT];
+};
+
+// Scores s of NP positions (bit 4 j of vis: position j is seen; `partial`: not all are, in some column) and their scales
+// vs to the weights' two f16 parts, and into l; the reference is raised where products pass 2^15.
+template <bool Q8, int NP, int DT>
+__device__ __forceinline__ void weigh(const float (&s)[NP], float cs, const float (&vs)[NP], bool partial, uint64_t vis, bool& coarse,
+                                      Sums<DT>& m, h8_t (&ph)[NP / 8], h8_t (&pl)[NP / 8])
+{
+    float w[NP], lc, mx;
+    const auto weights = [&]() {
+        lc = mx = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) w[j] = __builtin_amdgcn_exp2f(s[j] * cs - m.R);
+        if (partial) {
+            asm volatile("");  // a branch
+#pragma unroll
+            for (int j = 0; j < NP; ++j) w[j] = vis >> (4 * j) & 1 ? w[j] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            lc = lc + w[j];
+            if constexpr (Q8) w[j] = w[j] * vs[j];
+            mx = fmaxf(mx, w[j]);
+        }
+        if (Q8 && coarse) {
+            asm volatile("");
+            mx = mx * m.F;
+#pragma unroll
+            for (int j = 0; j < NP; ++j) w[j] = w[j] * m.F;
+        }
+    };
+    weights();
+    if (__ballot(mx > 0x1p15f || lc > 0x1p100f)) {
+        // the reference that leaves the largest product at 2^13 (and weights of small s_v below 2^90)
+        float m1 = -INFINITY, m2 = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const float h = vis >> (4 * j) & 1 ? s[j] * cs : -INFINITY;
+            m1 = fmaxf(m1, h);
+            m2 = fmaxf(m2, Q8 ? h + __builtin_amdgcn_logf(vs[j]) : h);
+        }
+        m1 = fmaxf(m1, lane_xor<16>(m1, 64));
+        m1 = fmaxf(m1, lane_xor<32>(m1, 64));
+        m2 = fmaxf(m2, lane_xor<16>(m2, 64));
+        m2 = fmaxf(m2, lane_xor<32>(m2, 64));
+        const float up = fmaxf(m.R, fmaxf(m2 - 13.0f, m1 - 90.0f));
+        float ratio = up > m.R ? __builtin_amdgcn_exp2f(m.R - up) : 1.0f;  // from -inf: 0, as l and O are
+        m.R = up;
+        m.l = m.l * ratio;
+        if constexpr (Q8) {
+            // beyond 2^20 a reference has no bits for the 13: the products are scaled down instead
+            const float over = m2 - up;
+            const float f = over > 15.0f && over < 1000.0f ? fminf(m.F, __builtin_amdgcn_exp2f(13.0f - rintf(over))) : m.F;
+            ratio = ratio * (f / m.F);
+            m.F = f;
+            coarse = coarse || __ballot(f != 1.0f) != 0;
+        }
+#pragma unroll
+        for (int e = 0; e < DT; ++e) m.o[e] = m.o[e] * ratio;
+        weights();
+    }
+    m.l = m.l + lc;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const _Float16 h = (_Float16)w[j];
+        ph[j >> 3][j & 7] = h;
+        pl[j >> 3][j & 7] = (_Float16)__builtin_fmaf((float)h, -1.0f, w[j]);
+    }
+}
+
+// Words of four (8-bit) or two (f16) dims at eight positions as the V^T operands of those dims
+template <bool Q8>
+__device__ __forceinline__ void v_operands(const uint32_t (&r)[8], u4_t (&vt)[Q8 ? 4 : 2])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (Q8) {
+            uint32_t y[4];
+            pairs_of_codes(r[2 * i], r[2 * i + 1], y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vt[e][i] = y[e];
+        } else {
+            vt[0][i] = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x05040100u);
+            vt[1][i] = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x07060302u);
+        }
+    }
+}
+
+// scores of a tile's 16 positions from the sums of q's parts
+__device__ __forceinline__ float score_of(int hi, int mid, int lo, float ks)
+{
+    return __builtin_fmaf((float)hi, 65536.0f, (float)(mid * 256 + lo)) * ks;
+}
+
+// ---- a block's results: its sums where the set is split, else the quotients; the sums of splits added by the last ----
+// COLS columns of a set from column col0 of the table on; a split's sums: [COLS][HD], then R and l, [COLS] each.
+template <int HD, int COLS>
+struct Results {
+    static constexpr uint32_t kPart = COLS * (HD + 2);
+    const MmaArgs& A;
+    const Work& k;
+    int table, col0, kvh;
+    __amdgpu_buffer_rsrc_t part;
+    __device__ __forceinline__ Results(const MmaArgs& A_, const Work& k_, int kvh_)
+        : A(A_), k(k_), table(k_.set / A_.tiles), col0((k_.set - table * A_.tiles) * COLS), kvh(kvh_), part(buffer_rsrc(A_.part, A_.part_bytes))
+    {
+    }
+    __device__ __forceinline__ int columns() const { return min(A.a.per * A.group - col0, COLS); }
+    __device__ __forceinline__ int row_of(int x) const { return table * A.a.per + (col0 + x) / A.group; }
+    __device__ __forceinline__ int head_of(int x) const { return kvh * A.group + (col0 + x) % A.group; }
+    __device__ __forceinline__ float* out_of(int x) const { return A.a.out + ((size_t)row_of(x) * A.a.n_heads + head_of(x)) * HD; }
+    __device__ __forceinline__ const float* q_of(int x) const { return A.a.q + ((size_t)row_of(x) * A.a.n_heads + head_of(x)) * HD; }
+    __device__ __forceinline__ uint32_t part_of(int sp) const { return (uint32_t)((k.slot0 + sp) * A.a.g.n_kv + kvh) * kPart; }
+    // four dims of column x from d on, ll the sum of all its weights; whether they are finite
+    __device__ __forceinline__ bool put(int x, int d, f4_t v, float ll) const
+    {
+        if (k.splits > 1) st_agent4(part, part_of(k.split) + x * HD + d, v);
+        else *reinterpret_cast<f4_t*>(out_of(x) + d) = v * (ll != 0.0f ? 1.0f / ll : 0.0f);
+        return finite_f32(v[0]) && finite_f32(v[1]) && finite_f32(v[2]) && finite_f32(v[3]) && finite_f32(ll);
+    }
+    __device__ __forceinline__ void put_sums(int x, float r, float ll) const
+    {
+        st_agent(part, part_of(k.split) + COLS * HD + x, r);
+        st_agent(part, part_of(k.split) + COLS * (HD + 1) + x, ll);
+    }
+    // f16 pages: the columns whose bits `again` has by plain sums; the whole block
+    template <int UNIT>
+    __device__ void put_plain(uint32_t again, unsigned char* lds) const
+    {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // their first values are written
+        __syncthreads();
+#pragma unroll 1
+        for (int x = 0; x < COLS; ++x) {
+            if (!(again >> x & 1)) continue;
+            Sight sc;
+            sight_of(A.a, A.cap, table, row_of(x), sc);
+            float mm, ll;
+            const float v = plain_range<HD, UNIT>(A.a, sc, table, row_of(x), head_of(x), k.lo, sc.end, k.step, k.splits > 1, lds, mm, ll);
+            const int t = threadIdx.x;
+            if (k.splits > 1) {
+                if (t < HD) st_agent(part, part_of(k.split) + x * HD + t, v);
+                if (t == 0) put_sums(x, mm, ll);
+            } else if (t < HD) {
+                out_of(x)[t] = ll != 0.0f ? v / ll : 0.0f;
+            }
+        }
+    }
+    // The last block of a split set to get here adds the splits; bit x of `here`: column x is there; lds: COLS * kMaxSplits * 8
+    // bytes, half of them at least 16 a thread.
+    __device__ void combine(const uint32_t& here, float* lsum, int* last, unsigned char* lds) const
+    {
+        const int t = threadIdx.x, lane = t & 63, wave = rfl(t >> 6), n = k.splits;
+        if (n <= 1) return;
+        // this block's sums are performed at the coherence point before it counts itself
+        uint32_t* const counter = A.counters + (size_t)k.set * A.a.g.n_kv + kvh;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (t == 0)
+            *last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(n - 1);
+        __syncthreads();
+        if (!*last) return;
+        // The splits' references and sums of weights to LDS, then weights 2^(R_k - R).  The values: an item is four dims
+        // of a column; few items share their splits among groups of threads, which meet in LDS.
+        float* const mk = reinterpret_cast<float*>(lds);  // [column][kMaxSplits], then the weights
+        float* const lk = mk + COLS * kMaxSplits;
+        f4_t* const red = reinterpret_cast<f4_t*>(lk);    // once lk is read
+        const uint32_t present = here;
+        const auto there = [&](int x) { return present >> x & 1; };
+        const int cols = columns(), items = cols * (HD / 4), groups = max(1, kThreads / items);
+        constexpr int U = 8;  // loads in flight
+        f4_t v[U];
+        const int group = t / items;
+        int item = t - group * items;
+        bool busy = group < groups && t < groups * items;
+        const auto load = [&](int sp) {
+#pragma unroll
+            for (int j = 0; j < U; ++j) v[j] = ld_agent4(part, part_of(min(sp + j * groups, n - 1)) + 4 * item);
+        };
+        if (busy) load(group);
+        for (int i = t; i < COLS * n; i += kThreads) {
+            const int sp = i / COLS, x = i % COLS;
+            if (!there(x)) continue;
+            mk[x * kMaxSplits + sp] = ld_agent(part, part_of(sp) + COLS * HD + x);
+            lk[x * kMaxSplits + sp] = ld_agent(part, part_of(sp) + COLS * (HD + 1) + x);
+        }
+        __syncthreads();
+        for (int x = wave; x < cols; x += kWaves) {
+            if (!there(x)) continue;
+            const float mv = lane < n ? mk[x * kMaxSplits + lane] : -INFINITY, lv = lane < n ? lk[x * kMaxSplits + lane] : 0.0f;
+            const float mm = group_max<64>(mv);
+            // a split without a score above -inf weighs nothing beside others; where all are so, its l is 0 (nothing
+            // seen: zeros) or NaN
+            const float ew = mv > -INFINITY ? __builtin_amdgcn_exp2f(mv - mm) : mm > -INFINITY ? 0.0f : 1.0f;
+            const float ll = group_sum<64>(mv > -INFINITY || !(mm > -INFINITY) ? lv * ew : 0.0f);
+            if (lane < n) mk[x * kMaxSplits + lane] = ew;
+            if (lane == 0) lsum[x] = ll;
+        }
+        __syncthreads();
+        for (;;) {  // more than 256 items: again for the others, in one group
+            f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            const int x = min(item / (HD / 4), COLS - 1);
+            if (busy) {
+                for (int sp = group; sp < n; sp += U * groups) {
+                    if (sp > group) load(sp);
+#pragma unroll
+                    for (int j = 0; j < U; ++j)
+                        if (sp + j * groups < n) acc = acc + v[j] * mk[x * kMaxSplits + sp + j * groups];
+                }
+            }
+            if (groups > 1) {
+                red[t] = acc;
+                __syncthreads();
+                if (group == 0)
+                    for (int y = 1; y < groups; ++y) acc = acc + red[y * items + t];
+            }
+            if (busy && group == 0 && there(x)) {
+                const float ll = lsum[x];
+                *reinterpret_cast<f4_t*>(out_of(x) + 4 * (item % (HD / 4))) = acc * (ll != 0.0f ? 1.0f / ll : 0.0f);
+            }
+            item += kThreads;
+            if (groups > 1 || item - t >= items) break;
+            busy = item < items;
+            if (busy) load(0);
+        }
+        if (t == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+};
+
+// One set of 16 CT columns a block; its waves take chunks of the positions in turn and meet in LDS.
 template <bool Q8, int HD, int CT, bool CAP>
 __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A)
 {
     using S = Shape<Q8, HD>;
     constexpr int CH = S::CH, NT = CH / 16, NP = CH / 4, KS = CH / 32;  // K tiles; positions of a lane; k steps of V
-    constexpr int KK = Q8 ? HD / 64 : HD / 32;                          // k steps of a K tile
-    constexpr int DT = HD / 16, VW = DT * S::ES / 4;                    // tiles of O^T; words of V per lane and position
+    constexpr int KK = S::KK, QP = S::QP, NE = S::NE, DT = S::DT, VW = DT * S::ES / 4;  // VW: words of V per lane and position
+    constexpr int NR = HD / 4 < 32 ? HD / 4 : 32;                       // registers of O^T that the waves add at a time
+    constexpr bool kQInLds = HD > 128 || CT > 1;                        // q's parts in LDS, for want of registers
     constexpr int COLS = kCols * CT;
-    constexpr int kMergeBytes = kWaves * S::NR * 64 * 4;
-    static_assert(kMergeBytes >= COLS * kMaxSplits * 8 && kMergeBytes >= kThreads * 16, "LDS of the later steps");
+    constexpr int kMergeBytes = std::max(kWaves * NR * 64 * 4, COLS * kMaxSplits * 8);
     __shared__ __align__(16) unsigned char merge[kMergeBytes];
-    __shared__ __align__(16) unsigned char qs[S::QP * COLS * S::QS];
-    __shared__ float qscale[COLS];
+    __shared__ __align__(16) u4_t qlds[kQInLds ? CT * KK * QP * 64 : 1];
     __shared__ __align__(16) uint32_t kidx[kWaves][CH], vidx[kWaves][CH];  // [c][tile], [g][j]
     __shared__ __align__(16) float kscl[kWaves][Q8 ? CH : 4], vscl[kWaves][Q8 ? CH : 4];
-    __shared__ float ml[kWaves][2][COLS];
-    __shared__ uint32_t flags;
+    __shared__ float ml[kWaves][2][COLS], lsum[COLS];
+    __shared__ uint32_t flags, here;
     __shared__ int last;
 
     const PagedAttnArgs& a = A.a;
@@ -379,110 +663,65 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     const int c = lane & 15, g4 = lane >> 4;
     const int kvh = blockIdx.x % a.g.n_kv;
     Work k;
-    if (!plan<S::UNIT>(A, blockIdx.x / a.g.n_kv, k)) return;  // the same for the whole block
-    const int table = k.set / A.tiles, col0 = (k.set - table * A.tiles) * COLS;
-    const auto row_of = [&](int col) { return table * a.per + (col0 + col) / A.group; };
-    const auto head_of = [&](int col) { return kvh * A.group + (col0 + col) % A.group; };
-    const int n_cols = a.per * A.group - col0;  // columns from n_cols on are none
+    if (!plan<kWaves * CH>(A, blockIdx.x / a.g.n_kv, k)) return;  // the same for the whole block
+    const Results<HD, COLS> res(A, k, kvh);
+    const int table = res.table, n_cols = res.columns();
 
-    // ---- the first chunk's page entries
+    // ---- the first chunk's page entries, q, and what this lane's column sees: loads that do not wait for each other
     const auto block_of = [&](int p) { return A.tpb_shift >= 0 ? p >> A.tpb_shift : p / a.g.tpb; };
     const uint32_t* const bt = a.g.bt + (size_t)table * a.g.max_blocks;
-    const int b_first = block_of(k.lo + wave * CH + (lane & (CH - 1)));
+    int p0 = k.lo + wave * CH;
+    const int b_first = block_of(p0 + (lane & (CH - 1)));
     const uint32_t blk_first = bt[min(b_first, a.g.max_blocks - 1)];
-
-    // ---- what column 16 u + c sees
     Sight si[CT];
     bool has[CT];
-    uint32_t present = 0;
+    u4_t qp[CT][KK][QP];
+    float qsc[CT], cs[CT];  // scale of the sums of q's parts, and of the exponents
+    Sums<DT> m[CT];
+    {
+        f4_t qf[CT][KK][NE / 4];
 #pragma unroll
-    for (int u = 0; u < CT; ++u) {
-        const int col = kCols * u + c;
-        si[u] = Sight{0, 0, 0, a.masks};
-        has[u] = col < n_cols && sight_of(a, A.cap, table, row_of(min(col, n_cols - 1)), si[u]);
-        if (!has[u]) si[u].start = si[u].ctx = si[u].end = 0;
-        present |= ((uint32_t)__ballot(has[u]) & 0xFFFFu) << (kCols * u);
-    }
-
-    // ---- q in LDS: 16 threads per column, HD / 16 elements each
+        for (int u = 0; u < CT; ++u) {
+            const f4_t* src = reinterpret_cast<const f4_t*>(res.q_of(min(kCols * u + c, n_cols - 1)) + NE * g4);
 #pragma unroll
-    for (int u = 0; u < CT; ++u) {
-        constexpr int NE = HD / 16;
-        const int col = kCols * u + (t >> 4), part = t & 15;
-        float x[NE];
-        if (present >> col & 1) {
-            const f4_t* src = reinterpret_cast<const f4_t*>(a.q + ((size_t)row_of(col) * a.n_heads + head_of(col)) * HD + part * NE);
+            for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-            for (int i = 0; i < NE / 4; ++i) {
-                const f4_t v = src[i];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[4 * i + j] = v[j];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NE; ++i) x[i] = 0.0f;
+                for (int i = 0; i < NE / 4; ++i) qf[u][kk][i] = src[NE * kk + i];
         }
-        uint32_t mx = 0;  // |x| in the order of its bits; f16 pages: of the finite ones
+        uint32_t b = 0;
 #pragma unroll
-        for (int i = 0; i < NE; ++i) {
-            const uint32_t b = __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu;
-            mx = max(mx, Q8 || b < 0x7F800000u ? b : 0u);
+        for (int u = 0; u < CT; ++u) {
+            si[u] = Sight{0, 0, 0, a.masks};
+            has[u] = sight_of(a, A.cap, table, res.row_of(min(kCols * u + c, n_cols - 1)), si[u]) && kCols * u + c < n_cols;
+            if (!has[u]) si[u] = Sight{0, 0, 0, a.masks};
+            b |= ((uint32_t)__ballot(has[u]) & 0xFFFFu) << (kCols * u);
         }
-        mx = team_max_u32<16>(mx);
-        const int top = max((int)(mx >> 23), 1) - 127;
-        unsigned char* dst = qs + col * S::QS + part * NE * S::ES;
-        if constexpr (Q8) {
-            const bool bad = mx >= 0x7F800000u;
-            const int e = mx > 0 && !bad ? 21 - top : 0;
-            uint32_t y[NE];
-#pragma unroll
-            for (int i = 0; i < NE; ++i) y[i] = (uint32_t)(int)rintf(bad ? 0.0f : ldexpf(x[i], e)) + 0x00808080u;
-#pragma unroll
-            for (int i = 0; i < NE / 4; ++i) {  // the three low bytes less 128 are the balanced digits
-                const uint32_t* w = y + 4 * i;
-                const uint32_t a01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), a23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
-                const uint32_t b01 = __builtin_amdgcn_perm(w[1], w[0], 0x0C0C0602u), b23 = __builtin_amdgcn_perm(w[3], w[2], 0x0C0C0602u);
-                const uint32_t d[3] = {__builtin_amdgcn_perm(a23, a01, 0x05040100u), __builtin_amdgcn_perm(a23, a01, 0x07060302u),
-                                       __builtin_amdgcn_perm(b23, b01, 0x05040100u)};
-#pragma unroll
-                for (int p = 0; p < 3; ++p)
-                    *reinterpret_cast<uint32_t*>(dst + p * COLS * S::QS + 4 * i) = d[p] ^ 0x80808080u;
-            }
-            if (part == 0) qscale[col] = bad ? __builtin_nanf("") : ldexpf(a.scale, -e);
-        } else {
-            const int e = mx > 0 ? 13 - top : 0;
-#pragma unroll
-            for (int i = 0; i < NE; i += 2) {
-                h2_t hi, lo;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float v = ldexpf(x[i + j], e);
-                    hi[j] = (_Float16)v;
-                    lo[j] = finite_f32(v) ? (_Float16)(v - (float)hi[j]) : (_Float16)0.0f;
-                }
-                *reinterpret_cast<uint32_t*>(dst + 2 * i) = as_u32(hi);
-                *reinterpret_cast<uint32_t*>(dst + COLS * S::QS + 2 * i) = as_u32(lo);
-            }
-            if (part == 0) qscale[col] = ldexpf(a.scale, -e);
+        if (t == 0) {
+            here = b;
+            flags = 0;
         }
-        if (t == 0) flags = 0;
-    }
-    __syncthreads();
-
-    f4_t o[CT][DT];
-    float R[CT], l[CT], qsc[CT], cs[CT];  // reference, sum of the weights; scale of the sums and of the exponents
-    float F[CT];                          // O is in units of 1 / F
-    bool coarse = false;                  // F is not 1 somewhere
 #pragma unroll
-    for (int u = 0; u < CT; ++u) {
-#pragma unroll
-        for (int e = 0; e < DT; ++e) o[u][e] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        F[u] = 1.0f;
-        R[u] = -INFINITY;  // the first chunk's weights pass any bound
-        l[u] = 0.0f;
-        qsc[u] = qscale[kCols * u + c];
-        cs[u] = CAP ? kLog2e : qsc[u] * kLog2e;
+        for (int u = 0; u < CT; ++u) {
+            q_parts<Q8, HD>(a, qf[u], qp[u], qsc[u]);
+            cs[u] = CAP ? kLog2e : qsc[u] * kLog2e;
+            m[u] = Sums<DT>{-INFINITY, 0.0f, 1.0f, {}};
+        }
     }
+    if constexpr (kQInLds) {
+#pragma unroll
+        for (int u = 0; u < CT; ++u)
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                for (int p = 0; p < QP; ++p)
+                    if (wave == 0) qlds[((u * KK + kk) * QP + p) * 64 + lane] = qp[u][kk][p];
+        __syncthreads();
+    }
+    const auto q_part = [&](int u, int p, int kk) {
+        if constexpr (kQInLds) return qlds[((u * KK + kk) * QP + p) * 64 + lane];
+        else return qp[u][kk][p];
+    };
+    bool coarse = false;  // F is not 1 somewhere
     const unsigned char* const kbase = static_cast<const unsigned char*>(a.kc) + 16 * g4;
     const unsigned char* const vbase = static_cast<const unsigned char*>(a.vc) + DT * S::ES * c;
 
@@ -550,7 +789,6 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         asm volatile("" ::: "memory");
     };
     const int step = k.step;
-    int p0 = k.lo + wave * CH;
     if (p0 < k.hi) {
         b_of = b_first;
         blk = blk_first;
@@ -579,10 +817,10 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                 for (int kk = 0; kk < KK; ++kk) kr[i][kk] = gone ? u4_t{0, 0, 0, 0} : kr[i][kk];
             }
         }
-        // ---- scores of positions p0 + 4 j + g4, less their scale qsc without a cap
         h8_t ph[CT][KS], pl[CT][KS];
 #pragma unroll
         for (int u = 0; u < CT; ++u) {
+            // ---- scores of positions p0 + 4 j + g4, less their scale qsc without a cap
             float s[NP];
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
@@ -591,337 +829,130 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
 #pragma unroll
                     for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-                        for (int p = 0; p < 3; ++p) {
-                            const i4_t qv = *reinterpret_cast<const i4_t*>(qs + (p * COLS + kCols * u + c) * S::QS + 64 * kk + 16 * g4);
-                            d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4_t, kr[i][kk]), qv, d[p], 0, 0, 0);
-                        }
+                        for (int p = 0; p < 3; ++p)
+                            d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4_t, kr[i][kk]),
+                                                                         __builtin_bit_cast(i4_t, q_part(u, p, kk)), d[p], 0, 0, 0);
                     const f4_t ksv = *reinterpret_cast<const f4_t*>(&kscl[wave][g4 * NP + 4 * i]);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        s[4 * i + x] = __builtin_fmaf((float)d[2][x], 65536.0f, (float)(d[1][x] * 256 + d[0][x])) * ksv[x];
+                    for (int x = 0; x < 4; ++x) s[4 * i + x] = score_of(d[2][x], d[1][x], d[0][x], ksv[x]);
                 } else {
                     f4_t d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int p = 1; p >= 0; --p)  // the low parts first
 #pragma unroll
-                        for (int kk = 0; kk < KK; ++kk) {
-                            const h8_t qv = *reinterpret_cast<const h8_t*>(qs + (p * COLS + kCols * u + c) * S::QS + 64 * kk + 16 * g4);
-                            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, kr[i][kk]), qv, d, 0, 0, 0);
-                        }
+                        for (int kk = 0; kk < KK; ++kk)
+                            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, kr[i][kk]),
+                                                                       __builtin_bit_cast(h8_t, q_part(u, p, kk)), d, 0, 0, 0);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) s[4 * i + x] = d[x];
                 }
             }
             if (u == CT - 1) load_k();
-            float vs[NP];
-#pragma unroll
-            for (int j = 0; j < NP; ++j) vs[j] = Q8 ? vscl[wave][g4 * NP + j] : 1.0f;
             if constexpr (CAP) {
 #pragma unroll
                 for (int j = 0; j < NP; ++j) s[j] = capped(a, s[j] * qsc[u]);
             }
             // ---- weights; of positions that some column does not see, those are 0 whatever they hold
+            float vs[NP];
+#pragma unroll
+            for (int j = 0; j < NP; ++j) vs[j] = Q8 ? vscl[wave][g4 * NP + j] : 1.0f;
             const bool partial = __ballot(has[u] && (p0 < si[u].start || p0 + CH > si[u].ctx)) != 0;
             uint64_t vis = ~0ull;  // bit 4 j: position j of this lane
-            float w[NP], lc, mx;
-            const auto weigh = [&]() {
-                lc = mx = 0.0f;
-#pragma unroll
-                for (int j = 0; j < NP; ++j) w[j] = __builtin_amdgcn_exp2f(s[j] * cs[u] - R[u]);
-                if (partial) {
-                    asm volatile("");  // a branch
-#pragma unroll
-                    for (int j = 0; j < NP; ++j) w[j] = vis >> (4 * j) & 1 ? w[j] : 0.0f;
-                }
-#pragma unroll
-                for (int j = 0; j < NP; ++j) {
-                    lc = lc + w[j];
-                    if constexpr (Q8) w[j] = w[j] * vs[j];
-                    mx = fmaxf(mx, w[j]);
-                }
-                if (Q8 && coarse) {
-                    asm volatile("");
-                    mx = mx * F[u];
-#pragma unroll
-                    for (int j = 0; j < NP; ++j) w[j] = w[j] * F[u];
-                }
-            };
             if (partial) {
                 vis = visible(a, si[u], p0) >> g4;
 #pragma unroll
                 for (int j = 0; j < NP; ++j) vs[j] = vis >> (4 * j) & 1 ? vs[j] : 0.0f;
             }
-            weigh();
-            if (__ballot(mx > 0x1p15f || lc > 0x1p100f)) {
-                // the reference that leaves the largest product at 2^13 (and weights of small s_v below 2^90)
-                float m1 = -INFINITY, m2 = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < NP; ++j) {
-                    const float h = vis >> (4 * j) & 1 ? s[j] * cs[u] : -INFINITY;
-                    m1 = fmaxf(m1, h);
-                    m2 = fmaxf(m2, Q8 ? h + __builtin_amdgcn_logf(vs[j]) : h);
-                }
-                m1 = fmaxf(m1, lane_xor<16>(m1, 64));
-                m1 = fmaxf(m1, lane_xor<32>(m1, 64));
-                m2 = fmaxf(m2, lane_xor<16>(m2, 64));
-                m2 = fmaxf(m2, lane_xor<32>(m2, 64));
-                const float up = fmaxf(R[u], fmaxf(m2 - 13.0f, m1 - 90.0f));
-                float ratio = up > R[u] ? __builtin_amdgcn_exp2f(R[u] - up) : 1.0f;  // from -inf: 0, as l and O are
-                R[u] = up;
-                l[u] = l[u] * ratio;
-                if constexpr (Q8) {
-                    // beyond 2^20 a reference has no bits for the 13: the products are scaled down instead
-                    const float over = m2 - up;
-                    const float f = over > 15.0f && over < 1000.0f ? fminf(F[u], __builtin_amdgcn_exp2f(13.0f - rintf(over))) : F[u];
-                    ratio = ratio * (f / F[u]);
-                    F[u] = f;
-                    coarse = coarse || __ballot(f != 1.0f) != 0;
-                }
-#pragma unroll
-                for (int e = 0; e < DT; ++e) o[u][e] = o[u][e] * ratio;
-                weigh();
-            }
-            l[u] = l[u] + lc;
-#pragma unroll
-            for (int j = 0; j < NP; ++j) {
-                const _Float16 h = (_Float16)w[j];
-                ph[u][j >> 3][j & 7] = h;
-                pl[u][j >> 3][j & 7] = (_Float16)(w[j] - (float)h);
-            }
+            weigh<Q8>(s, cs[u], vs, partial, vis, coarse, m[u], ph[u], pl[u]);
         }
         // ---- O^T += V^T . P^T
         if (!Q8 && miss) {
 #pragma unroll
             for (int j = 0; j < NP; ++j)
 #pragma unroll
-                for (int w = 0; w < VW; ++w) vr[j][w] = miss >> (4 * j + g4) & 1 ? 0u : vr[j][w];
+                for (int x = 0; x < VW; ++x) vr[j][x] = miss >> (4 * j + g4) & 1 ? 0u : vr[j][x];
         }
-        if constexpr (Q8) {
 #pragma unroll
-            for (int w = 0; w < VW; ++w)
+        for (int x = 0; x < VW; ++x)
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    u4_t vt[4];
+            for (int ks = 0; ks < KS; ++ks) {
+                constexpr int E = Q8 ? 4 : 2;  // tiles of a word
+                uint32_t r[8];
+                u4_t vt[E];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t x[4];
-                        pairs_of_codes(vr[8 * ks + 2 * i][w], vr[8 * ks + 2 * i + 1][w], x);
+                for (int j = 0; j < 8; ++j) r[j] = vr[8 * ks + j][x];
+                v_operands<Q8>(r, vt);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) vt[e][i] = x[e];
+                for (int e = 0; e < E; ++e)
+#pragma unroll
+                    for (int u = 0; u < CT; ++u) {
+                        const h8_t v = __builtin_bit_cast(h8_t, vt[e]);
+                        f4_t& o = m[u].o[E * x + e];
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u][ks], o, 0, 0, 0);
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u][ks], o, 0, 0, 0);
                     }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int u = 0; u < CT; ++u) {
-                            const h8_t v = __builtin_bit_cast(h8_t, vt[e]);
-                            o[u][4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u][ks], o[u][4 * w + e], 0, 0, 0);
-                            o[u][4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u][ks], o[u][4 * w + e], 0, 0, 0);
-                        }
-                }
-        } else {
-#pragma unroll
-            for (int w = 0; w < VW; ++w)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        u4_t vt;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            vt[i] = __builtin_amdgcn_perm(vr[8 * ks + 2 * i + 1][w], vr[8 * ks + 2 * i][w], e ? 0x07060302u : 0x05040100u);
-                        const h8_t v = __builtin_bit_cast(h8_t, vt);
-#pragma unroll
-                        for (int u = 0; u < CT; ++u) {
-                            o[u][2 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u][ks], o[u][2 * w + e], 0, 0, 0);
-                            o[u][2 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u][ks], o[u][2 * w + e], 0, 0, 0);
-                        }
-                    }
-        }
+            }
         load_v();
     }
 
-    // ---- the waves meet: lane (c, g) holds dims g HD / 4 + r of its column, r = 0..HD / 4 - 1, in register (r % DT, r / DT)
-#pragma unroll
-    for (int u = 0; u < CT; ++u) {
-        l[u] = l[u] + lane_xor<16>(l[u], 64);
-        l[u] = l[u] + lane_xor<32>(l[u], 64);
-        if (Q8 && coarse) {
-#pragma unroll
-            for (int e = 0; e < DT; ++e) o[u][e] = o[u][e] / F[u];
-        }
-        if (g4 == 0) {
-            ml[wave][0][kCols * u + c] = R[u];
-            ml[wave][1][kCols * u + c] = l[u];
-        }
-    }
-    const bool split = k.splits > 1;
-    const __amdgpu_buffer_rsrc_t part = buffer_rsrc(A.part, A.part_bytes);
-    constexpr uint32_t kPart = COLS * (HD + 2);  // floats of a block's sums: [COLS][HD], then R and l, [COLS] each
-    const auto part_of = [&](int sp) { return (uint32_t)((k.slot0 + sp) * a.g.n_kv + kvh) * kPart; };
-    const auto out_of = [&](int col) { return a.out + ((size_t)row_of(col) * a.n_heads + head_of(col)) * HD; };
+    // ---- the waves meet: each adds a quarter of the registers over all four; lane (c, g) holds dims g HD / 4 + r of its
+    // column, r = 0..HD / 4 - 1, in register (r % DT, r / DT)
     float* const mine = reinterpret_cast<float*>(merge) + lane;
+    bool fine[CT];
 #pragma unroll
     for (int u = 0; u < CT; ++u) {
         const int col = kCols * u + c;
-        bool odd = false;  // a sum that is not finite
+        m[u].l = m[u].l + lane_xor<16>(m[u].l, 64);
+        m[u].l = m[u].l + lane_xor<32>(m[u].l, 64);
+        if (Q8 && coarse) {
 #pragma unroll
-        for (int rd = 0; rd < HD / 4 / S::NR; ++rd) {
+            for (int e = 0; e < DT; ++e) m[u].o[e] = m[u].o[e] / m[u].F;
+        }
+        if (g4 == 0) {
+            ml[wave][0][col] = m[u].R;
+            ml[wave][1][col] = m[u].l;
+        }
+        fine[u] = true;
+#pragma unroll
+        for (int rd = 0; rd < HD / 4 / NR; ++rd) {
             if (u || rd) __syncthreads();
 #pragma unroll
-            for (int r = 0; r < S::NR; ++r) {
-                const int x = rd * S::NR + r;
-                mine[(wave * S::NR + r) * 64] = o[u][x % DT][x / DT];
+            for (int r = 0; r < NR; ++r) {
+                const int x = rd * NR + r;
+                mine[(wave * NR + r) * 64] = m[u].o[x % DT][x / DT];
             }
             __syncthreads();
-            float mm = ml[0][0][col], ll = 0.0f, acc[S::NR / 4];
+            float mm = ml[0][0][col], ll = 0.0f, acc[NR / 4];
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, ml[w][0][col]);
+            for (int x = 1; x < kWaves; ++x) mm = fmaxf(mm, ml[x][0][col]);
 #pragma unroll
-            for (int r = 0; r < S::NR / 4; ++r) acc[r] = 0.0f;
+            for (int r = 0; r < NR / 4; ++r) acc[r] = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
+            for (int x = 0; x < kWaves; ++x) {
                 // no weight (l is 0, or NaN)
-                const float ew = ml[w][0][col] > -INFINITY ? __builtin_amdgcn_exp2f(ml[w][0][col] - mm) : ml[w][1][col];
-                ll = ll + ml[w][1][col] * ew;
+                const float ew = ml[x][0][col] > -INFINITY ? __builtin_amdgcn_exp2f(ml[x][0][col] - mm) : ml[x][1][col];
+                ll = ll + ml[x][1][col] * ew;
 #pragma unroll
-                for (int r = 0; r < S::NR / 4; ++r) acc[r] = acc[r] + mine[(w * S::NR + wave * (S::NR / 4) + r) * 64] * ew;
+                for (int r = 0; r < NR / 4; ++r) acc[r] = acc[r] + mine[(x * NR + wave * (NR / 4) + r) * 64] * ew;
             }
             if (has[u]) {
-                const int d0 = g4 * (HD / 4) + rd * S::NR + wave * (S::NR / 4);
-                if (split) {
-                    const uint32_t at = part_of(k.split);
 #pragma unroll
-                    for (int r = 0; r < S::NR / 4; r += 4)
-                        st_agent4(part, at + col * HD + d0 + r, f4_t{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]});
-                    if (rd == 0 && wave == 0 && g4 == 0) {
-                        st_agent(part, at + COLS * HD + col, mm);
-                        st_agent(part, at + COLS * (HD + 1) + col, ll);
-                    }
-                } else {
-                    const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
-#pragma unroll
-                    for (int r = 0; r < S::NR / 4; r += 4)
-                        *reinterpret_cast<f4_t*>(out_of(col) + d0 + r) = f4_t{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]} * inv;
-                }
-                if constexpr (!Q8) {
-#pragma unroll
-                    for (int r = 0; r < S::NR / 4; ++r) odd |= !finite_f32(acc[r]);
-                    odd |= !finite_f32(ll);
-                }
+                for (int r = 0; r < NR / 4; r += 4)
+                    fine[u] &= res.put(col, g4 * (HD / 4) + rd * NR + wave * (NR / 4) + r,
+                                       f4_t{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]}, ll);
+                if (k.splits > 1 && rd == 0 && wave == 0 && g4 == 0) res.put_sums(col, mm, ll);
             }
-        }
-        if constexpr (!Q8) {
-            if (odd) atomicOr(&flags, 1u << col);
         }
     }
     if constexpr (!Q8) {
+#pragma unroll
+        for (int u = 0; u < CT; ++u)
+            if (!fine[u]) atomicOr(&flags, 1u << (kCols * u + c));
         __syncthreads();
         const uint32_t again = flags;
-        if (again) {  // rare: columns that are not finite over this block's positions
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // their first values are written
-            __syncthreads();
-#pragma unroll 1
-            for (int col = 0; col < COLS; ++col) {
-                if (!(again >> col & 1)) continue;
-                Sight sc;
-                sight_of(a, A.cap, table, row_of(col), sc);
-                float mm, ll;
-                const float v = plain_range<HD, S::UNIT>(a, sc, table, row_of(col), head_of(col), k.lo, min(k.hi, sc.end), k.step,
-                                                         split, merge, mm, ll);
-                if (split) {
-                    const uint32_t at = part_of(k.split);
-                    if (t < HD) st_agent(part, at + col * HD + t, v);
-                    if (t == 0) {
-                        st_agent(part, at + COLS * HD + col, mm);
-                        st_agent(part, at + COLS * (HD + 1) + col, ll);
-                    }
-                } else if (t < HD) {
-                    out_of(col)[t] = ll != 0.0f ? v / ll : 0.0f;
-                }
-            }
-        }
+        if (again) res.template put_plain<kWaves * CH>(again, merge);  // rare
     }
-    if (!split) return;
-    // ---- this block's partials are performed at the coherence point before it counts itself
-    uint32_t* const counter = A.counters + (size_t)k.set * a.g.n_kv + kvh;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t == 0)
-        last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(k.splits - 1);
-    __syncthreads();
-    if (!last) return;
-    // The splits' references and sums of weights to LDS, then weights 2^(R_k - R).  The values: an item is four dims of a
-    // column that is there; few items share their splits among groups of threads, which meet in LDS.
-    const int n = k.splits;
-    float* const mk = reinterpret_cast<float*>(merge);  // [column][kMaxSplits], then the weights
-    float* const lk = mk + COLS * kMaxSplits;
-    f4_t* const red = reinterpret_cast<f4_t*>(lk);      // once lk is read
-    const int items = __popc(present) * (HD / 4), groups = max(1, kThreads / items);
-    const auto column = [&](int i) {                    // of the i-th that is there
-        uint32_t left = present;
-        for (int x = 0; x < i; ++x) left &= left - 1;
-        return __builtin_ctz(left);
-    };
-    constexpr int U = 8;  // loads in flight
-    f4_t v[U];
-    const int group = t / items;
-    int item = t - group * items;
-    bool busy = group < groups && items > 0;
-    uint32_t at = busy ? column(item / (HD / 4)) * HD + 4 * (item % (HD / 4)) : 0u;
-    const auto load = [&](int sp) {
-#pragma unroll
-        for (int j = 0; j < U; ++j) v[j] = ld_agent4(part, part_of(min(sp + j * groups, n - 1)) + at);
-    };
-    if (busy) load(group);
-    for (int i = t; i < COLS * n; i += kThreads) {
-        const int sp = i / COLS, col = i % COLS;
-        if (!(present >> col & 1)) continue;
-        mk[col * kMaxSplits + sp] = ld_agent(part, part_of(sp) + COLS * HD + col);
-        lk[col * kMaxSplits + sp] = ld_agent(part, part_of(sp) + COLS * (HD + 1) + col);
-    }
-    __syncthreads();
-    for (int col = wave; col < COLS; col += kWaves) {
-        if (!(present >> col & 1)) continue;
-        const float mv = lane < n ? mk[col * kMaxSplits + lane] : -INFINITY, lv = lane < n ? lk[col * kMaxSplits + lane] : 0.0f;
-        const float mm = group_max<64>(mv);
-        // a split without a score above -inf weighs nothing beside others; where all are so, its l is 0 (nothing
-        // seen: zeros) or NaN
-        const float ew = mv > -INFINITY ? __builtin_amdgcn_exp2f(mv - mm) : mm > -INFINITY ? 0.0f : 1.0f;
-        const float ll = group_sum<64>(mv > -INFINITY || !(mm > -INFINITY) ? lv * ew : 0.0f);
-        if (lane < n) mk[col * kMaxSplits + lane] = ew;
-        if (lane == 0) ml[0][0][col] = ll;
-    }
-    __syncthreads();
-    for (;;) {  // more than 256 items: again for the others, in one group
-        f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        const int col = (int)(at / HD);
-        if (busy) {
-            for (int sp = group; sp < n; sp += U * groups) {
-                if (sp > group) load(sp);
-#pragma unroll
-                for (int j = 0; j < U; ++j)
-                    if (sp + j * groups < n) acc = acc + v[j] * mk[col * kMaxSplits + sp + j * groups];
-            }
-        }
-        if (groups > 1) {
-            red[t] = acc;
-            __syncthreads();
-            if (group == 0)
-                for (int x = 1; x < groups; ++x) acc = acc + red[x * items + t];
-        }
-        if (busy && group == 0) {
-            const float ll = ml[0][0][col];
-            *reinterpret_cast<f4_t*>(out_of(col) + at % HD) = acc * (ll != 0.0f ? 1.0f / ll : 0.0f);
-        }
-        item += kThreads;
-        if (groups > 1 || item - t >= items) break;
-        busy = item < items;
-        if (busy) {
-            at = column(item / (HD / 4)) * HD + 4 * (item % (HD / 4));
-            load(0);
-        }
-    }
-    if (t == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    res.combine(here, lsum, &last, merge);
 }
 
 template <typename F>
@@ -936,7 +967,7 @@ void by_shape(bool q8, int head_dim, F&& f)
 }
 
 struct Layout {
-    int group, ct, cols, tiles, sets, want;
+    int ct, group, cols, tiles, sets, want;
     long long works;  // per kv head
 };
 
@@ -944,16 +975,17 @@ Layout layout_of(const PagedAttnArgs& a)
 {
     Layout y{};
     y.group = a.n_heads / a.g.n_kv;
-    const long long columns = (long long)a.per * y.group;
-    y.ct = columns > CTMIN && a.head_dim <= 128 ? 2 : 1;
+    const long long columns = (long long)a.per * y.group, tables = a.rows / a.per;
+    y.ct = !a.ks && a.head_dim <= 128 && columns > kCols && tables * a.g.n_kv * ((columns + 31) / 32) >= CTMIN ? 2 : 1;
     y.cols = kCols * y.ct;
     y.tiles = (int)((columns + y.cols - 1) / y.cols);
-    y.sets = a.rows / a.per * y.tiles;
-    const long long cap = (long long)a.g.max_blocks * a.g.tpb;
+    y.sets = (int)(tables * y.tiles);
     int unit = 0;
-    by_shape(a.ks != nullptr, a.head_dim, [&](auto q, auto hd) { unit = Shape<decltype(q)::value, decltype(hd)::value>::UNIT; });
-    const long long units = (cap + unit - 1) / unit;
-    if (y.sets <= kPlanSets && (long long)y.sets * a.g.n_kv < kPlanBlocks && units > 1) y.want = std::max(1, std::max(kPlanBlocks / a.g.n_kv - y.sets, kPlanBlocks / 4 / a.g.n_kv));
+    by_shape(a.ks != nullptr, a.head_dim,
+             [&](auto q, auto hd) { unit = Shape<decltype(q)::value, decltype(hd)::value>::CH * kWaves; });
+    const long long cap = (long long)a.g.max_blocks * a.g.tpb, units = (cap + unit - 1) / unit;
+    if (y.sets <= kPlanSets && (long long)y.sets * a.g.n_kv < kPlanBlocks && units > kWholeUnits)
+        y.want = std::max(1, std::max(kPlanBlocks / a.g.n_kv - y.sets, kPlanBlocks / 4 / a.g.n_kv));
     // each set's last split may be short
     y.works = y.want ? std::min<long long>(y.want + y.sets, y.sets * std::min<long long>(kMaxSplits, units)) : y.sets;
     return y;
@@ -987,7 +1019,7 @@ hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipS
         constexpr bool Q8 = decltype(q)::value;
         constexpr int HD = decltype(hd)::value;
         const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, st, A); };
-        if constexpr (HD <= 128) {
+        if constexpr (!Q8 && HD <= 128) {
             if (y.ct == 2) return a.cap > 0.0f ? go(attn_paged_kernel<Q8, HD, 2, true>) : go(attn_paged_kernel<Q8, HD, 2, false>);
         }
         a.cap > 0.0f ? go(attn_paged_kernel<Q8, HD, 1, true>) : go(attn_paged_kernel<Q8, HD, 1, false>);
