@@ -244,7 +244,7 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
 __device__ __forceinline__ bool set_range(const MmaArgs& A, int set, int& lo, int& hi)
 {
     const PagedAttnArgs& a = A.a;
-    const int table = set / A.tiles, c0 = (set - table * A.tiles) * A.cols;
+    const int table = A.tiles == 1 ? set : set / A.tiles, c0 = (set - table * A.tiles) * A.cols;
     lo = A.cap;
     hi = 0;
     if (a.masks) {
@@ -266,7 +266,7 @@ __device__ __forceinline__ bool set_range(const MmaArgs& A, int set, int& lo, in
 }
 
 struct Work {
-    int set, lo, hi, step;      // units of positions lo, lo + step, ... below hi
+    int set, lo, hi, step;      // units of positions lo, lo + step, ... below hi (-1: below the columns' ends)
     int split, splits, slot0;   // slot0: work number of the set's split 0
 };
 
@@ -278,7 +278,9 @@ __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
 {
     const int lane = threadIdx.x & 63;
     if (A.want == 0) {
-        k = Work{A.sets - 1 - w, 0, 0, UNIT, 0, 1, 0};  // a prompt's last rows, which see the most, first
+        k = Work{A.sets - 1 - w, 0, -1, UNIT, 0, 1, 0};  // a prompt's last rows, which see the most, first
+        if (k.set < 0) return false;
+        if (!A.a.masks && A.a.window == 0) return true;  // all from 0 on: how far, the columns will say
         if (!set_range(A, k.set, k.lo, k.hi)) return false;
         k.lo = rfl(k.lo) & ~63;
         k.hi = rfl(k.hi);
@@ -330,9 +332,9 @@ __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
     return found;
 }
 
-template <bool Q8, int HD>
+template <bool Q8, int HD, int CT = 1>
 struct Shape {
-    static constexpr int CH = Q8 ? (HD <= 128 ? 64 : 32) : (HD <= 64 ? 64 : 32);  // positions of a chunk
+    static constexpr int CH = Q8 ? (HD == 64 || (HD == 128 && CT == 1) ? 64 : 32) : HD == 64 ? 64 : 32;  // positions of a chunk
     static constexpr int ES = Q8 ? 1 : 2;                    // bytes of an element of K and V
     static constexpr int KK = Q8 ? HD / 64 : HD / 32;        // k steps of a K tile
     static constexpr int QP = Q8 ? 3 : 2;                    // parts of q
@@ -515,20 +517,25 @@ struct Results {
     int table, col0, kvh;
     __amdgpu_buffer_rsrc_t part;
     __device__ __forceinline__ Results(const MmaArgs& A_, const Work& k_, int kvh_)
-        : A(A_), k(k_), table(k_.set / A_.tiles), col0((k_.set - table * A_.tiles) * COLS), kvh(kvh_), part(buffer_rsrc(A_.part, A_.part_bytes))
+        : A(A_), k(k_), table(A_.tiles == 1 ? k_.set : k_.set / A_.tiles), col0((k_.set - table * A_.tiles) * COLS), kvh(kvh_), part(buffer_rsrc(A_.part, A_.part_bytes))
     {
     }
     __device__ __forceinline__ int columns() const { return min(A.a.per * A.group - col0, COLS); }
-    __device__ __forceinline__ int row_of(int x) const { return table * A.a.per + (col0 + x) / A.group; }
-    __device__ __forceinline__ int head_of(int x) const { return kvh * A.group + (col0 + x) % A.group; }
-    __device__ __forceinline__ float* out_of(int x) const { return A.a.out + ((size_t)row_of(x) * A.a.n_heads + head_of(x)) * HD; }
-    __device__ __forceinline__ const float* q_of(int x) const { return A.a.q + ((size_t)row_of(x) * A.a.n_heads + head_of(x)) * HD; }
+    struct Column {
+        int row, head;
+    };
+    __device__ __forceinline__ Column column(int x) const
+    {
+        const int j = (col0 + x) / A.group;
+        return {table * A.a.per + j, kvh * A.group + (col0 + x) - j * A.group};
+    }
+    __device__ __forceinline__ size_t offset(Column c) const { return ((size_t)c.row * A.a.n_heads + c.head) * HD; }  // in q and out
     __device__ __forceinline__ uint32_t part_of(int sp) const { return (uint32_t)((k.slot0 + sp) * A.a.g.n_kv + kvh) * kPart; }
-    // four dims of column x from d on, ll the sum of all its weights; whether they are finite
-    __device__ __forceinline__ bool put(int x, int d, f4_t v, float ll) const
+    // four dims of column x (at offset `at` of out) from d on, ll the sum of all its weights; whether they are finite
+    __device__ __forceinline__ bool put(int x, size_t at, int d, f4_t v, float ll) const
     {
         if (k.splits > 1) st_agent4(part, part_of(k.split) + x * HD + d, v);
-        else *reinterpret_cast<f4_t*>(out_of(x) + d) = v * (ll != 0.0f ? 1.0f / ll : 0.0f);
+        else *reinterpret_cast<f4_t*>(A.a.out + at + d) = v * (ll != 0.0f ? 1.0f / ll : 0.0f);
         return finite_f32(v[0]) && finite_f32(v[1]) && finite_f32(v[2]) && finite_f32(v[3]) && finite_f32(ll);
     }
     __device__ __forceinline__ void put_sums(int x, float r, float ll) const
@@ -545,16 +552,17 @@ struct Results {
 #pragma unroll 1
         for (int x = 0; x < COLS; ++x) {
             if (!(again >> x & 1)) continue;
+            const Column c = column(x);
             Sight sc;
-            sight_of(A.a, A.cap, table, row_of(x), sc);
+            sight_of(A.a, A.cap, table, c.row, sc);
             float mm, ll;
-            const float v = plain_range<HD, UNIT>(A.a, sc, table, row_of(x), head_of(x), k.lo, sc.end, k.step, k.splits > 1, lds, mm, ll);
+            const float v = plain_range<HD, UNIT>(A.a, sc, table, c.row, c.head, k.lo, sc.end, k.step, k.splits > 1, lds, mm, ll);
             const int t = threadIdx.x;
             if (k.splits > 1) {
                 if (t < HD) st_agent(part, part_of(k.split) + x * HD + t, v);
                 if (t == 0) put_sums(x, mm, ll);
             } else if (t < HD) {
-                out_of(x)[t] = ll != 0.0f ? v / ll : 0.0f;
+                A.a.out[offset(c) + t] = ll != 0.0f ? v / ll : 0.0f;
             }
         }
     }
@@ -628,7 +636,7 @@ struct Results {
             }
             if (busy && group == 0 && there(x)) {
                 const float ll = lsum[x];
-                *reinterpret_cast<f4_t*>(out_of(x) + 4 * (item % (HD / 4))) = acc * (ll != 0.0f ? 1.0f / ll : 0.0f);
+                *reinterpret_cast<f4_t*>(A.a.out + offset(column(x)) + 4 * (item % (HD / 4))) = acc * (ll != 0.0f ? 1.0f / ll : 0.0f);
             }
             item += kThreads;
             if (groups > 1 || item - t >= items) break;
@@ -643,7 +651,7 @@ struct Results {
 template <bool Q8, int HD, int CT, bool CAP>
 __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A)
 {
-    using S = Shape<Q8, HD>;
+    using S = Shape<Q8, HD, CT>;
     constexpr int CH = S::CH, NT = CH / 16, NP = CH / 4, KS = CH / 32;  // K tiles; positions of a lane; k steps of V
     constexpr int KK = S::KK, QP = S::QP, NE = S::NE, DT = S::DT, VW = DT * S::ES / 4;  // VW: words of V per lane and position
     constexpr int NR = HD / 4 < 32 ? HD / 4 : 32;                       // registers of O^T that the waves add at a time
@@ -654,16 +662,16 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     __shared__ __align__(16) u4_t qlds[kQInLds ? CT * KK * QP * 64 : 1];
     __shared__ __align__(16) uint32_t kidx[kWaves][CH], vidx[kWaves][CH];  // [c][tile], [g][j]
     __shared__ __align__(16) float kscl[kWaves][Q8 ? CH : 4], vscl[kWaves][Q8 ? CH : 4];
-    __shared__ float ml[kWaves][2][COLS], lsum[COLS];
+    __shared__ float ml[kWaves][2][COLS], lsum[COLS], qs_lds[COLS];
     __shared__ uint32_t flags, here;
     __shared__ int last;
 
     const PagedAttnArgs& a = A.a;
     const int t = threadIdx.x, lane = t & 63, wave = rfl(t >> 6);
     const int c = lane & 15, g4 = lane >> 4;
-    const int kvh = blockIdx.x % a.g.n_kv;
+    const int kvh = blockIdx.x;
     Work k;
-    if (!plan<kWaves * CH>(A, blockIdx.x / a.g.n_kv, k)) return;  // the same for the whole block
+    if (!plan<kWaves * CH>(A, blockIdx.y + gridDim.y * blockIdx.z, k)) return;  // the same for the whole block
     const Results<HD, COLS> res(A, k, kvh);
     const int table = res.table, n_cols = res.columns();
 
@@ -675,47 +683,58 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     const uint32_t blk_first = bt[min(b_first, a.g.max_blocks - 1)];
     Sight si[CT];
     bool has[CT];
+    size_t at[CT];             // of the column in q and out
     u4_t qp[CT][KK][QP];
-    float qsc[CT], cs[CT];  // scale of the sums of q's parts, and of the exponents
+    float qsc[CT], cs[CT];     // scale of the sums of q's parts, and of the exponents
     Sums<DT> m[CT];
+    // with q's parts in LDS wave u makes those of the columns 16 u + c
+    const auto makes = [&](int u) { return !kQInLds || wave == u; };
     {
         f4_t qf[CT][KK][NE / 4];
-#pragma unroll
-        for (int u = 0; u < CT; ++u) {
-            const f4_t* src = reinterpret_cast<const f4_t*>(res.q_of(min(kCols * u + c, n_cols - 1)) + NE * g4);
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-                for (int i = 0; i < NE / 4; ++i) qf[u][kk][i] = src[NE * kk + i];
-        }
         uint32_t b = 0;
+        int top = 0;
 #pragma unroll
         for (int u = 0; u < CT; ++u) {
+            const auto x = res.column(min(kCols * u + c, n_cols - 1));
+            at[u] = res.offset(x);
+            if (makes(u)) {
+                const f4_t* src = reinterpret_cast<const f4_t*>(a.q + at[u] + NE * g4);
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                    for (int i = 0; i < NE / 4; ++i) qf[u][kk][i] = src[NE * kk + i];
+            }
             si[u] = Sight{0, 0, 0, a.masks};
-            has[u] = sight_of(a, A.cap, table, res.row_of(min(kCols * u + c, n_cols - 1)), si[u]) && kCols * u + c < n_cols;
+            has[u] = sight_of(a, A.cap, table, x.row, si[u]) && kCols * u + c < n_cols;
             if (!has[u]) si[u] = Sight{0, 0, 0, a.masks};
             b |= ((uint32_t)__ballot(has[u]) & 0xFFFFu) << (kCols * u);
+            top = max(top, si[u].end);
+            m[u] = Sums<DT>{-INFINITY, 0.0f, 1.0f, {}};
         }
+        if (k.hi < 0) k.hi = rfl((int)team_max_u32<16>((uint32_t)top));
         if (t == 0) {
             here = b;
             flags = 0;
         }
 #pragma unroll
         for (int u = 0; u < CT; ++u) {
+            if (!makes(u)) continue;
             q_parts<Q8, HD>(a, qf[u], qp[u], qsc[u]);
-            cs[u] = CAP ? kLog2e : qsc[u] * kLog2e;
-            m[u] = Sums<DT>{-INFINITY, 0.0f, 1.0f, {}};
+            if constexpr (kQInLds) {
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                    for (int p = 0; p < QP; ++p) qlds[((u * KK + kk) * QP + p) * 64 + lane] = qp[u][kk][p];
+                if (g4 == 0) qs_lds[kCols * u + c] = qsc[u];
+            }
         }
-    }
-    if constexpr (kQInLds) {
+        if constexpr (kQInLds) {
+            __syncthreads();
 #pragma unroll
-        for (int u = 0; u < CT; ++u)
+            for (int u = 0; u < CT; ++u) qsc[u] = qs_lds[kCols * u + c];
+        }
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-                for (int p = 0; p < QP; ++p)
-                    if (wave == 0) qlds[((u * KK + kk) * QP + p) * 64 + lane] = qp[u][kk][p];
-        __syncthreads();
+        for (int u = 0; u < CT; ++u) cs[u] = CAP ? kLog2e : qsc[u] * kLog2e;
     }
     const auto q_part = [&](int u, int p, int kk) {
         if constexpr (kQInLds) return qlds[((u * KK + kk) * QP + p) * 64 + lane];
@@ -938,7 +957,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             if (has[u]) {
 #pragma unroll
                 for (int r = 0; r < NR / 4; r += 4)
-                    fine[u] &= res.put(col, g4 * (HD / 4) + rd * NR + wave * (NR / 4) + r,
+                    fine[u] &= res.put(col, at[u], g4 * (HD / 4) + rd * NR + wave * (NR / 4) + r,
                                        f4_t{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]}, ll);
                 if (k.splits > 1 && rd == 0 && wave == 0 && g4 == 0) res.put_sums(col, mm, ll);
             }
@@ -976,13 +995,17 @@ Layout layout_of(const PagedAttnArgs& a)
     Layout y{};
     y.group = a.n_heads / a.g.n_kv;
     const long long columns = (long long)a.per * y.group, tables = a.rows / a.per;
-    y.ct = !a.ks && a.head_dim <= 128 && columns > kCols && tables * a.g.n_kv * ((columns + 31) / 32) >= CTMIN ? 2 : 1;
+        y.ct = a.head_dim <= 128 && columns > kCols && tables * a.g.n_kv * ((columns + 31) / 32) >= CTMIN ? 2 : 1;
     y.cols = kCols * y.ct;
     y.tiles = (int)((columns + y.cols - 1) / y.cols);
     y.sets = (int)(tables * y.tiles);
     int unit = 0;
     by_shape(a.ks != nullptr, a.head_dim,
-             [&](auto q, auto hd) { unit = Shape<decltype(q)::value, decltype(hd)::value>::CH * kWaves; });
+             [&](auto q, auto hd) {
+                 constexpr bool Q8 = decltype(q)::value;
+                 constexpr int HD = decltype(hd)::value;
+                 unit = (y.ct == 2 ? Shape<Q8, HD, 2>::CH : Shape<Q8, HD>::CH) * kWaves;
+             });
     const long long cap = (long long)a.g.max_blocks * a.g.tpb, units = (cap + unit - 1) / unit;
     if (y.sets <= kPlanSets && (long long)y.sets * a.g.n_kv < kPlanBlocks && units > kWholeUnits)
         y.want = std::max(1, std::max(kPlanBlocks / a.g.n_kv - y.sets, kPlanBlocks / 4 / a.g.n_kv));
@@ -1014,12 +1037,13 @@ hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipS
     A.counters = reinterpret_cast<uint32_t*>(workspace);
     A.part = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + attention_counter_bytes());
     A.part_bytes = (uint32_t)((size_t)y.works * a.g.n_kv * y.cols * (a.head_dim + 2) * sizeof(float));  // below 2^31: plan()'s blocks
-    const dim3 grid((unsigned)(y.works * a.g.n_kv));
+    const unsigned rows_of_grid = (unsigned)std::min<long long>(y.works, 32768);
+    const dim3 grid((unsigned)a.g.n_kv, rows_of_grid, (unsigned)((y.works + rows_of_grid - 1) / rows_of_grid));
     by_shape(a.ks != nullptr, a.head_dim, [&](auto q, auto hd) {
         constexpr bool Q8 = decltype(q)::value;
         constexpr int HD = decltype(hd)::value;
         const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, st, A); };
-        if constexpr (!Q8 && HD <= 128) {
+        if constexpr (HD <= 128) {
             if (y.ct == 2) return a.cap > 0.0f ? go(attn_paged_kernel<Q8, HD, 2, true>) : go(attn_paged_kernel<Q8, HD, 2, false>);
         }
         a.cap > 0.0f ? go(attn_paged_kernel<Q8, HD, 1, true>) : go(attn_paged_kernel<Q8, HD, 1, false>);
