@@ -52,13 +52,8 @@ constexpr int kWaves = 4, kThreads = kWaves * 64, kCols = 16;
 constexpr int kMaxSplits = 64;    // of a set's positions
 constexpr int kWholeUnits = 3;    // sets of so many units of positions are not split
 constexpr int kPlanSets = 512;   // sets that plan() looks at, 8 a lane; more run unsplit
-#ifndef PB
-#define PB 512
-#endif
-#ifndef CTMIN
-#define CTMIN 256
-#endif
-constexpr int kPlanBlocks = PB;
+constexpr int kPlanBlocks = 512;  // blocks that are at work at once: two on each of 256 CUs
+constexpr int kWideBlocks = 256;  // sets of 32 columns from so many blocks on
 
 struct MmaArgs {
     PagedAttnArgs a;
@@ -995,7 +990,7 @@ Layout layout_of(const PagedAttnArgs& a)
     Layout y{};
     y.group = a.n_heads / a.g.n_kv;
     const long long columns = (long long)a.per * y.group, tables = a.rows / a.per;
-        y.ct = a.head_dim <= 128 && columns > kCols && tables * a.g.n_kv * ((columns + 31) / 32) >= CTMIN ? 2 : 1;
+        y.ct = a.head_dim <= 128 && columns > kCols && tables * a.g.n_kv * ((columns + 31) / 32) >= kWideBlocks ? 2 : 1;
     y.cols = kCols * y.ct;
     y.tiles = (int)((columns + y.cols - 1) / y.cols);
     y.sets = (int)(tables * y.tiles);
@@ -1007,8 +1002,9 @@ Layout layout_of(const PagedAttnArgs& a)
                  unit = (y.ct == 2 ? Shape<Q8, HD, 2>::CH : Shape<Q8, HD>::CH) * kWaves;
              });
     const long long cap = (long long)a.g.max_blocks * a.g.tpb, units = (cap + unit - 1) / unit;
-    if (y.sets <= kPlanSets && (long long)y.sets * a.g.n_kv < kPlanBlocks && units > kWholeUnits)
-        y.want = std::max(1, std::max(kPlanBlocks / a.g.n_kv - y.sets, kPlanBlocks / 4 / a.g.n_kv));
+    const long long blocks = (long long)y.sets * a.g.n_kv;
+    if (y.sets <= kPlanSets && blocks < kPlanBlocks && units > kWholeUnits)
+        y.want = std::max(1, (blocks <= kPlanBlocks / 4 ? kPlanBlocks / 2 : kPlanBlocks) / a.g.n_kv - y.sets);
     // each set's last split may be short
     y.works = y.want ? std::min<long long>(y.want + y.sets, y.sets * std::min<long long>(kMaxSplits, units)) : y.sets;
     return y;

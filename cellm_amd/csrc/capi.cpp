@@ -1783,7 +1783,10 @@ int32_t get_graph_safe_scratch(cellm_hip_ctx* ctx, hipStream_t st, size_t need, 
     if (need == 0) return CELLM_HIP_OK;
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     unsigned long long id = 0;
-    HIP_TRY(hipStreamGetCaptureInfo(st, &status, &id), "hipStreamGetCaptureInfo");
+    if (hipStreamGetCaptureInfo(st, &status, &id) != hipSuccess) {  // the null stream during another's capture
+        (void)hipGetLastError();
+        status = hipStreamCaptureStatusNone;
+    }
     if (status == hipStreamCaptureStatusNone) return get_stream_buffer(ctx, ctx->attn, st, need, out, zero_prefix);
     if (status != hipStreamCaptureStatusActive) return set_error(CELLM_HIP_ERR_DEVICE, "the stream's capture is invalid");
     DeviceBuffer& b = ctx->graph_scratch[{id, st}];
@@ -1822,8 +1825,11 @@ int32_t check_kv(int64_t rows, int64_t per, int64_t n_kv_heads, int64_t head_dim
     if (rows < 0 || rows > (1 << 20) || per < 1 || rows % per != 0)
         return set_error(CELLM_HIP_ERR_INVALID_ARG, "rows=%lld (up to 2^20) must be a multiple of the %lld that share a table",
                          (long long)rows, (long long)per);
+    if (n_kv_heads > 4096 || rows * n_kv_heads > (1 << 25))  // threads are numbered in 32 bits
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "%lld rows of %lld kv heads: at most 4096 heads and 2^25 vectors a call",
+                         (long long)rows, (long long)n_kv_heads);
     // vectors of one array are numbered in 32 bits, positions with room for a step past the last
-    if (n_kv_heads < 1 || n_kv_heads > 4096 || max_blocks < 1 || total_blocks < 1 || n_layers < 1 || tpb < 1 || layer < 0 ||
+    if (n_kv_heads < 1 || max_blocks < 1 || total_blocks < 1 || n_layers < 1 || tpb < 1 || layer < 0 ||
         layer >= n_layers || max_blocks > (1 << 30) || tpb > (1 << 30) || max_blocks * tpb > (1 << 30) ||
         total_blocks > INT32_MAX || n_layers > INT32_MAX || n_layers * n_kv_heads > INT32_MAX ||
         n_layers * n_kv_heads * tpb > (int64_t)UINT32_MAX / total_blocks)
@@ -1848,7 +1854,7 @@ int32_t kv_write_q8_impl(cellm_hip_ctx* ctx, const float* q, const float* k, con
                          int64_t total_blocks, int64_t n_layers, int64_t tpb, int64_t layer, void* stream)
 {
     if (int32_t rc = check_kv(rows, per, n_kv_heads, head_dim, max_blocks, total_blocks, n_layers, tpb, layer)) return rc;
-    if (n_heads < 0 || n_heads > 4096 || (cos_sin && (table_positions < 1 || table_positions > INT32_MAX)))
+    if (n_heads < 0 || n_heads > 4096 || rows * n_heads > (1 << 28) || (cos_sin && (table_positions < 1 || table_positions > INT32_MAX)))
         return set_error(CELLM_HIP_ERR_INVALID_ARG, "bad heads %lld or table_positions %lld", (long long)n_heads,
                          (long long)table_positions);
     if (rows == 0) return CELLM_HIP_OK;

@@ -62,9 +62,9 @@ __global__ __launch_bounds__(kThreads) void kv_write_q8_kernel(const WriteArgs a
     constexpr int T = HD / 8, H = HD / 2;
     const int nq = a.q ? a.n_heads : 0, per_row = nq + 2 * a.g.n_kv;
     const int l = threadIdx.x % T;
-    const long long vec = (long long)blockIdx.x * (kThreads / T) + threadIdx.x / T;
-    if (vec >= (long long)a.rows * per_row) return;  // whole teams
-    const int r = (int)(vec / per_row), h = (int)(vec - (long long)r * per_row);
+    const uint32_t vec = blockIdx.x * (kThreads / T) + threadIdx.x / T;  // 32 bits: the host checks the count
+    if (vec >= (uint32_t)a.rows * (uint32_t)per_row) return;  // whole teams
+    const int r = (int)(vec / (uint32_t)per_row), h = (int)(vec - (uint32_t)r * (uint32_t)per_row);
     const bool is_q = h < nq, is_v = h >= nq + a.g.n_kv;
     const int kvh = is_q ? 0 : is_v ? h - nq - a.g.n_kv : h - nq;
     const int p = a.pos[r], slot = a.slots ? a.slots[r] : p;
@@ -135,9 +135,10 @@ __global__ __launch_bounds__(kThreads) void kv_read_q8_kernel(const int8_t* __re
                                                               void* __restrict__ ko, void* __restrict__ vo)
 {
     constexpr int E = DT == DT_F32 ? 4 : 8, T = HD / E;
-    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= (long long)rows * g.n_kv * T) return;
-    const int l = (int)(i % T), kvh = (int)(i / T % g.n_kv), r = (int)(i / T / g.n_kv);
+    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;  // 32 bits: the host checks the count
+    if (i >= (uint32_t)rows * (uint32_t)g.n_kv * T) return;
+    const uint32_t vec = i / T, row = vec / (uint32_t)g.n_kv;
+    const int l = (int)(i % T), kvh = (int)(vec - row * (uint32_t)g.n_kv), r = (int)row;
     const int p = pos[r];
     if (p < 0) return;
     const long long v0 = vector_of(g, r / per, p);

@@ -54,19 +54,21 @@ def _stream_ptr(stream):
     return C.c_void_p(stream.cuda_stream)
 
 
-# torch dtypes by name, filled on first use (this module is imported without torch)
-_DTYPE_NAMES: dict = {}
-_F32, _INT8, _INT32, _INT64 = ("float32",), ("int8",), ("int32", "uint32"), ("int64", "uint64")
-_HALF, _FLOATS = ("float16", "int16", "uint16"), ("float32", "float16", "bfloat16")
+class _Dtypes:
+    """torch dtypes that the paged-cache calls take, looked up on first use (this module is imported without torch)."""
 
+    names = dict(f32=("float32",), i8=("int8",), i32=("int32", "uint32"), i64=("int64", "uint64"),
+                 half=("float16", "int16", "uint16"), floats=("float32", "float16", "bfloat16"))
 
-def _name_dtypes() -> None:
-    if not _DTYPE_NAMES:
+    def __getattr__(self, kind):
         import torch
 
-        for name in {*_F32, *_INT8, *_INT32, *_INT64, *_HALF, *_FLOATS}:
-            if hasattr(torch, name):
-                _DTYPE_NAMES[getattr(torch, name)] = name
+        found = tuple(getattr(torch, n) for n in self.names[kind] if hasattr(torch, n))
+        setattr(self, kind, found)
+        return found
+
+
+_DT = _Dtypes()
 
 
 def argmax_key_index(key: int) -> int:
@@ -560,26 +562,26 @@ class HipOps:
     # [head_dim] with an f32 scale per vector; `rows_per_table` consecutive rows share a row of block_tables
 
     def _ptr(self, name: str, t, dtypes, count: int) -> int:
-        """Address of a device tensor of `count` elements of one of `dtypes` (names), on the context's device."""
-        if _DTYPE_NAMES.get(t.dtype, None) not in dtypes:
-            raise TypeError(f"{name} is {t.dtype}, not {' or '.join(dtypes)}")
+        """Address of a device tensor of `count` elements of one of `dtypes`, on the context's device."""
+        if t.dtype in dtypes and t.numel() == count and t.get_device() == self.device and t.is_contiguous():
+            return t.data_ptr()
+        if t.dtype not in dtypes:
+            raise TypeError(f"{name} is {t.dtype}, not {' or '.join(str(d) for d in dtypes)}")
         if t.numel() != count:
             raise ValueError(f"{name} holds {t.numel()} elements, not {count}")
         if t.get_device() != self.device:  # -1 for host tensors
             raise ValueError(f"encode_* expects device tensors: {name} is on {t.device}, the context on device {self.device}")
-        if not t.is_contiguous():
-            raise ValueError(f"encode_* expects contiguous tensors: {name} is not")
-        return t.data_ptr()
+        raise ValueError(f"encode_* expects contiguous tensors: {name} is not")
 
     def _q8_ptrs(self, kcodes, kscale, vcodes, vscale, head_dim: int, vectors: int):
-        return (self._ptr("kcodes", kcodes, _INT8, vectors * head_dim), self._ptr("kscale", kscale, _F32, vectors),
-                self._ptr("vcodes", vcodes, _INT8, vectors * head_dim), self._ptr("vscale", vscale, _F32, vectors))
+        return (self._ptr("kcodes", kcodes, _DT.i8, vectors * head_dim), self._ptr("kscale", kscale, _DT.f32, vectors),
+                self._ptr("vcodes", vcodes, _DT.i8, vectors * head_dim), self._ptr("vscale", vscale, _DT.f32, vectors))
 
     def _pages(self, kcache, vcache, kscale, vscale, head_dim: int, vectors: int):
         """K and V arrays of f16 pages (no scales) or 8-bit ones, in the order of the C calls."""
         if kscale is None and vscale is None:
-            return (self._ptr("kcache", kcache, _HALF, vectors * head_dim),
-                    self._ptr("vcache", vcache, _HALF, vectors * head_dim))
+            return (self._ptr("kcache", kcache, _DT.half, vectors * head_dim),
+                    self._ptr("vcache", vcache, _DT.half, vectors * head_dim))
         if kscale is None or vscale is None:
             raise ValueError("kscale and vscale go together")
         return self._q8_ptrs(kcache, kscale, vcache, vscale, head_dim, vectors)
@@ -588,21 +590,20 @@ class HipOps:
         if rows_per_table < 1 or rows % rows_per_table != 0:
             raise ValueError(f"{rows} rows are no multiple of rows_per_table {rows_per_table}")
         max_blocks = block_tables.shape[-1]
-        return self._ptr("block_tables", block_tables, _INT32, rows // rows_per_table * max_blocks), max_blocks
+        return self._ptr("block_tables", block_tables, _DT.i32, rows // rows_per_table * max_blocks), max_blocks
 
     def encode_kv_write_q8(self, k, v, n_kv_heads: int, head_dim: int, positions_i32, kcodes, kscale, vcodes, vscale,
                            block_tables, total_blocks: int, n_layers: int, tokens_per_block: int, layer: int,
                            rows_per_table: int = 1, stream=None) -> None:
         """K and V [rows][n_kv_heads * head_dim] f32 quantised into 8-bit pages (cellm_hip_kv_write_q8)."""
-        _name_dtypes()
         rows = positions_i32.numel()
         n = rows * n_kv_heads * head_dim
         bt, max_blocks = self._table_ptr(block_tables, rows, rows_per_table)
         cache = self._q8_ptrs(kcodes, kscale, vcodes, vscale, head_dim,
                               total_blocks * n_layers * n_kv_heads * tokens_per_block)
         check(self._lib.cellm_hip_kv_write_q8(
-            self._h, self._ptr("k", k, _F32, n), self._ptr("v", v, _F32, n), rows, rows_per_table, n_kv_heads, head_dim,
-            self._ptr("positions", positions_i32, _INT32, rows), *cache, bt, max_blocks, total_blocks, n_layers,
+            self._h, self._ptr("k", k, _DT.f32, n), self._ptr("v", v, _DT.f32, n), rows, rows_per_table, n_kv_heads, head_dim,
+            self._ptr("positions", positions_i32, _DT.i32, rows), *cache, bt, max_blocks, total_blocks, n_layers,
             tokens_per_block, layer, _stream_ptr(stream)))
 
     def encode_rope_kv_write_q8(self, q, k, v, q_out, n_heads: int, n_kv_heads: int, head_dim: int, positions_i32, cos_sin,
@@ -611,25 +612,23 @@ class HipOps:
                                 stream=None) -> None:
         """q_out = RoPE(q), and RoPE(k) and v quantised into 8-bit pages (cellm_hip_rope_kv_write_q8); q_out may be q.
         slots_i32: cache positions of the rows where they are not their positions (drafted tokens)."""
-        _name_dtypes()
         rows = positions_i32.numel()
         n, nq = rows * n_kv_heads * head_dim, rows * n_heads * head_dim
         bt, max_blocks = self._table_ptr(block_tables, rows, rows_per_table)
         cache = self._q8_ptrs(kcodes, kscale, vcodes, vscale, head_dim,
                               total_blocks * n_layers * n_kv_heads * tokens_per_block)
         check(self._lib.cellm_hip_rope_kv_write_q8(
-            self._h, self._ptr("q", q, _F32, nq), self._ptr("k", k, _F32, n), self._ptr("v", v, _F32, n),
-            self._ptr("q_out", q_out, _F32, nq), rows, rows_per_table, n_heads, n_kv_heads, head_dim,
-            self._ptr("positions", positions_i32, _INT32, rows),
-            None if slots_i32 is None else self._ptr("slots", slots_i32, _INT32, rows),
-            self._ptr("cos_sin", cos_sin, _F32, cos_sin.shape[0] * head_dim), cos_sin.shape[0], *cache, bt, max_blocks,
+            self._h, self._ptr("q", q, _DT.f32, nq), self._ptr("k", k, _DT.f32, n), self._ptr("v", v, _DT.f32, n),
+            self._ptr("q_out", q_out, _DT.f32, nq), rows, rows_per_table, n_heads, n_kv_heads, head_dim,
+            self._ptr("positions", positions_i32, _DT.i32, rows),
+            None if slots_i32 is None else self._ptr("slots", slots_i32, _DT.i32, rows),
+            self._ptr("cos_sin", cos_sin, _DT.f32, cos_sin.shape[0] * head_dim), cos_sin.shape[0], *cache, bt, max_blocks,
             total_blocks, n_layers, tokens_per_block, layer, _stream_ptr(stream)))
 
     def encode_kv_read_q8(self, kcodes, kscale, vcodes, vscale, block_tables, positions_i32, k_out, v_out,
                           n_kv_heads: int, head_dim: int, total_blocks: int, n_layers: int, tokens_per_block: int,
                           layer: int, rows_per_table: int = 1, stream=None) -> None:
         """The values of the rows' positions, [rows][n_kv_heads * head_dim] in k_out's type (cellm_hip_kv_read_q8)."""
-        _name_dtypes()
         rows = positions_i32.numel()
         n = rows * n_kv_heads * head_dim
         if k_out.dtype != v_out.dtype:
@@ -638,26 +637,25 @@ class HipOps:
         cache = self._q8_ptrs(kcodes, kscale, vcodes, vscale, head_dim,
                               total_blocks * n_layers * n_kv_heads * tokens_per_block)
         check(self._lib.cellm_hip_kv_read_q8(
-            self._h, *cache, bt, max_blocks, total_blocks, self._ptr("positions", positions_i32, _INT32, rows), rows,
+            self._h, *cache, bt, max_blocks, total_blocks, self._ptr("positions", positions_i32, _DT.i32, rows), rows,
             rows_per_table, n_kv_heads, head_dim, n_layers, tokens_per_block, layer, _torch_dtype_code(k_out),
-            self._ptr("k_out", k_out, _FLOATS, n), self._ptr("v_out", v_out, _FLOATS, n), _stream_ptr(stream)))
+            self._ptr("k_out", k_out, _DT.floats, n), self._ptr("v_out", v_out, _DT.floats, n), _stream_ptr(stream)))
 
     def encode_attention_q8(self, q, kcodes, kscale, vcodes, vscale, block_tables, positions_i32, out, n_heads: int,
                             n_kv_heads: int, head_dim: int, total_blocks: int, n_layers: int, tokens_per_block: int,
                             layer: int, attn_scale: float | None = None, soft_cap: float | None = None, window: int = 0,
                             rows_per_table: int = 1, stream=None) -> None:
         """encode_attention over 8-bit pages (cellm_hip_attention_gqa_q8kv)."""
-        _name_dtypes()
         rows = positions_i32.numel()
         n = rows * n_heads * head_dim
         bt, max_blocks = self._table_ptr(block_tables, rows, rows_per_table)
         cache = self._q8_ptrs(kcodes, kscale, vcodes, vscale, head_dim,
                               total_blocks * n_layers * n_kv_heads * tokens_per_block)
         check(self._lib.cellm_hip_attention_gqa_q8kv(
-            self._h, self._ptr("q", q, _F32, n), *cache, bt, max_blocks, total_blocks,
-            self._ptr("positions", positions_i32, _INT32, rows), rows, rows_per_table, n_heads, n_kv_heads, head_dim,
+            self._h, self._ptr("q", q, _DT.f32, n), *cache, bt, max_blocks, total_blocks,
+            self._ptr("positions", positions_i32, _DT.i32, rows), rows, rows_per_table, n_heads, n_kv_heads, head_dim,
             n_layers, tokens_per_block, layer, 0.0 if attn_scale is None else attn_scale,
-            0.0 if soft_cap is None else soft_cap, window, self._ptr("out", out, _F32, n), _stream_ptr(stream)))
+            0.0 if soft_cap is None else soft_cap, window, self._ptr("out", out, _DT.f32, n), _stream_ptr(stream)))
 
     def encode_attention_tree(self, q, kcache, vcache, block_tables, context_lens_i32, masks_i64, out, n_heads: int,
                               n_kv_heads: int, head_dim: int, total_blocks: int, n_layers: int, tokens_per_block: int,
@@ -666,7 +664,6 @@ class HipOps:
         """Attention of drafted trees: masks_i64 [sessions][tree][ceil(tree / 64)] words, bit i of node j set where j sees
         node i; node i stands in slot context_lens[t] + i.  f16 pages, or 8-bit ones with their scales
         (cellm_hip_attention_tree_f16kv / _q8kv)."""
-        _name_dtypes()
         if masks_i64.dim() != 3 or masks_i64.shape[2] != (masks_i64.shape[1] + 63) // 64:
             raise ValueError(f"masks {tuple(masks_i64.shape)} are not [sessions][tree][ceil(tree / 64)]")
         tables, tree, words = masks_i64.shape
@@ -674,26 +671,25 @@ class HipOps:
         bt, max_blocks = self._table_ptr(block_tables, tables, 1)
         cache = self._pages(kcache, vcache, kscale, vscale, head_dim, total_blocks * n_layers * n_kv_heads * tokens_per_block)
         fn = self._lib.cellm_hip_attention_tree_f16kv if kscale is None else self._lib.cellm_hip_attention_tree_q8kv
-        check(fn(self._h, self._ptr("q", q, _F32, n), *cache, bt, max_blocks, total_blocks,
-                 self._ptr("context_lens", context_lens_i32, _INT32, tables),
-                 self._ptr("masks", masks_i64, _INT64, tables * tree * words), tables, tree, n_heads, n_kv_heads, head_dim,
+        check(fn(self._h, self._ptr("q", q, _DT.f32, n), *cache, bt, max_blocks, total_blocks,
+                 self._ptr("context_lens", context_lens_i32, _DT.i32, tables),
+                 self._ptr("masks", masks_i64, _DT.i64, tables * tree * words), tables, tree, n_heads, n_kv_heads, head_dim,
                  n_layers, tokens_per_block, layer, 0.0 if attn_scale is None else attn_scale,
-                 0.0 if soft_cap is None else soft_cap, window, self._ptr("out", out, _F32, n), _stream_ptr(stream)))
+                 0.0 if soft_cap is None else soft_cap, window, self._ptr("out", out, _DT.f32, n), _stream_ptr(stream)))
 
     def encode_kv_accept(self, kcache, vcache, block_tables, context_lens_i32, accepted_i32, tree: int, n_kv_heads: int,
                          head_dim: int, total_blocks: int, n_layers: int, tokens_per_block: int, kscale=None, vscale=None,
                          stream=None) -> None:
         """Keeps the accepted path of each tree (cellm_hip_kv_accept_f16 / _q8): accepted_i32 [sessions][up to tree] rising
         node numbers, ended by -1."""
-        _name_dtypes()
         if accepted_i32.dim() != 2:
             raise ValueError(f"accepted {tuple(accepted_i32.shape)} is not [sessions][nodes]")
         tables, most = accepted_i32.shape
         bt, max_blocks = self._table_ptr(block_tables, tables, 1)
         cache = self._pages(kcache, vcache, kscale, vscale, head_dim, total_blocks * n_layers * n_kv_heads * tokens_per_block)
         fn = self._lib.cellm_hip_kv_accept_f16 if kscale is None else self._lib.cellm_hip_kv_accept_q8
-        check(fn(self._h, *cache, bt, max_blocks, total_blocks, self._ptr("context_lens", context_lens_i32, _INT32, tables),
-                 self._ptr("accepted", accepted_i32, _INT32, tables * most), most, tables, tree, n_kv_heads, head_dim,
+        check(fn(self._h, *cache, bt, max_blocks, total_blocks, self._ptr("context_lens", context_lens_i32, _DT.i32, tables),
+                 self._ptr("accepted", accepted_i32, _DT.i32, tables * most), most, tables, tree, n_kv_heads, head_dim,
                  n_layers, tokens_per_block, _stream_ptr(stream)))
 
     def encode_silu_mul(self, gate, up, stream=None) -> None:

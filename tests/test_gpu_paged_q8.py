@@ -241,6 +241,41 @@ def test_prompts(ops, tables, per, past, nh, nkv, hd, tpb, kw):
     _check(_attention(ops, q, cache, bt, pos, 0, per, **kw), ref)
 
 
+# enough sets of 32 columns for the kernel to take them so (tables * kv heads * ceil(rows * heads / kv heads / 32) >= 256),
+# whole ones and short ones, with more sets than are planned (512) and fewer
+@pytest.mark.parametrize("tables,per,past,nh,nkv,hd,tpb", [
+    (8, 21, 90, 16, 8, 64, 16), (5, 65, 7, 24, 8, 128, 16), (2, 160, 30, 32, 8, 64, 7), (1, 700, 0, 12, 3, 64, 16),
+    (64, 9, 50, 8, 2, 128, 32)])
+@pytest.mark.parametrize("kw", [{}, dict(window=45), dict(soft_cap=5.0)])
+def test_many_columns(ops, tables, per, past, nh, nkv, hd, tpb, kw):
+    g = torch.Generator().manual_seed(per + past)
+    n = past + per
+    bt, total = _table(g, tables, -(-n // tpb))
+    bt[-1, 1] = total  # a missing page
+    cache = P.cache_q8(total, 1, nkv, tpb, hd, per)
+    q = torch.randn(tables * per, nh, hd, generator=g) * 1.5
+    pos = (past + torch.arange(per)).repeat(tables)
+    pos[per // 2] = -1
+    got = _attention(ops, q, cache, bt, pos, 0, per, **kw)
+    some = torch.randperm(tables * per, generator=g)[:90]
+    some = torch.unique(torch.cat([some, torch.tensor([0, per // 2, tables * per - 1])]))
+    ref = torch.cat([P.causal(q[r:r + 1], *cache, bt[r // per:r // per + 1], pos[r:r + 1], 0, 1, None, kw.get("soft_cap", 0.0),
+                              kw.get("window", 0)) for r in some.tolist()])
+    _check(got[some], ref)
+
+
+def test_more_sets_than_a_grid_dimension_holds(ops):
+    g = torch.Generator().manual_seed(3)
+    tables, hd, tpb = 33000, 64, 16
+    cache = P.cache_q8(50, 1, 1, tpb, hd, 8)
+    bt = torch.randint(0, 50, (tables, 1), generator=g)
+    pos = torch.randint(-1, tpb, (tables,), generator=g)
+    q = torch.randn(tables, 1, hd, generator=g)
+    got = _attention(ops, q, cache, bt, pos, 0, 1)
+    some = torch.cat([torch.arange(20), torch.arange(tables - 20, tables), torch.randperm(tables, generator=g)[:60]])
+    _check(got[some], P.causal(q[some], *cache, bt[some], pos[some], 0, 1))
+
+
 def test_rows_of_a_table_in_any_order(ops):
     """Positions that jump, repeat, pass the table and are missing, with missing pages among the table's."""
     g = torch.Generator().manual_seed(11)
@@ -325,7 +360,7 @@ def _random_tree(g, tree):
 
 TREES = [(1, 26, 14, 2, 64, 16, 1000), (3, 1, 4, 4, 128, 16, 40), (2, 63, 8, 1, 128, 5, 130), (2, 64, 3, 3, 256, 16, 70),
          (1, 65, 6, 2, 64, 1, 5), (1, 200, 2, 1, 64, 32, 300), (4, 7, 20, 2, 128, 16, 0), (1, 256, 1, 1, 128, 16, 33),
-         (2, 12, 4, 2, 256, 16, 2500)]
+         (2, 12, 4, 2, 256, 16, 2500), (6, 61, 16, 8, 64, 16, 60), (11, 37, 24, 8, 128, 16, 30)]
 
 
 @pytest.mark.parametrize("f16", [True, False])
@@ -371,10 +406,11 @@ def test_trees_at_the_ends_of_their_tables(ops, f16):
 
 
 @pytest.mark.parametrize("f16", [True, False])
-@pytest.mark.parametrize("hd,ctx", [(64, 10), (128, 70), (256, 700)])
-def test_garbage_in_slots_that_a_node_does_not_see(ops, f16, hd, ctx):
+@pytest.mark.parametrize("hd,ctx,tables", [(64, 10, 1), (128, 70, 1), (256, 700, 1), (64, 900, 1), (64, 10, 64), (128, 70, 64)])
+def test_garbage_in_slots_that_a_node_does_not_see(ops, f16, hd, ctx, tables):
     """NaN, infinities and the largest numbers in other nodes' slots, behind the tree and before the window: a node that
-    does not see them keeps its result, one that does has theirs."""
+    does not see them keeps its result, one that does has theirs.  64 tables that are all the same take 32 columns at a
+    time."""
     g = torch.Generator().manual_seed(29)
     tree, nh, nkv, tpb = 20, 6, 2, 16
     bt, total = _table(g, 1, -(-(ctx + tree) // tpb) + 1)
@@ -398,7 +434,10 @@ def test_garbage_in_slots_that_a_node_does_not_see(ops, f16, hd, ctx):
         spoil(ctx + 5, what)
         for p in range(ctx + tree, bt.shape[1] * tpb):
             spoil(p, what)
-        got = _tree_call(ops, q, cache, bt, torch.tensor([ctx]), P.words_of(bits), 0, f16)[0]
+        got = _tree_call(ops, q.repeat(tables, 1, 1, 1), cache, bt.repeat(tables, 1), torch.tensor([ctx] * tables),
+                         P.words_of(bits).repeat(tables, 1, 1), 0, f16)
+        assert tables == 1 or torch.equal(torch.nan_to_num(got[0], nan=1e9), torch.nan_to_num(got[-1], nan=1e9))
+        got = got[-1]
         others = [j for j in range(tree) if j != 5]
         assert P.rel(got[others], clean[0, others]) <= TOL
         assert bool(torch.isnan(got[5]).all())
