@@ -337,17 +337,18 @@ struct Shape {
     static constexpr int DT = HD / 16;                       // tiles of O^T
 };
 
-// codes of four dims at positions j (a) and j + 1 (b) as exact f16 pairs by dim: 0x6400 | (c + 128) is 1152 + c
+// Codes of four dims at positions j (a) and j + 1 (b) as f16 pairs by dim, in units of 2^-9, all exact: the byte c + 128
+// alone is the f16 (c + 128) 2^-24, and (c + 128) 2^-24 * 2^15 - 2^-2 = c 2^-9.
+constexpr float kCodeUnit = 0x1p9f;
 __device__ __forceinline__ void pairs_of_codes(uint32_t a, uint32_t b, uint32_t (&o)[4])
 {
     a ^= 0x80808080u;
     b ^= 0x80808080u;
-    const uint32_t s01 = __builtin_amdgcn_perm(b, a, 0x05010400u), s23 = __builtin_amdgcn_perm(b, a, 0x07030602u);
-    const h2_t bias = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-    o[0] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, s01, 0x04010400u)) + bias);
-    o[1] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, s01, 0x04030402u)) + bias);
-    o[2] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, s23, 0x04010400u)) + bias);
-    o[3] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, s23, 0x04030402u)) + bias);
+    const h2_t up = {(_Float16)0x1p15f, (_Float16)0x1p15f}, off = {(_Float16)-0.25f, (_Float16)-0.25f};
+    o[0] = as_u32(__builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(b, a, 0x0C040C00u)), up, off));
+    o[1] = as_u32(__builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(b, a, 0x0C050C01u)), up, off));
+    o[2] = as_u32(__builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(b, a, 0x0C060C02u)), up, off));
+    o[3] = as_u32(__builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(b, a, 0x0C070C03u)), up, off));
 }
 
 // q's parts of the column `some`, the B operands of the scores, and the scale that is left out of them.
@@ -470,11 +471,17 @@ __device__ __forceinline__ void weigh(const float (&s)[NP], float cs, const floa
         weights();
     }
     m.l = m.l + lc;
+    // w - h, exact in f32, and its rounding to f16 are one instruction where the compiler sees a product
+    float minus1 = -1.0f;
+    asm("" : "+s"(minus1));
 #pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const _Float16 h = (_Float16)w[j];
-        ph[j >> 3][j & 7] = h;
-        pl[j >> 3][j & 7] = (_Float16)__builtin_fmaf((float)h, -1.0f, w[j]);
+    for (int j = 0; j < NP; j += 2) {
+        const h2_t h = {(_Float16)w[j], (_Float16)w[j + 1]};
+        const h2_t l = {(_Float16)__builtin_fmaf((float)h[0], minus1, w[j]), (_Float16)__builtin_fmaf((float)h[1], minus1, w[j + 1])};
+        ph[j >> 3][j & 7] = h[0];
+        ph[j >> 3][(j & 7) + 1] = h[1];
+        pl[j >> 3][j & 7] = l[0];
+        pl[j >> 3][(j & 7) + 1] = l[1];
     }
 }
 
@@ -947,7 +954,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                 const float ew = ml[x][0][col] > -INFINITY ? __builtin_amdgcn_exp2f(ml[x][0][col] - mm) : ml[x][1][col];
                 ll = ll + ml[x][1][col] * ew;
 #pragma unroll
-                for (int r = 0; r < NR / 4; ++r) acc[r] = acc[r] + mine[(x * NR + wave * (NR / 4) + r) * 64] * ew;
+                for (int r = 0; r < NR / 4; ++r) acc[r] = acc[r] + mine[(x * NR + wave * (NR / 4) + r) * 64] * (Q8 ? ew * kCodeUnit : ew);
             }
             if (has[u]) {
 #pragma unroll
@@ -990,7 +997,7 @@ Layout layout_of(const PagedAttnArgs& a)
     Layout y{};
     y.group = a.n_heads / a.g.n_kv;
     const long long columns = (long long)a.per * y.group, tables = a.rows / a.per;
-        y.ct = a.head_dim <= 128 && columns > kCols && tables * a.g.n_kv * ((columns + 31) / 32) >= kWideBlocks ? 2 : 1;
+    y.ct = a.head_dim <= 128 && columns > kCols && tables * a.g.n_kv * ((columns + 31) / 32) >= kWideBlocks ? 2 : 1;
     y.cols = kCols * y.ct;
     y.tiles = (int)((columns + y.cols - 1) / y.cols);
     y.sets = (int)(tables * y.tiles);
