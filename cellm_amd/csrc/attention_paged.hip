@@ -36,6 +36,12 @@
 // The positions of a set of columns are split over blocks by a rule on the device (plan()),
 // which knows how long every context is; the last block of a set to finish adds the others'
 // sums in split order.
+//
+// What bounds it (gfx950): decode, the reads, in part (8 sessions of 4096 to 8192 positions, 32/8 heads of 128: 28 us for 104 MB,
+// 3.7 TB/s, and one at 131072 58 us for 277 MB, 4.7, where a bare read of them takes 16.5 and 41), as 4 of 16 columns
+// are filled and V's unpacking stands beside them; short contexts, four dependent latencies a chunk and the meeting of
+// splits (9 us at 701 positions, 14/2 heads of 64); many columns, the latency of a chunk at two waves per SIMD (1024 tokens onto as
+// many, 32/8 heads of 128, 82 us: vector ALU busy 59 %, matrix units 19 %, 300 TFLOP/s of the formula's products).
 #include <algorithm>
 #include <cmath>
 
@@ -50,10 +56,21 @@ namespace {
 
 constexpr int kWaves = 4, kThreads = kWaves * 64, kCols = 16;
 constexpr int kMaxSplits = 64;    // of a set's positions
-constexpr int kWholeUnits = 3;    // sets of so many units of positions are not split
-constexpr int kPlanSets = 512;   // sets that plan() looks at, 8 a lane; more run unsplit
-constexpr int kPlanBlocks = 512;  // blocks that are at work at once: two on each of 256 CUs
-constexpr int kWideBlocks = 256;  // sets of 32 columns from so many blocks on
+// Sets of so many units of positions (a chunk for each wave) are not split: the meeting of splits costs about 4.5 us, a
+// walk of three units less.  300 positions (14/2 heads of 64) 8.3 us, 10.8 in splits; 701 10.1 and 11.0; a tree of 16
+// nodes at 500 10.0 and 12.3; a prompt of 512 10.4 and 15.9.  At four units splits win: 1000 positions 10.9, 12.4 in halves.
+constexpr int kWholeUnits = 3;
+constexpr int kPlanSets = 512;    // sets that plan() looks at, 8 a lane; more run unsplit
+// Splits aim at one block on each of the 256 CUs, though two run at once: fewer, longer walks keep the reads going and meet
+// faster (one session at 131072 positions, 32/8 heads of 128: 61.3 us, 66.1 with 512 blocks; 16 sessions at 8000, 8/1
+// heads of 256, 24.5 and 29.5; 300 rows at 600 of those 19.9 and 26.3).  Against it: 8 sessions at 1000 positions, 32/8
+// heads of 128, have 15.2 us and 13.8.
+constexpr int kPlanBlocks = 256;
+// Sets of 32 columns where they leave at least so many blocks: each K and V tile serves twice the columns (8 trees of
+// 63 nodes at 4096 positions, 32/8 heads of 128, f16: 90 us, 140 with 16 columns; a prompt of 1024 over 8-bit pages 90
+// and 104), but with fewer blocks the chip stands idle (16 trees of 8 nodes at 1000 positions 32.1 us, 18.3 with 16
+// columns; a prompt of 512 with 14/2 heads of 64 21.2 and 10.5; one f16 tree of 26 nodes 17.4 and 12.4).
+constexpr int kWideBlocks = 256;
 
 struct MmaArgs {
     PagedAttnArgs a;
@@ -158,9 +175,9 @@ __device__ __forceinline__ float capped(const PagedAttnArgs& a, float s)
     return a.cap > 0.0f ? tanhf(s / a.cap) * a.cap : s;
 }
 
-// The units of positions lo, lo + step, ... below up of one (row, head) over f16 pages by plain f32 sums, the whole block: reference R, log2(e) times
-// the largest score, sum l of the weights and, in threads below HD, the weighted sum of V (returned).  A unit at a time: a score
-// per thread, then HD threads per position.  For columns whose sums in f16 parts are not finite: inf * lo may be NaN where
+// The units of positions lo, lo + step, ... below up of one (row, head) over f16 pages by plain f32 sums, the whole block:
+// reference R, log2(e) times the largest score, sum l of the weights and, in threads below HD, the weighted sum of V
+// (returned).  A unit at a time: a score per thread, then HD threads per position.  For columns whose sums in f16 parts are not finite: inf * lo may be NaN where
 // inf * v is not, and so is the 0 * inf of a position that the column does not see.
 template <int HD, int UNIT>
 __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table, int row, int head, int lo, int up, int step,
@@ -1010,8 +1027,7 @@ Layout layout_of(const PagedAttnArgs& a)
              });
     const long long cap = (long long)a.g.max_blocks * a.g.tpb, units = (cap + unit - 1) / unit;
     const long long blocks = (long long)y.sets * a.g.n_kv;
-    if (y.sets <= kPlanSets && blocks < kPlanBlocks && units > kWholeUnits)
-        y.want = std::max(1, (blocks <= kPlanBlocks / 4 ? kPlanBlocks / 2 : kPlanBlocks) / a.g.n_kv - y.sets);
+    if (y.sets <= kPlanSets && blocks < kPlanBlocks && units > kWholeUnits) y.want = std::max(1, kPlanBlocks / a.g.n_kv - y.sets);
     // each set's last split may be short
     y.works = y.want ? std::min<long long>(y.want + y.sets, y.sets * std::min<long long>(kMaxSplits, units)) : y.sets;
     return y;

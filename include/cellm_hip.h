@@ -550,10 +550,10 @@ int32_t cellm_hip_attention_gqa_f16kv_noalloc(cellm_hip_ctx_t* ctx, const float*
 /* ---- the 8-bit paged cache ----------------------------------------------------
  * K and V as int8 codes with one f32 scale per (token, kv head): a head vector
  * x[head_dim] is held as s = max|x| / 127 (an f32 quotient; 0, and the codes 0,
- * where it is below the smallest normal f32; at most the largest f32
- * of which 127 are finite) and c = x / s rounded to the nearest
- * (halves to even) and held to +-127, and stands for c * s.  A vector with an
- * infinity or a NaN gets the scale NaN and reads as NaN.  Vector (block, layer,
+ * where it is below the smallest normal f32; at most the largest f32 of which 127 are
+ * finite) and c = x / s rounded to the nearest (halves to even) and held to +-127, and
+ * stands for c * s.  A vector with an infinity or a NaN gets the scale NaN and reads as
+ * NaN.  Vector (block, layer,
  * kv head h, slot) is number
  *   ((block * n_layers + layer) * n_kv_heads + h) * tokens_per_block + slot
  * of the codes (int8 [head_dim] each, 16-byte aligned array) and of the scales.
@@ -565,8 +565,15 @@ int32_t cellm_hip_attention_gqa_f16kv_noalloc(cellm_hip_ctx_t* ctx, const float*
  * session, the number of its tokens for a prompt.  Pages with block >= total_blocks
  * are missing: nothing is written to them and they read as zeros.  A row of position
  * < 0 is skipped, and its output left as it was (the padding of a batch of prompts).
- * head_dim 64, 128 or 256 (else CELLM_HIP_ERR_UNSUPPORTED), up to 2^20 rows, tables of
- * up to 2^30 positions, arrays of fewer than 2^32 vectors. */
+ * head_dim 64, 128 or 256 (else CELLM_HIP_ERR_UNSUPPORTED), up to 2^20 rows, 4096 kv
+ * heads and 2^25 (row, kv head) pairs, tables of up to 2^30 positions, arrays of fewer
+ * than 2^32 vectors.  Zero rows or tables are an empty call.
+ *
+ * Attention splits long contexts over blocks and adds their sums in context-owned
+ * scratch: one buffer per stream, grown on demand, or one per captured graph and stream,
+ * kept until the context is destroyed, so that graphs and eager calls may run at the same
+ * time; launches of what was made from one capture run one after the other.  The same
+ * call on the same values gives the same bits. */
 
 /* K and V [rows][n_kv_heads][head_dim] f32 into the pages of `layer` at each row's
  * position, as cellm_hip_kv_write_f16 does for f16.  The rows of one call go to
@@ -579,7 +586,7 @@ int32_t cellm_hip_kv_write_q8(cellm_hip_ctx_t* ctx, const float* k, const float*
 /* RoPE on q and k by each row's position and the K/V write in one launch, as
  * cellm_hip_rope_kv_write_f16 (the same rotation, pairs and table): q_out = RoPE(q)
  * (q_out may be q itself, and overlaps it in no other way), RoPE(k) and v quantised
- * into the pages; k is left as it was.  slots [rows], or NULL for the positions, are
+ * into the pages; k is left as it was; up to 2^28 (row, query head) pairs.  slots [rows], or NULL for the positions, are
  * the cache positions of the rows: drafted tokens stand in slots of their own behind
  * the context and are rotated by their depth.  A slot < 0 or past the table writes no
  * K and V. */
