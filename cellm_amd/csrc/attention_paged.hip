@@ -37,11 +37,11 @@
 // which knows how long every context is; the last block of a set to finish adds the others'
 // sums in split order.
 //
-// What bounds it (gfx950): decode, the reads, in part (8 sessions of 4096 to 8192 positions, 32/8 heads of 128: 28 us for 104 MB,
-// 3.7 TB/s, and one at 131072 58 us for 277 MB, 4.7, where a bare read of them takes 16.5 and 41), as 4 of 16 columns
-// are filled and V's unpacking stands beside them; short contexts, four dependent latencies a chunk and the meeting of
-// splits (9 us at 701 positions, 14/2 heads of 64); many columns, the latency of a chunk at two waves per SIMD (1024 tokens onto as
-// many, 32/8 heads of 128, 82 us: vector ALU busy 59 %, matrix units 19 %, 300 TFLOP/s of the formula's products).
+// What bounds it (gfx950).  Decode: the reads, in part (8 sessions of 4096 to 8192 positions, 32/8 heads of 128, 28 us for
+// 104 MB, 3.7 TB/s; one at 131072 58 us for 277 MB, 4.7; a bare read of them takes 16.5 and 41), as 4 of 16 columns are
+// filled and V's unpacking stands beside them.  Short contexts: four dependent latencies a chunk and the meeting of splits
+// (9 us at 701 positions, 14/2 heads of 64).  Many columns: vector instructions at two waves per SIMD (1024 tokens onto
+// as many, 32/8 heads of 128, 82 us: vector ALU busy 62 %, matrix units 20 %, 316 TFLOP/s of the formula's products).
 #include <algorithm>
 #include <cmath>
 
