@@ -1854,9 +1854,12 @@ int32_t kv_write_q8_impl(cellm_hip_ctx* ctx, const float* q, const float* k, con
                          int64_t total_blocks, int64_t n_layers, int64_t tpb, int64_t layer, void* stream)
 {
     if (int32_t rc = check_kv(rows, per, n_kv_heads, head_dim, max_blocks, total_blocks, n_layers, tpb, layer)) return rc;
-    if (n_heads < 0 || n_heads > 4096 || rows * n_heads > (1 << 28) || (cos_sin && (table_positions < 1 || table_positions > INT32_MAX)))
+    if (n_heads < 0 || n_heads > 4096 || (cos_sin && (table_positions < 1 || table_positions > INT32_MAX)))
         return set_error(CELLM_HIP_ERR_INVALID_ARG, "bad heads %lld or table_positions %lld", (long long)n_heads,
                          (long long)table_positions);
+    if (rows * (n_heads + 2 * n_kv_heads) * head_dim > (1ll << 34))  // 8 elements a thread, threads numbered in 32 bits
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "%lld rows of %lld heads of %lld: at most 2^34 elements of q, k and v a call",
+                         (long long)rows, (long long)(n_heads + 2 * n_kv_heads), (long long)head_dim);
     if (rows == 0) return CELLM_HIP_OK;
     if (!k || !v || !positions || !kcodes || !kscales || !vcodes || !vscales || !block_tables)
         return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");

@@ -203,7 +203,6 @@ struct AcceptArgs {
 
 constexpr int kPathStep = 8;  // tokens of a path in registers at a time
 
-template <typename W>
 __global__ __launch_bounds__(kThreads) void kv_accept_kernel(const AcceptArgs a)
 {
     __shared__ long long at[2][kMaxTree];  // row numbers of unit 0, source and target; -1: not moved
@@ -230,12 +229,12 @@ __global__ __launch_bounds__(kThreads) void kv_accept_kernel(const AcceptArgs a)
         at[1][i] = to;
     }
     __syncthreads();
-    const int n = count, cols = a.row / (int)sizeof(W);
+    const int n = count, cols = a.row / (int)sizeof(u4_t);
     const long long c = (long long)blockIdx.x * kThreads + t;
     const int unit = (int)(c / cols), col = (int)(c - (long long)unit * cols);
     if (unit >= a.units) return;
     for (int i0 = 0; i0 < n; i0 += kPathStep) {
-        W x[2][kPathStep];
+        u4_t x[2][kPathStep];
         float sc[2][kPathStep];
 #pragma unroll
         for (int j = 0; j < kPathStep; ++j) {
@@ -243,7 +242,7 @@ __global__ __launch_bounds__(kThreads) void kv_accept_kernel(const AcceptArgs a)
             const size_t row = from < 0 ? 0 : (size_t)from + (size_t)unit * a.tpb;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                x[w][j] = *reinterpret_cast<const W*>(a.a[w] + row * a.row + (size_t)col * sizeof(W));
+                x[w][j] = *reinterpret_cast<const u4_t*>(a.a[w] + row * a.row + (size_t)col * sizeof(u4_t));
                 if (a.s[w] && col == 0) sc[w][j] = a.s[w][row];
             }
         }
@@ -253,7 +252,7 @@ __global__ __launch_bounds__(kThreads) void kv_accept_kernel(const AcceptArgs a)
             const size_t row = (size_t)at[1][i0 + j] + (size_t)unit * a.tpb;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                *reinterpret_cast<W*>(a.a[w] + row * a.row + (size_t)col * sizeof(W)) = x[w][j];
+                *reinterpret_cast<u4_t*>(a.a[w] + row * a.row + (size_t)col * sizeof(u4_t)) = x[w][j];
                 if (a.s[w] && col == 0) a.s[w][row] = sc[w][j];
             }
         }
@@ -307,16 +306,9 @@ hipError_t launch_kv_accept(void* kc, float* ks, void* vc, float* vs, int units,
 {
     AcceptArgs a{{static_cast<unsigned char*>(kc), static_cast<unsigned char*>(vc)}, {ks, vs}, ctx, accepted, most, tree,
                  tpb, max_blocks, total_blocks, units, row_bytes, bt};
-    const auto go = [&](auto word) {
-        using W = decltype(word);
-        const long long n = (long long)units * (row_bytes / (int)sizeof(W));
-        hipLaunchKernelGGL((kv_accept_kernel<W>), dim3((unsigned)((n + kThreads - 1) / kThreads), (unsigned)tables),
-                           dim3(kThreads), 0, st, a);
-    };
-    const uintptr_t low = reinterpret_cast<uintptr_t>(kc) | reinterpret_cast<uintptr_t>(vc) | (uintptr_t)row_bytes;
-    if (low % 16 == 0) go(u4_t{});
-    else if (low % 4 == 0) go(uint32_t{});
-    else go(uint16_t{});
+    const long long n = (long long)units * (row_bytes / (int)sizeof(u4_t));  // rows are whole words: head_dim is 64 or more
+    hipLaunchKernelGGL(kv_accept_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads), (unsigned)tables), dim3(kThreads), 0,
+                       st, a);
     return hipGetLastError();
 }
 

@@ -586,7 +586,7 @@ int32_t cellm_hip_kv_write_q8(cellm_hip_ctx_t* ctx, const float* k, const float*
 /* RoPE on q and k by each row's position and the K/V write in one launch, as
  * cellm_hip_rope_kv_write_f16 (the same rotation, pairs and table): q_out = RoPE(q)
  * (q_out may be q itself, and overlaps it in no other way), RoPE(k) and v quantised
- * into the pages; k is left as it was; up to 2^28 (row, query head) pairs.  slots [rows], or NULL for the positions, are
+ * into the pages; k is left as it was; up to 2^34 elements of q, k and v together.  slots [rows], or NULL for the positions, are
  * the cache positions of the rows: drafted tokens stand in slots of their own behind
  * the context and are rotated by their depth.  A slot < 0 or past the table writes no
  * K and V. */

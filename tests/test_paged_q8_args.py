@@ -183,3 +183,11 @@ def test_host_tensors_and_rows_of_no_table_are_refused(ops, what):
         for per in (0, 3, -1):
             with pytest.raises(ValueError, match="rows_per_table"):
                 _do(ops, what, _tensors(), per)
+
+
+@pytest.mark.parametrize("bad", [dict(rows=1 << 20, nh=4096), dict(rows=1 << 20, nh=510, hd=128),
+                                 dict(rows=1 << 20, nh=63, hd=256)])
+def test_more_threads_than_a_grid_numbers_are_refused(ctx, bad):
+    args = _calls()["rope_kv_write_q8"]
+    assert _lib.load().cellm_hip_rope_kv_write_q8(ctx, *{**args, **bad}.values()) == _lib.ERR_INVALID_ARG
+    assert "2^34" in _lib.last_error()
