@@ -1825,11 +1825,11 @@ int32_t check_kv(int64_t rows, int64_t per, int64_t n_kv_heads, int64_t head_dim
     if (rows < 0 || rows > (1 << 20) || per < 1 || rows % per != 0)
         return set_error(CELLM_HIP_ERR_INVALID_ARG, "rows=%lld (up to 2^20) must be a multiple of the %lld that share a table",
                          (long long)rows, (long long)per);
-    if (n_kv_heads > 4096 || rows * n_kv_heads > (1 << 25))  // threads are numbered in 32 bits
-        return set_error(CELLM_HIP_ERR_INVALID_ARG, "%lld rows of %lld kv heads: at most 4096 heads and 2^25 vectors a call",
+    if (n_kv_heads < 1 || n_kv_heads > 4096 || rows * n_kv_heads > (1 << 25))  // threads are numbered in 32 bits
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "%lld rows of %lld kv heads: 1 to 4096 heads and 2^25 vectors a call",
                          (long long)rows, (long long)n_kv_heads);
     // vectors of one array are numbered in 32 bits, positions with room for a step past the last
-    if (n_kv_heads < 1 || max_blocks < 1 || total_blocks < 1 || n_layers < 1 || tpb < 1 || layer < 0 ||
+    if (max_blocks < 1 || total_blocks < 1 || n_layers < 1 || tpb < 1 || layer < 0 ||
         layer >= n_layers || max_blocks > (1 << 30) || tpb > (1 << 30) || max_blocks * tpb > (1 << 30) ||
         total_blocks > INT32_MAX || n_layers > INT32_MAX || n_layers * n_kv_heads > INT32_MAX ||
         n_layers * n_kv_heads * tpb > (int64_t)UINT32_MAX / total_blocks)
