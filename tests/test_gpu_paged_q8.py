@@ -601,6 +601,30 @@ def test_graphs_of_one_stream_run_at_once(ops):
             assert torch.equal(s["out"], w)
 
 
+def test_calls_of_one_graph_that_need_more_and_more(ops):
+    """A short context, then longer ones, captured one after the other: their scratch grows within the graph, whose earlier
+    nodes keep what they were given."""
+    sets = [_decode_set(s, ctx=c) for s, c in ((1, 900), (2, 4100), (3, 9000), (4, 900))]
+    want = []
+    for s in sets:
+        ops.encode_attention_q8(*s["args"])
+        torch.cuda.synchronize()
+        want.append(s["out"].clone())
+    cap, gr = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=cap):
+        for s in sets:
+            ops.encode_attention_q8(*s["args"], stream=cap)
+    for _ in range(4):
+        for s in sets:
+            s["out"].zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        for s, w in zip(sets, want):
+            assert torch.equal(s["out"], w)
+        ops.encode_attention_q8(*sets[2]["args"])
+        torch.cuda.synchronize()
+
+
 def test_calls_on_many_streams(ops):
     sets = [_decode_set(s, ctx=900 + 700 * s) for s in range(4)]
     want = []
