@@ -228,10 +228,11 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
         if (t < UNIT && p < up && si.sees(p)) {
             v = vector_at<false>(a.g, table, p, kvh);
             const float s = score(v);
-            // a range whose scores are all -inf weighs nothing beside others, and its l = NaN says that there were some
+            // a range whose scores are all -inf weighs nothing beside others, and its l = NaN says that there were some;
+            // a NaN among them (m leaves it out) has the weight NaN, which o brings to every split
             w = exp2f(__builtin_fmaf(s, kLog2e, -R));
             lt = lt + w;
-            if (part && m == -INFINITY) w = 0.0f;
+            if (part && m == -INFINITY && s == -INFINITY) w = 0.0f;
         }
         __syncthreads();
         vec[t] = v;

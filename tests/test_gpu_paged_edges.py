@@ -1,0 +1,124 @@
+"""Attention over shared pages (attention_paged.hip) where a result hangs on few positions of a split, on numbers near
+the ends of f32, or on what else runs on the stream: against plain 64-bit results.
+
+The bar is 3e-6 in the 2-norm, as for ordinary inputs: a score of size |s| <= 10 from f32 sums is off by a few 2^-24 |s|
+(6e-7 each), the exponentials by 2^-22, and the sums of weights and values by a few 2^-24.  Sizes of scores beyond that
+are equal among the positions that weigh anything, so that their rounding leaves the quotient."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import _paged as P
+
+pytestmark = pytest.mark.gpu
+
+TOL = 3e-6
+
+
+def _pages(f16, total, layers, nkv, tpb, hd, seed):
+    if not f16:
+        return P.cache_q8(total, layers, nkv, tpb, hd, seed)
+    g = torch.Generator().manual_seed(seed)
+    k, v = (torch.randn(total, layers, tpb, nkv, hd, generator=g).half() for _ in range(2))
+    return [k, None, v, None]
+
+
+def _random_tree(g, tree):
+    return P.tree_bits([-1 if j == 0 else int(torch.randint(-1, j, (1,), generator=g)) for j in range(tree)])
+
+
+def _tree_call(ops, q, cache, bt, ctx, bits, f16, **kw):
+    tables, tree, nh, hd = q.shape
+    kc, ks, vc, vs = cache
+    total, layers = kc.shape[:2]
+    tpb, nkv = (kc.shape[2], kc.shape[3]) if f16 else (kc.shape[3], kc.shape[2])
+    out = torch.full(q.shape, 7.0, device="cuda")
+    ops.encode_attention_tree(q.cuda(), kc.cuda(), vc.cuda(), bt.to(torch.int32).cuda(), ctx.to(torch.int32).cuda(),
+                              P.words_of(bits).cuda(), out, nh, nkv, hd, total, layers, tpb, 0,
+                              kscale=None if f16 else ks.cuda(), vscale=None if f16 else vs.cuda(), **kw)
+    torch.cuda.synchronize()
+    return out.cpu()
+
+
+def _attention(ops, q, cache, bt, pos, per, **kw):
+    rows, nh, hd = q.shape
+    total, layers, nkv, tpb, _ = cache[0].shape
+    out = torch.full((rows, nh, hd), 7.0, device="cuda")
+    ops.encode_attention_q8(q.cuda(), *[c.cuda() for c in cache], bt.to(torch.int32).cuda(), pos.to(torch.int32).cuda(), out,
+                            nh, nkv, hd, total, layers, tpb, 0, rows_per_table=per, **kw)
+    torch.cuda.synchronize()
+    return out.cpu()
+
+
+def _same_where_finite(got, ref):
+    """NaN in the same places, and the others near."""
+    bad = torch.isnan(ref)
+    assert torch.equal(torch.isnan(got), bad)
+    assert P.rel(got[~bad], ref[~bad]) <= TOL
+
+
+# ---- keys alone that are not finite, in a split of their own --------------------------------
+# ctx is a whole number of units (four waves of 64 or 32 positions), so that the drafted slots stand in a split of their
+# own, of which a root node sees nothing but itself
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("hd,ctx", [(64, 1024), (128, 1280), (256, 640)])
+@pytest.mark.parametrize("what", ["own slot", "a unit of the context", "NaN beside -inf"])
+def test_nan_keys_reach_every_node_that_sees_them(ops, f16, hd, ctx, what):
+    g = torch.Generator().manual_seed(hd)
+    tree, nh, nkv, tpb = 20, 6, 2, 16
+    bt = torch.randperm(ctx // tpb + 4, generator=g)[None, :ctx // tpb + 2]
+    cache = _pages(f16, ctx // tpb + 4, 1, nkv, tpb, hd, 37)
+    q = torch.randn(1, tree, nh, hd, generator=g)
+    q[..., 0] = q[..., 0].abs() + 0.1
+    bits = _random_tree(g, tree)[None]
+    bits[0, :, 7] = False
+    bits[0, 7] = False
+    bits[0, 7, 7] = True  # a root that no other node sees
+    at = dict(zip(["own slot", "a unit of the context", "NaN beside -inf"],
+                  [[ctx + 7], range(256, 512), [ctx + 7]]))[what]
+    for p in at:
+        blk, sl = int(bt[0, p // tpb]), p % tpb
+        if f16:
+            cache[0][blk, 0, sl] = math.nan
+        else:
+            cache[1][blk, 0, :, sl] = math.nan
+    if what == "NaN beside -inf" and f16:  # the root sees -inf scores in its split too
+        bits[0, 7, 8:12] = True
+        for p in range(ctx + 8, ctx + 12):
+            cache[0][int(bt[0, p // tpb]), 0, p % tpb, :, 0] = -math.inf
+    ref = P.tree(q, *cache, bt, torch.tensor([ctx]), bits, 0)
+    assert bool(torch.isnan(ref[0, 7]).all())
+    got = _tree_call(ops, q, cache, bt, torch.tensor([ctx]), bits, f16)
+    if what == "a unit of the context":
+        assert bool(torch.isnan(got).all())
+    else:
+        _same_where_finite(got, ref)
+
+
+@pytest.mark.parametrize("hd,ctx", [(64, 1024), (128, 1280), (256, 640)])
+def test_keys_of_minus_infinity_weigh_nothing(ops, hd, ctx):
+    """Units of the context and the drafted slots whose scores are all -inf, beside others; and nothing but those."""
+    g = torch.Generator().manual_seed(hd + 1)
+    tree, nh, nkv, tpb = 20, 6, 2, 16
+    bt = torch.randperm(ctx // tpb + 4, generator=g)[None, :ctx // tpb + 2]
+    cache = _pages(True, ctx // tpb + 4, 1, nkv, tpb, hd, 39)
+    q = torch.randn(1, tree, nh, hd, generator=g)
+    q[..., 0] = q[..., 0].abs() + 0.1
+    bits = _random_tree(g, tree)[None]
+
+    def spoil(positions):
+        for p in positions:
+            cache[0][int(bt[0, p // tpb]), 0, p % tpb, :, 0] = -math.inf
+
+    spoil([*range(256, 512), *range(ctx, ctx + tree)])
+    ref = P.tree(q, *cache, bt, torch.tensor([ctx]), bits, 0)
+    assert bool(torch.isfinite(ref).all())
+    _same_where_finite(_tree_call(ops, q, cache, bt, torch.tensor([ctx]), bits, True), ref)
+    spoil(range(ctx))
+    assert bool(torch.isnan(_tree_call(ops, q, cache, bt, torch.tensor([ctx]), bits, True)).all())
