@@ -190,14 +190,13 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
     const float* qr = a.q + ((size_t)row * a.n_heads + head) * HD;
     const auto score = [&](long long v) {
         float d = 0.0f;
-        if (v >= 0) {
-            const u4_t* src = reinterpret_cast<const u4_t*>(static_cast<const uint16_t*>(a.kc) + v * HD);
+        const u4_t* src = reinterpret_cast<const u4_t*>(static_cast<const uint16_t*>(a.kc) + v * HD);
 #pragma unroll 1
-            for (int i = 0; i < HD / 8; ++i) {
-                const h8_t w = __builtin_bit_cast(h8_t, src[i]);
+        for (int i = 0; i < HD / 8; ++i) {
+            // a missing page counts as zeros, of which an element of q that is not finite makes NaN
+            const h8_t w = __builtin_bit_cast(h8_t, v >= 0 ? src[i] : u4_t{0, 0, 0, 0});
 #pragma unroll
-                for (int j = 0; j < 8; ++j) d = d + qr[8 * i + j] * (float)w[j];
-            }
+            for (int j = 0; j < 8; ++j) d = d + qr[8 * i + j] * (float)w[j];
         }
         return capped(a, d * a.scale);
     };
@@ -240,7 +239,7 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
         __syncthreads();
 #pragma unroll 1
         for (int j = t / HD; j < min(UNIT, up - p0); j += NP)
-            if (vec[j] >= 0) o = o + ws[j] * (float)static_cast<const _Float16*>(a.vc)[vec[j] * HD + d];
+            o = o + ws[j] * (vec[j] >= 0 ? (float)static_cast<const _Float16*>(a.vc)[vec[j] * HD + d] : 0.0f);
     }
     l = reduce(lt, [](float x, float y) { return x + y; });
     __syncthreads();

@@ -122,3 +122,29 @@ def test_keys_of_minus_infinity_weigh_nothing(ops, hd, ctx):
     _same_where_finite(_tree_call(ops, q, cache, bt, torch.tensor([ctx]), bits, True), ref)
     spoil(range(ctx))
     assert bool(torch.isnan(_tree_call(ops, q, cache, bt, torch.tensor([ctx]), bits, True)).all())
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("hd,ctx", [(64, 60), (64, 1024), (256, 640)])
+@pytest.mark.parametrize("some", [True, False])
+def test_queries_that_are_not_finite_over_missing_pages(ops, f16, hd, ctx, some):
+    """A missing page is zeros, so a q with an infinity or a NaN has the score NaN there: its row is NaN, where some
+    pages are missing and its other scores are -inf, and where all are."""
+    g = torch.Generator().manual_seed(hd + 2)
+    tree, nh, nkv, tpb = 12, 4, 2, 16
+    bt = torch.randperm(ctx // tpb + 4, generator=g)[None, :ctx // tpb + 2]
+    bt[0, (1 if some else slice(None))] = -1
+    cache = _pages(f16, ctx // tpb + 4, 1, nkv, tpb, hd, 41)
+    cache[0][..., 3] = -cache[0][..., 3].abs().clamp(min=1)
+    q = torch.randn(1, tree, nh, hd, generator=g)
+    bits = _random_tree(g, tree)[None]
+    clean = P.tree(q, *cache, bt, torch.tensor([ctx]), bits, 0)
+    q[0, 2, 1, 3], q[0, 5, 2, 3] = math.inf, math.nan
+    got = _tree_call(ops, q, cache, bt, torch.tensor([ctx]), bits, f16)
+    bad = torch.zeros(1, tree, nh, dtype=torch.bool)
+    bad[0, 2, 1] = bad[0, 5, 2] = True
+    assert bool(torch.isnan(got[bad]).all())
+    if some:
+        assert P.rel(got[~bad], clean[~bad]) <= TOL
+    else:
+        assert bool((got[~bad] == 0).all())
