@@ -368,10 +368,17 @@ __device__ __forceinline__ void pairs_of_codes(uint32_t a, uint32_t b, uint32_t 
     o[3] = as_u32(__builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(b, a, 0x0C070C03u)), up, off));
 }
 
-// q's parts of the column `some`, the B operands of the scores, and the scale that is left out of them.
+// The sums of q's integers reach 2^37, so scales of keys near the end of f32 would take them past it before the scale of a
+// tiny q brings them back: in a chunk that has a scale above kHugeKey all are taken 2^kHugeShift times smaller, and the
+// column's scale as much larger.
+constexpr float kHugeKey = 0x1p80f;
+constexpr int kHugeShift = 40;
+
+// q's parts of a column, the B operands of the scores, and the scale that is left out of them: for scales of the keys as
+// they are and, of 8-bit pages, for those of a chunk with huge ones (kHugeKey).
 template <bool Q8, int HD>
 __device__ __forceinline__ void q_parts(const PagedAttnArgs& a, const f4_t (&qf)[Shape<Q8, HD>::KK][Shape<Q8, HD>::NE / 4],
-                                        u4_t (&d)[Shape<Q8, HD>::KK][Shape<Q8, HD>::QP], float& qsc)
+                                        u4_t (&d)[Shape<Q8, HD>::KK][Shape<Q8, HD>::QP], float (&qsc)[2])
 {
     using S = Shape<Q8, HD>;
     uint32_t mx = 0;  // |q| in the order of its bits; f16 pages: of the finite ones
@@ -388,7 +395,8 @@ __device__ __forceinline__ void q_parts(const PagedAttnArgs& a, const f4_t (&qf)
     const int top = max((int)(mx >> 23), 1) - 127;
     const bool bad = Q8 && mx >= 0x7F800000u;
     const int e = mx > 0 && !bad ? (Q8 ? 21 : 13) - top : 0;
-    qsc = bad ? __builtin_nanf("") : ldexpf(a.scale, -e);
+    qsc[0] = bad ? __builtin_nanf("") : ldexpf(a.scale, -e);
+    qsc[1] = Q8 ? (bad ? __builtin_nanf("") : ldexpf(a.scale, kHugeShift - e)) : 0.0f;
 #pragma unroll
     for (int kk = 0; kk < S::KK; ++kk) {
         if constexpr (Q8) {
@@ -681,7 +689,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     __shared__ __align__(16) u4_t qlds[kQInLds ? CT * KK * QP * 64 : 1];
     __shared__ __align__(16) uint32_t kidx[kWaves][CH], vidx[kWaves][CH];  // [c][tile], [g][j]
     __shared__ __align__(16) float kscl[kWaves][Q8 ? CH : 4], vscl[kWaves][Q8 ? CH : 4];
-    __shared__ float ml[kWaves][2][COLS], lsum[COLS], qs_lds[COLS];
+    __shared__ float ml[kWaves][2][COLS], lsum[COLS], qs_lds[2][COLS];
     __shared__ uint32_t flags, here;
     __shared__ int last;
 
@@ -704,7 +712,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     bool has[CT];
     size_t at[CT];             // of the column in q and out
     u4_t qp[CT][KK][QP];
-    float qsc[CT], cs[CT];     // scale of the sums of q's parts, and of the exponents
+    float qsc[CT][2];          // scale of the sums of q's parts
     Sums<DT> m[CT];
     // with q's parts in LDS wave u makes those of the columns 16 u + c
     const auto makes = [&](int u) { return !kQInLds || wave == u; };
@@ -744,16 +752,27 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                 for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
                     for (int p = 0; p < QP; ++p) qlds[((u * KK + kk) * QP + p) * 64 + lane] = qp[u][kk][p];
-                if (g4 == 0) qs_lds[kCols * u + c] = qsc[u];
+                if (g4 == 0) {
+                    qs_lds[0][kCols * u + c] = qsc[u][0];
+                    qs_lds[1][kCols * u + c] = qsc[u][1];
+                }
             }
         }
         if constexpr (kQInLds) {
             __syncthreads();
 #pragma unroll
-            for (int u = 0; u < CT; ++u) qsc[u] = qs_lds[kCols * u + c];
+            for (int u = 0; u < CT; ++u) {
+                qsc[u][0] = qs_lds[0][kCols * u + c];
+                qsc[u][1] = qs_lds[1][kCols * u + c];
+            }
         }
+        if constexpr (!CAP) {  // and of the exponents
 #pragma unroll
-        for (int u = 0; u < CT; ++u) cs[u] = CAP ? kLog2e : qsc[u] * kLog2e;
+            for (int u = 0; u < CT; ++u) {
+                qsc[u][0] = qsc[u][0] * kLog2e;
+                qsc[u][1] = qsc[u][1] * kLog2e;
+            }
+        }
     }
     const auto q_part = [&](int u, int p, int kk) {
         if constexpr (kQInLds) return qlds[((u * KK + kk) * QP + p) * 64 + lane];
@@ -837,7 +856,10 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     }
     for (; p0 < k.hi; p0 += step) {
         miss = miss_next;
+        bool huge = false;
         if constexpr (Q8) {
+            huge = __ballot(ks_own > kHugeKey) != 0;
+            if (huge) ks_own = ldexpf(ks_own, -kHugeShift);
             if (lane < CH) {
                 const int tile = lane >> 4, i = lane >> 2 & 3, g = lane & 3;
                 const bool gone = miss >> lane & 1;  // a missing page counts as zeros
@@ -886,9 +908,11 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                 }
             }
             if (u == CT - 1) load_k();
+            float cs = huge ? qsc[u][1] : qsc[u][0];
             if constexpr (CAP) {
 #pragma unroll
-                for (int j = 0; j < NP; ++j) s[j] = capped(a, s[j] * qsc[u]);
+                for (int j = 0; j < NP; ++j) s[j] = capped(a, s[j] * cs);
+                cs = kLog2e;
             }
             // ---- weights; of positions that some column does not see, those are 0 whatever they hold
             float vs[NP];
@@ -901,7 +925,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
 #pragma unroll
                 for (int j = 0; j < NP; ++j) vs[j] = vis >> (4 * j) & 1 ? vs[j] : 0.0f;
             }
-            weigh<Q8>(s, cs[u], vs, partial, vis, coarse, m[u], ph[u], pl[u]);
+            weigh<Q8>(s, cs, vs, partial, vis, coarse, m[u], ph[u], pl[u]);
         }
         // ---- O^T += V^T . P^T
         if (!Q8 && miss) {

@@ -148,3 +148,25 @@ def test_queries_that_are_not_finite_over_missing_pages(ops, f16, hd, ctx, some)
         assert P.rel(got[~bad], clean[~bad]) <= TOL
     else:
         assert bool((got[~bad] == 0).all())
+
+
+# ---- numbers near the ends of f32 ---------------------------------------------------------
+
+
+@pytest.mark.parametrize("hd,ctx", [(64, 701), (128, 2500), (256, 1300)])
+@pytest.mark.parametrize("keys,queries", [(1e34, 1e-34), (1e-34, 1e34), (1e36, 1e-36), (1e-36, 1e36), (1e32, 1e-20)])
+@pytest.mark.parametrize("kw", [{}, dict(soft_cap=5.0)])
+def test_scores_in_range_of_keys_and_queries_that_are_not(ops, hd, ctx, keys, queries, kw):
+    """Keys of 1e34 against queries of 1e-34 have ordinary scores, and so the other way round; scores of 1e12 are finite
+    too, and the largest takes all the weight."""
+    g = torch.Generator().manual_seed(ctx)
+    nh, nkv, tpb = 6, 2, 16
+    bt = torch.randperm(-(-ctx // tpb) + 1, generator=g)[None, :-(-ctx // tpb)]
+    cache = P.cache_q8(bt.shape[1] + 1, 1, nkv, tpb, hd, 43)
+    cache[1] *= keys
+    q = torch.randn(1, nh, hd, generator=g) * 1.2
+    q = (q / q.abs().max() * 3).mul(queries)
+    assert bool(torch.isfinite(q).all())
+    ref = P.causal(q, *cache, bt, torch.tensor([ctx - 1]), 0, 1, cap=kw.get("soft_cap", 0.0))
+    got = _attention(ops, q, cache, bt, torch.tensor([ctx - 1]), 1, **kw)
+    assert bool(torch.isfinite(got).all()) and P.rel(got, ref) <= TOL
