@@ -437,7 +437,7 @@ struct Sums {
 };
 
 // Scores s of NP positions (bit 4 j of vis: position j is seen; `partial`: not all are, in some column) and their scales
-// vs to the weights' two f16 parts, and into l; the reference is raised where products pass 2^15.
+// vs to the weights' two f16 parts, and into l; the reference is raised where products pass 2^15 (or weights 2^80).
 template <bool Q8, int NP, int DT>
 __device__ __forceinline__ void weigh(const float (&s)[NP], float cs, const float (&vs)[NP], bool partial, uint64_t vis, bool& coarse,
                                       Sums<DT>& m, h8_t (&ph)[NP / 8], h8_t (&pl)[NP / 8])
@@ -466,31 +466,39 @@ __device__ __forceinline__ void weigh(const float (&s)[NP], float cs, const floa
         }
     };
     weights();
-    if (__ballot(mx > 0x1p15f || lc > 0x1p100f)) {
-        // the reference that leaves the largest product at 2^13 (and weights of small s_v below 2^90)
+    if (__ballot(mx > 0x1p15f || lc > 0x1p80f)) {
+        // The reference that leaves the largest product at 2^13.  8-bit pages: not so far from the largest score that a
+        // sum of weights under another reference (of another wave or split, or this one so far) would leave f32 beside
+        // it; what the scales of the values then miss of 2^13, and what a reference beyond 2^20 has no bits for, F makes up.
         float m1 = -INFINITY, m2 = -INFINITY;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const float h = vis >> (4 * j) & 1 ? s[j] * cs : -INFINITY;
             m1 = fmaxf(m1, h);
-            m2 = fmaxf(m2, Q8 ? h + __builtin_amdgcn_logf(vs[j]) : h);
+            if constexpr (Q8) m2 = fmaxf(m2, h + __builtin_amdgcn_logf(vs[j]));
         }
         m1 = fmaxf(m1, lane_xor<16>(m1, 64));
         m1 = fmaxf(m1, lane_xor<32>(m1, 64));
-        m2 = fmaxf(m2, lane_xor<16>(m2, 64));
-        m2 = fmaxf(m2, lane_xor<32>(m2, 64));
-        const float up = fmaxf(m.R, fmaxf(m2 - 13.0f, m1 - 90.0f));
+        if constexpr (Q8) {
+            m2 = fmaxf(m2, lane_xor<16>(m2, 64));
+            m2 = fmaxf(m2, lane_xor<32>(m2, 64));
+        }
+        const float up = fmaxf(m.R, Q8 ? fminf(fmaxf(m2 - 13.0f, m1 - 60.0f), m1 + 30.0f) : m1 - 13.0f);
         float ratio = up > m.R ? __builtin_amdgcn_exp2f(m.R - up) : 1.0f;  // from -inf: 0, as l and O are
-        m.R = up;
         m.l = m.l * ratio;
         if constexpr (Q8) {
-            // beyond 2^20 a reference has no bits for the 13: the products are scaled down instead
-            const float over = m2 - up;
-            const float f = over > 15.0f && over < 1000.0f ? fminf(m.F, __builtin_amdgcn_exp2f(13.0f - rintf(over))) : m.F;
-            ratio = ratio * (f / m.F);
-            m.F = f;
-            coarse = coarse || __ballot(f != 1.0f) != 0;
+            const float over = m2 - up;  // NaN: nothing is seen here, nor was before
+            if (over < 1000.0f) {
+                const float want = __builtin_amdgcn_exp2f(fminf(fmaxf(13.0f - rintf(over), -100.0f), 100.0f));
+                // up by as much as R rose at most: what O holds is not to pass its bound
+                const float most = up > m.R ? m.F * __builtin_amdgcn_exp2f(up - m.R) : m.F;
+                const float f = m.F > 4.0f * want ? want : fminf(fmaxf(m.F, want), most);
+                if (ratio > 0.0f) ratio = ratio * (f / m.F);
+                m.F = f;
+            }
+            coarse = coarse || __ballot(m.F != 1.0f) != 0;
         }
+        m.R = up;
 #pragma unroll
         for (int e = 0; e < DT; ++e) m.o[e] = m.o[e] * ratio;
         weights();

@@ -170,3 +170,43 @@ def test_scores_in_range_of_keys_and_queries_that_are_not(ops, hd, ctx, keys, qu
     ref = P.causal(q, *cache, bt, torch.tensor([ctx - 1]), 0, 1, cap=kw.get("soft_cap", 0.0))
     got = _attention(ops, q, cache, bt, torch.tensor([ctx - 1]), 1, **kw)
     assert bool(torch.isfinite(got).all()) and P.rel(got, ref) <= TOL
+
+
+def _values_of_size(order, nv, tpb, hd, g):
+    """One table of 8-bit pages whose keys are 127 s in their first element, zero elsewhere: a query of 1 there scores
+    127 s / sqrt(hd).  order: (positions, score, size of the values) in turn; a size of 0: zero scales."""
+    n = sum(o[0] for o in order)
+    pages = -(-n // tpb)
+    bt = torch.randperm(pages + 1, generator=g)[None, :pages]
+    kc, ks, vc, vs = P.cache_q8(pages + 1, 1, nv, tpb, hd, 53)
+    kc.zero_()
+    kc[..., 0] = 127
+    p = 0
+    for count, score, size in order:
+        for i in range(p, p + count):
+            at = (int(bt[0, i // tpb]), 0, slice(None), i % tpb)
+            ks[at] = score * math.sqrt(hd) / 127
+            vs[at] *= size
+        p += count
+    return (kc, ks, vc, vs), bt, n
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("order", [
+    [(700, 0.0, 1e-32)], [(1500, 0.0, 1e-36)], [(1, 0.0, 1e-34)],
+    [(600, 0.0, 0.0), (600, 0.0, 1e-33)],                # zeros first
+    [(900, 0.0, 1.0), (900, 80.0, 1e-32)],               # small values of a weight e^80 times that of the others
+    [(900, 80.0, 1e-32), (900, 0.0, 1.0)],
+    [(64, 80.0, 1e-32), (64, 0.0, 1.0)] * 12, [(64, 0.0, 1e-30), (64, 0.0, 1e-10), (64, 0.0, 1e5)] * 3,
+    [(64, 0.0, 1e5), (64, 0.0, 0.0), (64, 0.0, 1e-34)] * 5, [(64, 0.0, 1e33), (64, 0.0, 1e-34)] * 4, [(300, 0.0, 1e33), (300, 0.0, 1e-34)],
+    [(64, 0.0, 1e3), (64, 85.0, 1e-30)] * 5])
+def test_small_values_keep_their_bits(ops, hd, order):
+    """Values whose scales the cache holds exactly, down to the smallest: the quotient is as near as that of ordinary
+    ones, with large values, zeros and other weights before and behind."""
+    g = torch.Generator().manual_seed(len(order))
+    cache, bt, n = _values_of_size(order, 1, 16, hd, g)
+    q = torch.zeros(1, 2, hd)
+    q[..., 0] = 1.0
+    ref = P.causal(q, *cache, bt, torch.tensor([n - 1]), 0, 1)
+    got = _attention(ops, q, cache, bt, torch.tensor([n - 1]), 1)
+    assert P.rel(got, ref) <= TOL
