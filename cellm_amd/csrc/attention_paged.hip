@@ -139,8 +139,8 @@ __device__ __forceinline__ bool sight_of(const PagedAttnArgs& a, int cap, int ta
     for (int w = 0; w < a.words; ++w) nodes += __popcll(tree_word(a, s.bits, w));
     s.ctx = min(c, cap);
     s.end = min(s.ctx + a.per, cap);
-    // the node stands at position ctx + nodes - 1 (its ancestors and itself)
-    s.start = a.window > 0 ? max(s.ctx + nodes - a.window, 0) : 0;
+    // the node stands at position c + nodes - 1 (its ancestors and itself), in the table or past it; window >= nodes
+    s.start = a.window > 0 ? max(max(c, 0) + (nodes - a.window), 0) : 0;
     return c >= 0 && nodes > 0;
 }
 
@@ -263,7 +263,7 @@ __device__ __forceinline__ bool set_range(const MmaArgs& A, int set, int& lo, in
         const int c = a.pos[table], ctx = min(c, A.cap);
         if (c < 0) return false;
         hi = min(ctx + a.per, A.cap);
-        lo = a.window > 0 ? min(max(ctx + 1 - a.window, 0), hi - 1) : 0;  // a position at least: rows that see none get zeros
+        lo = a.window > 0 ? min(max(c - a.window + 1, 0), hi - 1) : 0;  // a position at least: rows that see none get zeros
         return true;
     }
     const int j1 = min(a.per - 1, (c0 + A.cols - 1) / A.group);

@@ -210,3 +210,35 @@ def test_small_values_keep_their_bits(ops, hd, order):
     ref = P.causal(q, *cache, bt, torch.tensor([n - 1]), 0, 1)
     got = _attention(ops, q, cache, bt, torch.tensor([n - 1]), 1)
     assert P.rel(got, ref) <= TOL
+
+
+# ---- a window behind a context that is longer than the table -------------------------------------
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("tables,hd", [(7, 64), (7, 256), (70, 128)])  # the last: 32 columns at a time
+def test_windows_of_contexts_past_the_table(ops, f16, tables, hd):
+    """A node sees the positions above context + nodes - 1 - window that the table has, which may be none."""
+    g = torch.Generator().manual_seed(61)
+    tree, nh, nkv, tpb, pages, window = 9, 8, 2, 16, 5, 40
+    room = pages * tpb
+    bt = torch.randperm(tables * pages + 1, generator=g)[:tables * pages].view(tables, pages)
+    cache = _pages(f16, tables * pages + 1, 1, nkv, tpb, hd, 59)
+    q = torch.randn(tables, tree, nh, hd, generator=g)
+    ctx = torch.tensor([room - 4, room, room + 7, room + 29, room + 33, room + 200, 2**31 - 1] * (tables // 7))
+    bits = np.stack([_random_tree(g, tree) for _ in range(tables)])
+    got = _tree_call(ops, q, cache, bt, ctx, bits, f16, window=window)
+    ref = torch.zeros(q.shape, dtype=torch.float64)
+    at = torch.arange(room)
+    for t in range(tables):
+        k, v = (P.gather(c, s, bt[t], 0, range(room), cache[0].shape[0], tpb) for c, s in (cache[:2], cache[2:]))
+        for j in range(tree):
+            c = int(ctx[t])
+            sees = (at < c) & (at > c + int(bits[t, j].sum()) - 1 - window)
+            for i in range(tree):
+                if bits[t, j, i] and c + i < room:
+                    sees[c + i] = True
+            ref[t, j] = P.attend(q[t, j], k, v, sees)
+    none = (ref == 0).all(-1)
+    assert bool(none.any()) and bool((got[none] == 0).all())
+    assert P.rel(got, ref) <= TOL
