@@ -487,16 +487,18 @@ __device__ __forceinline__ void weigh(const float (&s)[NP], float cs, const floa
         float ratio = up > m.R ? __builtin_amdgcn_exp2f(m.R - up) : 1.0f;  // from -inf: 0, as l and O are
         m.l = m.l * ratio;
         if constexpr (Q8) {
-            const float over = m2 - up;  // NaN: nothing is seen here, nor was before
-            if (over < 1000.0f) {
-                const float want = __builtin_amdgcn_exp2f(fminf(fmaxf(13.0f - rintf(over), -100.0f), 100.0f));
-                // up by as much as R rose at most: what O holds is not to pass its bound
-                const float most = up > m.R ? m.F * __builtin_amdgcn_exp2f(up - m.R) : m.F;
-                const float f = m.F > 4.0f * want ? want : fminf(fmaxf(m.F, want), most);
-                if (ratio > 0.0f) ratio = ratio * (f / m.F);
-                m.F = f;
+            const float over = m2 - up;  // the largest product; NaN: nothing is seen here, nor was before
+            if (coarse || __ballot(over > 15.0f || (up > m.R && over < 12.0f))) {
+                if (over < 1000.0f) {
+                    const float want = __builtin_amdgcn_exp2f(fminf(fmaxf(13.0f - rintf(over), -100.0f), 100.0f));
+                    // up by as much as R rose at most: what O holds is not to pass its bound
+                    const float most = up > m.R ? m.F * __builtin_amdgcn_exp2f(up - m.R) : m.F;
+                    const float f = m.F > 4.0f * want ? want : fminf(fmaxf(m.F, want), most);
+                    if (ratio > 0.0f) ratio = ratio * (f / m.F);
+                    m.F = f;
+                }
+                coarse = coarse || __ballot(m.F != 1.0f) != 0;
             }
-            coarse = coarse || __ballot(m.F != 1.0f) != 0;
         }
         m.R = up;
 #pragma unroll
