@@ -172,6 +172,25 @@ def test_scores_in_range_of_keys_and_queries_that_are_not(ops, hd, ctx, keys, qu
     assert bool(torch.isfinite(got).all()) and P.rel(got, ref) <= TOL
 
 
+@pytest.mark.parametrize("hd,nh,nkv,ctx,rows", [(64, 14, 2, 300, 1), (128, 8, 2, 2500, 1), (256, 4, 1, 600, 1),
+                                                (64, 32, 8, 400, 300), (128, 32, 8, 400, 300)])
+def test_a_loud_element_of_q_leaves_the_others_their_bits(ops, hd, nh, nkv, ctx, rows):
+    """One element of q 300 times the others where the keys hold zeros: the scores come from the others alone.  They are
+    integers of 2^-29 of the largest's power of two, some 1000: a rounding of 0.29 * 2^-29 * 1000 = 5.4e-7 (rms) each, and
+    as much of a score of keys of size 1."""
+    g = torch.Generator().manual_seed(hd)
+    tpb = 16
+    bt = torch.randperm(-(-ctx // tpb) + 1, generator=g)[None, :-(-ctx // tpb)]
+    cache = P.cache_q8(bt.shape[1] + 1, 1, nkv, tpb, hd, 47)
+    cache[0][..., 5] = 0
+    q = torch.randn(rows, nh, hd, generator=g) * 1.2
+    q[..., 5] *= 300.0
+    pos = torch.arange(ctx - rows, ctx)
+    some = sorted({0, rows // 2, rows - 1})
+    ref = torch.cat([P.causal(q[r:r + 1], *cache, bt, pos[r:r + 1], 0, 1) for r in some])
+    assert P.rel(_attention(ops, q, cache, bt, pos, rows)[some], ref) <= TOL
+
+
 def _values_of_size(order, nv, tpb, hd, g):
     """One table of 8-bit pages whose keys are 127 s in their first element, zero elsewhere: a query of 1 there scores
     127 s / sqrt(hd).  order: (positions, score, size of the values) in turn; a size of 0: zero scales."""
