@@ -105,6 +105,7 @@ struct cellm_hip_ctx {
     std::unordered_map<hipStream_t, DeviceBuffer> aux;         // unfused gate/up: the up rows, one per stream
     std::unordered_map<hipStream_t, DeviceBuffer> attn;        // split-sequence attention partials, one per stream
     std::unordered_map<hipStream_t, DeviceBuffer> argmax;      // argmax row counters + chunk partials, one per stream
+    std::unordered_map<hipStream_t, DeviceBuffer> paged;       // attention over shared pages: eager calls' counters + sums, one per stream
     std::map<std::pair<unsigned long long, hipStream_t>, DeviceBuffer> graph_scratch;  // one per capture and stream
     std::vector<void*> retired;                                // outgrown scratch that captured graphs still write to
     float* attn_static = nullptr;  // this device's static attention scratch (cellm_hip_attention_gqa_f16kv_noalloc)
@@ -700,7 +701,7 @@ void cellm_hip_destroy(cellm_hip_ctx_t* ctx)
     if (!ctx) return;
     DeviceGuard g(ctx->device);
     if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
-    for (auto* map : {&ctx->workspaces, &ctx->aux, &ctx->attn, &ctx->argmax})
+    for (auto* map : {&ctx->workspaces, &ctx->aux, &ctx->attn, &ctx->argmax, &ctx->paged})
         for (auto& kv : *map) {
             (void)hipStreamSynchronize(kv.first);
             if (kv.second.ptr) (void)hipFree(kv.second.ptr);
@@ -1774,9 +1775,10 @@ int32_t cellm_hip_argmax_f32_keys(cellm_hip_ctx_t* ctx, const float* logits, int
 namespace {
 
 // Scratch of a call that its kernel leaves as it found it in its first zero_prefix bytes (zero): the stream's
-// attention scratch, or, under a capture, scratch of that graph's own, so that graphs captured on one stream may
-// run at once and beside eager calls.  It lasts as long as the context, as the graph may.  The caller holds ctx->mu
-// until the kernel is enqueued.
+// scratch of these calls (not ctx->attn, which graphs of cellm_hip_attention_gqa_f16kv on that stream hold), or,
+// under a capture, scratch of that graph's own, so that graphs captured on one stream may run at once and beside
+// eager calls.  It lasts as long as the context, as the graph may.  The caller holds ctx->mu until the kernel is
+// enqueued.
 int32_t get_graph_safe_scratch(cellm_hip_ctx* ctx, hipStream_t st, size_t need, float** out, size_t zero_prefix)
 {
     *out = nullptr;
@@ -1787,7 +1789,7 @@ int32_t get_graph_safe_scratch(cellm_hip_ctx* ctx, hipStream_t st, size_t need, 
         (void)hipGetLastError();
         status = hipStreamCaptureStatusNone;
     }
-    if (status == hipStreamCaptureStatusNone) return get_stream_buffer(ctx, ctx->attn, st, need, out, zero_prefix);
+    if (status == hipStreamCaptureStatusNone) return get_stream_buffer(ctx, ctx->paged, st, need, out, zero_prefix);
     if (status != hipStreamCaptureStatusActive) return set_error(CELLM_HIP_ERR_DEVICE, "the stream's capture is invalid");
     DeviceBuffer& b = ctx->graph_scratch[{id, st}];
     if (b.bytes < need) {

@@ -261,3 +261,82 @@ def test_windows_of_contexts_past_the_table(ops, f16, tables, hd):
     none = (ref == 0).all(-1)
     assert bool(none.any()) and bool((got[none] == 0).all())
     assert P.rel(got, ref) <= TOL
+
+
+# ---- beside graphs of the f16 cache's attention -----------------------------------------------------
+
+
+def _f16_set(seed, ctx=4000):
+    """Four sessions of the f16 cache whose positions cellm_hip_attention_gqa_f16kv splits."""
+    g = torch.Generator().manual_seed(seed)
+    tables, nh, nkv, hd, tpb = 4, 8, 2, 64, 16
+    pages = -(-ctx // tpb)
+    kc, vc = (torch.randn(tables * pages, 1, tpb, nkv, hd, generator=g).half().cuda() for _ in range(2))
+    bt = torch.randperm(tables * pages, generator=g).view(tables, pages).to(torch.int32).cuda()
+    q = torch.randn(tables, nh, hd, generator=g).cuda()
+    pos = torch.randint(ctx // 2, ctx, (tables,), generator=g).to(torch.int32).cuda()
+    out = torch.zeros_like(q)
+    return dict(args=(q, kc, vc, bt, pos, out, nh, nkv, hd, tables * pages, 1, tpb, 0), out=out)
+
+
+def _q8_set(seed, ctx=3000, hd=64):
+    g = torch.Generator().manual_seed(seed)
+    tables, nh, nkv, tpb = 3, 4, 2, 16
+    pages = -(-ctx // tpb)
+    bt = torch.randperm(tables * pages + 1, generator=g)[:tables * pages].view(tables, pages)
+    cache = [c.cuda() for c in P.cache_q8(tables * pages + 1, 1, nkv, tpb, hd, seed)]
+    q = torch.randn(tables, nh, hd, generator=g).cuda()
+    pos = torch.randint(ctx // 2, ctx, (tables,), generator=g).to(torch.int32).cuda()
+    out = torch.zeros_like(q)
+    return dict(args=(q, *cache, bt.to(torch.int32).cuda(), pos, out, nh, nkv, hd, tables * pages + 1, 1, tpb, 0), out=out)
+
+
+def _results(calls):
+    out = []
+    for call, s in calls:
+        call(*s["args"])
+        torch.cuda.synchronize()
+        out.append(s["out"].clone())
+        s["out"].zero_()
+    return out
+
+
+def test_eager_calls_have_scratch_that_no_graph_of_the_f16_cache_holds():
+    """The scratch that an f16 call left on a stream, and a graph of that stream may hold, is not what an 8-bit call there
+    uses: the free memory tells."""
+    from cellm_amd import HipOps
+
+    side, f16, q8 = torch.cuda.Stream(), _f16_set(1, 30000), _q8_set(2, hd=256)
+    with HipOps(0) as own:
+        own.encode_attention_q8(*q8["args"])  # the kernel's module is loaded, another stream's scratch taken
+        own.encode_attention(*f16["args"], stream=side)
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        own.encode_attention_q8(*q8["args"], stream=side)  # 64 KiB and some 250 splits of 16 x 258 floats
+        torch.cuda.synchronize()
+        assert before - torch.cuda.mem_get_info()[0] >= 2**21
+
+
+def test_graphs_of_the_f16_cache_run_beside_eager_calls_of_their_stream(ops):
+    """A graph of the f16 cache's attention replayed on one stream while 8-bit calls and trees run on the stream that it
+    was captured on: each has its own result."""
+    f16, q8 = _f16_set(3), [_q8_set(s) for s in (4, 5)]
+    want_f16, *want_q8 = _results([(ops.encode_attention, f16), *((ops.encode_attention_q8, s) for s in q8)])
+    cap, other, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    ops.encode_attention(*f16["args"], stream=cap)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=cap):
+        for _ in range(20):
+            ops.encode_attention(*f16["args"], stream=cap)
+    for _ in range(6):
+        for s in (f16, *q8):
+            s["out"].zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            graph.replay()
+        for _ in range(10):
+            for s in q8:
+                ops.encode_attention_q8(*s["args"], stream=cap)
+        torch.cuda.synchronize()
+        for s, w in zip((f16, *q8), (want_f16, *want_q8)):
+            assert torch.equal(s["out"], w)
