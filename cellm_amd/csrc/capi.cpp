@@ -210,8 +210,9 @@ struct RelaxedCapture {
 // every kernel that uses the buffer is enqueued: calls on one stream then
 // queue their scratch users back to back, and a grow (which waits for the
 // stream, then frees) cannot happen between a get and its launches.
-// A buffer that was handed to a capture is never freed before the context is:
-// the graph writes to it on every replay, so a grow sets it aside.  A capture
+// A buffer that was handed to a capture is not freed before the context is (or
+// cellm_hip_release_graph_scratch says that no graph runs again): the graph
+// writes to it on every replay, so a grow sets it aside.  A capture
 // itself takes the buffer as it stands; one that is too small is refused before
 // anything is done to the stream.
 // zero_prefix: bytes at the start of a freshly allocated buffer that are cleared
@@ -1777,8 +1778,8 @@ namespace {
 // Scratch of a call that its kernel leaves as it found it in its first zero_prefix bytes (zero): the stream's
 // scratch of these calls (not ctx->attn, which graphs of cellm_hip_attention_gqa_f16kv on that stream hold), or,
 // under a capture, scratch of that graph's own, so that graphs captured on one stream may run at once and beside
-// eager calls.  It lasts as long as the context, as the graph may.  The caller holds ctx->mu until the kernel is
-// enqueued.
+// eager calls.  It lasts as long as the context, as the graph may, or until the caller says that no graph is launched
+// again (cellm_hip_release_graph_scratch).  The caller holds ctx->mu until the kernel is enqueued.
 int32_t get_graph_safe_scratch(cellm_hip_ctx* ctx, hipStream_t st, size_t need, float** out, size_t zero_prefix)
 {
     *out = nullptr;
@@ -2082,6 +2083,28 @@ int32_t cellm_hip_attention_tree_f16kv(cellm_hip_ctx_t* ctx, const float* q, con
     a.out = out;
     return attention_tree_impl(ctx, a, masks, tables, tree, n_heads, n_kv_heads, head_dim, max_blocks, total_blocks, n_layers,
                                tokens_per_block, layer, window, stream);
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_release_graph_scratch(cellm_hip_ctx_t* ctx)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    DeviceGuard g(ctx->device);
+    const std::lock_guard<std::recursive_mutex> lk(ctx->mu);
+    const RelaxedCapture relaxed;
+    hipError_t failed = hipSuccess;
+    const auto release = [&](void* p) {  // waits for the device
+        if (const hipError_t e = p ? hipFree(p) : hipSuccess; e != hipSuccess) failed = e;
+    };
+    for (auto& kv : ctx->graph_scratch) release(kv.second.ptr);
+    ctx->graph_scratch.clear();
+    for (void* p : ctx->retired) release(p);
+    ctx->retired.clear();
+    for (auto* map : {&ctx->workspaces, &ctx->aux, &ctx->attn, &ctx->argmax, &ctx->paged})
+        for (auto& kv : *map) kv.second.captured = false;
+    HIP_TRY(failed, "hipFree(graph scratch)");
+    return CELLM_HIP_OK;
     CELLM_API_END(report_exception)
 }
 

@@ -692,6 +692,11 @@ class HipOps:
                  self._ptr("accepted", accepted_i32, _DT.i32, tables * most), most, tables, tree, n_kv_heads, head_dim,
                  n_layers, tokens_per_block, _stream_ptr(stream)))
 
+    def release_graph_scratch(self) -> None:
+        """Frees what the context keeps for captured graphs, none of which is launched again: for programs that capture
+        again and again (cellm_hip_release_graph_scratch)."""
+        check(self._lib.cellm_hip_release_graph_scratch(self._h))
+
     def encode_silu_mul(self, gate, up, stream=None) -> None:
         """gate = silu(gate) * up in place (f32), silu_mul_f32_inplace."""
         check(self._lib.cellm_hip_silu_mul_f32(self._h, _dev_ptr(gate), _dev_ptr(up), gate.numel(),

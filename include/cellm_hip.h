@@ -571,9 +571,17 @@ int32_t cellm_hip_attention_gqa_f16kv_noalloc(cellm_hip_ctx_t* ctx, const float*
  *
  * Attention splits long contexts over blocks and adds their sums in context-owned
  * scratch: one buffer per stream, grown on demand, or one per captured graph and stream,
- * kept until the context is destroyed, so that graphs and eager calls may run at the same
- * time; launches of what was made from one capture run one after the other.  The same
- * call on the same values gives the same bits. */
+ * kept until the context is destroyed or cellm_hip_release_graph_scratch is called, so that
+ * graphs and eager calls may run at the same time; launches of what was made from one
+ * capture run one after the other.  The same call on the same values gives the same bits. */
+
+/* Frees what this context keeps for captured graphs: the scratch of captured attention
+ * over shared pages, and scratch of any call that a graph held when its stream needed more.
+ * For programs that capture again and again, whose context would otherwise grow with every
+ * capture.  The caller has seen to it that no graph captured from this context's calls is
+ * launched afterwards, that their launches have ended, and that no capture of such calls is
+ * under way.  Waits for the device. */
+int32_t cellm_hip_release_graph_scratch(cellm_hip_ctx_t* ctx);
 
 /* K and V [rows][n_kv_heads][head_dim] f32 into the pages of `layer` at each row's
  * position, as cellm_hip_kv_write_f16 does for f16.  The rows of one call go to

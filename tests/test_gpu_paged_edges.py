@@ -317,6 +317,42 @@ def test_eager_calls_have_scratch_that_no_graph_of_the_f16_cache_holds():
         assert before - torch.cuda.mem_get_info()[0] >= 2**21
 
 
+def test_scratch_of_captures_is_given_back():
+    """A program that captures again and again: the context's memory stands where it was once the graphs are gone and it
+    says so, graphs captured afterwards give the eager result, and so do eager calls on the capture's stream."""
+    from cellm_amd import HipOps
+
+    s, cap = _q8_set(6, hd=256), torch.cuda.Stream()
+    with HipOps(0) as own:
+        (want,) = _results([(own.encode_attention_q8, s)])
+
+        def captured():
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=cap):
+                own.encode_attention_q8(*s["args"], stream=cap)
+            return graph
+
+        captured().replay()
+        torch.cuda.synchronize()
+        own.release_graph_scratch()
+        before = torch.cuda.mem_get_info()[0]
+        for _ in range(3):
+            graphs = [captured() for _ in range(30)]
+            for graph in graphs:
+                s["out"].zero_()
+                graph.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(s["out"], want)
+            assert before - torch.cuda.mem_get_info()[0] >= 30 * 2**21  # each its own
+            del graph, graphs
+            own.release_graph_scratch()
+            assert before - torch.cuda.mem_get_info()[0] <= 10 * 2**21  # what the runtime keeps of its own
+            s["out"].zero_()
+            own.encode_attention_q8(*s["args"], stream=cap)
+            torch.cuda.synchronize()
+            assert torch.equal(s["out"], want)
+
+
 def test_graphs_of_the_f16_cache_run_beside_eager_calls_of_their_stream(ops):
     """A graph of the f16 cache's attention replayed on one stream while 8-bit calls and trees run on the stream that it
     was captured on: each has its own result."""
