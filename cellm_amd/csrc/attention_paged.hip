@@ -61,12 +61,13 @@ constexpr int kMaxSplits = 64;    // of a set's positions
 // walk of three units less.  300 positions (14/2 heads of 64) 8.3 us, 10.8 in splits; 701 10.1 and 11.0; a tree of 16
 // nodes at 500 10.0 and 12.3; a prompt of 512 10.4 and 15.9.  At four units splits win: 1000 positions 10.9, 12.4 in halves.
 constexpr int kWholeUnits = 3;
-constexpr int kPlanSets = 512;    // sets that plan() looks at, 8 a lane; more run unsplit
+constexpr int kPlanSets = 256;    // sets that plan() looks at, 4 a lane: fewer than kPlanBlocks
 // Splits aim at one block on each of the 256 CUs, though two run at once: fewer, longer walks keep the reads going and meet
 // faster (one session at 131072 positions, 32/8 heads of 128: 61.3 us, 66.1 with 512 blocks; 16 sessions at 8000, 8/1
 // heads of 256, 24.5 and 29.5; 300 rows at 600 of those 19.9 and 26.3).  Against it: 8 sessions at 1000 positions, 32/8
 // heads of 128, have 15.2 us and 13.8.
 constexpr int kPlanBlocks = 256;
+static_assert(kPlanSets >= kPlanBlocks);
 // Sets of 32 columns where they leave at least so many blocks: each K and V tile serves twice the columns (8 trees of
 // 63 nodes at 4096 positions, 32/8 heads of 128, f16: 90 us, 140 with 16 columns; a prompt of 1024 over 8-bit pages 90
 // and 104), but with fewer blocks the chip stands idle (16 trees of 8 nodes at 1000 positions 32.1 us, 18.3 with 16
@@ -283,14 +284,14 @@ struct Work {
     int split, splits, slot0;   // slot0: work number of the set's split 0
 };
 
-// Work number w of a kv head.  Every wave looks at all sets (64 lanes, up to 8 sets each): their positions in units of
-// UNIT add up to the work, each set gets as many splits as units, in shares of the same size for all (so that
+// Work number w of a kv head.  SPLITS: every wave looks at all sets (64 lanes, up to 4 sets each): their positions in units
+// of UNIT add up to the work, each set gets as many splits as units, in shares of the same size for all (so that
 // contexts of different lengths end together) and at most kMaxSplits, and the splits are numbered through.
-template <int UNIT>
+template <int UNIT, bool SPLITS>
 __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
 {
     const int lane = threadIdx.x & 63;
-    if (A.want == 0) {
+    if (!SPLITS || A.want == 0) {
         k = Work{A.sets - 1 - w, 0, -1, UNIT, 0, 1, 0};  // a prompt's last rows, which see the most, first
         if (k.set < 0) return false;
         if (!A.a.masks && A.a.window == 0) return true;  // all from 0 on: how far, the columns will say
@@ -564,9 +565,12 @@ __device__ __forceinline__ float score_of(int hi, int mid, int lo, float ks)
 }
 
 // ---- a block's results: its sums where the set is split, else the quotients; the sums of splits added by the last ----
-// COLS columns of a set from column col0 of the table on; a split's sums: [COLS][HD], then R and l, [COLS] each.
+// COLS columns of a set from column col0 of the table on; a split's sums: [COLS][HD], then R and l, [COLS] each.  Sets of
+// 32 columns are taken where they leave kWideBlocks blocks, and split where there are fewer than kPlanBlocks: never.
 template <int HD, int COLS>
 struct Results {
+    static constexpr bool kSplits = COLS == kCols;
+    static_assert(kSplits || kWideBlocks >= kPlanBlocks);
     static constexpr uint32_t kPart = COLS * (HD + 2);
     const MmaArgs& A;
     const Work& k;
@@ -590,7 +594,7 @@ struct Results {
     // four dims of column x (at offset `at` of out) from d on, ll the sum of all its weights; whether they are finite
     __device__ __forceinline__ bool put(int x, size_t at, int d, f4_t v, float ll) const
     {
-        if (k.splits > 1) st_agent4(part, part_of(k.split) + x * HD + d, v);
+        if (kSplits && k.splits > 1) st_agent4(part, part_of(k.split) + x * HD + d, v);
         else *reinterpret_cast<f4_t*>(A.a.out + at + d) = v * (ll != 0.0f ? 1.0f / ll : 0.0f);
         return finite_f32(v[0]) && finite_f32(v[1]) && finite_f32(v[2]) && finite_f32(v[3]) && finite_f32(ll);
     }
@@ -612,9 +616,9 @@ struct Results {
             Sight sc;
             sight_of(A.a, A.cap, table, c.row, sc);
             float mm, ll;
-            const float v = plain_range<HD, UNIT>(A.a, sc, table, c.row, c.head, k.lo, sc.end, k.step, k.splits > 1, lds, mm, ll);
+            const float v = plain_range<HD, UNIT>(A.a, sc, table, c.row, c.head, k.lo, sc.end, k.step, kSplits && k.splits > 1, lds, mm, ll);
             const int t = threadIdx.x;
-            if (k.splits > 1) {
+            if (kSplits && k.splits > 1) {
                 if (t < HD) st_agent(part, part_of(k.split) + x * HD + t, v);
                 if (t == 0) put_sums(x, mm, ll);
             } else if (t < HD) {
@@ -713,14 +717,15 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     constexpr int NR = HD / 4 < 32 ? HD / 4 : 32;                       // registers of O^T that the waves add at a time
     constexpr bool kQInLds = HD > 128 || CT > 1;                        // q's parts in LDS, for want of registers
     constexpr int COLS = kCols * CT;
-    constexpr int kMergeBytes = std::max(kWaves * NR * 64 * 4, COLS * kMaxSplits * 8);
+    constexpr bool kSplits = Results<HD, COLS>::kSplits;
+    constexpr int kMergeBytes = std::max(kWaves * NR * 64 * 4, kSplits ? COLS * kMaxSplits * 8 : 0);
     __shared__ __align__(16) unsigned char merge[kMergeBytes];
     __shared__ __align__(16) u4_t qlds[kQInLds ? CT * KK * QP * 64 : 1];
     __shared__ __align__(16) u4_t qlow[Q8 ? CT * KK * 64 : 1];          // the fourth digits
     __shared__ uint32_t loud_lds[CT];
     __shared__ __align__(16) uint32_t kidx[kWaves][CH], vidx[kWaves][CH];  // [c][tile], [g][j]
     __shared__ __align__(16) float kscl[kWaves][Q8 ? CH : 4], vscl[kWaves][Q8 ? CH : 4];
-    __shared__ float ml[kWaves][2][COLS], lsum[COLS], qs_lds[2][COLS];
+    __shared__ float ml[kWaves][2][COLS], lsum[kSplits ? COLS : 1], qs_lds[2][COLS];
     __shared__ uint32_t flags, here;
     __shared__ int last;
 
@@ -729,7 +734,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     const int c = lane & 15, g4 = lane >> 4;
     const int kvh = blockIdx.x;
     Work k;
-    if (!plan<kWaves * CH>(A, blockIdx.y + gridDim.y * blockIdx.z, k)) return;  // the same for the whole block
+    if (!plan<kWaves * CH, kSplits>(A, blockIdx.y + gridDim.y * blockIdx.z, k)) return;  // the same for the whole block
     const Results<HD, COLS> res(A, k, kvh);
     const int table = res.table, n_cols = res.columns();
 
@@ -1058,7 +1063,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                 for (int r = 0; r < NR / 4; r += 4)
                     fine[u] &= res.put(col, at[u], g4 * (HD / 4) + rd * NR + wave * (NR / 4) + r,
                                        f4_t{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]}, ll);
-                if (k.splits > 1 && rd == 0 && wave == 0 && g4 == 0) res.put_sums(col, mm, ll);
+                if (kSplits && k.splits > 1 && rd == 0 && wave == 0 && g4 == 0) res.put_sums(col, mm, ll);
             }
         }
     }
@@ -1070,7 +1075,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         const uint32_t again = flags;
         if (again) res.template put_plain<kWaves * CH>(again, merge);  // rare
     }
-    res.combine(here, lsum, &last, merge);
+    if constexpr (kSplits) res.combine(here, lsum, &last, merge);
 }
 
 template <typename F>
@@ -1107,7 +1112,7 @@ Layout layout_of(const PagedAttnArgs& a)
              });
     const long long cap = (long long)a.g.max_blocks * a.g.tpb, units = (cap + unit - 1) / unit;
     const long long blocks = (long long)y.sets * a.g.n_kv;
-    if (y.sets <= kPlanSets && blocks < kPlanBlocks && units > kWholeUnits) y.want = std::max(1, kPlanBlocks / a.g.n_kv - y.sets);
+    if (blocks < kPlanBlocks && units > kWholeUnits) y.want = std::max(1, kPlanBlocks / a.g.n_kv - y.sets);
     // each set's last split may be short
     y.works = y.want ? std::min<long long>(y.want + y.sets, y.sets * std::min<long long>(kMaxSplits, units)) : y.sets;
     return y;

@@ -263,6 +263,26 @@ def test_windows_of_contexts_past_the_table(ops, f16, tables, hd):
     assert P.rel(got, ref) <= TOL
 
 
+# ---- both sides of the rule that plans splits: fewer than 256 blocks, over tables of more than three units -------------
+
+
+@pytest.mark.parametrize("tables,nkv", [(255, 1), (256, 1), (257, 1), (85, 3), (86, 3)])
+def test_sessions_on_both_sides_of_256_blocks(ops, tables, nkv):
+    g = torch.Generator().manual_seed(tables)
+    hd, tpb, pages = 64, 16, 57  # 912 positions: four units of 256
+    bt = torch.randint(0, 200, (tables, pages), generator=g)
+    cache = P.cache_q8(200, 1, nkv, tpb, hd, 71)
+    q = torch.randn(tables, 2 * nkv, hd, generator=g)
+    pos = torch.randint(-1, pages * tpb, (tables,), generator=g)
+    pos[0], pos[-1] = pages * tpb - 1, 800
+    got = _attention(ops, q, cache, bt, pos, 1)
+    some = torch.unique(torch.cat([torch.tensor([0, 1, tables // 2, tables - 1]), torch.randperm(tables, generator=g)[:10]]))
+    ref = P.causal(q[some], *cache, bt[some], pos[some], 0, 1)
+    none = pos[some] < 0
+    assert bool((got[some][none] == 7.0).all())
+    assert P.rel(got[some][~none], ref[~none]) <= TOL
+
+
 # ---- beside graphs of the f16 cache's attention -----------------------------------------------------
 
 
