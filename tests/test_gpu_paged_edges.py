@@ -396,3 +396,65 @@ def test_graphs_of_the_f16_cache_run_beside_eager_calls_of_their_stream(ops):
         torch.cuda.synchronize()
         for s, w in zip((f16, *q8), (want_f16, *want_q8)):
             assert torch.equal(s["out"], w)
+
+
+# ---- drafts over the f16 cache, as a serving loop runs them --------------------------------------------
+
+
+def test_drafted_decode_over_the_f16_cache(ops):
+    """A prompt enters the f16 cache, a tree of drafts is written behind it, checked in one call and its accepted path
+    kept; the next token attends to it.  The pages are those of the path entered token by token, and every accepted
+    node's attention and the next token's are near what encode_attention gives there."""
+    g = torch.Generator().manual_seed(73)
+    nh, nkv, hd, tpb, prompt, tree, pages = 6, 2, 64, 8, 45, 13, 9
+    parents = [-1, -1, 0, 0, 1, 2, 2, 5, 5, 4, 8, 8, 10]
+    path = [0, 2, 5, 8, 10, 12]
+    bits = P.tree_bits(parents)
+    depth = torch.from_numpy(bits.sum(1).astype(np.int32)) - 1
+    bt = torch.randperm(pages, generator=g)[None].to(torch.int32).cuda()
+    a = np.arange(80)[:, None] * 10000.0 ** (-2.0 * np.arange(hd // 2) / hd)
+    cs = torch.from_numpy(np.stack([np.cos(a), np.sin(a)], -1).astype(np.float32)).cuda()
+    x = [torch.randn(prompt + tree + 1, n, hd, generator=g).cuda() for n in (nh, nkv, nkv)]
+    geo = (pages, 1, tpb, 0)
+
+    def ints(values):
+        return torch.tensor(list(values), dtype=torch.int32).cuda()
+
+    def enter(cache, rows, pos, slots):
+        q, k, v = (t[list(rows)].contiguous() for t in x)
+        ops.encode_rope_half(q, nh, hd, pos, cs)
+        ops.encode_rope_half(k, nkv, hd, pos, cs)
+        ops.encode_kv_write(k.view(k.shape[0], -1), v.view(v.shape[0], -1), slots, *cache,
+                            bt.expand(k.shape[0], -1).contiguous(), *geo)
+        return q
+
+    def attend(cache, q, pos):
+        out = torch.empty_like(q)
+        ops.encode_attention(q, *cache, bt.expand(q.shape[0], -1).contiguous(), pos, out, nh, nkv, hd, *geo)
+        return out
+
+    def fresh():
+        return [torch.zeros(pages, 1, tpb, nkv, hd, dtype=torch.float16, device="cuda") for _ in range(2)]
+
+    one, outs = fresh(), []
+    enter(one, range(prompt), ints(range(prompt)), ints(range(prompt)))
+    for i, node in enumerate(path):
+        at = ints([prompt + i])
+        outs.append(attend(one, enter(one, [prompt + node], at, at), at))
+    at = ints([prompt + len(path)])
+    last = attend(one, enter(one, [prompt + tree], at, at), at)
+
+    two = fresh()
+    enter(two, range(prompt), ints(range(prompt)), ints(range(prompt)))
+    q = enter(two, range(prompt, prompt + tree), (prompt + depth).cuda(), ints(range(prompt, prompt + tree)))
+    out = torch.empty_like(q)
+    ops.encode_attention_tree(q, *two, bt, ints([prompt]), P.words_of(bits[None]).cuda(), out, nh, nkv, hd, *geo)
+    ops.encode_kv_accept(*two, bt, ints([prompt]), torch.tensor([path + [-1] * 3], dtype=torch.int32).cuda(), tree, nkv, hd,
+                         pages, 1, tpb)
+    for o, node in zip(outs, path):
+        assert P.rel(out[node].cpu(), o[0].cpu().double()) <= 2 * TOL
+    assert torch.equal(attend(two, enter(two, [prompt + tree], at, at), at), last)
+    where = torch.arange(prompt + len(path) + 1)
+    blocks = bt[0].long()[where.cuda() // tpb]
+    for c1, c2 in zip(one, two):
+        assert torch.equal(c1[blocks, 0, where.cuda() % tpb], c2[blocks, 0, where.cuda() % tpb])
