@@ -38,11 +38,13 @@
 // which knows how long every context is; the last block of a set to finish adds the others'
 // sums in split order.
 //
-// What bounds it (gfx950).  Decode: the reads, in part (8 sessions of 4096 to 8192 positions, 32/8 heads of 128, 28 us for
-// 104 MB, 3.7 TB/s; one at 131072 58 us for 277 MB, 4.7; a bare read of them takes 16.5 and 41), as 4 of 16 columns are
-// filled and V's unpacking stands beside them.  Short contexts: four dependent latencies a chunk and the meeting of splits
-// (9 us at 701 positions, 14/2 heads of 64).  Many columns: vector instructions at two waves per SIMD (1024 tokens onto
-// as many, 32/8 heads of 128, 82 us: vector ALU busy 62 %, matrix units 20 %, 316 TFLOP/s of the formula's products).
+// What bounds it (gfx950).  Decode: the reads and how they are shared out.  One session at 131072 positions, 32/8 heads of
+// 128, takes 58 to 61 us for 277 MB, 4.7 TB/s; 8 sessions of 4096 to 8192 28 to 29 for 104 MB, 3.7 TB/s, with a block on
+// 208 of the 256 CUs and walks of up to 9 units where 7 would do (a bare read of them takes 42 and 16.5; vector ALU
+// busy 23 %, matrix units 6).  Short contexts: latency.  A block of one unit of positions takes 6.2 us (100 positions, 14/2
+// heads of 64), each further one 1.8 (page entry, K, scores, weights, V one after the other): 9.7 at 701, unsplit.
+// Many columns: vector instructions at two waves per SIMD (1024 tokens onto as many, 32/8 heads of 128, 84 us: vector ALU
+// busy 62 %, matrix units 20 %, 307 TFLOP/s of the formula's products).
 #include <algorithm>
 #include <cmath>
 
@@ -58,14 +60,18 @@ namespace {
 constexpr int kWaves = 4, kThreads = kWaves * 64, kCols = 16;
 constexpr int kMaxSplits = 64;    // of a set's positions
 // Sets of so many units of positions (a chunk for each wave) are not split: the meeting of splits costs about 4.5 us, a
-// walk of three units less.  300 positions (14/2 heads of 64) 8.3 us, 10.8 in splits; 701 10.1 and 11.0; a tree of 16
-// nodes at 500 10.0 and 12.3; a prompt of 512 10.4 and 15.9.  At four units splits win: 1000 positions 10.9, 12.4 in halves.
+// walk of three units less.  Units of 256 positions: 300 (14/2 heads of 64) 8.3 us, 10.8 in splits; 701 9.7 and 10.9; a
+// tree of 16 nodes at 500 10.0 and 12.3; a prompt of 512 10.4 and 15.9.  At four units splits win: 1000 positions 10.9,
+// 11.4 whole; 4 sessions of 1000, 32/8 heads of 128, 12.7 and 14.1.  Units of 128 (8-bit heads of 256, f16 of 128 and 256)
+// walk faster: three units 12.5 us, 14.7 in splits (370 positions, 8/1 heads of 256), and four still lose in splits, 15.1
+// to 14.1, and a tree of 16 nodes at 490 over f16 heads of 128 14.9 to 11.4.
 constexpr int kWholeUnits = 3;
 constexpr int kPlanSets = 256;    // sets that plan() looks at, 4 a lane: fewer than kPlanBlocks
 // Splits aim at one block on each of the 256 CUs, though two run at once: fewer, longer walks keep the reads going and meet
 // faster (one session at 131072 positions, 32/8 heads of 128: 61.3 us, 66.1 with 512 blocks; 16 sessions at 8000, 8/1
-// heads of 256, 24.5 and 29.5; 300 rows at 600 of those 19.9 and 26.3).  Against it: 8 sessions at 1000 positions, 32/8
-// heads of 128, have 15.2 us and 13.8.
+// heads of 256, 24.5 and 29.5; 300 rows at 600 of those 19.9 and 26.3).  Fewer stand than that: the sets are taken off
+// for their last splits, which may be short, and the share is rounded up (8 sessions of 4096 to 8192 positions, 32/8
+// heads of 128, 208 blocks; 24 such 192; 8 at 1000 positions 128, which have 15.3 us, and 13.8 under a bound of 512).
 constexpr int kPlanBlocks = 256;
 static_assert(kPlanSets >= kPlanBlocks);
 // Sets of 32 columns where they leave at least so many blocks: each K and V tile serves twice the columns (8 trees of

@@ -15,8 +15,8 @@
 //
 // All three are bound by bytes or, where there are few, by their launch and the chain position -> page -> data.  Write: a
 // team of lanes per head vector, 32 bytes of f32 a lane, the maximum by lane exchanges, so that a vector is read once;
-// 2048 tokens of 32/8 heads of 128 with RoPE move 89 MB in 20 us, 4.5 TB/s (a large copy: 4.7); one token of 14/2 heads
-// of 64 takes 3.4 us.
+// 2048 tokens of 32/8 heads of 128 with RoPE move 89 MB in 20 us, 4.5 TB/s (large copies: 4.7 to 5.3); one token of 9/3
+// heads of 64 takes 3.4 us.
 // Read: 16 bytes of output a thread; 8000 tokens of 8 heads of 128 to f16 move 50 MB in 10.3 us, 4.8 TB/s.  The move of
 // accepted tokens: 4.1 us for 24 layers of 2 heads of 64, 4.6 for 32 layers of 8 heads of 128 in 8 sessions (5.4 MB).
 #include <algorithm>

@@ -618,9 +618,11 @@ int32_t cellm_hip_kv_read_q8(cellm_hip_ctx_t* ctx, const int8_t* kcodes, const f
  * [rows][n_heads][head_dim] f32, row r attends to the positions up to its own of its
  * table (the table's last at most), the last `window` of them with a window > 0;
  * attn_scale and soft_cap as there.  Any number of query heads per kv head.
- * Positions may differ from row to row of a table in any way.  A q vector with an
- * infinity or a NaN gives a row of NaN, and so does an attended vector of scale NaN;
- * what a row does not attend to never reaches it. */
+ * Positions may differ from row to row of a table in any way; out overlaps no input.
+ * q is held as integers of 2^-22 of its head's largest element, or of 2^-30 where that is
+ * more than 8 times the mean |q|; scores and sums are f32, and a score past f32's range
+ * gives a row of NaN.  A q vector with an infinity or a NaN gives a row of NaN, and so
+ * does an attended vector of scale NaN; what a row does not attend to never reaches it. */
 int32_t cellm_hip_attention_gqa_q8kv(cellm_hip_ctx_t* ctx, const float* q, const int8_t* kcodes, const float* kscales,
                                      const int8_t* vcodes, const float* vscales, const uint32_t* block_tables,
                                      int64_t max_blocks, int64_t total_blocks, const int32_t* positions, int64_t rows,
@@ -641,7 +643,9 @@ int32_t cellm_hip_attention_gqa_q8kv(cellm_hip_ctx_t* ctx, const float* q, const
  * session with a context < 0, is skipped and its output left as it was; context
  * positions and slots past the table are not there, and a node that sees none gets
  * zeros.  Otherwise as cellm_hip_attention_gqa_q8kv, and over f16 pages
- * (cellm_hip_attention_gqa_f16kv's) for head_dim 64, 128 and 256. */
+ * (cellm_hip_attention_gqa_f16kv's) for head_dim 64, 128 and 256, with q as two f16 parts
+ * (23 bits of an element, 2^-38 of its head's largest) and keys and values with infinities
+ * and NaN counted as they are. */
 int32_t cellm_hip_attention_tree_f16kv(cellm_hip_ctx_t* ctx, const float* q, const uint16_t* kcache, const uint16_t* vcache,
                                        const uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks,
                                        const int32_t* context_lens, const uint64_t* masks, int64_t tables, int64_t tree,
