@@ -458,3 +458,112 @@ def test_drafted_decode_over_the_f16_cache(ops):
     blocks = bt[0].long()[where.cuda() // tpb]
     for c1, c2 in zip(one, two):
         assert torch.equal(c1[blocks, 0, where.cuda() % tpb], c2[blocks, 0, where.cuda() % tpb])
+
+
+def _loop(ops, cache, state, stream=None):
+    """Write of a tree of drafts, its check, the accepted path, and what then stands in the pages."""
+    nh, nkv, hd, geo, tree = state["nh"], state["nkv"], state["hd"], state["geo"], state["tree"]
+    kw = dict(stream=stream)
+    ops.encode_rope_kv_write_q8(state["q"], state["k"], state["v"], state["qr"], nh, nkv, hd, state["pos"], state["cs"], *cache,
+                                state["bt"], *geo, slots_i32=state["slots"], rows_per_table=tree, **kw)
+    ops.encode_attention_tree(state["qr"], cache[0], cache[2], state["bt"], state["ctx"], state["masks"], state["out"], nh, nkv,
+                              hd, *geo, kscale=cache[1], vscale=cache[3], **kw)
+    ops.encode_kv_accept(cache[0], cache[2], state["bt"], state["ctx"], state["acc"], tree, nkv, hd, *geo[:3], kscale=cache[1],
+                         vscale=cache[3], **kw)
+    ops.encode_kv_read_q8(*cache, state["bt"], state["where"], state["ko"], state["vo"], nkv, hd, *geo,
+                          rows_per_table=state["where"].numel() // state["bt"].shape[0], **kw)
+
+
+def _loop_state(seed, tables=3, tree=21, ctx=1300):
+    g = torch.Generator().manual_seed(seed)
+    nh, nkv, hd, tpb = 6, 2, 64, 16
+    pages = -(-(ctx + tree) // tpb)
+    total, n = tables * pages, tables * tree
+    bits = np.stack([_random_tree(g, tree) for _ in range(tables)])
+    lens = torch.randint(ctx // 2, ctx, (tables,), generator=g)
+    a = np.arange(ctx + tree)[:, None] * 10000.0 ** (-2.0 * np.arange(hd // 2) / hd)
+    acc = torch.full((tables, 8), -1)
+    for t in range(tables):
+        path = np.flatnonzero(bits[t, tree - 1 - t])[:8]
+        acc[t, :len(path)] = torch.from_numpy(path)
+    where = (lens[:, None] + torch.arange(-4, 8)).reshape(-1)
+    depth = torch.from_numpy(bits.sum(2)) - 1
+
+    def ints(t):
+        return t.to(torch.int32).cuda()
+
+    def rows(heads):
+        return torch.randn(n, heads, hd, generator=g).cuda()
+
+    st = dict(nh=nh, nkv=nkv, hd=hd, tree=tree, geo=(total, 1, tpb, 0), bt=ints(torch.randperm(total, generator=g).view(tables, pages)),
+              q=rows(nh), k=rows(nkv), v=rows(nkv), pos=ints((lens[:, None] + depth).reshape(-1)),
+              slots=ints((lens[:, None] + torch.arange(tree)).reshape(-1)), ctx=ints(lens), masks=P.words_of(bits).cuda(),
+              acc=ints(acc), where=ints(where), cs=torch.from_numpy(np.stack([np.cos(a), np.sin(a)], -1).astype(np.float32)).cuda())
+    st["qr"], st["out"] = torch.zeros_like(st["q"]), torch.zeros_like(st["q"])
+    st["ko"], st["vo"] = (torch.zeros(where.numel(), nkv * hd, device="cuda") for _ in range(2))
+    return st, [c.cuda() for c in P.cache_q8(total, 1, nkv, tpb, hd, seed)]
+
+
+_RESULTS = ("qr", "out", "ko", "vo")
+
+
+def test_the_loop_in_one_graph(ops):
+    """Write, check, acceptance and read captured together and replayed with new tokens each time: the eager calls' bits."""
+    st, first = _loop_state(79)
+    cap, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    cache = [c.clone() for c in first]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=cap):
+        _loop(ops, cache, st, cap)
+    g = torch.Generator().manual_seed(83)
+    for turn in range(4):
+        for name in "qkv":
+            st[name].copy_(torch.randn(st[name].shape, generator=g))
+        eager = [c.clone() for c in first]
+        _loop(ops, eager, st)
+        torch.cuda.synchronize()
+        want = [st[n].clone() for n in _RESULTS]
+        for n in _RESULTS:
+            st[n].zero_()
+        for c, f in zip(cache, first):
+            c.copy_(f)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(st[n], w) for n, w in zip(_RESULTS, want))
+        assert all(torch.equal(a, b) for a, b in zip(cache, eager))
+
+
+def test_loops_of_two_threads(ops):
+    """Two threads with one context, each on a stream of its own."""
+    import threading
+
+    both = [_loop_state(s, ctx=c) for s, c in ((89, 1300), (97, 4200))]
+    want = []
+    for st, first in both:
+        _loop(ops, [c.clone() for c in first], st)
+        torch.cuda.synchronize()
+        want.append([st[n].clone() for n in _RESULTS])
+    wrong = []
+
+    def work(st, first, expected):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    for n in _RESULTS:
+                        st[n].zero_()
+                    cache = [c.clone() for c in first]
+                    _loop(ops, cache, st, stream)
+                    stream.synchronize()
+                    if not all(torch.equal(st[n], w) for n, w in zip(_RESULTS, expected)):
+                        wrong.append("results")
+        except Exception as e:  # told below: a thread's own exception would be lost
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(*b, w)) for b, w in zip(both, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
