@@ -867,8 +867,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     };
     const auto load_k = [&]() {
         if constexpr (Q8) {
-            ks_own = a.ks[vn];
-            vs_own = a.vs[vn];
+            ks_own = static_cast<const float*>(a.ks)[vn];
+            vs_own = static_cast<const float*>(a.vs)[vn];
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -1110,7 +1110,7 @@ Layout layout_of(const PagedAttnArgs& a)
     y.tiles = (int)((columns + y.cols - 1) / y.cols);
     y.sets = (int)(tables * y.tiles);
     int unit = 0;
-    by_shape(a.ks != nullptr, a.head_dim,
+    by_shape(a.fmt == KV_Q8, a.head_dim,
              [&](auto q, auto hd) {
                  constexpr bool Q8 = decltype(q)::value;
                  constexpr int HD = decltype(hd)::value;
@@ -1149,7 +1149,7 @@ hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipS
     A.part_bytes = (uint32_t)((size_t)y.works * a.g.n_kv * y.cols * (a.head_dim + 2) * sizeof(float));  // below 2^31: plan()'s blocks
     const unsigned rows_of_grid = (unsigned)std::min<long long>(y.works, 32768);
     const dim3 grid((unsigned)a.g.n_kv, rows_of_grid, (unsigned)((y.works + rows_of_grid - 1) / rows_of_grid));
-    by_shape(a.ks != nullptr, a.head_dim, [&](auto q, auto hd) {
+    by_shape(a.fmt == KV_Q8, a.head_dim, [&](auto q, auto hd) {
         constexpr bool Q8 = decltype(q)::value;
         constexpr int HD = decltype(hd)::value;
         const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, st, A); };

@@ -1904,6 +1904,10 @@ int32_t attention_paged_impl(cellm_hip_ctx* ctx, const PagedAttnArgs& in, int64_
     DeviceGuard g(ctx->device);
     const std::lock_guard<std::recursive_mutex> lk(ctx->mu);  // held until the scratch user is enqueued
     const hipStream_t st = pick_stream(ctx, stream);
+    if (a.fmt == KV_Q4) {
+        HIP_TRY(launch_attention_q4(a, st), "attention launch");
+        return CELLM_HIP_OK;
+    }
     float* ws = nullptr;
     if (int32_t rc = get_graph_safe_scratch(ctx, st, attention_paged_workspace_bytes(a), &ws, attention_counter_bytes()))
         return rc;
@@ -2022,6 +2026,7 @@ int32_t cellm_hip_attention_gqa_q8kv(cellm_hip_ctx_t* ctx, const float* q, const
     if (rows > 0 && (!kscales || !vscales)) return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
     PagedAttnArgs a{};
     a.q = q;
+    a.fmt = KV_Q8;
     a.kc = kcodes;
     a.ks = kscales;
     a.vc = vcodes;
@@ -2049,6 +2054,7 @@ int32_t cellm_hip_attention_tree_q8kv(cellm_hip_ctx_t* ctx, const float* q, cons
     if (tables > 0 && (!kscales || !vscales)) return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
     PagedAttnArgs a{};
     a.q = q;
+    a.fmt = KV_Q8;
     a.kc = kcodes;
     a.ks = kscales;
     a.vc = vcodes;
@@ -2131,6 +2137,186 @@ int32_t cellm_hip_kv_accept_q8(cellm_hip_ctx_t* ctx, int8_t* kcodes, float* ksca
     if (int32_t rc = check_ctx(ctx)) return rc;
     return kv_accept_impl(ctx, kcodes, kscales, vcodes, vscales, true, block_tables, max_blocks, total_blocks, context_lens,
                           accepted, max_accept, tables, tree, n_kv_heads, head_dim, n_layers, tokens_per_block, stream);
+    CELLM_API_END(report_exception)
+}
+
+}  // extern "C"
+
+// ---- a step over a paged cache whose lengths the device knows (kv_step.hip), and 4-bit pages ----
+
+namespace {
+
+int32_t norm_rope_write_impl(cellm_hip_ctx* ctx, const NormRopeArgs& in, int64_t rows, int64_t n_heads, int64_t n_kv_heads,
+                             int64_t head_dim, int64_t table_positions, int fmt, int64_t total_blocks, int64_t n_layers,
+                             int64_t tpb, int64_t layer, void* stream)
+{
+    if (int32_t rc = check_kv(rows, 1, n_kv_heads, head_dim, 1, total_blocks, n_layers, tpb, layer)) return rc;
+    if (n_heads < 1 || n_heads > 4096 || (in.cos_sin && (table_positions < 1 || table_positions > INT32_MAX)))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "bad heads %lld or table_positions %lld", (long long)n_heads,
+                         (long long)table_positions);
+    if (rows * (n_heads + 2 * n_kv_heads) * head_dim > (1ll << 34))  // 8 elements a thread, threads numbered in 32 bits
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "%lld rows of %lld heads of %lld: at most 2^34 elements of q, k and v a call",
+                         (long long)rows, (long long)(n_heads + 2 * n_kv_heads), (long long)head_dim);
+    if ((in.q_weight || in.k_weight) && (!valid_dtype(in.weight_dtype) || !(in.eps >= 0.0f) || std::isinf(in.eps)))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "bad weight dtype %d, or eps not finite and >= 0", (int)in.weight_dtype);
+    if (rows == 0) return CELLM_HIP_OK;
+    if (!in.q || !in.k || !in.v || !in.q_out || !in.pos || !in.slots || !in.kc || !in.vc || (fmt != KV_F16 && (!in.ks || !in.vs)))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
+    if (!aligned16(in.q) || !aligned16(in.k) || !aligned16(in.v) || !aligned16(in.q_out) || !aligned16(in.q_weight) ||
+        !aligned16(in.k_weight) || !aligned16(in.cos_sin) || !aligned16(in.kc) || !aligned16(in.vc) ||
+        (fmt == KV_Q4 && (!aligned16(in.ks) || !aligned16(in.vs))))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "q, k, v, weights, cos_sin and the pages must be 16-byte aligned");
+    NormRopeArgs a = in;
+    a.table_positions = (int)table_positions;
+    a.interleaved = ctx->rope_interleaved.load();
+    DeviceGuard g(ctx->device);
+    HIP_TRY(launch_norm_rope_write(a, (int)rows, (int)n_heads, (int)head_dim, fmt,
+                                   kv_geom(nullptr, 1, total_blocks, n_layers, n_kv_heads, tpb, layer), pick_stream(ctx, stream)),
+            "norm_rope_write launch");
+    return CELLM_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t cellm_hip_kv_plan(cellm_hip_ctx_t* ctx, const int32_t* context_lens, const int32_t* new_lens, int64_t tables,
+                          uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks, int64_t tokens_per_block,
+                          uint32_t* free_blocks, const int32_t* free_count, int64_t free_capacity, int32_t* lens_out,
+                          int32_t* free_out, int32_t* row_starts, int32_t* positions, int32_t* slots, int64_t rows,
+                          void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    // page counts of 1024 sessions add up in 32 bits, slots are 32-bit numbers
+    if (tables < 0 || tables > (1 << 20) || rows < 0 || rows > (1 << 20) || max_blocks < 1 || max_blocks > (1 << 20) ||
+        tokens_per_block < 1 || tokens_per_block > (1 << 30) || max_blocks * tokens_per_block > (1 << 30) ||
+        total_blocks < 1 || total_blocks > INT32_MAX / tokens_per_block || free_capacity < 0 || free_capacity > INT32_MAX)
+        return set_error(CELLM_HIP_ERR_INVALID_ARG,
+                         "bad geometry tables=%lld rows=%lld max_blocks=%lld total_blocks=%lld tpb=%lld free_capacity=%lld (at "
+                         "most 2^20 tables, rows and pages of a table, 2^30 positions of a table, 2^31 slots)",
+                         (long long)tables, (long long)rows, (long long)max_blocks, (long long)total_blocks,
+                         (long long)tokens_per_block, (long long)free_capacity);
+    if (!free_count || !free_out || !row_starts || (tables > 0 && (!context_lens || !new_lens || !block_tables || !lens_out)) ||
+        (free_capacity > 0 && !free_blocks) || (rows > 0 && (!positions || !slots)))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
+    KvPlanArgs a{context_lens, new_lens, (int)tables, block_tables, (int)max_blocks, (int)total_blocks, (int)tokens_per_block,
+                 free_blocks, free_count, (int)free_capacity, lens_out, free_out, row_starts, positions, slots, (int)rows};
+    DeviceGuard g(ctx->device);
+    HIP_TRY(launch_kv_plan(a, pick_stream(ctx, stream)), "kv_plan launch");
+    return CELLM_HIP_OK;
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_norm_rope_kv_write_f16(cellm_hip_ctx_t* ctx, const float* q, const float* k, const float* v, float* q_out,
+                                         const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+                                         int64_t rows, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                         const int32_t* positions, const float* cos_sin, int64_t table_positions,
+                                         const int32_t* slots, uint16_t* kcache, uint16_t* vcache, int64_t total_blocks,
+                                         int64_t n_layers, int64_t tokens_per_block, int64_t layer, void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    const NormRopeArgs a{q, k, v, q_out, q_weight, k_weight, weight_dtype, eps, positions, slots, cos_sin, 0, 0, kcache, nullptr,
+                         vcache, nullptr};
+    return norm_rope_write_impl(ctx, a, rows, n_heads, n_kv_heads, head_dim, table_positions, KV_F16, total_blocks, n_layers,
+                                tokens_per_block, layer, stream);
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_norm_rope_kv_write_q8(cellm_hip_ctx_t* ctx, const float* q, const float* k, const float* v, float* q_out,
+                                        const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+                                        int64_t rows, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                        const int32_t* positions, const float* cos_sin, int64_t table_positions,
+                                        const int32_t* slots, int8_t* kcodes, float* kscales, int8_t* vcodes, float* vscales,
+                                        int64_t total_blocks, int64_t n_layers, int64_t tokens_per_block, int64_t layer,
+                                        void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    const NormRopeArgs a{q, k, v, q_out, q_weight, k_weight, weight_dtype, eps, positions, slots, cos_sin, 0, 0, kcodes, kscales,
+                         vcodes, vscales};
+    return norm_rope_write_impl(ctx, a, rows, n_heads, n_kv_heads, head_dim, table_positions, KV_Q8, total_blocks, n_layers,
+                                tokens_per_block, layer, stream);
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_norm_rope_kv_write_q4(cellm_hip_ctx_t* ctx, const float* q, const float* k, const float* v, float* q_out,
+                                        const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+                                        int64_t rows, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                        const int32_t* positions, const float* cos_sin, int64_t table_positions,
+                                        const int32_t* slots, uint8_t* kcodes, uint16_t* kscales, uint8_t* vcodes,
+                                        uint16_t* vscales, int64_t total_blocks, int64_t n_layers, int64_t tokens_per_block,
+                                        int64_t layer, void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    const NormRopeArgs a{q, k, v, q_out, q_weight, k_weight, weight_dtype, eps, positions, slots, cos_sin, 0, 0, kcodes, kscales,
+                         vcodes, vscales};
+    return norm_rope_write_impl(ctx, a, rows, n_heads, n_kv_heads, head_dim, table_positions, KV_Q4, total_blocks, n_layers,
+                                tokens_per_block, layer, stream);
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_kv_read_q4(cellm_hip_ctx_t* ctx, const uint8_t* kcodes, const uint16_t* kscales, const uint8_t* vcodes,
+                             const uint16_t* vscales, const uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks,
+                             const int32_t* positions, int64_t rows, int64_t rows_per_table, int64_t n_kv_heads,
+                             int64_t head_dim, int64_t n_layers, int64_t tokens_per_block, int64_t layer, int32_t out_dtype,
+                             void* k_out, void* v_out, void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    if (int32_t rc = check_kv(rows, rows_per_table, n_kv_heads, head_dim, max_blocks, total_blocks, n_layers,
+                              tokens_per_block, layer))
+        return rc;
+    if (!valid_dtype(out_dtype)) return set_error(CELLM_HIP_ERR_INVALID_ARG, "bad dtype");
+    if (rows == 0) return CELLM_HIP_OK;
+    if (!kcodes || !kscales || !vcodes || !vscales || !block_tables || !positions || !k_out || !v_out)
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
+    if (!aligned16(kcodes) || !aligned16(vcodes) || !aligned16(kscales) || !aligned16(vscales) || !aligned16(k_out) ||
+        !aligned16(v_out))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "the codes, scales and outputs must be 16-byte aligned");
+    DeviceGuard g(ctx->device);
+    HIP_TRY(launch_kv_read_q4(kcodes, kscales, vcodes, vscales, positions, (int)rows, (int)rows_per_table, (int)head_dim,
+                              kv_geom(block_tables, max_blocks, total_blocks, n_layers, n_kv_heads, tokens_per_block, layer),
+                              k_out, v_out, out_dtype, pick_stream(ctx, stream)),
+            "kv_read_q4 launch");
+    return CELLM_HIP_OK;
+    CELLM_API_END(report_exception)
+}
+
+int32_t cellm_hip_attention_gqa_q4kv(cellm_hip_ctx_t* ctx, const float* q, const uint8_t* kcodes, const uint16_t* kscales,
+                                     const uint8_t* vcodes, const uint16_t* vscales, const uint32_t* block_tables,
+                                     int64_t max_blocks, int64_t total_blocks, const int32_t* positions, int64_t rows,
+                                     int64_t rows_per_table, const int32_t* row_starts, int64_t tables, int64_t n_heads,
+                                     int64_t n_kv_heads, int64_t head_dim, int64_t n_layers, int64_t tokens_per_block,
+                                     int64_t layer, float attn_scale, float soft_cap, int64_t window, float* out, void* stream)
+{
+    CELLM_API_BEGIN
+    if (int32_t rc = check_ctx(ctx)) return rc;
+    if (rows > 0 && (!kscales || !vscales)) return set_error(CELLM_HIP_ERR_INVALID_ARG, "null pointer");
+    if (!aligned16(kscales) || !aligned16(vscales))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "the scales must be 16-byte aligned");
+    if (row_starts && (tables < 0 || tables > (1 << 20) || rows_per_table != 1))
+        return set_error(CELLM_HIP_ERR_INVALID_ARG, "row_starts of %lld tables (up to 2^20) go with rows_per_table 1, not %lld",
+                         (long long)tables, (long long)rows_per_table);
+    if (row_starts && tables == 0) return CELLM_HIP_OK;
+    PagedAttnArgs a{};
+    a.q = q;
+    a.fmt = KV_Q4;
+    a.kc = kcodes;
+    a.ks = kscales;
+    a.vc = vcodes;
+    a.vs = vscales;
+    a.starts = row_starts;
+    a.tables = row_starts ? (int)tables : 0;
+    a.g.bt = block_tables;
+    a.pos = positions;
+    a.scale = attn_scale;
+    a.cap = soft_cap;
+    a.out = out;
+    return attention_paged_impl(ctx, a, rows, rows_per_table, n_heads, n_kv_heads, head_dim, max_blocks, total_blocks,
+                                n_layers, tokens_per_block, layer, window, stream);
     CELLM_API_END(report_exception)
 }
 

@@ -200,14 +200,60 @@ hipError_t launch_kv_read_q8(const int8_t* kc, const float* ks, const int8_t* vc
 hipError_t launch_kv_accept(void* kc, float* ks, void* vc, float* vs, int units, int row_bytes, int tables,
                             const int32_t* ctx, const int32_t* accepted, int most, int tree, int tpb, int max_blocks,
                             int total_blocks, const uint32_t* bt, hipStream_t st);
-// Attention over pages that `per` consecutive rows share (attention_paged.hip): of 8-bit pages (ks, vs) or f16
-// ones (null), up to each row's position, or (masks) of the nodes of trees drafted behind ctx positions.
+// What pages hold: f16, or codes of 8 or 4 bits with their scales (kv_pages.hpp)
+enum KvFormat : int { KV_F16 = 0, KV_Q8 = 1, KV_Q4 = 2 };
+// A serving step (kv_step.hip): its pages and rows from the sessions' lengths ...
+struct KvPlanArgs {
+    const int32_t* ctx;      // tokens held; lens_out may be the same array
+    const int32_t* add;      // tokens asked for; < 0: finished
+    int tables;
+    uint32_t* bt;
+    int max_blocks, total_blocks, tpb;
+    uint32_t* free_blocks;
+    const int32_t* free_count;
+    int free_capacity;
+    int32_t* lens_out;
+    int32_t* free_out;       // may be free_count
+    int32_t* starts;
+    int32_t* pos;
+    int32_t* slots;
+    int rows;
+};
+hipError_t launch_kv_plan(const KvPlanArgs& a, hipStream_t st);
+// ... and q and k normed per head (weights null: not), rotated (cos_sin null: not), k and v written by slot.
+struct NormRopeArgs {
+    const float* q;
+    const float* k;
+    const float* v;
+    float* q_out;
+    const void* q_weight;
+    const void* k_weight;
+    int weight_dtype;
+    float eps;
+    const int32_t* pos;
+    const int32_t* slots;
+    const float* cos_sin;
+    int table_positions, interleaved;
+    void* kc;
+    void* ks;
+    void* vc;
+    void* vs;
+};
+hipError_t launch_norm_rope_write(const NormRopeArgs& n, int rows, int n_heads, int head_dim, int fmt, const KvGeom& g,
+                                  hipStream_t st);  // g.bt and g.max_blocks are not used
+hipError_t launch_kv_read_q4(const void* kc, const void* ks, const void* vc, const void* vs, const int32_t* pos, int rows,
+                             int per, int head_dim, const KvGeom& g, void* k_out, void* v_out, int out_dtype, hipStream_t st);
+// Attention over pages that `per` consecutive rows share (attention_paged.hip), or (starts) the rows starts[t] ..
+// starts[t + 1] - 1 of table t: up to each row's position, or (masks) of the nodes of trees drafted behind ctx positions.
 struct PagedAttnArgs {
     const float* q;
     const void* kc;
-    const float* ks;
+    const void* ks;          // 8-bit pages: f32; 4-bit ones: words of scale and base
     const void* vc;
-    const float* vs;
+    const void* vs;
+    int fmt;                 // KvFormat
+    const int32_t* starts;   // [tables + 1], or null; 4-bit pages only
+    int tables;              // of starts
     KvGeom g;
     const int32_t* pos;      // [rows]; with masks the contexts, [rows / per]
     const uint64_t* masks;   // [rows][words], or null
@@ -221,6 +267,7 @@ constexpr int kMaxTree = 256;  // nodes of a drafted tree
 // every one, then the splits' sums.
 size_t attention_paged_workspace_bytes(const PagedAttnArgs& a);
 hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipStream_t st);
+hipError_t launch_attention_q4(const PagedAttnArgs& a, hipStream_t st);  // over 4-bit pages, no scratch
 
 // First maximum per row (non-finite -> -inf): chunk blocks of 4096 elements in one launch; rows past
 // one chunk need scratch of argmax_scratch_bytes whose first argmax_counter_bytes (the per-row

@@ -23,6 +23,7 @@
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "kv_pages.hpp"
 
 #pragma clang fp contract(off)  // RoPE's products and sums are rounded one by one, as in decode.hip
 
@@ -31,17 +32,6 @@ namespace cellm {
 namespace {
 
 constexpr int kThreads = 256;
-
-// vector number of token `slot` of row table `table` for head 0, or -1: no position, or its page is missing
-__device__ __forceinline__ long long vector_of(const KvGeom& g, int table, int slot)
-{
-    if (slot < 0) return -1;
-    const int b = slot / g.tpb;
-    if (b >= g.max_blocks) return -1;
-    const uint32_t blk = g.bt[(size_t)table * g.max_blocks + b];
-    if (blk >= (uint32_t)g.total_blocks) return -1;
-    return ((long long)blk * g.n_layers + g.layer) * g.n_kv * (long long)g.tpb + (slot - b * g.tpb);
-}
 
 struct WriteArgs {
     const float* q;       // nullptr: no q
@@ -103,34 +93,13 @@ __global__ __launch_bounds__(kThreads) void kv_write_q8_kernel(const WriteArgs a
     }
     const long long v0 = vector_of(a.g, r / a.per, slot);
     if (v0 < 0) return;  // the same for the whole team
-    uint32_t m = 0;      // |x| in the order of its bits: NaN above infinity above the finite
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu);
-    m = team_max_u32<T>(m);
-    float s = __builtin_bit_cast(float, m) / 127.0f;
-    if (!(s >= 1.1754943508222875e-38f)) s = 0.0f;
-    s = fminf(s, 0x1.0204060000000p+121f);  // 127 of it are finite: the quotient of the largest f32 is rounded up
-    const bool finite = m < 0x7F800000u;
-    uint32_t w[2] = {0, 0};
-    if (finite && s > 0.0f) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int c = (int)fminf(fmaxf(rintf(x[i] / s), -127.0f), 127.0f);
-            w[i >> 2] |= (uint32_t)(c & 0xFF) << (8 * (i & 3));
-        }
-    }
+    uint32_t w[2];
+    const float s = quantise8<T>(x, w);
     const size_t vn = (size_t)v0 + (size_t)kvh * a.g.tpb;
     int8_t* dst = (is_v ? a.vc : a.kc) + vn * HD;
     *reinterpret_cast<uint32_t*>(dst + e0) = w[0];
     *reinterpret_cast<uint32_t*>(dst + e1) = w[1];
-    if (l == 0) (is_v ? a.vs : a.ks)[vn] = finite ? s : __builtin_nanf("");
-}
-
-__device__ __forceinline__ uint16_t bf16_rne(float v)
-{
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0x7FC0;
-    return (uint16_t)((u + 0x7FFFu + (u >> 16 & 1u)) >> 16);
+    if (l == 0) (is_v ? a.vs : a.ks)[vn] = s;
 }
 
 // E codes per thread, one 16-byte store of the output (eight 2-byte or four 4-byte values); a row

@@ -57,7 +57,7 @@ def _stream_ptr(stream):
 class _Dtypes:
     """torch dtypes that the paged-cache calls take, looked up on first use (this module is imported without torch)."""
 
-    names = dict(f32=("float32",), i8=("int8",), i32=("int32", "uint32"), i64=("int64", "uint64"),
+    names = dict(f32=("float32",), i8=("int8",), u8=("uint8",), i32=("int32", "uint32"), i64=("int64", "uint64"),
                  half=("float16", "int16", "uint16"), floats=("float32", "float16", "bfloat16"))
 
     def __getattr__(self, kind):
@@ -691,6 +691,102 @@ class HipOps:
         check(fn(self._h, *cache, bt, max_blocks, total_blocks, self._ptr("context_lens", context_lens_i32, _DT.i32, tables),
                  self._ptr("accepted", accepted_i32, _DT.i32, tables * most), most, tables, tree, n_kv_heads, head_dim,
                  n_layers, tokens_per_block, _stream_ptr(stream)))
+
+    # ---- a step whose lengths the device knows, and the 4-bit paged cache: uint8 codes [total_blocks][n_layers][n_kv_heads]
+    # [tokens_per_block][head_dim / 2] with float16 (scale, base) [..., head_dim / 32, 2]
+
+    def _q4_ptrs(self, kcodes, kscale, vcodes, vscale, head_dim: int, vectors: int):
+        codes, scales = vectors * head_dim // 2, vectors * head_dim // 16
+        return (self._ptr("kcodes", kcodes, _DT.u8, codes), self._ptr("kscale", kscale, _DT.half, scales),
+                self._ptr("vcodes", vcodes, _DT.u8, codes), self._ptr("vscale", vscale, _DT.half, scales))
+
+    def encode_kv_plan(self, context_lens_i32, new_lens_i32, block_tables, total_blocks: int, tokens_per_block: int,
+                       free_blocks, free_count_i32, lens_out, free_out, row_starts, positions, slots, stream=None) -> None:
+        """Pages and rows of a step from the sessions' lengths (cellm_hip_kv_plan): sessions hold context_lens tokens and
+        ask for new_lens more (< 0: finished).  Writes block_tables [sessions][max_blocks], free_blocks, lens_out (may be
+        context_lens), free_out [1] (may be free_count), row_starts [sessions + 1], positions and slots [rows]."""
+        if block_tables.dim() != 2:
+            raise ValueError(f"block_tables {tuple(block_tables.shape)} is not [sessions][pages]")
+        (tables, max_blocks), rows, i32 = block_tables.shape, positions.numel(), _DT.i32
+        check(self._lib.cellm_hip_kv_plan(
+            self._h, self._ptr("context_lens", context_lens_i32, i32, tables), self._ptr("new_lens", new_lens_i32, i32, tables),
+            tables, self._ptr("block_tables", block_tables, i32, tables * max_blocks), max_blocks, total_blocks,
+            tokens_per_block, self._ptr("free_blocks", free_blocks, i32, free_blocks.numel()),
+            self._ptr("free_count", free_count_i32, i32, 1), free_blocks.numel(), self._ptr("lens_out", lens_out, i32, tables),
+            self._ptr("free_out", free_out, i32, 1), self._ptr("row_starts", row_starts, i32, tables + 1),
+            self._ptr("positions", positions, i32, rows), self._ptr("slots", slots, i32, rows), rows, _stream_ptr(stream)))
+
+    def encode_norm_rope_kv_write(self, q, k, v, q_out, n_heads: int, n_kv_heads: int, head_dim: int, q_weight, k_weight,
+                                  eps: float, positions_i32, cos_sin, slots_i32, kcache, vcache, total_blocks: int,
+                                  n_layers: int, tokens_per_block: int, layer: int, kscale=None, vscale=None,
+                                  stream=None) -> None:
+        """Norm of each head of q and k, RoPE, and K and V into the pages by slot (cellm_hip_norm_rope_kv_write_*); q_out
+        may be q.  Weights [head_dim] or None (not normed), cos_sin or None (not rotated).  Pages by their type: float16
+        (or its bits), int8 codes or, for 4 bits, uint8 codes, these two with their scales."""
+        rows, vectors = positions_i32.numel(), total_blocks * n_layers * n_kv_heads * tokens_per_block
+        n, nq = rows * n_kv_heads * head_dim, rows * n_heads * head_dim
+        weights = [w for w in (q_weight, k_weight) if w is not None]
+        if len(weights) == 2 and q_weight.dtype != k_weight.dtype:
+            raise TypeError("q_weight and k_weight must share a dtype")
+        if kscale is None or kcache.dtype not in _DT.u8:
+            cache = self._pages(kcache, vcache, kscale, vscale, head_dim, vectors)
+            fn = self._lib.cellm_hip_norm_rope_kv_write_f16 if kscale is None else self._lib.cellm_hip_norm_rope_kv_write_q8
+        else:
+            if vscale is None:
+                raise ValueError("kscale and vscale go together")
+            cache = self._q4_ptrs(kcache, kscale, vcache, vscale, head_dim, vectors)
+            fn = self._lib.cellm_hip_norm_rope_kv_write_q4
+        check(fn(
+            self._h, self._ptr("q", q, _DT.f32, nq), self._ptr("k", k, _DT.f32, n), self._ptr("v", v, _DT.f32, n),
+            self._ptr("q_out", q_out, _DT.f32, nq),
+            None if q_weight is None else self._ptr("q_weight", q_weight, _DT.floats, head_dim),
+            None if k_weight is None else self._ptr("k_weight", k_weight, _DT.floats, head_dim),
+            _torch_dtype_code(weights[0]) if weights else DTYPE_F32, eps, rows, n_heads, n_kv_heads, head_dim,
+            self._ptr("positions", positions_i32, _DT.i32, rows),
+            None if cos_sin is None else self._ptr("cos_sin", cos_sin, _DT.f32, cos_sin.shape[0] * head_dim),
+            0 if cos_sin is None else cos_sin.shape[0], self._ptr("slots", slots_i32, _DT.i32, rows), *cache, total_blocks,
+            n_layers, tokens_per_block, layer, _stream_ptr(stream)))
+
+    def encode_kv_read_q4(self, kcodes, kscale, vcodes, vscale, block_tables, positions_i32, k_out, v_out,
+                          n_kv_heads: int, head_dim: int, total_blocks: int, n_layers: int, tokens_per_block: int,
+                          layer: int, rows_per_table: int = 1, stream=None) -> None:
+        """encode_kv_read_q8 of 4-bit pages (cellm_hip_kv_read_q4)."""
+        rows = positions_i32.numel()
+        n = rows * n_kv_heads * head_dim
+        if k_out.dtype != v_out.dtype:
+            raise TypeError("k_out and v_out must share a dtype")
+        bt, max_blocks = self._table_ptr(block_tables, rows, rows_per_table)
+        cache = self._q4_ptrs(kcodes, kscale, vcodes, vscale, head_dim,
+                              total_blocks * n_layers * n_kv_heads * tokens_per_block)
+        check(self._lib.cellm_hip_kv_read_q4(
+            self._h, *cache, bt, max_blocks, total_blocks, self._ptr("positions", positions_i32, _DT.i32, rows), rows,
+            rows_per_table, n_kv_heads, head_dim, n_layers, tokens_per_block, layer, _torch_dtype_code(k_out),
+            self._ptr("k_out", k_out, _DT.floats, n), self._ptr("v_out", v_out, _DT.floats, n), _stream_ptr(stream)))
+
+    def encode_attention_q4(self, q, kcodes, kscale, vcodes, vscale, block_tables, positions_i32, out, n_heads: int,
+                            n_kv_heads: int, head_dim: int, total_blocks: int, n_layers: int, tokens_per_block: int,
+                            layer: int, attn_scale: float | None = None, soft_cap: float | None = None, window: int = 0,
+                            rows_per_table: int = 1, row_starts_i32=None, stream=None) -> None:
+        """encode_attention over 4-bit pages (cellm_hip_attention_gqa_q4kv).  row_starts_i32 [sessions + 1]: rows
+        row_starts[t] .. row_starts[t + 1] - 1 are session t's (encode_kv_plan), instead of rows_per_table each."""
+        rows = positions_i32.numel()
+        n = rows * n_heads * head_dim
+        if row_starts_i32 is None:
+            tables, starts = 0, None
+            bt, max_blocks = self._table_ptr(block_tables, rows, rows_per_table)
+        else:
+            tables = row_starts_i32.numel() - 1
+            if rows_per_table != 1 or tables < 0:
+                raise ValueError("row_starts [sessions + 1] take the place of rows_per_table")
+            starts = self._ptr("row_starts", row_starts_i32, _DT.i32, tables + 1)
+            bt, max_blocks = self._table_ptr(block_tables, tables, 1)
+        cache = self._q4_ptrs(kcodes, kscale, vcodes, vscale, head_dim,
+                              total_blocks * n_layers * n_kv_heads * tokens_per_block)
+        check(self._lib.cellm_hip_attention_gqa_q4kv(
+            self._h, self._ptr("q", q, _DT.f32, n), *cache, bt, max_blocks, total_blocks,
+            self._ptr("positions", positions_i32, _DT.i32, rows), rows, rows_per_table, starts, tables, n_heads, n_kv_heads,
+            head_dim, n_layers, tokens_per_block, layer, 0.0 if attn_scale is None else attn_scale,
+            0.0 if soft_cap is None else soft_cap, window, self._ptr("out", out, _DT.f32, n), _stream_ptr(stream)))
 
     def release_graph_scratch(self) -> None:
         """Frees what the context keeps for captured graphs, none of which is launched again: for programs that capture

@@ -678,6 +678,106 @@ int32_t cellm_hip_kv_accept_q8(cellm_hip_ctx_t* ctx, int8_t* kcodes, float* ksca
                                int64_t tree, int64_t n_kv_heads, int64_t head_dim, int64_t n_layers,
                                int64_t tokens_per_block, void* stream);
 
+/* ---- a serving step over a paged cache whose lengths only the device knows ----------
+ * cellm_hip_kv_plan makes a step's pages and rows from the sessions' lengths,
+ * cellm_hip_norm_rope_kv_write_* puts the rows' K and V into the pages by its slots, and
+ * cellm_hip_attention_gqa_q4kv takes its rows as they are: the host needs to know no length,
+ * so that a step (and a graph of it) is the same launches whatever the sessions hold. */
+
+/* The pages and rows of a step (the counterpart of the reference's BlockAllocator and
+ * PageTable, crates/cellm-cache/src/allocator.rs:11-93, pagetable.rs:8-120, which run on
+ * the host).  Session t of `tables` holds context_lens[t] tokens in the first
+ * ceil(context_lens[t] / tokens_per_block) entries of its row of block_tables and asks for
+ * new_lens[t] more; 0 asks for none, and with new_lens[t] < 0 the session is finished and
+ * gives its pages back.  context_lens[t] < 0: no session.
+ *   - The pages of finished sessions go behind the free_count[0] entries of free_blocks, in
+ *     the order of sessions and positions (entries that are no page are left out, and so
+ *     is what does not fit into free_capacity).
+ *   - Sessions are then served in order, up to the first for whose pages or rows
+ *     there is no room: it and those after it get nothing and wait.  (A session that asks
+ *     for more than max_blocks * tokens_per_block positions hold gets nothing, and is passed
+ *     over.)  Pages are taken from the end of the free list, and their numbers written
+ *     behind the session's own in block_tables; other entries are left as they are.
+ *   - lens_out[t]: tokens held after the step (0: finished).  May be context_lens itself.
+ *     free_out[0]: pages left in the list.  May be free_count itself.
+ *   - row_starts [tables + 1]: the rows of session t are row_starts[t] .. row_starts[t + 1]
+ *     - 1, none if it waits.  positions and slots [rows]: each row's position, and its slot
+ *     block * tokens_per_block + position % tokens_per_block (-1 where its page is missing);
+ *     both are -1 for the rows behind the last.
+ * Sessions hold different pages, and the arrays do not overlap otherwise.  Up to 2^20 tables,
+ * rows and pages of a table, 2^30 positions of a table and 2^31 slots. */
+int32_t cellm_hip_kv_plan(cellm_hip_ctx_t* ctx, const int32_t* context_lens, const int32_t* new_lens, int64_t tables,
+                          uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks, int64_t tokens_per_block,
+                          uint32_t* free_blocks, const int32_t* free_count, int64_t free_capacity, int32_t* lens_out,
+                          int32_t* free_out, int32_t* row_starts, int32_t* positions, int32_t* slots, int64_t rows,
+                          void* stream);
+
+/* Norm of every head of q and k, RoPE and the K/V write in one launch (the q_norm and k_norm
+ * of models that have them, before cellm_hip_rope_kv_write_f16 and its 8-bit form):
+ *   y = (x * inv) * w,  inv = f32(1 / sqrt(sum x^2 / head_dim + eps)),
+ * the sum and the root in 64 bits, then the rotation of each row's position (pairs as
+ * cellm_hip_set_rope_interleaved says, table as cellm_hip_rope_half_f32) -- q to q_out (may be
+ * q itself, and overlaps it in no other way), k and v into `layer` of the pages at each
+ * row's slot (cellm_hip_kv_plan); q, k and v are otherwise left as they were.  q_weight and
+ * k_weight [head_dim] in weight_dtype; NULL: that one is not normed.  cos_sin NULL: no
+ * rotation.  A row of position < 0 is skipped and its q_out left as it was; a slot < 0 or past
+ * the pages writes no K and V.  The rows of one call go to different slots.  Limits as
+ * cellm_hip_rope_kv_write_q8; f16 pages of cellm_hip_kv_write_f16, 8-bit pages of
+ * cellm_hip_kv_write_q8, or 4-bit pages: */
+int32_t cellm_hip_norm_rope_kv_write_f16(cellm_hip_ctx_t* ctx, const float* q, const float* k, const float* v, float* q_out,
+                                         const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+                                         int64_t rows, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                         const int32_t* positions, const float* cos_sin, int64_t table_positions,
+                                         const int32_t* slots, uint16_t* kcache, uint16_t* vcache, int64_t total_blocks,
+                                         int64_t n_layers, int64_t tokens_per_block, int64_t layer, void* stream);
+int32_t cellm_hip_norm_rope_kv_write_q8(cellm_hip_ctx_t* ctx, const float* q, const float* k, const float* v, float* q_out,
+                                        const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+                                        int64_t rows, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                        const int32_t* positions, const float* cos_sin, int64_t table_positions,
+                                        const int32_t* slots, int8_t* kcodes, float* kscales, int8_t* vcodes, float* vscales,
+                                        int64_t total_blocks, int64_t n_layers, int64_t tokens_per_block, int64_t layer,
+                                        void* stream);
+int32_t cellm_hip_norm_rope_kv_write_q4(cellm_hip_ctx_t* ctx, const float* q, const float* k, const float* v, float* q_out,
+                                        const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+                                        int64_t rows, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                        const int32_t* positions, const float* cos_sin, int64_t table_positions,
+                                        const int32_t* slots, uint8_t* kcodes, uint16_t* kscales, uint8_t* vcodes,
+                                        uint16_t* vscales, int64_t total_blocks, int64_t n_layers, int64_t tokens_per_block,
+                                        int64_t layer, void* stream);
+
+/* ---- the 4-bit paged cache -------------------------------------------------------
+ * Vectors numbered as those of the 8-bit cache, each of head_dim / 2 bytes of codes (dim i is
+ * nibble i % 2 of byte i / 2, the low one first) and head_dim / 32 pairs of f16 (scale s, base z),
+ * one for 32 neighbouring dims, both arrays 16-byte aligned: 5 bits an element.  With f32 arithmetic,
+ * every operation rounded once,
+ *   z = f16(min), s = f16((max - z) / 15), c = clamp(rint((x - z) / s), 0, 15)
+ * and a code stands for f16(c * s + z), rounded once (s one step smaller where the last
+ * code would stand for an infinity; codes 0 where s is 0).  Elements beyond f16's range are held
+ * to its ends; 32 dims with an infinity or a NaN read as NaN.  The reference's low-bit cache
+ * (crates/cellm-cache/src/kvcache.rs:792-1205) is its counterpart; format and layout are
+ * this library's own. */
+
+/* The values at each row's position as cellm_hip_kv_read_q8: f16 values, widened to f32
+ * exactly, or rounded once more to bf16. */
+int32_t cellm_hip_kv_read_q4(cellm_hip_ctx_t* ctx, const uint8_t* kcodes, const uint16_t* kscales, const uint8_t* vcodes,
+                             const uint16_t* vscales, const uint32_t* block_tables, int64_t max_blocks, int64_t total_blocks,
+                             const int32_t* positions, int64_t rows, int64_t rows_per_table, int64_t n_kv_heads,
+                             int64_t head_dim, int64_t n_layers, int64_t tokens_per_block, int64_t layer, int32_t out_dtype,
+                             void* k_out, void* v_out, void* stream);
+
+/* cellm_hip_attention_gqa_q8kv over 4-bit pages.  With row_starts (NULL: rows_per_table
+ * consecutive rows share a table) the rows row_starts[t] .. row_starts[t + 1] - 1 are those of
+ * table t, in any number and none (prompts and decoding sessions in one call;
+ * cellm_hip_kv_plan's): row_starts [tables + 1] rises from 0 up to `rows` at most, and rows from
+ * row_starts[tables] on are left as they were; rows_per_table is 1 then.  Without row_starts
+ * `tables` is ignored. */
+int32_t cellm_hip_attention_gqa_q4kv(cellm_hip_ctx_t* ctx, const float* q, const uint8_t* kcodes, const uint16_t* kscales,
+                                     const uint8_t* vcodes, const uint16_t* vscales, const uint32_t* block_tables,
+                                     int64_t max_blocks, int64_t total_blocks, const int32_t* positions, int64_t rows,
+                                     int64_t rows_per_table, const int32_t* row_starts, int64_t tables, int64_t n_heads,
+                                     int64_t n_kv_heads, int64_t head_dim, int64_t n_layers, int64_t tokens_per_block,
+                                     int64_t layer, float attn_scale, float soft_cap, int64_t window, float* out, void* stream);
+
 /* MetalOps::encode_silu_mul_f32_inplace (metal.rs:232-243, the CPU loop of
  * llama.rs:477-484): gate[i] = silu(gate[i]) * up[i], silu(g) = g / (1 + exp(-g)),
  * in place on gate. */
