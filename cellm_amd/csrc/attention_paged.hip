@@ -50,6 +50,7 @@
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "kv_pages.hpp"
 
 #pragma clang fp contract(off)
 
@@ -167,14 +168,14 @@ __device__ __forceinline__ uint64_t visible(const PagedAttnArgs& a, const Sight&
 }
 
 // vector number of head kvh at position p, or -1 where its page is missing
-template <bool Q8>
+template <int F>
 __device__ __forceinline__ long long vector_at(const KvGeom& g, int table, int p, int kvh)
 {
     const int b = p / g.tpb;
     const uint32_t blk = g.bt[(size_t)table * g.max_blocks + b];
     if (blk >= (uint32_t)g.total_blocks) return -1;
     const long long page = (long long)blk * g.n_layers + g.layer;
-    if constexpr (Q8) return (page * g.n_kv + kvh) * g.tpb + (p - b * g.tpb);
+    if constexpr (F != KV_F16) return (page * g.n_kv + kvh) * g.tpb + (p - b * g.tpb);
     else return (page * g.tpb + (p - b * g.tpb)) * g.n_kv + kvh;
 }
 
@@ -183,11 +184,28 @@ __device__ __forceinline__ float capped(const PagedAttnArgs& a, float s)
     return a.cap > 0.0f ? tanhf(s / a.cap) * a.cap : s;
 }
 
-// The units of positions lo, lo + step, ... below up of one (row, head) over f16 pages by plain f32 sums, the whole block:
+// Eight dims of a vector of f16 or 4-bit pages, from dim 8 i on; none (< 0): a missing page counts as zeros
+template <int F, int HD>
+__device__ __forceinline__ h8_t eight_dims(const void* pages, const void* scales, long long v, int i)
+{
+    h8_t x = {};
+    if (v < 0) return x;
+    if constexpr (F == KV_F16) return static_cast<const h8_t*>(pages)[v * (HD / 8) + i];
+    const uint32_t w = static_cast<const uint32_t*>(pages)[v * (HD / 8) + i], m = static_cast<const uint32_t*>(scales)[v * (HD / 32) + i / 4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const h2_t y = values4(w >> (4 * j) & 0x000F000Fu, as_h2(both_low(m)), as_h2(both_high(m)));
+        x[j] = y[0];
+        x[j + 4] = y[1];
+    }
+    return x;
+}
+
+// The units of positions lo, lo + step, ... below up of one (row, head) over f16 or 4-bit pages by plain f32 sums, the whole block:
 // reference R, log2(e) times the largest score, sum l of the weights and, in threads below HD, the weighted sum of V
 // (returned).  A unit at a time: a score per thread, then HD threads per position.  For columns whose sums in f16 parts are not finite: inf * lo may be NaN where
 // inf * v is not, and so is the 0 * inf of a position that the column does not see.
-template <int HD, int UNIT>
+template <int F, int HD, int UNIT>
 __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table, int row, int head, int lo, int up, int step,
                              bool part, unsigned char* lds, float& R, float& l)
 {
@@ -198,11 +216,10 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
     const float* qr = a.q + ((size_t)row * a.n_heads + head) * HD;
     const auto score = [&](long long v) {
         float d = 0.0f;
-        const u4_t* src = reinterpret_cast<const u4_t*>(static_cast<const uint16_t*>(a.kc) + v * HD);
 #pragma unroll 1
         for (int i = 0; i < HD / 8; ++i) {
-            // a missing page counts as zeros, of which an element of q that is not finite makes NaN
-            const h8_t w = __builtin_bit_cast(h8_t, v >= 0 ? src[i] : u4_t{0, 0, 0, 0});
+            // of a missing page's zeros an element of q that is not finite makes NaN
+            const h8_t w = eight_dims<F, HD>(a.kc, a.ks, v, i);
 #pragma unroll
             for (int j = 0; j < 8; ++j) d = d + qr[8 * i + j] * (float)w[j];
         }
@@ -221,7 +238,7 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
     float mt = -INFINITY;
 #pragma unroll 1
     for (int p = lo + t; p < up; p += step)
-        if (t < UNIT && si.sees(p)) mt = fmaxf(mt, score(vector_at<false>(a.g, table, p, kvh)));
+        if (t < UNIT && si.sees(p)) mt = fmaxf(mt, score(vector_at<F>(a.g, table, p, kvh)));
     const float m = reduce(mt, [](float x, float y) { return fmaxf(x, y); });
     R = m * kLog2e;
     constexpr int NP = kThreads / HD;
@@ -233,7 +250,7 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
         long long v = -1;
         float w = 0.0f;
         if (t < UNIT && p < up && si.sees(p)) {
-            v = vector_at<false>(a.g, table, p, kvh);
+            v = vector_at<F>(a.g, table, p, kvh);
             const float s = score(v);
             // a range whose scores are all -inf weighs nothing beside others, and its l = NaN says that there were some;
             // a NaN among them (m leaves it out) has the weight NaN, which o brings to every split
@@ -246,8 +263,13 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
         ws[t] = w;
         __syncthreads();
 #pragma unroll 1
-        for (int j = t / HD; j < min(UNIT, up - p0); j += NP)
-            o = o + ws[j] * (vec[j] >= 0 ? (float)static_cast<const _Float16*>(a.vc)[vec[j] * HD + d] : 0.0f);
+        for (int j = t / HD; j < min(UNIT, up - p0); j += NP) {
+            const h8_t w = eight_dims<F, HD>(a.vc, a.vs, vec[j], d / 8);
+            float x = (float)w[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) x = d % 8 == i ? (float)w[i] : x;
+            o = o + ws[j] * x;
+        }
     }
     l = reduce(lt, [](float x, float y) { return x + y; });
     __syncthreads();
@@ -260,11 +282,38 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
     return o;
 }
 
-// Positions lo..hi - 1 that the columns of a set may see; false: none of its rows has a position.
-__device__ __forceinline__ bool set_range(const MmaArgs& A, int set, int& lo, int& hi)
+// The table of a set, its rows, and the set's first column among those of the table
+struct Span {
+    int table, row0, rows, col0;
+};
+// RAGGED (4-bit pages): table t has the rows starts[t] .. starts[t + 1] - 1.  Its sets are numbered from
+// floor(starts[t] group / cols) + t on, which leaves it at least as many numbers as it has tiles, so that a set finds its table by
+// a search alone; numbers behind its last tile are sets without columns.
+template <bool RAGGED>
+__device__ __forceinline__ Span span_of(const MmaArgs& A, int set)
 {
     const PagedAttnArgs& a = A.a;
-    const int table = A.tiles == 1 ? set : set / A.tiles, c0 = (set - table * A.tiles) * A.cols;
+    if (RAGGED && a.starts) {
+        const auto start = [&](int t) { return min(max(a.starts[t], 0), a.rows); };
+        const auto base = [&](int t) { return start(t) * A.group / A.cols + t; };
+        int lo = 0, hi = a.tables;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (base(mid) <= set) lo = mid;
+            else hi = mid;
+        }
+        const int row0 = start(lo);
+        return {lo, row0, max(start(lo + 1) - row0, 0), (set - base(lo)) * A.cols};
+    }
+    const int table = A.tiles == 1 ? set : set / A.tiles;
+    return {table, table * a.per, a.per, (set - table * A.tiles) * A.cols};
+}
+
+// Positions lo..hi - 1 that the columns of a set may see; false: none of its rows has a position.
+__device__ __forceinline__ bool set_range(const MmaArgs& A, const Span& sp, int& lo, int& hi)
+{
+    const PagedAttnArgs& a = A.a;
+    const int table = sp.table, c0 = sp.col0;
     lo = A.cap;
     hi = 0;
     if (a.masks) {
@@ -274,9 +323,9 @@ __device__ __forceinline__ bool set_range(const MmaArgs& A, int set, int& lo, in
         lo = a.window > 0 ? min(max(c - a.window + 1, 0), hi - 1) : 0;  // a position at least: rows that see none get zeros
         return true;
     }
-    const int j1 = min(a.per - 1, (c0 + A.cols - 1) / A.group);
+    const int j1 = min(sp.rows - 1, (c0 + A.cols - 1) / A.group);
     for (int j = c0 / A.group; j <= j1; ++j) {
-        const int p = a.pos[table * a.per + j];
+        const int p = a.pos[sp.row0 + j];
         if (p < 0) continue;
         const int end = min(p, A.cap - 1) + 1;
         hi = max(hi, end);
@@ -286,6 +335,7 @@ __device__ __forceinline__ bool set_range(const MmaArgs& A, int set, int& lo, in
 }
 
 struct Work {
+    Span span;
     int set, lo, hi, step;      // units of positions lo, lo + step, ... below hi (-1: below the columns' ends)
     int split, splits, slot0;   // slot0: work number of the set's split 0
 };
@@ -293,27 +343,31 @@ struct Work {
 // Work number w of a kv head.  SPLITS: every wave looks at all sets (64 lanes, up to 4 sets each): their positions in units
 // of UNIT add up to the work, each set gets as many splits as units, in shares of the same size for all (so that
 // contexts of different lengths end together) and at most kMaxSplits, and the splits are numbered through.
-template <int UNIT, bool SPLITS>
+template <int UNIT, bool SPLITS, bool RAGGED>
 __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
 {
     const int lane = threadIdx.x & 63;
     if (!SPLITS || A.want == 0) {
-        k = Work{A.sets - 1 - w, 0, -1, UNIT, 0, 1, 0};  // a prompt's last rows, which see the most, first
+        k = Work{{}, A.sets - 1 - w, 0, -1, UNIT, 0, 1, 0};  // a prompt's last rows, which see the most, first
         if (k.set < 0) return false;
+        k.span = span_of<RAGGED>(A, k.set);
+        if (RAGGED && k.span.col0 >= k.span.rows * A.group) return false;
         if (!A.a.masks && A.a.window == 0) return true;  // all from 0 on: how far, the columns will say
-        if (!set_range(A, k.set, k.lo, k.hi)) return false;
+        if (!set_range(A, k.span, k.lo, k.hi)) return false;
         k.lo = rfl(k.lo) & ~63;
         k.hi = rfl(k.hi);
         return true;
     }
     constexpr int N = kPlanSets / 64;
     int units[N], from[N], to[N], total = 0;
+    Span spans[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         units[i] = from[i] = to[i] = 0;
         if (64 * i >= A.sets) continue;  // the same for the whole wave
         const int e = lane + 64 * i;
-        if (e < A.sets && set_range(A, e, from[i], to[i])) {
+        spans[i] = span_of<RAGGED>(A, min(e, A.sets - 1));
+        if (e < A.sets && set_range(A, spans[i], from[i], to[i])) {
             from[i] &= ~63;
             units[i] = (to[i] - from[i] + UNIT - 1) / UNIT;
         }
@@ -340,6 +394,14 @@ __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
             const int src = __builtin_ctzll(hit);
             found = true;
             k.set = src + 64 * i;
+            if constexpr (RAGGED) {
+                k.span.table = __builtin_amdgcn_readlane(spans[i].table, src);
+                k.span.row0 = __builtin_amdgcn_readlane(spans[i].row0, src);
+                k.span.rows = __builtin_amdgcn_readlane(spans[i].rows, src);
+                k.span.col0 = __builtin_amdgcn_readlane(spans[i].col0, src);
+            } else {
+                k.span = span_of<false>(A, k.set);
+            }
             k.splits = __builtin_amdgcn_readlane(n, src);
             k.slot0 = __builtin_amdgcn_readlane(first, src);
             k.split = w - k.slot0;
@@ -352,10 +414,12 @@ __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
     return found;
 }
 
-template <bool Q8, int HD, int CT = 1>
+template <int F, int HD, int CT = 1>
 struct Shape {
-    static constexpr int CH = Q8 ? (HD == 64 || (HD == 128 && CT == 1) ? 64 : 32) : HD == 64 ? 64 : 32;  // positions of a chunk
-    static constexpr int ES = Q8 ? 1 : 2;                    // bytes of an element of K and V
+    static constexpr bool Q8 = F == KV_Q8, Q4 = F == KV_Q4;
+    // positions of a chunk
+    static constexpr int CH = Q4 ? 64 : Q8 ? (HD == 64 || (HD == 128 && CT == 1) ? 64 : 32) : HD == 64 ? 64 : 32;
+    static constexpr int VB = Q4 ? HD / 2 : Q8 ? HD : 2 * HD;  // bytes of a vector of K and V
     static constexpr int KK = Q8 ? HD / 64 : HD / 32;        // k steps of a K tile
     static constexpr int QP = Q8 ? 3 : 2;                    // parts of q
     static constexpr int NE = Q8 ? 16 : 8;                   // elements of q of a lane and k step: NE (4 kk + g) + 0, 1, ...
@@ -382,6 +446,14 @@ __device__ __forceinline__ void pairs_of_codes(uint32_t a, uint32_t b, uint32_t 
 constexpr float kHugeKey = 0x1p80f;
 constexpr int kHugeShift = 40;
 
+// 4-bit pages: an f16 below 2^-14 has its bits in the low end of its fraction, and the matrix unit adds products aligned
+// by their exponents as if it had 2^-14 (values of 2.5e-7 in all pages: the output 1.9e-5 off, 244 times what others have,
+// 2^-14 over those).  Where the groups of a chunk are all that small, s and z are taken 2^10 times larger, which makes
+// the values exactly that much larger: c s + z is a multiple of 2^-24 and below 2^-13 has 11 bits at most.
+constexpr float kTinyUp = 0x1p10f;
+constexpr uint32_t kTinyScale = 0x0040, kTinyBase = 0x0400;  // the f16 2^-18 and 2^-14: values below 2^-13
+__device__ __forceinline__ bool tiny_group(uint32_t m) { return (m & 0x7FFFu) < kTinyScale && (m >> 16 & 0x7FFFu) < kTinyBase; }
+
 // Three digits leave every element a rounding of 2^-23 of the largest, f32 one of 2^-25 of itself, beside sums that cost
 // some 2^-24: heads whose largest |q| is more than kLoud times the mean |q| take the fourth digit (normally distributed
 // elements have 3 to 5 times).  Error of the output with one element 30 and 300 times the others, where the keys hold
@@ -393,12 +465,13 @@ constexpr float kLoud = 8.0f;
 // q's parts of a column, the B operands of the scores, and the scale that is left out of them: for scales of the keys as
 // they are and, of 8-bit pages, for those of a chunk with huge ones (kHugeKey).  8-bit pages: the fourth digits, and
 // whether some column of the wave needs them.
-template <bool Q8, int HD>
-__device__ __forceinline__ void q_parts(const PagedAttnArgs& a, const f4_t (&qf)[Shape<Q8, HD>::KK][Shape<Q8, HD>::NE / 4],
-                                        u4_t (&d)[Shape<Q8, HD>::KK][Shape<Q8, HD>::QP], u4_t (&low)[Shape<Q8, HD>::KK],
+template <int F, int HD>
+__device__ __forceinline__ void q_parts(const PagedAttnArgs& a, const f4_t (&qf)[Shape<F, HD>::KK][Shape<F, HD>::NE / 4],
+                                        u4_t (&d)[Shape<F, HD>::KK][Shape<F, HD>::QP], u4_t (&low)[Shape<F, HD>::KK],
                                         bool& loud, float (&qsc)[2])
 {
-    using S = Shape<Q8, HD>;
+    using S = Shape<F, HD>;
+    constexpr bool Q8 = S::Q8;
     uint32_t mx = 0;  // |q| in the order of its bits; f16 pages: of the finite ones
     float sum = 0.0f;
 #pragma unroll
@@ -438,7 +511,7 @@ __device__ __forceinline__ void q_parts(const PagedAttnArgs& a, const f4_t (&qf)
                 h2_t hi, lo;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const int x = 2 * i + j;
+                    const int x = S::Q4 ? i + 4 * j : 2 * i + j;  // 4-bit pages: nibbles i and i + 4 of a word
                     const float v = ldexpf(qf[kk][x >> 2][x & 3], e);
                     hi[j] = (_Float16)v;
                     lo[j] = finite_f32(v) ? (_Float16)(v - (float)hi[j]) : (_Float16)0.0f;
@@ -546,13 +619,22 @@ __device__ __forceinline__ void weigh(const float (&s)[NP], float cs, const floa
     }
 }
 
-// Words of four (8-bit) or two (f16) dims at eight positions as the V^T operands of those dims
-template <bool Q8>
-__device__ __forceinline__ void v_operands(const uint32_t (&r)[8], u4_t (&vt)[Q8 ? 4 : 2])
+// Words of four (8-bit) or two (f16) dims at eight positions as the V^T operands of those dims; of eight dims
+// (4-bit, with their scale words m) those of the lower (HALF 0) or upper four.
+template <int F, int HALF = 0>
+__device__ __forceinline__ void v_operands(const uint32_t (&r)[8], const uint32_t (&m)[F == KV_Q4 ? 8 : 1], u4_t (&vt)[F == KV_F16 ? 2 : 4])
 {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if constexpr (Q8) {
+        if constexpr (F == KV_Q4) {
+            // nibble e of both positions' halves
+            uint32_t y[4];
+            four_values4(__builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], HALF ? 0x07060302u : 0x05040100u),
+                         as_h2(__builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x05040100u)),
+                         as_h2(__builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x07060302u)), y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vt[e][i] = y[e];
+        } else if constexpr (F == KV_Q8) {
             uint32_t y[4];
             pairs_of_codes(r[2 * i], r[2 * i + 1], y);
 #pragma unroll
@@ -573,7 +655,7 @@ __device__ __forceinline__ float score_of(int hi, int mid, int lo, float ks)
 // ---- a block's results: its sums where the set is split, else the quotients; the sums of splits added by the last ----
 // COLS columns of a set from column col0 of the table on; a split's sums: [COLS][HD], then R and l, [COLS] each.  Sets of
 // 32 columns are taken where they leave kWideBlocks blocks, and split where there are fewer than kPlanBlocks: never.
-template <int HD, int COLS>
+template <int F, int HD, int COLS>
 struct Results {
     static constexpr bool kSplits = COLS == kCols;
     static_assert(kSplits || kWideBlocks >= kPlanBlocks);
@@ -583,17 +665,17 @@ struct Results {
     int table, col0, kvh;
     __amdgpu_buffer_rsrc_t part;
     __device__ __forceinline__ Results(const MmaArgs& A_, const Work& k_, int kvh_)
-        : A(A_), k(k_), table(A_.tiles == 1 ? k_.set : k_.set / A_.tiles), col0((k_.set - table * A_.tiles) * COLS), kvh(kvh_), part(buffer_rsrc(A_.part, A_.part_bytes))
+        : A(A_), k(k_), table(k_.span.table), col0(k_.span.col0), kvh(kvh_), part(buffer_rsrc(A_.part, A_.part_bytes))
     {
     }
-    __device__ __forceinline__ int columns() const { return min(A.a.per * A.group - col0, COLS); }
+    __device__ __forceinline__ int columns() const { return min(k.span.rows * A.group - col0, COLS); }
     struct Column {
         int row, head;
     };
     __device__ __forceinline__ Column column(int x) const
     {
         const int j = (col0 + x) / A.group;
-        return {table * A.a.per + j, kvh * A.group + (col0 + x) - j * A.group};
+        return {k.span.row0 + j, kvh * A.group + (col0 + x) - j * A.group};
     }
     __device__ __forceinline__ size_t offset(Column c) const { return ((size_t)c.row * A.a.n_heads + c.head) * HD; }  // in q and out
     __device__ __forceinline__ uint32_t part_of(int sp) const { return (uint32_t)((k.slot0 + sp) * A.a.g.n_kv + kvh) * kPart; }
@@ -609,7 +691,7 @@ struct Results {
         st_agent(part, part_of(k.split) + COLS * HD + x, r);
         st_agent(part, part_of(k.split) + COLS * (HD + 1) + x, ll);
     }
-    // f16 pages: the columns whose bits `again` has by plain sums; the whole block
+    // f16 and 4-bit pages: the columns whose bits `again` has by plain sums; the whole block
     template <int UNIT>
     __device__ void put_plain(uint32_t again, unsigned char* lds) const
     {
@@ -622,7 +704,7 @@ struct Results {
             Sight sc;
             sight_of(A.a, A.cap, table, c.row, sc);
             float mm, ll;
-            const float v = plain_range<HD, UNIT>(A.a, sc, table, c.row, c.head, k.lo, sc.end, k.step, kSplits && k.splits > 1, lds, mm, ll);
+            const float v = plain_range<F, HD, UNIT>(A.a, sc, table, c.row, c.head, k.lo, sc.end, k.step, kSplits && k.splits > 1, lds, mm, ll);
             const int t = threadIdx.x;
             if (kSplits && k.splits > 1) {
                 if (t < HD) st_agent(part, part_of(k.split) + x * HD + t, v);
@@ -714,16 +796,19 @@ struct Results {
 };
 
 // One set of 16 CT columns a block; its waves take chunks of the positions in turn and meet in LDS.
-template <bool Q8, int HD, int CT, bool CAP>
+template <int F, int HD, int CT, bool CAP>
 __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A)
 {
-    using S = Shape<Q8, HD, CT>;
+    using S = Shape<F, HD, CT>;
+    constexpr bool Q8 = S::Q8, Q4 = S::Q4;
     constexpr int CH = S::CH, NT = CH / 16, NP = CH / 4, KS = CH / 32;  // K tiles; positions of a lane; k steps of V
-    constexpr int KK = S::KK, QP = S::QP, NE = S::NE, DT = S::DT, VW = DT * S::ES / 4;  // VW: words of V per lane and position
+    constexpr int KK = S::KK, QP = S::QP, NE = S::NE, DT = S::DT, VB = S::VB;
+    constexpr int VW = (VB / 16 + 3) / 4;                               // words of V per lane and position (a half: 4 bits, 64 dims)
+    constexpr int KR = Q4 ? (KK + 3) / 4 : KK, G = Q4 ? HD / 32 : 1;    // loads of K per lane and tile; scale words of a vector
     constexpr int NR = HD / 4 < 32 ? HD / 4 : 32;                       // registers of O^T that the waves add at a time
     constexpr bool kQInLds = HD > 128 || CT > 1;                        // q's parts in LDS, for want of registers
     constexpr int COLS = kCols * CT;
-    constexpr bool kSplits = Results<HD, COLS>::kSplits;
+    constexpr bool kSplits = Results<F, HD, COLS>::kSplits;
     constexpr int kMergeBytes = std::max(kWaves * NR * 64 * 4, kSplits ? COLS * kMaxSplits * 8 : 0);
     __shared__ __align__(16) unsigned char merge[kMergeBytes];
     __shared__ __align__(16) u4_t qlds[kQInLds ? CT * KK * QP * 64 : 1];
@@ -731,6 +816,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     __shared__ uint32_t loud_lds[CT];
     __shared__ __align__(16) uint32_t kidx[kWaves][CH], vidx[kWaves][CH];  // [c][tile], [g][j]
     __shared__ __align__(16) float kscl[kWaves][Q8 ? CH : 4], vscl[kWaves][Q8 ? CH : 4];
+    __shared__ __align__(16) uint32_t kmeta[kWaves][Q4 ? G * CH : 4], vmeta[kWaves][Q4 ? G * CH : 4];  // [group], then as kidx and vidx
     __shared__ float ml[kWaves][2][COLS], lsum[kSplits ? COLS : 1], qs_lds[2][COLS];
     __shared__ uint32_t flags, here;
     __shared__ int last;
@@ -740,8 +826,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     const int c = lane & 15, g4 = lane >> 4;
     const int kvh = blockIdx.x;
     Work k;
-    if (!plan<kWaves * CH, kSplits>(A, blockIdx.y + gridDim.y * blockIdx.z, k)) return;  // the same for the whole block
-    const Results<HD, COLS> res(A, k, kvh);
+    if (!plan<kWaves * CH, kSplits, Q4>(A, blockIdx.y + gridDim.y * blockIdx.z, k)) return;  // the same for the whole block
+    const Results<F, HD, COLS> res(A, k, kvh);
     const int table = res.table, n_cols = res.columns();
 
     // ---- the first chunk's page entries, q, and what this lane's column sees: loads that do not wait for each other
@@ -768,11 +854,12 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             const auto x = res.column(min(kCols * u + c, n_cols - 1));
             at[u] = res.offset(x);
             if (makes(u)) {
-                const f4_t* src = reinterpret_cast<const f4_t*>(a.q + at[u] + NE * g4);
+                // 4-bit pages: the words of the lane's loads of K, each a k step
+                const f4_t* src = reinterpret_cast<const f4_t*>(a.q + at[u] + (Q4 ? (HD == 64 ? 16 : 32) : NE) * g4);
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-                    for (int i = 0; i < NE / 4; ++i) qf[u][kk][i] = src[NE * kk + i];
+                    for (int i = 0; i < NE / 4; ++i) qf[u][kk][i] = src[(Q4 ? kk / 4 * 32 + kk % 4 * 2 : NE * kk) + i];
             }
             si[u] = Sight{0, 0, 0, a.masks};
             has[u] = sight_of(a, A.cap, table, x.row, si[u]) && kCols * u + c < n_cols;
@@ -790,7 +877,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         for (int u = 0; u < CT; ++u) {
             if (!makes(u)) continue;
             u4_t low[KK];
-            q_parts<Q8, HD>(a, qf[u], qp[u], low, loud, qsc[u]);
+            q_parts<F, HD>(a, qf[u], qp[u], low, loud, qsc[u]);
             if (Q8 && (kQInLds || (loud && wave == 0))) {
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) qlow[(u * KK + kk) * 64 + lane] = low[kk];
@@ -832,8 +919,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         else return qp[u][kk][p];
     };
     bool coarse = false;  // F is not 1 somewhere
-    const unsigned char* const kbase = static_cast<const unsigned char*>(a.kc) + 16 * g4;
-    const unsigned char* const vbase = static_cast<const unsigned char*>(a.vc) + DT * S::ES * c;
+    const unsigned char* const kbase = static_cast<const unsigned char*>(a.kc) + (VB == 32 ? 8 : 16) * g4;
+    const unsigned char* const vbase = static_cast<const unsigned char*>(a.vc) + VB / 16 * c;
 
     // A chunk's loads are issued an iteration ahead, into the registers that its predecessor has just used: K and the
     // scales after the scores, V after the weighted sums, page entries two chunks ahead.  The last iteration loads too:
@@ -842,8 +929,9 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     int b_of;                           // its place in the table
     unsigned long long miss, miss_next; // positions without a page, or past the range
     float ks_own = 0.0f, vs_own = 0.0f;
-    u4_t kr[NT][KK];
+    u4_t kr[NT][KR];
     uint32_t vr[NP][VW];
+    uint32_t km[G], vm[G];              // 4-bit pages: the scale words of this lane's position
     uint32_t vn = 0;
     const auto load_page = [&](int p0) {
         b_of = block_of(p0 + (lane & (CH - 1)));
@@ -854,8 +942,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         const bool ok = pp < k.hi && b_of < a.g.max_blocks && blk < (uint32_t)a.g.total_blocks;
         const uint32_t page = blk * (uint32_t)a.g.n_layers + (uint32_t)a.g.layer, off = (uint32_t)(pp - b_of * a.g.tpb);
         // where there is none: the last vector again, loaded but not used
-        vn = !ok ? vn : Q8 ? (page * (uint32_t)a.g.n_kv + (uint32_t)kvh) * (uint32_t)a.g.tpb + off
-                           : (page * (uint32_t)a.g.tpb + off) * (uint32_t)a.g.n_kv + (uint32_t)kvh;
+        vn = !ok ? vn : F != KV_F16 ? (page * (uint32_t)a.g.n_kv + (uint32_t)kvh) * (uint32_t)a.g.tpb + off
+                                      : (page * (uint32_t)a.g.tpb + off) * (uint32_t)a.g.n_kv + (uint32_t)kvh;
         miss_next = __ballot(!ok);
         wave_lds_fence();
         if (lane < CH) {  // position 16 tile + 4 i + g
@@ -870,19 +958,44 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             ks_own = static_cast<const float*>(a.ks)[vn];
             vs_own = static_cast<const float*>(a.vs)[vn];
         }
+        if constexpr (Q4) {
+            const auto meta = [&](const void* from, uint32_t (&to)[G]) {
+                const uint32_t* src = static_cast<const uint32_t*>(from) + (size_t)vn * G;
+                if constexpr (G == 2) {
+                    const u2_t m = *reinterpret_cast<const u2_t*>(src);
+                    to[0] = m[0];
+                    to[1] = m[1];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < G / 4; ++i) {
+                        const u4_t m = reinterpret_cast<const u4_t*>(src)[i];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) to[4 * i + x] = m[x];
+                    }
+                }
+            };
+            meta(a.ks, km);
+            meta(a.vs, vm);
+        }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            const unsigned char* src = kbase + (size_t)kidx[wave][c * NT + i] * (HD * S::ES);
+            const unsigned char* src = kbase + (size_t)kidx[wave][c * NT + i] * VB;
+            if constexpr (VB == 32) {
+                const u2_t w = *reinterpret_cast<const u2_t*>(src);
+                kr[i][0] = u4_t{w[0], w[1], 0, 0};
+            } else {
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) kr[i][kk] = *reinterpret_cast<const u4_t*>(src + 64 * kk);
+                for (int kk = 0; kk < KR; ++kk) kr[i][kk] = *reinterpret_cast<const u4_t*>(src + 64 * kk);
+            }
         }
         asm volatile("" ::: "memory");  // issued here
     };
     const auto load_v = [&]() {
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-            const unsigned char* src = vbase + (size_t)vidx[wave][g4 * NP + j] * (HD * S::ES);
-            if constexpr (VW == 1) vr[j][0] = *reinterpret_cast<const uint32_t*>(src);
+            const unsigned char* src = vbase + (size_t)vidx[wave][g4 * NP + j] * VB;
+            if constexpr (VB == 32) vr[j][0] = *reinterpret_cast<const uint16_t*>(src);
+            else if constexpr (VW == 1) vr[j][0] = *reinterpret_cast<const uint32_t*>(src);
             else if constexpr (VW == 2) {
                 const u2_t v = *reinterpret_cast<const u2_t*>(src);
                 vr[j][0] = v[0];
@@ -899,6 +1012,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         asm volatile("" ::: "memory");
     };
     const int step = k.step;
+    bool first = true, vup = false;     // 4-bit pages: no chunk yet; V's sums are kTinyUp times larger
     if (p0 < k.hi) {
         b_of = b_first;
         blk = blk_first;
@@ -920,14 +1034,53 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                 vscl[wave][g * NP + 4 * tile + i] = gone ? 0.0f : vs_own;
             }
         }
+        bool ktiny = false;
+        if constexpr (Q4) {
+            const int tile = lane >> 4, i = lane >> 2 & 3, g = lane & 3;
+            const bool gone = miss >> lane & 1;  // a missing page counts as zeros
+            bool kt = true, vt = true;
+#pragma unroll
+            for (int x = 0; x < G; ++x) {
+                km[x] = gone ? 0 : km[x];
+                vm[x] = gone ? 0 : vm[x];
+                kt = kt && tiny_group(km[x]);
+                vt = vt && tiny_group(vm[x]);
+            }
+            const h2_t up = {(_Float16)kTinyUp, (_Float16)kTinyUp};
+            ktiny = __ballot(kt) == ~0ull;
+            if (ktiny) {
+#pragma unroll
+                for (int x = 0; x < G; ++x) km[x] = as_u32(as_h2(km[x]) * up);
+            }
+            // V's sums hold one factor: larger values end it
+            const bool small = __ballot(vt) == ~0ull;
+            if (first && small) vup = true;
+            if (vup && !small) {
+                vup = false;
+#pragma unroll
+                for (int u = 0; u < CT; ++u)
+#pragma unroll
+                    for (int e = 0; e < DT; ++e) m[u].o[e] = m[u].o[e] * (1.0f / kTinyUp);
+            }
+            if (vup) {
+#pragma unroll
+                for (int x = 0; x < G; ++x) vm[x] = as_u32(as_h2(vm[x]) * up);
+            }
+            first = false;
+#pragma unroll
+            for (int x = 0; x < G; ++x) {
+                kmeta[wave][x * CH + (4 * g + i) * NT + tile] = km[x];
+                vmeta[wave][x * CH + g * NP + 4 * tile + i] = vm[x];
+            }
+        }
         index(p0 + step);
         load_page(p0 + 2 * step);
-        if (!Q8 && miss) {  // a missing page counts as zeros, and so do the positions past the range
+        if (F == KV_F16 && miss) {  // a missing page counts as zeros, and so do the positions past the range
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
                 const bool gone = miss >> (16 * i + 4 * (c & 3) + (c >> 2)) & 1;
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk) kr[i][kk] = gone ? u4_t{0, 0, 0, 0} : kr[i][kk];
+                for (int kk = 0; kk < KR; ++kk) kr[i][kk] = gone ? u4_t{0, 0, 0, 0} : kr[i][kk];
             }
         }
         h8_t ph[CT][KS], pl[CT][KS];
@@ -950,11 +1103,23 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                     for (int x = 0; x < 4; ++x) s[4 * i + x] = score_of(d[2][x], d[1][x], d[0][x], ksv[x]);
                 } else {
                     f4_t d = {0.0f, 0.0f, 0.0f, 0.0f};
+                    u4_t kt[KK];
+#pragma unroll
+                    for (int kk = 0; kk < KK; ++kk) {
+                        if constexpr (Q4) {
+                            const uint32_t m = kmeta[wave][(HD == 64 ? g4 >> 1 : kk / 4 * 4 + g4) * CH + c * NT + i];
+                            uint32_t y[4];
+                            four_values4(kr[i][kk / 4][kk % 4], as_h2(both_low(m)), as_h2(both_high(m)), y);
+                            kt[kk] = u4_t{y[0], y[1], y[2], y[3]};
+                        } else {
+                            kt[kk] = kr[i][kk];
+                        }
+                    }
 #pragma unroll
                     for (int p = 1; p >= 0; --p)  // the low parts first
 #pragma unroll
                         for (int kk = 0; kk < KK; ++kk)
-                            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, kr[i][kk]),
+                            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, kt[kk]),
                                                                        __builtin_bit_cast(h8_t, q_part(u, p, kk)), d, 0, 0, 0);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) s[4 * i + x] = d[x];
@@ -976,6 +1141,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             }
             if (u == CT - 1) load_k();
             float cs = huge ? qsc[u][1] : qsc[u][0];
+            if (Q4 && ktiny) cs = cs * (1.0f / kTinyUp);
             if constexpr (CAP) {
 #pragma unroll
                 for (int j = 0; j < NP; ++j) s[j] = capped(a, s[j] * cs);
@@ -995,7 +1161,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             weigh<Q8>(s, cs, vs, partial, vis, coarse, m[u], ph[u], pl[u]);
         }
         // ---- O^T += V^T . P^T
-        if (!Q8 && miss) {
+        if (F == KV_F16 && miss) {
 #pragma unroll
             for (int j = 0; j < NP; ++j)
 #pragma unroll
@@ -1005,21 +1171,30 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         for (int x = 0; x < VW; ++x)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                constexpr int E = Q8 ? 4 : 2;  // tiles of a word
-                uint32_t r[8];
-                u4_t vt[E];
+                constexpr int E = F == KV_F16 ? 2 : 4, W = Q4 && VB > 32 ? 8 : E;  // tiles at a time, and of a word
+                uint32_t r[8], mw[Q4 ? 8 : 1];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[j] = vr[8 * ks + j][x];
-                v_operands<Q8>(r, vt);
+                if constexpr (Q4) {
 #pragma unroll
-                for (int e = 0; e < E; ++e)
+                    for (int j = 0; j < 8; ++j) mw[j] = vmeta[wave][c * HD / 512 * CH + g4 * NP + 8 * ks + j];
+                }
+                const auto tiles = [&](auto half) {
+                    constexpr int H = decltype(half)::value;
+                    u4_t vt[E];
+                    v_operands<F, H>(r, mw, vt);
 #pragma unroll
-                    for (int u = 0; u < CT; ++u) {
-                        const h8_t v = __builtin_bit_cast(h8_t, vt[e]);
-                        f4_t& o = m[u].o[E * x + e];
-                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u][ks], o, 0, 0, 0);
-                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u][ks], o, 0, 0, 0);
-                    }
+                    for (int e = 0; e < E; ++e)
+#pragma unroll
+                        for (int u = 0; u < CT; ++u) {
+                            const h8_t v = __builtin_bit_cast(h8_t, vt[e]);
+                            f4_t& o = m[u].o[W * x + E * H + e];
+                            o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u][ks], o, 0, 0, 0);
+                            o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u][ks], o, 0, 0, 0);
+                        }
+                };
+                tiles(std::integral_constant<int, 0>{});
+                if constexpr (W > E) tiles(std::integral_constant<int, 1>{});
             }
         load_v();
     }
@@ -1036,6 +1211,10 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         if (Q8 && coarse) {
 #pragma unroll
             for (int e = 0; e < DT; ++e) m[u].o[e] = m[u].o[e] / m[u].F;
+        }
+        if (Q4 && vup) {
+#pragma unroll
+            for (int e = 0; e < DT; ++e) m[u].o[e] = m[u].o[e] * (1.0f / kTinyUp);
         }
         if (g4 == 0) {
             ml[wave][0][col] = m[u].R;
@@ -1084,15 +1263,17 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     if constexpr (kSplits) res.combine(here, lsum, &last, merge);
 }
 
-template <typename F>
-void by_shape(bool q8, int head_dim, F&& f)
+template <typename Fn>
+void by_shape(int fmt, int head_dim, Fn&& f)
 {
     const auto with = [&](auto q) {
         if (head_dim == 64) f(q, std::integral_constant<int, 64>{});
         else if (head_dim == 128) f(q, std::integral_constant<int, 128>{});
         else f(q, std::integral_constant<int, 256>{});
     };
-    q8 ? with(std::true_type{}) : with(std::false_type{});
+    if (fmt == KV_Q8) with(std::integral_constant<int, KV_Q8>{});
+    else if (fmt == KV_Q4) with(std::integral_constant<int, KV_Q4>{});
+    else with(std::integral_constant<int, KV_F16>{});
 }
 
 struct Layout {
@@ -1104,17 +1285,25 @@ Layout layout_of(const PagedAttnArgs& a)
 {
     Layout y{};
     y.group = a.n_heads / a.g.n_kv;
-    const long long columns = (long long)a.per * y.group, tables = a.rows / a.per;
-    y.ct = a.head_dim <= 128 && columns > kCols && tables * a.g.n_kv * ((columns + 31) / 32) >= kWideBlocks ? 2 : 1;
-    y.cols = kCols * y.ct;
-    y.tiles = (int)((columns + y.cols - 1) / y.cols);
-    y.sets = (int)(tables * y.tiles);
+    if (a.starts) {  // the host knows no table's rows: their mean, and set numbers for any
+        const long long columns = (long long)a.rows * y.group;
+        const auto sets = [&](int cols) { return columns / cols + a.tables; };
+        y.ct = a.head_dim <= 128 && columns > (long long)kCols * a.tables && a.g.n_kv * sets(32) >= kWideBlocks ? 2 : 1;
+        y.cols = kCols * y.ct;
+        y.tiles = 1;
+        y.sets = (int)sets(y.cols);
+    } else {
+        const long long columns = (long long)a.per * y.group, tables = a.rows / a.per;
+        y.ct = a.head_dim <= 128 && columns > kCols && tables * a.g.n_kv * ((columns + 31) / 32) >= kWideBlocks ? 2 : 1;
+        y.cols = kCols * y.ct;
+        y.tiles = (int)((columns + y.cols - 1) / y.cols);
+        y.sets = (int)(tables * y.tiles);
+    }
     int unit = 0;
-    by_shape(a.fmt == KV_Q8, a.head_dim,
+    by_shape(a.fmt, a.head_dim,
              [&](auto q, auto hd) {
-                 constexpr bool Q8 = decltype(q)::value;
-                 constexpr int HD = decltype(hd)::value;
-                 unit = (y.ct == 2 ? Shape<Q8, HD, 2>::CH : Shape<Q8, HD>::CH) * kWaves;
+                 constexpr int F = decltype(q)::value, HD = decltype(hd)::value;
+                 unit = (y.ct == 2 ? Shape<F, HD, 2>::CH : Shape<F, HD>::CH) * kWaves;
              });
     const long long cap = (long long)a.g.max_blocks * a.g.tpb, units = (cap + unit - 1) / unit;
     const long long blocks = (long long)y.sets * a.g.n_kv;
@@ -1149,14 +1338,13 @@ hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipS
     A.part_bytes = (uint32_t)((size_t)y.works * a.g.n_kv * y.cols * (a.head_dim + 2) * sizeof(float));  // below 2^31: plan()'s blocks
     const unsigned rows_of_grid = (unsigned)std::min<long long>(y.works, 32768);
     const dim3 grid((unsigned)a.g.n_kv, rows_of_grid, (unsigned)((y.works + rows_of_grid - 1) / rows_of_grid));
-    by_shape(a.fmt == KV_Q8, a.head_dim, [&](auto q, auto hd) {
-        constexpr bool Q8 = decltype(q)::value;
-        constexpr int HD = decltype(hd)::value;
+    by_shape(a.fmt, a.head_dim, [&](auto q, auto hd) {
+        constexpr int F = decltype(q)::value, HD = decltype(hd)::value;
         const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, st, A); };
         if constexpr (HD <= 128) {
-            if (y.ct == 2) return a.cap > 0.0f ? go(attn_paged_kernel<Q8, HD, 2, true>) : go(attn_paged_kernel<Q8, HD, 2, false>);
+            if (y.ct == 2) return a.cap > 0.0f ? go(attn_paged_kernel<F, HD, 2, true>) : go(attn_paged_kernel<F, HD, 2, false>);
         }
-        a.cap > 0.0f ? go(attn_paged_kernel<Q8, HD, 1, true>) : go(attn_paged_kernel<Q8, HD, 1, false>);
+        a.cap > 0.0f ? go(attn_paged_kernel<F, HD, 1, true>) : go(attn_paged_kernel<F, HD, 1, false>);
     });
     return hipGetLastError();
 }

@@ -1904,10 +1904,6 @@ int32_t attention_paged_impl(cellm_hip_ctx* ctx, const PagedAttnArgs& in, int64_
     DeviceGuard g(ctx->device);
     const std::lock_guard<std::recursive_mutex> lk(ctx->mu);  // held until the scratch user is enqueued
     const hipStream_t st = pick_stream(ctx, stream);
-    if (a.fmt == KV_Q4) {
-        HIP_TRY(launch_attention_q4(a, st), "attention launch");
-        return CELLM_HIP_OK;
-    }
     float* ws = nullptr;
     if (int32_t rc = get_graph_safe_scratch(ctx, st, attention_paged_workspace_bytes(a), &ws, attention_counter_bytes()))
         return rc;

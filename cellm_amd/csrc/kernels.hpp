@@ -267,7 +267,6 @@ constexpr int kMaxTree = 256;  // nodes of a drafted tree
 // every one, then the splits' sums.
 size_t attention_paged_workspace_bytes(const PagedAttnArgs& a);
 hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipStream_t st);
-hipError_t launch_attention_q4(const PagedAttnArgs& a, hipStream_t st);  // over 4-bit pages, no scratch
 
 // First maximum per row (non-finite -> -inf): chunk blocks of 4096 elements in one launch; rows past
 // one chunk need scratch of argmax_scratch_bytes whose first argmax_counter_bytes (the per-row

@@ -105,5 +105,22 @@ __device__ __forceinline__ h2_t values4(uint32_t codes, h2_t s, h2_t z)
     const h2_t c = as_h2(codes | 0x64006400u) - h2_t{(_Float16)1024.0f, (_Float16)1024.0f};  // the f16 1024 + c, exactly
     return __builtin_elementwise_fma(c, s, z);
 }
+// The same of nibbles 0 .. 3 of both halves of w, 13 instructions: a nibble at bit 4 makes the f16 1024 + 16 c.
+__device__ __forceinline__ void four_values4(uint32_t w, h2_t s, h2_t z, uint32_t (&y)[4])
+{
+    const h2_t k = {(_Float16)1024.0f, (_Float16)1024.0f}, sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f},
+               k16 = {(_Float16)-64.0f, (_Float16)-64.0f};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t x = i ? w >> 8 : w;
+        const h2_t lo = as_h2(and_or(x, 0x000F000Fu, 0x64006400u)) - k;
+        const h2_t hi = __builtin_elementwise_fma(as_h2(and_or(x, 0x00F000F0u, 0x64006400u)), sixteenth, k16);
+        y[2 * i] = as_u32(__builtin_elementwise_fma(lo, s, z));
+        y[2 * i + 1] = as_u32(__builtin_elementwise_fma(hi, s, z));
+    }
+}
+// The lower or upper half of a word in both of them
+__device__ __forceinline__ uint32_t both_low(uint32_t m) { return __builtin_amdgcn_perm(m, m, 0x01000100u); }
+__device__ __forceinline__ uint32_t both_high(uint32_t m) { return __builtin_amdgcn_perm(m, m, 0x03020302u); }
 
 }  // namespace cellm

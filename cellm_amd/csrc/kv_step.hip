@@ -279,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void kv_read_q4_kernel(const uint32_t* __
     const size_t vn = v0 < 0 ? 0 : (size_t)v0 + (size_t)kvh * g.tpb;
     const auto one = [&](const uint32_t* c, const uint32_t* s, void* out) {
         const uint32_t w = v0 < 0 ? 0 : c[vn * T + l], m = v0 < 0 ? 0 : s[vn * (HD / 32) + l / 4];
-        const h2_t sc = as_h2(__builtin_amdgcn_perm(m, m, 0x01000100u)), z = as_h2(__builtin_amdgcn_perm(m, m, 0x03020302u));
+        const h2_t sc = as_h2(both_low(m)), z = as_h2(both_high(m));
         _Float16 x[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {  // nibbles j and j + 4
