@@ -21,78 +21,118 @@ constexpr int kThreads = 256;
 //   it gets them where P <= pages free and R <= rows: in order, up to the first that does not fit.
 // Page i of those handed out (counted over the sessions) is entry count - 1 - i of the free
 // list, after the pages of finished sessions (add < 0) have been put onto its end.
-constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+//
+// Latency bounds it: one block goes over the sessions, a thread each, and what differs in size from session to
+// session (a finished one's pages, a prompt's) is shared out flat, an entry a thread, by a search in the running
+// sums (four entries a thread: 11.3 us for 11.8 where 13 sessions give 1600 pages back, but 6.9 for 5.8 where few do).
+// The rows' positions and slots are filled by the same block where they are few, else by a second launch over
+// the whole chip (kFillRows).  8 sessions that take a token each 4.4 us, 256 with 24 prompts 11.8, 64 prompts of 64 thousand
+// rows 8.4 (one thread per session for all of its pages, and one block for all rows: 6.6, 22 and 73).
+constexpr int kFillRows = 2048;      // 256 sessions: 1024 rows 6.7 us in one launch and 8.2 in two, 4096 9.4 and 8.4, 8192 20.1 and 11.9
+constexpr int kPlanSmall = 256;      // sessions for which a block of 256 threads is launched, not of 1024: 5.8 us at 256, 8.0
+constexpr int kFillThreads = 256;
+constexpr int kFillSessions = 4096;  // of which the filling blocks hold the row starts in LDS
 
-// inclusive sum over the block's threads; scan: kPlanWaves words
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* scan)
+// Running sum of v over the block's threads; sums: a word per wave.  All threads get the block's total.
+template <int N, typename T>
+__device__ __forceinline__ T block_scan(T v, T* sums, T& total)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t u = __shfl_up(v, o);
+        const T u = __shfl_up(v, o);
         if (lane >= o) v += u;
     }
     __syncthreads();
-    if (lane == 63) scan[wave] = v;
+    if (lane == 63) sums[wave] = v;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) v += scan[w];
-    return v;
+    T before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < N / 64; ++w) {
+        if (w < wave) before += sums[w];
+        total += sums[w];
+    }
+    return v + before;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(const KvPlanArgs a)
+// The first of n rising sums that is above i
+__device__ __forceinline__ int above(const uint32_t* sums, int n, uint32_t i)
 {
-    __shared__ uint32_t scan[kPlanWaves];
+    int lo = 0;
+    for (int step = n >> 1; step; step >>= 1)  // n: a power of two
+        if (sums[lo + step - 1] <= i) lo += step;
+    return lo;
+}
+
+__device__ __forceinline__ int slot_of(const KvPlanArgs& a, int session, int pos)
+{
+    const int b = pos / a.tpb;
+    const uint32_t blk = a.bt[(size_t)session * a.max_blocks + b];
+    return blk < (uint32_t)a.total_blocks ? (int)(blk * (uint32_t)a.tpb) + (pos - b * a.tpb) : -1;
+}
+
+// N threads; FILL: the rows too
+template <int N, bool FILL>
+__global__ __launch_bounds__(N) void kv_plan_kernel(const KvPlanArgs a)
+{
+    __shared__ uint32_t sums[N], row_sums[FILL ? N : 1], wave_sums[N / 64];
+    __shared__ unsigned long long wave_pairs[N / 64];
+    __shared__ int held_of[N], lens_of[FILL ? N : 1];
     __shared__ uint32_t last[2];   // pages and rows of the last session that fits
     const int t = threadIdx.x, lane = t & 63;
     const auto pages_of = [&](long long tokens) { return (uint32_t)((tokens + a.tpb - 1) / a.tpb); };
     long long count = max(a.free_count[0], 0);
     if (count > a.free_capacity) count = a.free_capacity;
+    int ctx = t < a.tables ? a.ctx[t] : -1, add = t < a.tables ? a.add[t] : 0;  // of the round at hand
 
     // ---- finished sessions give their pages back, in the order of sessions and positions
-    for (int t0 = 0; t0 < a.tables; t0 += kPlanThreads) {
-        const int s = t0 + t;
-        const int ctx = s < a.tables ? a.ctx[s] : -1, add = s < a.tables ? a.add[s] : 0;
-        uint32_t entries = 0, valid = 0;
-        if (ctx >= 0 && add < 0) entries = min(pages_of(ctx), (uint32_t)a.max_blocks);
-        const auto each = [&](auto&& f) {  // the wave's finished sessions, 64 entries at a time
-            for (unsigned long long todo = __ballot(entries > 0); todo; todo &= todo - 1) {
-                const int src = __builtin_ctzll(todo);
-                const uint32_t n = __shfl(entries, src);
-                const uint32_t* row = a.bt + (size_t)(t0 + (t & ~63) + src) * a.max_blocks;
-                for (uint32_t e0 = 0; e0 < n; e0 += 64) {
-                    const uint32_t blk = e0 + lane < n ? row[e0 + lane] : ~0u;
-                    f(src, blk, __ballot(blk < (uint32_t)a.total_blocks));
-                }
+    for (int t0 = 0; t0 < a.tables; t0 += N) {
+        if (t0) {
+            const int s = t0 + t;
+            ctx = s < a.tables ? a.ctx[s] : -1;
+            add = s < a.tables ? a.add[s] : 0;
+        }
+        const uint32_t entries = ctx >= 0 && add < 0 ? min(pages_of(ctx), (uint32_t)a.max_blocks) : 0;
+        if (!__syncthreads_or(entries > 0)) continue;
+        uint32_t all;
+        sums[t] = block_scan<N>(entries, wave_sums, all);
+        for (uint32_t i0 = 0; i0 < all; i0 += N) {
+            __syncthreads();
+            const uint32_t i = i0 + t;
+            uint32_t blk = ~0u, n;
+            if (i < all) {
+                const int s = above(sums, N, i);
+                blk = a.bt[(size_t)(t0 + s) * a.max_blocks + (i - (s ? sums[s - 1] : 0))];
             }
-        };
-        each([&](int src, uint32_t, unsigned long long there) {
-            if (lane == src) valid += (uint32_t)__popcll(there);
-        });
-        const uint32_t up = block_scan(valid, scan);
-        uint32_t at = up - valid;  // of the pages that this round gives back
-        each([&](int src, uint32_t blk, unsigned long long there) {
-            const uint32_t first = __shfl(at, src);
-            const long long i = count + first + __popcll(there & ((1ull << lane) - 1));
-            if (there >> lane & 1 && i < a.free_capacity) a.free_blocks[i] = blk;
-            if (lane == src) at += (uint32_t)__popcll(there);
-        });
-        __syncthreads();
-        if (t == kPlanThreads - 1) last[0] = up;
-        __syncthreads();
-        count = min(count + last[0], (long long)a.free_capacity);
+            const uint32_t there = blk < (uint32_t)a.total_blocks ? 1 : 0;
+            const long long at = count + block_scan<N>(there, wave_sums, n) - 1;
+            if (there && at < a.free_capacity) a.free_blocks[at] = blk;
+            count = min(count + n, (long long)a.free_capacity);
+        }
     }
     __syncthreads();  // the free list as it is now
+    if (a.tables > N) {
+        ctx = a.ctx[t];
+        add = a.add[t];
+    }
 
     // ---- sessions in order, up to the first whose pages or rows are not there
     long long pages0 = 0, rows0 = 0;  // of the sessions before this round's
     if (t == 0) a.starts[0] = 0;
-    for (int t0 = 0; t0 < a.tables; t0 += kPlanThreads) {
+    for (int t0 = 0; t0 < a.tables; t0 += N) {
         const int s = t0 + t;
-        const int ctx = s < a.tables ? a.ctx[s] : -1, add = s < a.tables ? a.add[s] : 0;
+        if (t0) {
+            ctx = s < a.tables ? a.ctx[s] : -1;
+            add = s < a.tables ? a.add[s] : 0;
+        }
         const bool valid = ctx >= 0 && add > 0 && (long long)ctx + add <= (long long)a.max_blocks * a.tpb;
         const uint32_t held = ctx > 0 ? pages_of(ctx) : 0;
         const uint32_t need = valid ? pages_of((long long)ctx + add) - held : 0;
         const uint32_t asked = valid ? (uint32_t)min(add, a.rows + 1) : 0;
-        const uint32_t p = block_scan(need, scan), r = block_scan(asked, scan);
+        // both sums stay below 2^31: 2^20 pages or rows and one of each of 1024 sessions
+        unsigned long long all;
+        const unsigned long long up = block_scan<N>((unsigned long long)need << 32 | asked, wave_pairs, all);
+        const uint32_t p = (uint32_t)(up >> 32), r = (uint32_t)up;
         const bool fits = pages0 + p <= count && rows0 + r <= a.rows;
         if (t < 2) last[t] = 0;
         __syncthreads();
@@ -102,48 +142,76 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(const KvPlanArgs 
             atomicMax(&last[1], r);
         }
         __syncthreads();
+        const uint32_t pages = last[0], rows = last[1];
+        const int len = fits && valid ? ctx + add : ctx >= 0 && add < 0 ? 0 : ctx;
+        sums[t] = fits ? p : pages;
+        held_of[t] = (int)(held + (fits ? need : 0) - sums[t]);  // entry of page i: held_of + i, of a session that has it
+        if constexpr (FILL) {
+            row_sums[t] = fits ? r : rows;
+            lens_of[t] = len - (int)row_sums[t];
+        }
         if (s < a.tables) {
-            a.starts[s + 1] = (int32_t)(rows0 + (fits ? r : last[1]));
-            a.lens_out[s] = fits && valid ? ctx + add : ctx >= 0 && add < 0 ? 0 : ctx;
+            a.starts[s + 1] = (int32_t)(rows0 + (fits ? r : rows));
+            a.lens_out[s] = len;
         }
-        if (fits && valid) {
-            uint32_t* row = a.bt + (size_t)s * a.max_blocks + held;
-            const uint32_t* top = a.free_blocks + (count - 1 - (pages0 + p - need));
-            for (uint32_t j = 0; j < need; ++j) row[j] = top[-(long long)j];
+        __syncthreads();
+        for (uint32_t i = t; i < pages; i += N) {
+            const int e = above(sums, N, i);
+            a.bt[(size_t)(t0 + e) * a.max_blocks + (held_of[e] + (int)i)] = a.free_blocks[count - 1 - (pages0 + i)];
         }
-        const bool full = !__syncthreads_and(fits);
-        pages0 += last[0];
-        rows0 += last[1];
-        if (full) {  // nothing more fits: the others wait
-            for (int e = t0 + kPlanThreads + t; e < a.tables; e += kPlanThreads) {
+        __syncthreads();
+        if constexpr (FILL) {
+            for (uint32_t i = t; i < rows; i += N) {
+                const int e = above(row_sums, N, i), pos = lens_of[e] + (int)i;
+                a.pos[rows0 + i] = pos;
+                a.slots[rows0 + i] = slot_of(a, t0 + e, pos);
+            }
+        }
+        pages0 += pages;
+        rows0 += rows;
+        if (!__syncthreads_and(fits)) {  // nothing more fits: the others wait
+            for (int e = t0 + N + t; e < a.tables; e += N) {
                 const int c = a.ctx[e];
                 a.starts[e + 1] = (int32_t)rows0;
                 a.lens_out[e] = c >= 0 && a.add[e] < 0 ? 0 : c;
             }
             break;
         }
-        __syncthreads();
     }
     if (t == 0) a.free_out[0] = (int32_t)(count - pages0);
-    __syncthreads();
-
-    // ---- positions and slots of the rows
-    for (int r = t; r < a.rows; r += kPlanThreads) {
-        int pos = -1, slot = -1;
-        if (r < rows0) {
-            int lo = 0, hi = a.tables;  // starts[lo] <= r < starts[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                (a.starts[mid] <= r ? lo : hi) = mid;
-            }
-            pos = a.lens_out[lo] - (a.starts[lo + 1] - r);
-            const int b = pos / a.tpb;
-            const uint32_t blk = a.bt[(size_t)lo * a.max_blocks + b];
-            if (blk < (uint32_t)a.total_blocks) slot = (int)(blk * (uint32_t)a.tpb) + (pos - b * a.tpb);
+    if constexpr (FILL) {
+        for (long long i = rows0 + t; i < a.rows; i += N) {
+            a.pos[i] = -1;
+            a.slots[i] = -1;
         }
-        a.pos[r] = pos;
-        a.slots[r] = slot;
     }
+}
+
+// Positions and slots of many rows, a row a thread, once the sessions have theirs.
+__global__ __launch_bounds__(kFillThreads) void kv_fill_kernel(const KvPlanArgs a)
+{
+    __shared__ int32_t lds[kFillSessions + 1];
+    const bool small = a.tables <= kFillSessions;
+    if (small) {
+        for (int i = threadIdx.x; i <= a.tables; i += kFillThreads) lds[i] = a.starts[i];
+        __syncthreads();
+    }
+    const auto start = [&](int t) { return small ? lds[t] : a.starts[t]; };
+    const int r = (int)(blockIdx.x * kFillThreads + threadIdx.x);
+    if (r >= a.rows) return;
+    int pos = -1, slot = -1;
+    if (r < start(a.tables)) {
+        int lo = 0, hi = a.tables;  // start(lo) <= r < start(hi)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start(mid) <= r) lo = mid;
+            else hi = mid;
+        }
+        pos = a.lens_out[lo] - (start(lo + 1) - r);
+        slot = slot_of(a, lo, pos);
+    }
+    a.pos[r] = pos;
+    a.slots[r] = slot;
 }
 
 // ---- norm, rotation and write ---------------------------------------------------------
@@ -309,7 +377,20 @@ __global__ __launch_bounds__(kThreads) void kv_read_q4_kernel(const uint32_t* __
 
 hipError_t launch_kv_plan(const KvPlanArgs& a, hipStream_t st)
 {
-    hipLaunchKernelGGL(kv_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
+    const auto go = [&](auto n, auto fill) {
+        constexpr int N = decltype(n)::value;
+        hipLaunchKernelGGL((kv_plan_kernel<N, decltype(fill)::value>), dim3(1), dim3(N), 0, st, a);
+    };
+    const auto by_size = [&](auto fill) {
+        if (a.tables <= kPlanSmall) go(std::integral_constant<int, 256>{}, fill);
+        else go(std::integral_constant<int, 1024>{}, fill);
+    };
+    if (a.rows <= kFillRows) {
+        by_size(std::true_type{});
+    } else {
+        by_size(std::false_type{});
+        hipLaunchKernelGGL(kv_fill_kernel, dim3((unsigned)((a.rows + kFillThreads - 1) / kFillThreads)), dim3(kFillThreads), 0, st, a);
+    }
     return hipGetLastError();
 }
 
