@@ -286,9 +286,9 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
 struct Span {
     int table, row0, rows, col0;
 };
-// RAGGED (4-bit pages): table t has the rows starts[t] .. starts[t + 1] - 1.  Its sets are numbered from
-// floor(starts[t] group / cols) + t on, which leaves it at least as many numbers as it has tiles, so that a set finds its table by
-// a search alone; numbers behind its last tile are sets without columns.
+// RAGGED (4-bit pages): table t may have the rows starts[t] .. starts[t + 1] - 1.  Its sets are numbered from
+// floor(starts[t] group / cols) + t on, which leaves it at least as many numbers as it has tiles, so that a set finds its table
+// by a search alone; numbers behind its last tile are sets without columns.
 template <bool RAGGED>
 __device__ __forceinline__ Span span_of(const MmaArgs& A, int set)
 {
@@ -451,8 +451,95 @@ constexpr int kHugeShift = 40;
 // 2^-14 over those).  Where the groups of a chunk are all that small, s and z are taken 2^10 times larger, which makes
 // the values exactly that much larger: c s + z is a multiple of 2^-24 and below 2^-13 has 11 bits at most.
 constexpr float kTinyUp = 0x1p10f;
-constexpr uint32_t kTinyScale = 0x0040, kTinyBase = 0x0400;  // the f16 2^-18 and 2^-14: values below 2^-13
-__device__ __forceinline__ bool tiny_group(uint32_t m) { return (m & 0x7FFFu) < kTinyScale && (m >> 16 & 0x7FFFu) < kTinyBase; }
+constexpr uint32_t kTinyBits = 0x7C007FC0u;  // of a scale word: none of these is set where s < 2^-18 and |z| < 2^-14
+
+// Whether the groups of a chunk are all tiny, K's and V's (the words of a position in every lane)
+template <int G>
+struct Tiny {
+    bool k, v;
+    __device__ __forceinline__ Tiny(const uint32_t (&km)[G], const uint32_t (&vm)[G])
+    {
+        uint32_t kb = km[0], vb = vm[0];
+#pragma unroll
+        for (int x = 1; x < G; ++x) {
+            kb |= km[x];
+            vb |= vm[x];
+        }
+        k = !__ballot(kb & kTinyBits);
+        v = !__ballot(vb & kTinyBits);
+    }
+    // V's sums hold one factor, which larger values end: true where they do
+    __device__ __forceinline__ bool v_factor(bool& first, bool& vup) const
+    {
+        if (first && v) vup = true;
+        first = false;
+        const bool drop = vup && !v;
+        if (drop) vup = false;
+        return drop;
+    }
+    __device__ __forceinline__ void scale(uint32_t (&km)[G], uint32_t (&vm)[G], bool vup) const
+    {
+        const h2_t up = {(_Float16)kTinyUp, (_Float16)kTinyUp};
+        if (k) {
+            asm volatile("");  // a branch
+#pragma unroll
+            for (int x = 0; x < G; ++x) km[x] = as_u32(as_h2(km[x]) * up);
+        }
+        if (vup) {
+            asm volatile("");
+#pragma unroll
+            for (int x = 0; x < G; ++x) vm[x] = as_u32(as_h2(vm[x]) * up);
+        }
+    }
+};
+
+// The scale words of positions without a page become those of zeros; bit of `miss`: the lane's position
+template <int G>
+__device__ __forceinline__ void drop_missing(unsigned long long miss, uint32_t (&km)[G], uint32_t (&vm)[G])
+{
+    if (!miss) return;
+    const bool gone = miss >> (threadIdx.x & 63) & 1;
+#pragma unroll
+    for (int x = 0; x < G; ++x) {
+        km[x] = gone ? 0 : km[x];
+        vm[x] = gone ? 0 : vm[x];
+    }
+}
+
+// BYTES bytes at off of vector `vector` (VB bytes each) of a 4-bit page's codes or scales.  Offsets of 32 bits where the
+// array has no more (BIG: false): one sum beside a base in scalar registers, where an address of 64 bits takes four times
+// that (131072 positions 44 us, 63 with those; both in one kernel behind a branch, which parts what the loads run beside, 55).
+template <bool BIG, int VB, int BYTES>
+__device__ __forceinline__ void load_bytes(const void* base, uint32_t vector, uint32_t off, uint32_t (&to)[(BYTES + 3) / 4])
+{
+    const size_t at = BIG ? (size_t)vector * VB + off : (size_t)(uint32_t)(vector * VB + off);
+    const unsigned char* src = static_cast<const unsigned char*>(base) + at;
+    const auto put = [&](auto v) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 4; ++i) to[i] = v[i];
+    };
+    if constexpr (BYTES == 2) to[0] = *reinterpret_cast<const uint16_t*>(src);
+    else if constexpr (BYTES == 4) to[0] = *reinterpret_cast<const uint32_t*>(src);
+    else if constexpr (BYTES == 8) put(*reinterpret_cast<const u2_t*>(src));
+    else put(*reinterpret_cast<const u4_t*>(src));
+}
+
+// The G scale words of vector vn
+template <bool BIG, int G>
+__device__ __forceinline__ void load_words(const void* from, uint32_t vn, uint32_t (&to)[G])
+{
+    if constexpr (G == 2) {
+        load_bytes<BIG, 8, 8>(from, vn, 0, to);
+    } else {
+#pragma unroll
+        for (int i = 0; i < G / 4; ++i) {
+            uint32_t w[4];
+            load_bytes<BIG, 4 * G, 16>(from, vn, 16 * i, w);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) to[4 * i + x] = w[x];
+        }
+    }
+}
 
 // Three digits leave every element a rounding of 2^-23 of the largest, f32 one of 2^-25 of itself, beside sums that cost
 // some 2^-24: heads whose largest |q| is more than kLoud times the mean |q| take the fourth digit (normally distributed
@@ -468,7 +555,7 @@ constexpr float kLoud = 8.0f;
 template <int F, int HD>
 __device__ __forceinline__ void q_parts(const PagedAttnArgs& a, const f4_t (&qf)[Shape<F, HD>::KK][Shape<F, HD>::NE / 4],
                                         u4_t (&d)[Shape<F, HD>::KK][Shape<F, HD>::QP], u4_t (&low)[Shape<F, HD>::KK],
-                                        bool& loud, float (&qsc)[2])
+                                        bool& loud, float (&qsc)[2], [[maybe_unused]] float fold = 1.0f)
 {
     using S = Shape<F, HD>;
     constexpr bool Q8 = S::Q8;
@@ -480,15 +567,18 @@ __device__ __forceinline__ void q_parts(const PagedAttnArgs& a, const f4_t (&qf)
         for (int i = 0; i < S::NE; ++i) {
             const float x = qf[kk][i >> 2][i & 3];  // a bit_cast of the element itself reads the vector's first
             const uint32_t b = __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu;
-            mx = max(mx, Q8 || b < 0x7F800000u ? b : 0u);
+            mx = max(mx, F != KV_F16 || b < 0x7F800000u ? b : 0u);
             if constexpr (Q8) sum = sum + fabsf(x);
         }
     mx = max(mx, __builtin_bit_cast(uint32_t, lane_xor<16>(__builtin_bit_cast(float, mx), 64)));
     mx = max(mx, __builtin_bit_cast(uint32_t, lane_xor<32>(__builtin_bit_cast(float, mx), 64)));
     const int top = max((int)(mx >> 23), 1) - 127;
-    const bool bad = Q8 && mx >= 0x7F800000u;
+    const bool bad = F != KV_F16 && mx >= 0x7F800000u;
     const int e = mx > 0 && !bad ? (Q8 ? 21 : 13) - top : 0;
-    qsc[0] = bad ? __builtin_nanf("") : ldexpf(a.scale, -e);
+    // 4-bit pages: `fold`, the scores' scale, goes into q and leaves a power of two
+    [[maybe_unused]] int fold_e = 0;
+    [[maybe_unused]] const float fold_m = S::Q4 ? frexpf(fold, &fold_e) : 1.0f;
+    qsc[0] = bad ? __builtin_nanf("") : S::Q4 ? ldexpf(1.0f, fold_e - e) : ldexpf(a.scale, -e);
     qsc[1] = Q8 ? (bad ? __builtin_nanf("") : ldexpf(a.scale, kHugeShift - e)) : 0.0f;
 #pragma unroll
     for (int kk = 0; kk < S::KK; ++kk) {
@@ -511,8 +601,12 @@ __device__ __forceinline__ void q_parts(const PagedAttnArgs& a, const f4_t (&qf)
                 h2_t hi, lo;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const int x = S::Q4 ? i + 4 * j : 2 * i + j;  // 4-bit pages: nibbles i and i + 4 of a word
-                    const float v = ldexpf(qf[kk][x >> 2][x & 3], e);
+                    const int x = S::Q4 ? 4 * (i & 1) + (i >> 1) + 2 * j : 2 * i + j;  // 4-bit pages: the pairs of values4x8
+                    float v = ldexpf(qf[kk][x >> 2][x & 3], e);
+                    if constexpr (S::Q4) {
+                        v = v * fold_m;
+                        asm("" : "+v"(v));  // the f32 product is what both parts are of (v_fma_mixlo_f16 would round the exact one)
+                    }
                     hi[j] = (_Float16)v;
                     lo[j] = finite_f32(v) ? (_Float16)(v - (float)hi[j]) : (_Float16)0.0f;
                 }
@@ -619,6 +713,63 @@ __device__ __forceinline__ void weigh(const float (&s)[NP], float cs, const floa
     }
 }
 
+// Bit j: whether the row sees position p0 + 4 j + g4 (no masks of trees)
+template <int NP>
+__device__ __forceinline__ uint32_t seen_of(const Sight& s, int p0, int g4)
+{
+    const auto below = [&](int end) { return (1u << min(max((end - p0 - g4 + 3) >> 2, 0), NP)) - 1; };  // positions before end
+    return below(s.ctx) & ~below(s.start);
+}
+
+// The reference of a column that has seen nothing: below any score, and finite, so that what is not seen (-inf) weighs 0
+constexpr float kNoScore = -0x1p120f;
+
+// weigh() for 4-bit pages: scores d times the power of two pw are the weights' exponents, so that one fma takes the
+// reference off them exactly; the high parts are cut off, not rounded (the low ones keep 2^-22 of the weight).
+template <int NP, int DT>
+__device__ __forceinline__ void weigh4(float (&d)[NP], float pw, bool partial, uint32_t seen, Sums<DT>& m, h8_t (&ph)[NP / 8],
+                                       h8_t (&pl)[NP / 8])
+{
+    float w[NP], lc, mx;
+    if (partial) {
+        asm volatile("s_nop 0" ::: "memory");  // a branch: few chunks have positions that some row does not see
+#pragma unroll
+        for (int j = 0; j < NP; ++j) d[j] = seen >> j & 1 ? d[j] : -INFINITY;
+    }
+    const auto weights = [&]() {
+        lc = mx = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(d[j], pw, -m.R));
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            lc = lc + w[j];
+            mx = fmaxf(mx, w[j]);
+        }
+    };
+    weights();
+    if (__ballot(mx > 0x1p15f)) {
+        float m1 = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) m1 = fmaxf(m1, d[j] * pw);
+        m1 = fmaxf(m1, lane_xor<16>(m1, 64));
+        m1 = fmaxf(m1, lane_xor<32>(m1, 64));
+        const float up = fmaxf(m.R, m1 - 13.0f);
+        const float ratio = up > m.R ? __builtin_amdgcn_exp2f(m.R - up) : 1.0f;
+        m.l = m.l * ratio;
+        m.R = up;
+#pragma unroll
+        for (int e = 0; e < DT; ++e) m.o[e] = m.o[e] * ratio;
+        weights();
+    }
+    m.l = m.l + lc;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const float hi = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, w[j]) & 0xFFFFE000u);  // f16's bits
+        ph[j >> 3][j & 7] = (_Float16)hi;
+        pl[j >> 3][j & 7] = (_Float16)(w[j] - hi);
+    }
+}
+
 // Words of four (8-bit) or two (f16) dims at eight positions as the V^T operands of those dims; of eight dims
 // (4-bit, with their scale words m) those of the lower (HALF 0) or upper four.
 template <int F, int HALF = 0>
@@ -627,13 +778,12 @@ __device__ __forceinline__ void v_operands(const uint32_t (&r)[8], const uint32_
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if constexpr (F == KV_Q4) {
-            // nibble e of both positions' halves
-            uint32_t y[4];
-            four_values4(__builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], HALF ? 0x07060302u : 0x05040100u),
-                         as_h2(__builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x05040100u)),
-                         as_h2(__builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x07060302u)), y);
+            uint32_t y[4];  // bytes of both positions side by side: dims 0, 2, 1, 3 of the half
+            values4x8(__builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], HALF ? 0x07030602u : 0x05010400u),
+                      as_h2(__builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x05040100u)),
+                      as_h2(__builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x07060302u)), y);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) vt[e][i] = y[e];
+            for (int e = 0; e < 4; ++e) vt[2 * (e & 1) + (e >> 1)][i] = y[e];
         } else if constexpr (F == KV_Q8) {
             uint32_t y[4];
             pairs_of_codes(r[2 * i], r[2 * i + 1], y);
@@ -796,7 +946,7 @@ struct Results {
 };
 
 // One set of 16 CT columns a block; its waves take chunks of the positions in turn and meet in LDS.
-template <int F, int HD, int CT, bool CAP>
+template <int F, int HD, int CT, bool CAP, bool BIG = false>
 __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A)
 {
     using S = Shape<F, HD, CT>;
@@ -866,7 +1016,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             if (!has[u]) si[u] = Sight{0, 0, 0, a.masks};
             b |= ((uint32_t)__ballot(has[u]) & 0xFFFFu) << (kCols * u);
             top = max(top, si[u].end);
-            m[u] = Sums<DT>{-INFINITY, 0.0f, 1.0f, {}};
+            m[u] = Sums<DT>{Q4 ? kNoScore : -INFINITY, 0.0f, 1.0f, {}};
         }
         if (k.hi < 0) k.hi = rfl((int)team_max_u32<16>((uint32_t)top));
         if (t == 0) {
@@ -877,7 +1027,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         for (int u = 0; u < CT; ++u) {
             if (!makes(u)) continue;
             u4_t low[KK];
-            q_parts<F, HD>(a, qf[u], qp[u], low, loud, qsc[u]);
+            q_parts<F, HD>(a, qf[u], qp[u], low, loud, qsc[u], CAP ? a.scale : a.scale * kLog2e);
             if (Q8 && (kQInLds || (loud && wave == 0))) {
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) qlow[(u * KK + kk) * 64 + lane] = low[kk];
@@ -906,7 +1056,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         } else if (Q8 && loud) {
             __syncthreads();  // the same for all waves, whose columns are the same
         }
-        if constexpr (!CAP) {  // and of the exponents
+        if constexpr (!CAP && !Q4) {  // and of the exponents
 #pragma unroll
             for (int u = 0; u < CT; ++u) {
                 qsc[u][0] = qsc[u][0] * kLog2e;
@@ -919,7 +1069,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         else return qp[u][kk][p];
     };
     bool coarse = false;  // F is not 1 somewhere
-    const unsigned char* const kbase = static_cast<const unsigned char*>(a.kc) + (VB == 32 ? 8 : 16) * g4;
+    const unsigned char* const kbase = static_cast<const unsigned char*>(a.kc) + 16 * g4;
     const unsigned char* const vbase = static_cast<const unsigned char*>(a.vc) + VB / 16 * c;
 
     // A chunk's loads are issued an iteration ahead, into the registers that its predecessor has just used: K and the
@@ -932,6 +1082,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     u4_t kr[NT][KR];
     uint32_t vr[NP][VW];
     uint32_t km[G], vm[G];              // 4-bit pages: the scale words of this lane's position
+    constexpr bool kRegs = Q4 && HD <= 128 && CT == 1;
+    uint32_t ki[kRegs ? NT : 1], vi[kRegs ? NP : 1];  // and the vectors that it loads, out of LDS before they are needed
     uint32_t vn = 0;
     const auto load_page = [&](int p0) {
         b_of = block_of(p0 + (lane & (CH - 1)));
@@ -952,6 +1104,12 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             vidx[wave][g * NP + 4 * tile + i] = vn;
         }
         wave_lds_fence();
+        if constexpr (kRegs) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) ki[i] = kidx[wave][c * NT + i];
+#pragma unroll
+            for (int j = 0; j < NP; ++j) vi[j] = vidx[wave][g4 * NP + j];
+        }
     };
     const auto load_k = [&]() {
         if constexpr (Q8) {
@@ -959,53 +1117,52 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             vs_own = static_cast<const float*>(a.vs)[vn];
         }
         if constexpr (Q4) {
-            const auto meta = [&](const void* from, uint32_t (&to)[G]) {
-                const uint32_t* src = static_cast<const uint32_t*>(from) + (size_t)vn * G;
-                if constexpr (G == 2) {
-                    const u2_t m = *reinterpret_cast<const u2_t*>(src);
-                    to[0] = m[0];
-                    to[1] = m[1];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < G / 4; ++i) {
-                        const u4_t m = reinterpret_cast<const u4_t*>(src)[i];
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) to[4 * i + x] = m[x];
-                    }
-                }
-            };
-            meta(a.ks, km);
-            meta(a.vs, vm);
+            load_words<BIG>(a.ks, vn, km);
+            load_words<BIG>(a.vs, vn, vm);
         }
+        if constexpr (Q4) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const unsigned char* src = kbase + (size_t)kidx[wave][c * NT + i] * VB;
-            if constexpr (VB == 32) {
-                const u2_t w = *reinterpret_cast<const u2_t*>(src);
-                kr[i][0] = u4_t{w[0], w[1], 0, 0};
-            } else {
+            for (int i = 0; i < NT; ++i) {
+                const uint32_t vec = kRegs ? ki[i] : kidx[wave][c * NT + i];
 #pragma unroll
-                for (int kk = 0; kk < KR; ++kk) kr[i][kk] = *reinterpret_cast<const u4_t*>(src + 64 * kk);
+                for (int kk = 0; kk < KR; ++kk) {
+                    constexpr int N = VB == 32 ? 8 : 16;
+                    uint32_t w[N / 4];
+                    load_bytes<BIG, VB, N>(a.kc, vec, N * g4 + 64 * kk, w);
+                    kr[i][kk] = N == 8 ? u4_t{w[0], w[1], 0, 0} : u4_t{w[0], w[1], w[N / 4 - 2], w[N / 4 - 1]};
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const unsigned char* src = kbase + (size_t)kidx[wave][c * NT + i] * VB;
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) kr[i][kk] = *reinterpret_cast<const u4_t*>(src + 64 * kk);
             }
         }
         asm volatile("" ::: "memory");  // issued here
     };
     const auto load_v = [&]() {
+        if constexpr (Q4) {
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            const unsigned char* src = vbase + (size_t)vidx[wave][g4 * NP + j] * VB;
-            if constexpr (VB == 32) vr[j][0] = *reinterpret_cast<const uint16_t*>(src);
-            else if constexpr (VW == 1) vr[j][0] = *reinterpret_cast<const uint32_t*>(src);
-            else if constexpr (VW == 2) {
-                const u2_t v = *reinterpret_cast<const u2_t*>(src);
-                vr[j][0] = v[0];
-                vr[j][1] = v[1];
-            } else {
+            for (int j = 0; j < NP; ++j)
+                load_bytes<BIG, VB, VB / 16>(a.vc, kRegs ? vi[j] : vidx[wave][g4 * NP + j], VB / 16 * c, vr[j]);
+        } else {
 #pragma unroll
-                for (int w = 0; w < VW / 4; ++w) {
-                    const u4_t v = *reinterpret_cast<const u4_t*>(src + 16 * w);
+            for (int j = 0; j < NP; ++j) {
+                const unsigned char* src = vbase + (size_t)vidx[wave][g4 * NP + j] * VB;
+                if constexpr (VW == 1) vr[j][0] = *reinterpret_cast<const uint32_t*>(src);
+                else if constexpr (VW == 2) {
+                    const u2_t v = *reinterpret_cast<const u2_t*>(src);
+                    vr[j][0] = v[0];
+                    vr[j][1] = v[1];
+                } else {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) vr[j][4 * w + x] = v[x];
+                    for (int w = 0; w < VW / 4; ++w) {
+                        const u4_t v = *reinterpret_cast<const u4_t*>(src + 16 * w);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) vr[j][4 * w + x] = v[x];
+                    }
                 }
             }
         }
@@ -1037,36 +1194,16 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         bool ktiny = false;
         if constexpr (Q4) {
             const int tile = lane >> 4, i = lane >> 2 & 3, g = lane & 3;
-            const bool gone = miss >> lane & 1;  // a missing page counts as zeros
-            bool kt = true, vt = true;
-#pragma unroll
-            for (int x = 0; x < G; ++x) {
-                km[x] = gone ? 0 : km[x];
-                vm[x] = gone ? 0 : vm[x];
-                kt = kt && tiny_group(km[x]);
-                vt = vt && tiny_group(vm[x]);
-            }
-            const h2_t up = {(_Float16)kTinyUp, (_Float16)kTinyUp};
-            ktiny = __ballot(kt) == ~0ull;
-            if (ktiny) {
-#pragma unroll
-                for (int x = 0; x < G; ++x) km[x] = as_u32(as_h2(km[x]) * up);
-            }
-            // V's sums hold one factor: larger values end it
-            const bool small = __ballot(vt) == ~0ull;
-            if (first && small) vup = true;
-            if (vup && !small) {
-                vup = false;
+            drop_missing(miss, km, vm);  // a missing page counts as zeros
+            const Tiny<G> tiny(km, vm);
+            ktiny = tiny.k;
+            if (tiny.v_factor(first, vup)) {
 #pragma unroll
                 for (int u = 0; u < CT; ++u)
 #pragma unroll
                     for (int e = 0; e < DT; ++e) m[u].o[e] = m[u].o[e] * (1.0f / kTinyUp);
             }
-            if (vup) {
-#pragma unroll
-                for (int x = 0; x < G; ++x) vm[x] = as_u32(as_h2(vm[x]) * up);
-            }
-            first = false;
+            tiny.scale(km, vm, vup);
 #pragma unroll
             for (int x = 0; x < G; ++x) {
                 kmeta[wave][x * CH + (4 * g + i) * NT + tile] = km[x];
@@ -1109,7 +1246,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                         if constexpr (Q4) {
                             const uint32_t m = kmeta[wave][(HD == 64 ? g4 >> 1 : kk / 4 * 4 + g4) * CH + c * NT + i];
                             uint32_t y[4];
-                            four_values4(kr[i][kk / 4][kk % 4], as_h2(both_low(m)), as_h2(both_high(m)), y);
+                            values4x8(kr[i][kk / 4][kk % 4], as_h2(both_low(m)), as_h2(both_high(m)), y);
                             kt[kk] = u4_t{y[0], y[1], y[2], y[3]};
                         } else {
                             kt[kk] = kr[i][kk];
@@ -1144,8 +1281,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             if (Q4 && ktiny) cs = cs * (1.0f / kTinyUp);
             if constexpr (CAP) {
 #pragma unroll
-                for (int j = 0; j < NP; ++j) s[j] = capped(a, s[j] * cs);
-                cs = kLog2e;
+                for (int j = 0; j < NP; ++j) s[j] = Q4 ? capped(a, s[j] * cs) * kLog2e : capped(a, s[j] * cs);
+                cs = Q4 ? 1.0f : kLog2e;
             }
             // ---- weights; of positions that some column does not see, those are 0 whatever they hold
             float vs[NP];
@@ -1153,12 +1290,13 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             for (int j = 0; j < NP; ++j) vs[j] = Q8 ? vscl[wave][g4 * NP + j] : 1.0f;
             const bool partial = __ballot(has[u] && (p0 < si[u].start || p0 + CH > si[u].ctx)) != 0;
             uint64_t vis = ~0ull;  // bit 4 j: position j of this lane
-            if (partial) {
+            if (!Q4 && partial) {
                 vis = visible(a, si[u], p0) >> g4;
 #pragma unroll
                 for (int j = 0; j < NP; ++j) vs[j] = vis >> (4 * j) & 1 ? vs[j] : 0.0f;
             }
-            weigh<Q8>(s, cs, vs, partial, vis, coarse, m[u], ph[u], pl[u]);
+            if constexpr (Q4) weigh4(s, cs, partial, partial ? seen_of<NP>(si[u], p0, g4) : ~0u, m[u], ph[u], pl[u]);
+            else weigh<Q8>(s, cs, vs, partial, vis, coarse, m[u], ph[u], pl[u]);
         }
         // ---- O^T += V^T . P^T
         if (F == KV_F16 && miss) {
@@ -1338,13 +1476,26 @@ hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipS
     A.part_bytes = (uint32_t)((size_t)y.works * a.g.n_kv * y.cols * (a.head_dim + 2) * sizeof(float));  // below 2^31: plan()'s blocks
     const unsigned rows_of_grid = (unsigned)std::min<long long>(y.works, 32768);
     const dim3 grid((unsigned)a.g.n_kv, rows_of_grid, (unsigned)((y.works + rows_of_grid - 1) / rows_of_grid));
+    // whether offsets in the codes of 4-bit pages take more than 32 bits
+    const bool big = ((unsigned long long)a.g.total_blocks * a.g.n_layers * a.g.n_kv * a.g.tpb * (a.head_dim / 2)) >> 32 != 0;
     by_shape(a.fmt, a.head_dim, [&](auto q, auto hd) {
         constexpr int F = decltype(q)::value, HD = decltype(hd)::value;
         const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, st, A); };
-        if constexpr (HD <= 128) {
-            if (y.ct == 2) return a.cap > 0.0f ? go(attn_paged_kernel<F, HD, 2, true>) : go(attn_paged_kernel<F, HD, 2, false>);
+        const auto by_size = [&](auto ct, auto wide) {
+            constexpr int CT = decltype(ct)::value;
+            constexpr bool BIG = decltype(wide)::value;
+            a.cap > 0.0f ? go(attn_paged_kernel<F, HD, CT, true, BIG>) : go(attn_paged_kernel<F, HD, CT, false, BIG>);
+        };
+        const auto by_columns = [&](auto wide) {
+            if constexpr (HD <= 128) {
+                if (y.ct == 2) return by_size(std::integral_constant<int, 2>{}, wide);
+            }
+            by_size(std::integral_constant<int, 1>{}, wide);
+        };
+        if constexpr (F == KV_Q4) {
+            if (big) return by_columns(std::true_type{});
         }
-        a.cap > 0.0f ? go(attn_paged_kernel<F, HD, 1, true>) : go(attn_paged_kernel<F, HD, 1, false>);
+        by_columns(std::false_type{});
     });
     return hipGetLastError();
 }

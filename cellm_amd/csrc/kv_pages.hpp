@@ -105,19 +105,16 @@ __device__ __forceinline__ h2_t values4(uint32_t codes, h2_t s, h2_t z)
     const h2_t c = as_h2(codes | 0x64006400u) - h2_t{(_Float16)1024.0f, (_Float16)1024.0f};  // the f16 1024 + c, exactly
     return __builtin_elementwise_fma(c, s, z);
 }
-// The same of nibbles 0 .. 3 of both halves of w, 13 instructions: a nibble at bit 4 makes the f16 1024 + 16 c.
-__device__ __forceinline__ void four_values4(uint32_t w, h2_t s, h2_t z, uint32_t (&y)[4])
+// Eight f16 values from the nibbles 0 .. 7 of w, 11 instructions: pairs (0, 2), (4, 6), (1, 3), (5, 7), with the scales of
+// the first and of the second of each pair.  A byte below 16 is the 8-bit float (1 sign, 4 exponent, 3 fraction bits)
+// that is 2^-9 of it: numbers below 8 are the subnormal ones, and the first exponent goes on where those end.
+__device__ __forceinline__ void values4x8(uint32_t w, h2_t s, h2_t z, uint32_t (&y)[4])
 {
-    const h2_t k = {(_Float16)1024.0f, (_Float16)1024.0f}, sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f},
-               k16 = {(_Float16)-64.0f, (_Float16)-64.0f};
+    const uint32_t even = w & 0x0F0F0F0Fu, odd = w >> 4 & 0x0F0F0F0Fu;
+    const h2_t c[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(even, 512.0f, false), __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(even, 512.0f, true),
+                       __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(odd, 512.0f, false), __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(odd, 512.0f, true)};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t x = i ? w >> 8 : w;
-        const h2_t lo = as_h2(and_or(x, 0x000F000Fu, 0x64006400u)) - k;
-        const h2_t hi = __builtin_elementwise_fma(as_h2(and_or(x, 0x00F000F0u, 0x64006400u)), sixteenth, k16);
-        y[2 * i] = as_u32(__builtin_elementwise_fma(lo, s, z));
-        y[2 * i + 1] = as_u32(__builtin_elementwise_fma(hi, s, z));
-    }
+    for (int i = 0; i < 4; ++i) y[i] = as_u32(__builtin_elementwise_fma(c[i], s, z));
 }
 // The lower or upper half of a word in both of them
 __device__ __forceinline__ uint32_t both_low(uint32_t m) { return __builtin_amdgcn_perm(m, m, 0x01000100u); }
