@@ -340,6 +340,50 @@ struct Work {
     int split, splits, slot0;   // slot0: work number of the set's split 0
 };
 
+// 4-bit pages: the smallest share, in units, with which the sets have no more splits together than `want`, one block on
+// each CU; it is looked for between the mean and the share whose short last splits fit too.  Where long ones come out
+// well above the mean, twice as many splits, two blocks on a CU: 16 sessions of 8000 to 16000 positions, 32/8 heads of 128,
+// 61.5 us, 82 with the share of want less the sets; 24 of 4096 to 8192 50 and 60; 32 of lengths apart 19.6 and 23.3, 32
+// of the same 2048 (whole, but now planned) 21.1 and 19.9; with two blocks everywhere one session at 131072 had 46 and not 41.5.
+// Splits of one set meet one after the other, 16 of them in the time that a unit takes: 8192 positions of 8 kv heads in
+// 16 splits of two units 14.9 us, in 32 of one 16.4.
+constexpr int kLongShare = 8;   // units from which two blocks on a CU are looked at
+constexpr int kMeetUnits = 16;
+template <int N>
+__device__ __forceinline__ int share_of(const int (&units)[N], int sets, int total, int want)
+{
+    int most = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) most = max(most, units[i]);
+    most = (int)group_max<64>((float)most);
+    const auto splits = [&](int share) {
+        const float inv = 1.0f / (float)share;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (64 * i >= sets) break;
+            int q = (int)((float)units[i] * inv);  // the quotient's floor or a neighbour
+            if (q * share < units[i]) ++q;
+            n += units[i] <= kWholeUnits ? min(units[i], 1) : min(kMaxSplits, q);
+        }
+        return (int)group_sum<64>((float)n);
+    };
+    const auto least = [&](int w) {
+        int lo = max(1, (total + w - 1) / w);  // the mean
+        while (kMeetUnits * lo * lo < most) ++lo;
+        int hi = max(lo, w > sets ? (total + w - sets - 1) / (w - sets) : most);  // each set's last split short, or none split
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (splits(mid) <= w) hi = mid;
+            else lo = mid + 1;
+        }
+        return rfl(lo);
+    };
+    const int share = least(want);
+    if (share >= kLongShare && 5 * share * want > 6 * total) return least(2 * want);
+    return share;
+}
+
 // Work number w of a kv head.  SPLITS: every wave looks at all sets (64 lanes, up to 4 sets each): their positions in units
 // of UNIT add up to the work, each set gets as many splits as units, in shares of the same size for all (so that
 // contexts of different lengths end together) and at most kMaxSplits, and the splits are numbered through.
@@ -374,7 +418,8 @@ __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
         total += units[i];
     }
     for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-    const int share = max(1, (total + A.want - 1) / A.want);
+    int share = max(1, (total + A.want - 1) / A.want);
+    if constexpr (RAGGED) share = share_of(units, A.sets, total, A.want);
     int base = 0;
     bool found = false;
 #pragma unroll
@@ -724,10 +769,25 @@ __device__ __forceinline__ uint32_t seen_of(const Sight& s, int p0, int g4)
 // The reference of a column that has seen nothing: below any score, and finite, so that what is not seen (-inf) weighs 0
 constexpr float kNoScore = -0x1p120f;
 
+// The value of the lane N further round in its row of 16
+template <int N>
+__device__ __forceinline__ float lane_ror(float v)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + N, 0xF, 0xF, false));
+}
+
+// y where mask is ~0, x where it is 0 (a choice between elements of two arrays would put both into memory)
+__device__ __forceinline__ uint32_t pick(uint32_t mask, uint32_t x, uint32_t y) { return (y & mask) | (x & ~mask); }
+__device__ __forceinline__ float pick(uint32_t mask, float x, float y)
+{
+    return __builtin_bit_cast(float, pick(mask, __builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)));
+}
+
 // weigh() for 4-bit pages: scores d times the power of two pw are the weights' exponents, so that one fma takes the
 // reference off them exactly; the high parts are cut off, not rounded (the low ones keep 2^-22 of the weight).
-template <int NP, int DT>
-__device__ __forceinline__ void weigh4(float (&d)[NP], float pw, bool partial, uint32_t seen, Sums<DT>& m, h8_t (&ph)[NP / 8],
+// FEW columns: a lane gives one of the parts, `low` which, and the lanes 4 further round have other positions.
+template <bool FEW, int NP, int DT>
+__device__ __forceinline__ void weigh4(float (&d)[NP], float pw, bool partial, uint32_t seen, uint32_t low, Sums<DT>& m, h8_t (&ph)[NP / 8],
                                        h8_t (&pl)[NP / 8])
 {
     float w[NP], lc, mx;
@@ -751,6 +811,7 @@ __device__ __forceinline__ void weigh4(float (&d)[NP], float pw, bool partial, u
         float m1 = -INFINITY;
 #pragma unroll
         for (int j = 0; j < NP; ++j) m1 = fmaxf(m1, d[j] * pw);
+        if constexpr (FEW) m1 = fmaxf(m1, lane_ror<4>(m1));
         m1 = fmaxf(m1, lane_xor<16>(m1, 64));
         m1 = fmaxf(m1, lane_xor<32>(m1, 64));
         const float up = fmaxf(m.R, m1 - 13.0f);
@@ -765,8 +826,12 @@ __device__ __forceinline__ void weigh4(float (&d)[NP], float pw, bool partial, u
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
         const float hi = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, w[j]) & 0xFFFFE000u);  // f16's bits
-        ph[j >> 3][j & 7] = (_Float16)hi;
-        pl[j >> 3][j & 7] = (_Float16)(w[j] - hi);
+        if constexpr (FEW) {
+            ph[j >> 3][j & 7] = (_Float16)pick(low, hi, w[j] - hi);
+        } else {
+            ph[j >> 3][j & 7] = (_Float16)hi;
+            pl[j >> 3][j & 7] = (_Float16)(w[j] - hi);
+        }
     }
 }
 
@@ -946,7 +1011,14 @@ struct Results {
 };
 
 // One set of 16 CT columns a block; its waves take chunks of the positions in turn and meet in LDS.
-template <int F, int HD, int CT, bool CAP, bool BIG = false>
+//
+// 4-bit pages, FEW: sets of up to 4 columns, of which an operand's 16 columns have each four times: columns c and c + 8 are
+// the high and the low parts of q and of the weights, so that both take one product and meet at its end (those of the
+// scores at once), and c + 4 is column c again, with the weights of the other half of the chunk's positions: each lane
+// makes half as many.  131072 positions, 32/8 heads of 128: 41.5 us, 45 without; 24 sessions of 4096 to 8192 60 and 63.5;
+// 4 at 1000, where it has more to begin and to end with, 11.9 and 11.5.  (Parts side by side for up to 8 columns: 14/2 heads
+// of 64 at 65536 20.1, 19.7 without.)
+template <int F, int HD, int CT, bool CAP, bool BIG = false, bool FEW = false>
 __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A)
 {
     using S = Shape<F, HD, CT>;
@@ -956,7 +1028,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     constexpr int VW = (VB / 16 + 3) / 4;                               // words of V per lane and position (a half: 4 bits, 64 dims)
     constexpr int KR = Q4 ? (KK + 3) / 4 : KK, G = Q4 ? HD / 32 : 1;    // loads of K per lane and tile; scale words of a vector
     constexpr int NR = HD / 4 < 32 ? HD / 4 : 32;                       // registers of O^T that the waves add at a time
-    constexpr bool kQInLds = HD > 128 || CT > 1;                        // q's parts in LDS, for want of registers
+    constexpr bool kQInLds = (HD > 128 && !FEW) || CT > 1;            // q's parts in LDS, for want of registers
+    static_assert(!FEW || (Q4 && CT == 1));
     constexpr int COLS = kCols * CT;
     constexpr bool kSplits = Results<F, HD, COLS>::kSplits;
     constexpr int kMergeBytes = std::max(kWaves * NR * 64 * 4, kSplits ? COLS * kMaxSplits * 8 : 0);
@@ -993,6 +1066,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     float qsc[CT][2];          // scale of the sums of q's parts
     bool loud = false;         // some column needs the fourth digits
     Sums<DT> m[CT];
+    const uint32_t low_part = FEW && (c & 8) ? ~0u : 0u, half_part = FEW && (c & 4) ? ~0u : 0u;
     // with q's parts in LDS wave u makes those of the columns 16 u + c
     const auto makes = [&](int u) { return !kQInLds || wave == u; };
     {
@@ -1001,7 +1075,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         int top = 0;
 #pragma unroll
         for (int u = 0; u < CT; ++u) {
-            const auto x = res.column(min(kCols * u + c, n_cols - 1));
+            const auto x = res.column(min(kCols * u + (FEW ? c & 3 : c), n_cols - 1));
             at[u] = res.offset(x);
             if (makes(u)) {
                 // 4-bit pages: the words of the lane's loads of K, each a k step
@@ -1012,8 +1086,9 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                     for (int i = 0; i < NE / 4; ++i) qf[u][kk][i] = src[(Q4 ? kk / 4 * 32 + kk % 4 * 2 : NE * kk) + i];
             }
             si[u] = Sight{0, 0, 0, a.masks};
-            has[u] = sight_of(a, A.cap, table, x.row, si[u]) && kCols * u + c < n_cols;
+            has[u] = sight_of(a, A.cap, table, x.row, si[u]) && kCols * u + (FEW ? c & 3 : c) < n_cols;
             if (!has[u]) si[u] = Sight{0, 0, 0, a.masks};
+            has[u] = has[u] && !(FEW && c >= 4);
             b |= ((uint32_t)__ballot(has[u]) & 0xFFFFu) << (kCols * u);
             top = max(top, si[u].end);
             m[u] = Sums<DT>{Q4 ? kNoScore : -INFINITY, 0.0f, 1.0f, {}};
@@ -1028,6 +1103,12 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             if (!makes(u)) continue;
             u4_t low[KK];
             q_parts<F, HD>(a, qf[u], qp[u], low, loud, qsc[u], CAP ? a.scale : a.scale * kLog2e);
+            if constexpr (FEW) {
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) qp[u][kk][0][x] = pick(low_part, qp[u][kk][0][x], qp[u][kk][1][x]);
+            }
             if (Q8 && (kQInLds || (loud && wave == 0))) {
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) qlow[(u * KK + kk) * 64 + lane] = low[kk];
@@ -1253,7 +1334,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                         }
                     }
 #pragma unroll
-                    for (int p = 1; p >= 0; --p)  // the low parts first
+                    for (int p = FEW ? 0 : 1; p >= 0; --p)  // the low parts first
 #pragma unroll
                         for (int kk = 0; kk < KK; ++kk)
                             d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, kt[kk]),
@@ -1279,9 +1360,21 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             if (u == CT - 1) load_k();
             float cs = huge ? qsc[u][1] : qsc[u][0];
             if (Q4 && ktiny) cs = cs * (1.0f / kTinyUp);
-            if constexpr (CAP) {
+            // few columns: both parts' scores, of the lane's half of the positions
+            float mine[FEW ? NP / 2 : 1];
+            if constexpr (FEW) {
 #pragma unroll
-                for (int j = 0; j < NP; ++j) s[j] = Q4 ? capped(a, s[j] * cs) * kLog2e : capped(a, s[j] * cs);
+                for (int j = 0; j < NP / 2; ++j) {
+                    mine[j] = pick(half_part, s[j], s[NP / 2 + j]);
+                    mine[j] = mine[j] + lane_ror<8>(mine[j]);
+                }
+            }
+            if constexpr (CAP) {
+                const auto cap_all = [&](auto& x) {
+                    for (float& v : x) v = Q4 ? capped(a, v * cs) * kLog2e : capped(a, v * cs);
+                };
+                if constexpr (FEW) cap_all(mine);
+                else cap_all(s);
                 cs = Q4 ? 1.0f : kLog2e;
             }
             // ---- weights; of positions that some column does not see, those are 0 whatever they hold
@@ -1295,8 +1388,21 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
 #pragma unroll
                 for (int j = 0; j < NP; ++j) vs[j] = vis >> (4 * j) & 1 ? vs[j] : 0.0f;
             }
-            if constexpr (Q4) weigh4(s, cs, partial, partial ? seen_of<NP>(si[u], p0, g4) : ~0u, m[u], ph[u], pl[u]);
-            else weigh<Q8>(s, cs, vs, partial, vis, coarse, m[u], ph[u], pl[u]);
+            if constexpr (FEW) {
+                h8_t p[1], none[1];
+                weigh4<FEW>(mine, cs, partial, partial ? seen_of<NP / 2>(si[u], p0 + (half_part ? CH / 2 : 0), g4) : ~0u, low_part, m[u], p, none);
+                const u4_t all = __builtin_bit_cast(u4_t, p[0]);
+                u4_t w0, w1;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    w0[x] = pick(half_part, all[x], 0u);
+                    w1[x] = pick(half_part, 0u, all[x]);
+                }
+                ph[u][0] = __builtin_bit_cast(h8_t, w0);
+                ph[u][1] = __builtin_bit_cast(h8_t, w1);
+            } else if constexpr (Q4) {
+                weigh4<FEW>(s, cs, partial, partial ? seen_of<NP>(si[u], p0, g4) : ~0u, low_part, m[u], ph[u], pl[u]);
+            } else weigh<Q8>(s, cs, vs, partial, vis, coarse, m[u], ph[u], pl[u]);
         }
         // ---- O^T += V^T . P^T
         if (F == KV_F16 && miss) {
@@ -1327,7 +1433,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                         for (int u = 0; u < CT; ++u) {
                             const h8_t v = __builtin_bit_cast(h8_t, vt[e]);
                             f4_t& o = m[u].o[W * x + E * H + e];
-                            o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u][ks], o, 0, 0, 0);
+                            if constexpr (!FEW) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u][ks], o, 0, 0, 0);
                             o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u][ks], o, 0, 0, 0);
                         }
                 };
@@ -1346,6 +1452,16 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
         const int col = kCols * u + c;
         m[u].l = m[u].l + lane_xor<16>(m[u].l, 64);
         m[u].l = m[u].l + lane_xor<32>(m[u].l, 64);
+        if constexpr (FEW) {
+            m[u].l = m[u].l + lane_ror<4>(m[u].l);
+#pragma unroll
+            for (int e = 0; e < DT; ++e)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    m[u].o[e][x] = m[u].o[e][x] + lane_ror<8>(m[u].o[e][x]);
+                    m[u].o[e][x] = m[u].o[e][x] + lane_ror<4>(m[u].o[e][x]);
+                }
+        }
         if (Q8 && coarse) {
 #pragma unroll
             for (int e = 0; e < DT; ++e) m[u].o[e] = m[u].o[e] / m[u].F;
@@ -1445,9 +1561,14 @@ Layout layout_of(const PagedAttnArgs& a)
              });
     const long long cap = (long long)a.g.max_blocks * a.g.tpb, units = (cap + unit - 1) / unit;
     const long long blocks = (long long)y.sets * a.g.n_kv;
-    if (blocks < kPlanBlocks && units > kWholeUnits) y.want = std::max(1, kPlanBlocks / a.g.n_kv - y.sets);
-    // each set's last split may be short
-    y.works = y.want ? std::min<long long>(y.want + y.sets, y.sets * std::min<long long>(kMaxSplits, units)) : y.sets;
+    if (a.fmt == KV_Q4) {  // share_of(): up to twice as many splits as wanted, or sets
+        if (blocks < 2 * kPlanBlocks && y.sets <= kPlanSets && units > kWholeUnits) y.want = std::max(1, kPlanBlocks / a.g.n_kv);
+        y.works = y.want ? std::min<long long>(std::max<long long>(2 * y.want, y.sets), y.sets * std::min<long long>(kMaxSplits, units)) : y.sets;
+    } else {
+        if (blocks < kPlanBlocks && units > kWholeUnits) y.want = std::max(1, kPlanBlocks / a.g.n_kv - y.sets);
+        // each set's last split may be short
+        y.works = y.want ? std::min<long long>(y.want + y.sets, y.sets * std::min<long long>(kMaxSplits, units)) : y.sets;
+    }
     return y;
 }
 
@@ -1494,6 +1615,11 @@ hipError_t launch_attention_paged(const PagedAttnArgs& a, float* workspace, hipS
         };
         if constexpr (F == KV_Q4) {
             if (big) return by_columns(std::true_type{});
+            const long long columns = a.starts ? kCols : (long long)a.per * y.group;
+            if (columns <= 4) {
+                a.cap > 0.0f ? go(attn_paged_kernel<F, HD, 1, true, false, true>) : go(attn_paged_kernel<F, HD, 1, false, false, true>);
+                return;
+            }
         }
         by_columns(std::false_type{});
     });
