@@ -36,6 +36,28 @@ __device__ __forceinline__ uint16_t bf16_rne(float v)
     return (uint16_t)((u + 0x7FFFu + (u >> 16 & 1u)) >> 16);
 }
 
+// rint(f32(x / s)) of the N values for which that is an integer from lo to hi; what lies outside may be any value beyond
+// the end that it is nearest to.  x times the approximate 1 / s is off by 1.5 2^-23 of it (2.3e-5 at 127, with the quotient's own
+// rounding 2.7e-5): where that stays clear of half way between two integers, both have the same; the few lanes that
+// come nearer divide.
+template <int N>
+__device__ __forceinline__ void rounded_quotients(const float (&x)[N], float s, float (&c)[N])
+{
+    constexpr float kClear = 0.5f - 0x1p-14f;
+    const float r = __builtin_amdgcn_rcpf(s);
+    float far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float q = x[i] * r;
+        c[i] = rintf(q);
+        far = fmaxf(far, fabsf(q - c[i]));
+    }
+    if (far > kClear) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) c[i] = rintf(x[i] / s);
+    }
+}
+
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
 
 // The 8-bit codes of a vector of which each of T lanes has x[0..3] and x[4..7] (a word each), and its scale.
@@ -52,11 +74,10 @@ __device__ __forceinline__ float quantise8(const float (&x)[8], uint32_t (&w)[2]
     const bool finite = m < 0x7F800000u;
     w[0] = w[1] = 0;
     if (finite && s > 0.0f) {
+        float c[8];
+        rounded_quotients(x, s, c);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int c = (int)fminf(fmaxf(rintf(x[i] / s), -127.0f), 127.0f);
-            w[i >> 2] |= (uint32_t)(c & 0xFF) << (8 * (i & 3));
-        }
+        for (int i = 0; i < 8; ++i) w[i >> 2] |= (uint32_t)((int)fminf(fmaxf(c[i], -127.0f), 127.0f) & 0xFF) << (8 * (i & 3));
     }
     return finite ? s : __builtin_nanf("");
 }
@@ -92,9 +113,12 @@ __device__ __forceinline__ uint32_t quantise4(const float (&in)[4], uint32_t& sc
     const float s = (float)s16;
     uint32_t w = 0;
     if (s > 0.0f) {
+        float d[4], c[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w |= (uint32_t)(int)fminf(fmaxf(rintf((x[i] - z) / s), 0.0f), 15.0f) << (4 * i);
+        for (int i = 0; i < 4; ++i) d[i] = x[i] - z;
+        rounded_quotients(d, s, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= (uint32_t)(int)fminf(fmaxf(c[i], 0.0f), 15.0f) << (4 * i);
     }
     return w;
 }

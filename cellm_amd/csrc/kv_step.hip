@@ -15,6 +15,22 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// n / d by the upper half of a product with 2^(32 + shift) / d rounded up: n below 2^31
+struct Divisor {
+    uint32_t mul;
+    int shift;  // -1: d is 1
+};
+Divisor divisor_of(uint32_t d)
+{
+    int shift = -1;
+    while (1ull << (shift + 1) < d) ++shift;
+    return {shift < 0 ? 0u : (uint32_t)(((1ull << (32 + shift)) + d - 1) / d), shift};
+}
+__device__ __forceinline__ uint32_t over(uint32_t n, Divisor d)
+{
+    return d.shift < 0 ? n : __umulhi(n, d.mul) >> d.shift;
+}
+
 // ---- the pages and rows of a step -----------------------------------------------------
 // Session t holds ctx tokens in ceil(ctx / tpb) pages and asks for `add` more.  With running sums
 // over the sessions, P of the pages that these need and R of their rows,
@@ -219,71 +235,127 @@ __global__ __launch_bounds__(kFillThreads) void kv_fill_kernel(const KvPlanArgs 
 // for each head of q and k, the sum and the root in 64 bits, so that inv (and with it every bit of
 // the result) does not hang on the order of the sum; then RoPE as in kv_cache.hip, and q to q_out,
 // k and v to the row's slot.
-__device__ __forceinline__ double lane_xor64(double v, int o)
+template <int O>
+__device__ __forceinline__ double lane_xor64(double v)
 {
-    return __shfl_xor(v, o);
+    const u2_t b = __builtin_bit_cast(u2_t, v);
+    const auto half = [](uint32_t w) { return __builtin_bit_cast(uint32_t, lane_xor<O>(__builtin_bit_cast(float, w), 64)); };
+    return __builtin_bit_cast(double, u2_t{half(b[0]), half(b[1])});
+}
+template <int T>
+__device__ __forceinline__ double team_sum64(double v)
+{
+    if constexpr (T >= 32) v += lane_xor64<16>(v);
+    if constexpr (T >= 16) v += lane_xor64<8>(v);
+    v += lane_xor64<4>(v);
+    v += lane_xor64<2>(v);
+    return v + lane_xor64<1>(v);
+}
+// 1 / sqrt(m) to some 2^-50: the approximate one y (2^-24 and better) and the first two terms of (1 - e)^(-1/2),
+// e = 1 - m y^2.
+__device__ __forceinline__ double inv_sqrt64(double m)
+{
+    const double y = __builtin_amdgcn_rsq(m);
+    const double e = __builtin_fma(-(m * y), y, 1.0);
+    const double z = __builtin_fma(y * e, __builtin_fma(0.375, e, 0.5), y);
+    return m > 0.0 && m < __builtin_inf() ? z : y;
+}
+// Four weights as they lie in memory, and as floats
+template <int WDT>
+using Raw4 = std::conditional_t<WDT == DT_F32, u4_t, u2_t>;
+template <int WDT>
+__device__ __forceinline__ f4_t floats(Raw4<WDT> w)
+{
+    if constexpr (WDT == DT_F32) {
+        return __builtin_bit_cast(f4_t, w);
+    } else if constexpr (WDT == DT_F16) {
+        const h2_t a = as_h2(w[0]), b = as_h2(w[1]);
+        return f4_t{(float)a[0], (float)a[1], (float)b[0], (float)b[1]};
+    } else {
+        const auto f = [](uint32_t u) { return __builtin_bit_cast(float, u); };
+        return f4_t{f(w[0] << 16), f(w[0] & 0xFFFF0000u), f(w[1] << 16), f(w[1] & 0xFFFF0000u)};
+    }
 }
 
 struct NormWriteArgs {
     NormRopeArgs n;
     int rows, n_heads;
-    int units, tpb, layer, n_layers, n_kv;
-    long long slots_end;
+    Divisor per_row, tokens;  // heads of a row, tokens of a page
+    int tpb, layer, n_layers, n_kv;
+    uint32_t slots_end;
 };
 
 // One team of HD / 8 lanes per head vector: a row's query heads, then its K heads, then its V heads.  Lane l holds dims
 // 4 l .. 4 l + 3 and HD / 2 + 4 l .. HD / 2 + 4 l + 3: the pairs of the rotate-half layout, two pairs of each run of
 // the interleaved one, and 8 lanes hold two groups of 4-bit codes.
+//
+// Bytes bound it at many rows, latency at few.  2048 rows of 32/8/8 heads of 128 to 8-bit pages (88 MB) 17.1 us,
+// 5.1 TB/s where a copy of that kind reaches 5.3; 7996 rows of 4/1/1 heads of 256 to 4-bit pages (84 MB) 18.7; one row
+// 2.4.  A vector's loads are all on their way before its position and slot are looked at, the sum goes round by lane
+// moves, quotients by integers are products, codes take no division, and of 4-bit codes two lanes share out their two
+// words (shuffles, divisions and 2-byte stores: 18.6, 21.1 and 2.7 us); rows in order within each XCD read the table
+// of cosines from its own L2 (7996 rows written and read back 25.5 us, 26.1 with blocks dealt out in turn).
 template <int HD, int FMT, int WDT>
 __global__ __launch_bounds__(kThreads) void norm_rope_write_kernel(const NormWriteArgs A)
 {
     constexpr int T = HD / 8, H = HD / 2;
     const NormRopeArgs& a = A.n;
     const int per_row = A.n_heads + 2 * A.n_kv, l = threadIdx.x % T;
-    const uint32_t vec = blockIdx.x * (kThreads / T) + threadIdx.x / T;  // 32 bits: the host checks the count
+    const uint32_t block = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);  // each XCD has rows that follow one another
+    const uint32_t vec = block * (kThreads / T) + threadIdx.x / T;  // the host checks the count
     if (vec >= (uint32_t)A.rows * (uint32_t)per_row) return;              // whole teams
-    const int r = (int)(vec / (uint32_t)per_row), h = (int)(vec - (uint32_t)r * (uint32_t)per_row);
+    const int r = (int)over(vec, A.per_row), h = (int)(vec - (uint32_t)r * (uint32_t)per_row);
     const bool is_q = h < A.n_heads, is_v = h >= A.n_heads + A.n_kv;
     const int kvh = is_q ? 0 : is_v ? h - A.n_heads - A.n_kv : h - A.n_heads;
     const int p = a.pos[r];
-    if (p < 0) return;
-    const int slot = a.slots[r];
-    if (!is_q && (slot < 0 || slot >= A.slots_end)) return;
+    const uint32_t slot = (uint32_t)a.slots[r];
     const int e0 = 4 * l, e1 = H + 4 * l;
     const float* src = is_q ? a.q + ((size_t)r * A.n_heads + h) * HD
                             : (is_v ? a.v : a.k) + ((size_t)r * A.n_kv + kvh) * HD;
     const f4_t x0 = *reinterpret_cast<const f4_t*>(src + e0), x1 = *reinterpret_cast<const f4_t*>(src + e1);
-    float x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
     const void* weight = is_q ? a.q_weight : is_v ? nullptr : a.k_weight;
+    Raw4<WDT> w0 = {}, w1 = {};
+    if (weight) {
+        w0 = static_cast<const Raw4<WDT>*>(weight)[e0 / 4];
+        w1 = static_cast<const Raw4<WDT>*>(weight)[e1 / 4];
+    }
+    if (p < 0 || (!is_q && slot >= A.slots_end)) return;
+    const bool turned = a.cos_sin && !is_v;
+    f4_t c0 = {}, c1 = {};  // (cos, sin) of two pairs each
+    if (turned) {
+        const float* cs = a.cos_sin + (size_t)min(p, a.table_positions - 1) * HD;
+        c0 = *reinterpret_cast<const f4_t*>(cs + (a.interleaved ? e0 : 8 * l));
+        c1 = *reinterpret_cast<const f4_t*>(cs + (a.interleaved ? e1 : 8 * l + 4));
+    }
+    float x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
     if (weight) {
         double ss = 0.0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss += (double)x[i] * (double)x[i];
-#pragma unroll
-        for (int o = 1; o < T; o <<= 1) ss += lane_xor64(ss, o);
-        const float inv = (float)(1.0 / sqrt(ss / HD + (double)a.eps));
+        for (int i = 0; i < 8; ++i) ss = __builtin_fma((double)x[i], (double)x[i], ss);
+        const f4_t y0 = floats<WDT>(w0), y1 = floats<WDT>(w1);
+        const float inv = (float)inv_sqrt64(team_sum64<T>(ss) * (1.0 / HD) + (double)a.eps);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float y = x[i] * inv;
-            x[i] = y * load_f32<WDT>(weight, (i < 4 ? e0 : e1 - 4) + i);
+            x[i] = y * (i < 4 ? y0[i] : y1[i - 4]);
         }
     }
-    if (a.cos_sin && !is_v) {
-        const float2* cs = reinterpret_cast<const float2*>(a.cos_sin) + (size_t)min(p, a.table_positions - 1) * H;
-        const auto turn = [&](int u, int w, float2 c) {
+    if (turned) {
+        const auto turn = [&](int u, int w, float co, float si) {
             const float lo = x[u], hi = x[w];
-            x[u] = lo * c.x - hi * c.y;
-            x[w] = hi * c.x + lo * c.y;
+            x[u] = lo * co - hi * si;
+            x[w] = hi * co + lo * si;
         };
         if (!a.interleaved) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) turn(i, 4 + i, cs[4 * l + i]);
+            turn(0, 4, c0[0], c0[1]);
+            turn(1, 5, c0[2], c0[3]);
+            turn(2, 6, c1[0], c1[1]);
+            turn(3, 7, c1[2], c1[3]);
         } else {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                turn(2 * i, 2 * i + 1, cs[2 * l + i]);
-                turn(4 + 2 * i, 5 + 2 * i, cs[H / 2 + 2 * l + i]);
-            }
+            turn(0, 1, c0[0], c0[1]);
+            turn(2, 3, c0[2], c0[3]);
+            turn(4, 5, c1[0], c1[1]);
+            turn(6, 7, c1[2], c1[3]);
         }
     }
     if (is_q) {
@@ -292,7 +364,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_write_kernel(const NormWri
         *reinterpret_cast<f4_t*>(dst + e1) = f4_t{x[4], x[5], x[6], x[7]};
         return;
     }
-    const int blk = slot / A.tpb, off = slot - blk * A.tpb;
+    const uint32_t blk = over(slot, A.tokens), off = slot - blk * (uint32_t)A.tpb;
     const size_t page = (size_t)blk * A.n_layers + A.layer;
     if constexpr (FMT == KV_F16) {
         uint16_t* dst = static_cast<uint16_t*>(is_v ? a.vc : a.kc) + ((page * A.tpb + off) * A.n_kv + kvh) * HD;
@@ -316,61 +388,81 @@ __global__ __launch_bounds__(kThreads) void norm_rope_write_kernel(const NormWri
         if (l == 0) static_cast<float*>(is_v ? a.vs : a.ks)[vn] = s;
     }
     if constexpr (FMT == KV_Q4) {
-        uint16_t* dst = static_cast<uint16_t*>(is_v ? a.vc : a.kc) + vn * (HD / 4);
+        uint32_t* dst = static_cast<uint32_t*>(is_v ? a.vc : a.kc) + vn * (HD / 8);
         uint32_t* sc = static_cast<uint32_t*>(is_v ? a.vs : a.ks) + vn * (HD / 32);
+        uint32_t w[2], s[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const float y[4] = {x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]};
-            uint32_t s;
-            dst[u * (H / 4) + l] = (uint16_t)quantise4(y, s);
-            if (l % 8 == 0) sc[u * (H / 32) + l / 8] = s;
+            w[u] = quantise4(y, s[u]);
         }
+        // of two lanes the even one stores their word of the first half, the odd one that of the second
+        const bool odd = l & 1;
+        const uint32_t other = __builtin_bit_cast(uint32_t, dpp_xor1(__builtin_bit_cast(float, odd ? w[0] : w[1])));
+        dst[(odd ? H / 8 : 0) + l / 2] = odd ? other | w[1] << 16 : w[0] | other << 16;
+        if (l % 8 < 2) sc[(odd ? H / 32 : 0) + l / 8] = odd ? s[1] : s[0];
     }
 }
 
 // ---- 4-bit pages read back --------------------------------------------------------------
-// A word of codes per thread.
+struct ReadArgs {
+    const void *kc, *ks, *vc, *vs;
+    const int32_t* pos;
+    void *ko, *vo;
+    KvGeom g;
+    int rows;
+    Divisor heads, per, tokens;  // of a row, rows of a table, of a page
+};
+
+// E codes of K and of V per thread, one 16-byte store of each.  The outputs' bytes bound it, and at the sizes of a step the
+// way there, position, page, codes: 7996 rows of one head of 256 to f32 (19 MB) 5.9 us, 7.3 with a word of codes and
+// 32 bytes out per thread.
 template <int HD, int DT>
-__global__ __launch_bounds__(kThreads) void kv_read_q4_kernel(const uint32_t* __restrict__ kc, const uint32_t* __restrict__ ks,
-                                                              const uint32_t* __restrict__ vc, const uint32_t* __restrict__ vs,
-                                                              const int32_t* __restrict__ pos, int rows, int per, KvGeom g,
-                                                              void* __restrict__ ko, void* __restrict__ vo)
+__global__ __launch_bounds__(kThreads) void kv_read_q4_kernel(const ReadArgs A)
 {
-    constexpr int T = HD / 8;
-    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;  // 32 bits: the host checks the count
-    if (i >= (uint32_t)rows * (uint32_t)g.n_kv * T) return;
-    const uint32_t vec = i / T, row = vec / (uint32_t)g.n_kv;
-    const int l = (int)(i % T), kvh = (int)(vec - row * (uint32_t)g.n_kv), r = (int)row;
-    const int p = pos[r];
+    constexpr int E = DT == DT_F32 ? 4 : 8, T = HD / E;
+    const KvGeom& g = A.g;
+    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;  // the host checks the count
+    if (i >= (uint32_t)A.rows * (uint32_t)g.n_kv * T) return;
+    const uint32_t vec = i / T, row = over(vec, A.heads), l = i % T, kvh = vec - row * (uint32_t)g.n_kv;
+    const int p = A.pos[row];
     if (p < 0) return;
-    const long long v0 = vector_of(g, r / per, p);
-    const size_t vn = v0 < 0 ? 0 : (size_t)v0 + (size_t)kvh * g.tpb;
-    const auto one = [&](const uint32_t* c, const uint32_t* s, void* out) {
-        const uint32_t w = v0 < 0 ? 0 : c[vn * T + l], m = v0 < 0 ? 0 : s[vn * (HD / 32) + l / 4];
-        const h2_t sc = as_h2(both_low(m)), z = as_h2(both_high(m));
-        _Float16 x[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {  // nibbles j and j + 4
-            const h2_t v = values4(w >> (4 * j) & 0x000F000Fu, sc, z);
-            x[j] = v[0];
-            x[j + 4] = v[1];
+    const uint32_t b = over((uint32_t)p, A.tokens);
+    uint32_t blk = ~0u;
+    if (b < (uint32_t)g.max_blocks) blk = g.bt[(size_t)over(row, A.per) * g.max_blocks + b];
+    const bool there = blk < (uint32_t)g.total_blocks;
+    const size_t vn = (((size_t)blk * g.n_layers + g.layer) * g.n_kv + kvh) * g.tpb + ((uint32_t)p - b * (uint32_t)g.tpb);
+    const auto one = [&](const void* codes, const void* scales, void* out) {
+        uint32_t w = 0, m = 0;
+        if (there) {
+            if constexpr (E == 4) w = static_cast<const uint16_t*>(codes)[vn * T + l];
+            else w = static_cast<const uint32_t*>(codes)[vn * T + l];
+            m = static_cast<const uint32_t*>(scales)[vn * (HD / 32) + E * l / 32];
         }
-        if constexpr (DT == DT_F32) {
-            f4_t* o = reinterpret_cast<f4_t*>(out) + 2 * (size_t)i;
-            o[0] = f4_t{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
-            o[1] = f4_t{(float)x[4], (float)x[5], (float)x[6], (float)x[7]};
+        const h2_t s = as_h2(both_low(m)), z = as_h2(both_high(m));
+        u4_t o;
+        if constexpr (E == 4) {
+            w |= w << 12;  // nibbles 0 and 1, 2 and 3 at bits 0 and 16, 8 and 24
+            const h2_t a = values4(w & 0x000F000Fu, s, z), c = values4(w >> 8 & 0x000F000Fu, s, z);
+            o = __builtin_bit_cast(u4_t, f4_t{(float)a[0], (float)a[1], (float)c[0], (float)c[1]});
         } else {
-            u4_t o;
+            _Float16 x[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // nibbles j and j + 4
+                const h2_t v = values4(w >> (4 * j) & 0x000F000Fu, s, z);
+                x[j] = v[0];
+                x[j + 4] = v[1];
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (DT == DT_F16) o[j] = as_u32(h2_t{x[2 * j], x[2 * j + 1]});
                 else o[j] = (uint32_t)bf16_rne((float)x[2 * j]) | (uint32_t)bf16_rne((float)x[2 * j + 1]) << 16;
             }
-            reinterpret_cast<u4_t*>(out)[i] = o;
         }
+        static_cast<u4_t*>(out)[i] = o;
     };
-    one(kc, ks, ko);
-    one(vc, vs, vo);
+    one(A.kc, A.ks, A.ko);
+    one(A.vc, A.vs, A.vo);
 }
 
 }  // namespace
@@ -405,12 +497,14 @@ hipError_t launch_norm_rope_write(const NormRopeArgs& n, int rows, int n_heads, 
     a.layer = g.layer;
     a.n_layers = g.n_layers;
     a.n_kv = g.n_kv;
-    a.slots_end = (long long)g.total_blocks * g.tpb;
+    a.slots_end = (uint32_t)std::min((long long)g.total_blocks * g.tpb, 1ll << 31);  // slots: numbers of 31 bits
+    a.per_row = divisor_of((uint32_t)(n_heads + 2 * g.n_kv));
+    a.tokens = divisor_of((uint32_t)g.tpb);
     const long long vecs = (long long)rows * (n_heads + 2 * g.n_kv);
     const auto go = [&](auto hd, auto fm, auto wt) {
         constexpr int HD = decltype(hd)::value, V = kThreads / (HD / 8);
         hipLaunchKernelGGL((norm_rope_write_kernel<HD, decltype(fm)::value, decltype(wt)::value>),
-                           dim3((unsigned)((vecs + V - 1) / V)), dim3(kThreads), 0, st, a);
+                           dim3((unsigned)((vecs + 8 * V - 1) / (8 * V) * 8)), dim3(kThreads), 0, st, a);
     };
     const auto by_weight = [&](auto hd, auto fm) {
         if (n.weight_dtype == DT_F32) go(hd, fm, std::integral_constant<int, DT_F32>{});
@@ -431,12 +525,13 @@ hipError_t launch_norm_rope_write(const NormRopeArgs& n, int rows, int n_heads, 
 hipError_t launch_kv_read_q4(const void* kc, const void* ks, const void* vc, const void* vs, const int32_t* pos, int rows,
                              int per, int head_dim, const KvGeom& g, void* k_out, void* v_out, int out_dtype, hipStream_t st)
 {
+    const ReadArgs a{kc, ks, vc, vs, pos, k_out, v_out, g, rows, divisor_of((uint32_t)g.n_kv), divisor_of((uint32_t)per),
+                     divisor_of((uint32_t)g.tpb)};
     const auto go = [&](auto hd, auto dt) {
         constexpr int HD = decltype(hd)::value, DT = decltype(dt)::value;
-        const long long n = (long long)rows * g.n_kv * (HD / 8);
-        const auto words = [](const void* p) { return static_cast<const uint32_t*>(p); };
+        const long long n = (long long)rows * g.n_kv * (HD / (DT == DT_F32 ? 4 : 8));
         hipLaunchKernelGGL((kv_read_q4_kernel<HD, DT>), dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0,
-                           st, words(kc), words(ks), words(vc), words(vs), pos, rows, per, g, k_out, v_out);
+                           st, a);
     };
     const auto by_type = [&](auto hd) {
         if (out_dtype == DT_F32) go(hd, std::integral_constant<int, DT_F32>{});
