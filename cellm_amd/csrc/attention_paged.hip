@@ -289,27 +289,53 @@ struct Span {
 // RAGGED (4-bit pages): table t may have the rows starts[t] .. starts[t + 1] - 1.  Its sets are numbered from
 // floor(starts[t] group / cols) + t on, which leaves it at least as many numbers as it has tiles, so that a set finds its table
 // by a search alone; numbers behind its last tile are sets without columns.
+__device__ __forceinline__ int start_of(const PagedAttnArgs& a, int t) { return min(max(a.starts[t], 0), a.rows); }
+__device__ __forceinline__ int first_set(const MmaArgs& A, int start, int t) { return start * A.group / A.cols + t; }
+
+// starts: those of all tables in LDS, where a.starts are given
 template <bool RAGGED>
-__device__ __forceinline__ Span span_of(const MmaArgs& A, int set)
+__device__ __forceinline__ Span span_of(const MmaArgs& A, int set, const int* starts)
 {
     const PagedAttnArgs& a = A.a;
     if (RAGGED && a.starts) {
-        const auto start = [&](int t) { return min(max(a.starts[t], 0), a.rows); };
-        const auto base = [&](int t) { return start(t) * A.group / A.cols + t; };
         int lo = 0, hi = a.tables;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (base(mid) <= set) lo = mid;
+            if (first_set(A, starts[mid], mid) <= set) lo = mid;
             else hi = mid;
         }
-        const int row0 = start(lo);
-        return {lo, row0, max(start(lo + 1) - row0, 0), (set - base(lo)) * A.cols};
+        const int row0 = starts[lo];
+        return {lo, row0, max(starts[lo + 1] - row0, 0), (set - first_set(A, row0, lo)) * A.cols};
     }
     const int table = A.tiles == 1 ? set : set / A.tiles;
     return {table, table * a.per, a.per, (set - table * A.tiles) * A.cols};
 }
+// One set for the whole wave: 64 tables at a look, so that up to 64 of them cost one way to memory and 2^18 three (20 sessions,
+// 700 blocks that see 64 positions each, 17.2 us; a search by halves 17.8).
+template <bool RAGGED>
+__device__ __forceinline__ Span wave_span_of(const MmaArgs& A, int set)
+{
+    const PagedAttnArgs& a = A.a;
+    if (!RAGGED || !a.starts) return span_of<false>(A, set, nullptr);
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = a.tables, here, next, at;
+    for (;;) {  // the table is one of the n from lo on
+        const int step = (n + 63) >> 6, t = min(lo + lane * step, lo + n - 1);
+        here = start_of(a, t);
+        next = start_of(a, t + 1);
+        at = __popcll(__ballot(lane * step < n && first_set(A, here, t) <= set)) - 1;
+        at = max(at, 0);  // starts that do not begin with 0
+        lo += at * step;
+        n = min(step, n - at * step);
+        if (step == 1) break;
+    }
+    const int row0 = __builtin_amdgcn_readlane(here, at);
+    return {lo, row0, max(__builtin_amdgcn_readlane(next, at) - row0, 0), (set - first_set(A, row0, lo)) * A.cols};
+}
 
-// Positions lo..hi - 1 that the columns of a set may see; false: none of its rows has a position.
+// Positions lo..hi - 1 that the columns of a set may see; false: none of its rows has a position.  WAVE: the set is the
+// same for the whole wave.
+template <bool WAVE>
 __device__ __forceinline__ bool set_range(const MmaArgs& A, const Span& sp, int& lo, int& hi)
 {
     const PagedAttnArgs& a = A.a;
@@ -324,13 +350,30 @@ __device__ __forceinline__ bool set_range(const MmaArgs& A, const Span& sp, int&
         return true;
     }
     const int j1 = min(sp.rows - 1, (c0 + A.cols - 1) / A.group);
-    for (int j = c0 / A.group; j <= j1; ++j) {
-        const int p = a.pos[sp.row0 + j];
-        if (p < 0) continue;
+    int most = 0, least = A.cap;  // ends of the rows
+    const auto row = [&](int p) {
         const int end = min(p, A.cap - 1) + 1;
-        hi = max(hi, end);
-        lo = min(lo, a.window > 0 ? max(end - a.window, 0) : 0);
+        most = max(most, end);
+        least = min(least, p < 0 ? A.cap : end);
+    };
+    if constexpr (WAVE) {
+        const int j = c0 / A.group + (int)(threadIdx.x & 63);  // at most 33 rows
+        row(j <= j1 ? a.pos[sp.row0 + j] : -1);
+        most = (int)team_max_u32<32>((uint32_t)most);
+        least = A.cap - (int)team_max_u32<32>((uint32_t)(A.cap - least));
+        most = max(__builtin_amdgcn_readlane(most, 0), __builtin_amdgcn_readlane(most, 32));
+        least = min(__builtin_amdgcn_readlane(least, 0), __builtin_amdgcn_readlane(least, 32));
+    } else {
+        for (int j = c0 / A.group; j <= j1; j += 4) {  // loads that do not wait for each other
+            int p[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = a.pos[sp.row0 + min(j + i, j1)];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) row(p[i]);
+        }
     }
+    hi = most;
+    lo = hi > 0 && a.window > 0 ? max(least - a.window, 0) : 0;
     return hi > 0;
 }
 
@@ -388,16 +431,16 @@ __device__ __forceinline__ int share_of(const int (&units)[N], int sets, int tot
 // of UNIT add up to the work, each set gets as many splits as units, in shares of the same size for all (so that
 // contexts of different lengths end together) and at most kMaxSplits, and the splits are numbered through.
 template <int UNIT, bool SPLITS, bool RAGGED>
-__device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
+__device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k, int* starts)
 {
     const int lane = threadIdx.x & 63;
     if (!SPLITS || A.want == 0) {
         k = Work{{}, A.sets - 1 - w, 0, -1, UNIT, 0, 1, 0};  // a prompt's last rows, which see the most, first
         if (k.set < 0) return false;
-        k.span = span_of<RAGGED>(A, k.set);
+        k.span = wave_span_of<RAGGED>(A, k.set);
         if (RAGGED && k.span.col0 >= k.span.rows * A.group) return false;
         if (!A.a.masks && A.a.window == 0) return true;  // all from 0 on: how far, the columns will say
-        if (!set_range(A, k.span, k.lo, k.hi)) return false;
+        if (!set_range<true>(A, k.span, k.lo, k.hi)) return false;
         k.lo = rfl(k.lo) & ~63;
         k.hi = rfl(k.hi);
         return true;
@@ -405,13 +448,17 @@ __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
     constexpr int N = kPlanSets / 64;
     int units[N], from[N], to[N], total = 0;
     Span spans[N];
+    if (RAGGED && A.a.starts) {  // no more tables than sets
+        for (int t = lane; t <= A.a.tables; t += 64) starts[t] = start_of(A.a, t);
+        wave_lds_fence();        // every wave writes them all
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         units[i] = from[i] = to[i] = 0;
         if (64 * i >= A.sets) continue;  // the same for the whole wave
         const int e = lane + 64 * i;
-        spans[i] = span_of<RAGGED>(A, min(e, A.sets - 1));
-        if (e < A.sets && set_range(A, spans[i], from[i], to[i])) {
+        spans[i] = span_of<RAGGED>(A, min(e, A.sets - 1), starts);
+        if (e < A.sets && set_range<false>(A, spans[i], from[i], to[i])) {
             from[i] &= ~63;
             units[i] = (to[i] - from[i] + UNIT - 1) / UNIT;
         }
@@ -445,7 +492,7 @@ __device__ __forceinline__ bool plan(const MmaArgs& A, int w, Work& k)
                 k.span.rows = __builtin_amdgcn_readlane(spans[i].rows, src);
                 k.span.col0 = __builtin_amdgcn_readlane(spans[i].col0, src);
             } else {
-                k.span = span_of<false>(A, k.set);
+                k.span = span_of<false>(A, k.set, nullptr);
             }
             k.splits = __builtin_amdgcn_readlane(n, src);
             k.slot0 = __builtin_amdgcn_readlane(first, src);
@@ -1030,6 +1077,10 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     constexpr int NR = HD / 4 < 32 ? HD / 4 : 32;                       // registers of O^T that the waves add at a time
     constexpr bool kQInLds = (HD > 128 && !FEW) || CT > 1;            // q's parts in LDS, for want of registers
     static_assert(!FEW || (Q4 && CT == 1));
+    // Of two waves on a SIMD the one that has products to issue goes first, beside the other's weights: 20 sessions, 3 of 200
+    // rows, 16/4 heads of 128 72.3 us, 76.1 without; a prompt of 1024 with 32/8 72.9 and 74; those three beside them 128.6
+    // and 125.8; heads of 256 at 700 rows 31.9 and 33.6; heads of 64 lose (701 positions 8.6 and 8.3).
+    constexpr bool kPrio = Q4 && HD >= 128;
     constexpr int COLS = kCols * CT;
     constexpr bool kSplits = Results<F, HD, COLS>::kSplits;
     constexpr int kMergeBytes = std::max(kWaves * NR * 64 * 4, kSplits ? COLS * kMaxSplits * 8 : 0);
@@ -1049,7 +1100,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     const int c = lane & 15, g4 = lane >> 4;
     const int kvh = blockIdx.x;
     Work k;
-    if (!plan<kWaves * CH, kSplits, Q4>(A, blockIdx.y + gridDim.y * blockIdx.z, k)) return;  // the same for the whole block
+    __shared__ int starts_lds[Q4 ? kPlanSets + 1 : 1];
+    if (!plan<kWaves * CH, kSplits, Q4>(A, blockIdx.y + gridDim.y * blockIdx.z, k, starts_lds)) return;  // the same for the whole block
     const Results<F, HD, COLS> res(A, k, kvh);
     const int table = res.table, n_cols = res.columns();
 
@@ -1302,13 +1354,62 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             }
         }
         h8_t ph[CT][KS], pl[CT][KS];
+        f4_t d4[Q4 ? CT : 1][NT];
+        if constexpr (Q4) {  // K's values once for all columns (a product's beside the next one's unpacking: 73 us, 76 set by set)
+            if (kPrio) __builtin_amdgcn_s_setprio(1);
+            const auto words = [&](int i, int kk) {
+                const uint32_t m = kmeta[wave][(HD == 64 ? g4 >> 1 : kk / 4 * 4 + g4) * CH + c * NT + i];
+                uint32_t y[4];
+                values4x8(kr[i][kk / 4][kk % 4], as_h2(both_low(m)), as_h2(both_high(m)), y);
+                return __builtin_bit_cast(h8_t, u4_t{y[0], y[1], y[2], y[3]});
+            };
+#pragma unroll
+            for (int u = 0; u < CT; ++u)
+#pragma unroll
+                for (int i = 0; i < NT; ++i) d4[u][i] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            const auto add = [&](int u, int i, int p, int kk, h8_t k) {
+                d4[u][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(h8_t, q_part(u, p, kk)), d4[u][i], 0, 0, 0);
+            };
+            if constexpr (CT > 1) {  // q's parts are read from LDS once
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    h8_t kt[NT];
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) kt[i] = words(i, kk);
+#pragma unroll
+                    for (int p = 1; p >= 0; --p)
+#pragma unroll
+                        for (int u = 0; u < CT; ++u)
+#pragma unroll
+                            for (int i = 0; i < NT; ++i) add(u, i, p, kk, kt[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    h8_t kt[KK];
+#pragma unroll
+                    for (int kk = 0; kk < KK; ++kk) kt[kk] = words(i, kk);
+#pragma unroll
+                    for (int p = FEW ? 0 : 1; p >= 0; --p)  // the low parts first
+#pragma unroll
+                        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                            for (int u = 0; u < CT; ++u) add(u, i, p, kk, kt[kk]);
+                }
+            }
+            load_k();
+            if (kPrio) __builtin_amdgcn_s_setprio(0);
+        }
 #pragma unroll
         for (int u = 0; u < CT; ++u) {
             // ---- scores of positions p0 + 4 j + g4, less their scale qsc without a cap
             float s[NP];
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                if constexpr (Q8) {
+                if constexpr (Q4) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[4 * i + x] = d4[u][i][x];
+                } else if constexpr (Q8) {
                     i4_t d[3] = {};
 #pragma unroll
                     for (int kk = 0; kk < KK; ++kk)
@@ -1321,23 +1422,11 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                     for (int x = 0; x < 4; ++x) s[4 * i + x] = score_of(d[2][x], d[1][x], d[0][x], ksv[x]);
                 } else {
                     f4_t d = {0.0f, 0.0f, 0.0f, 0.0f};
-                    u4_t kt[KK];
 #pragma unroll
-                    for (int kk = 0; kk < KK; ++kk) {
-                        if constexpr (Q4) {
-                            const uint32_t m = kmeta[wave][(HD == 64 ? g4 >> 1 : kk / 4 * 4 + g4) * CH + c * NT + i];
-                            uint32_t y[4];
-                            values4x8(kr[i][kk / 4][kk % 4], as_h2(both_low(m)), as_h2(both_high(m)), y);
-                            kt[kk] = u4_t{y[0], y[1], y[2], y[3]};
-                        } else {
-                            kt[kk] = kr[i][kk];
-                        }
-                    }
-#pragma unroll
-                    for (int p = FEW ? 0 : 1; p >= 0; --p)  // the low parts first
+                    for (int p = 1; p >= 0; --p)  // the low parts first
 #pragma unroll
                         for (int kk = 0; kk < KK; ++kk)
-                            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, kt[kk]),
+                            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, kr[i][kk]),
                                                                        __builtin_bit_cast(h8_t, q_part(u, p, kk)), d, 0, 0, 0);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) s[4 * i + x] = d[x];
@@ -1357,7 +1446,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                     for (int x = 0; x < 4; ++x) s[4 * i + x] = s[4 * i + x] + (float)d[x] * 0x1p-8f * ksv[x];
                 }
             }
-            if (u == CT - 1) load_k();
+            if (!Q4 && u == CT - 1) load_k();
             float cs = huge ? qsc[u][1] : qsc[u][0];
             if (Q4 && ktiny) cs = cs * (1.0f / kTinyUp);
             // few columns: both parts' scores, of the lane's half of the positions
@@ -1405,6 +1494,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
             } else weigh<Q8>(s, cs, vs, partial, vis, coarse, m[u], ph[u], pl[u]);
         }
         // ---- O^T += V^T . P^T
+        if (kPrio) __builtin_amdgcn_s_setprio(1);
         if (F == KV_F16 && miss) {
 #pragma unroll
             for (int j = 0; j < NP; ++j)
@@ -1440,6 +1530,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                 tiles(std::integral_constant<int, 0>{});
                 if constexpr (W > E) tiles(std::integral_constant<int, 1>{});
             }
+        if (kPrio) __builtin_amdgcn_s_setprio(0);
         load_v();
     }
 
