@@ -1,5 +1,5 @@
-// Attention over paged K/V whose pages many query rows share (gfx950): 8-bit pages for
-// decode and prompts, and 8-bit or f16 pages for trees of drafted tokens.
+// Attention over paged K/V whose pages many query rows share (gfx950): 8-bit and 4-bit pages
+// for decode and prompts, and 8-bit or f16 pages for trees of drafted tokens.
 //
 //   s_p = scale * (q . k_p), capped: s = cap * tanh(s / cap)
 //   o   = sum_p e^(s_p - M) v_p / sum_p e^(s_p - M),   M = max_p s_p
@@ -33,6 +33,14 @@
 // two f16 parts like q's, over the codes as exact f16 integers or f16 values, and R is raised
 // (and l and O with it) only where one of them passes 2^15, to leave the largest at 2^13: a
 // test of the lanes' own values, where a maximum of each chunk would be sums over lanes.
+//
+// 4-bit pages: a code stands for the f16 value f16(c s + z) of its group of 32 dims (kv_pages.hpp), so K's and V's
+// operands are unpacked to those values, exactly, and both products are f16's with q (its scale and log2(e) inside) and the
+// weights in two parts each.  Unpacking bounds it where reads do not: 11 instructions for 8 values, 350 of the 560
+// vector instructions of 64 positions beside 16 columns and their 64 products.  131072 positions of one session with
+// 32/8 heads of 128 (168 MB) 41.5 us, 4.0 TB/s; 8 sessions of 4096 to 8192 22.6; a prompt of 1024 behind 1024 73;
+// 20 sessions, 3 of them with prompts of 200, window 1024 and a cap 43.8; 701 positions of 14/2 heads of 64 8.2.
+// Rows need not be the same number of each table: a set finds its table in the rows' starts (span_of()).
 //
 // The positions of a set of columns are split over blocks by a rule on the device (plan()),
 // which knows how long every context is; the last block of a set to finish adds the others'

@@ -99,7 +99,7 @@ __global__ __launch_bounds__(N) void kv_plan_kernel(const KvPlanArgs a)
     const auto pages_of = [&](long long tokens) { return (uint32_t)((tokens + a.tpb - 1) / a.tpb); };
     long long count = max(a.free_count[0], 0);
     if (count > a.free_capacity) count = a.free_capacity;
-    int ctx = t < a.tables ? a.ctx[t] : -1, add = t < a.tables ? a.add[t] : 0;  // of the round at hand
+    int ctx = t < a.tables ? a.ctx[t] : -1, add = t < a.tables ? a.add[t] : 0;  // of the turn at hand
 
     // ---- finished sessions give their pages back, in the order of sessions and positions
     for (int t0 = 0; t0 < a.tables; t0 += N) {
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(N) void kv_plan_kernel(const KvPlanArgs a)
     }
 
     // ---- sessions in order, up to the first whose pages or rows are not there
-    long long pages0 = 0, rows0 = 0;  // of the sessions before this round's
+    long long pages0 = 0, rows0 = 0;  // of the sessions of earlier turns
     if (t == 0) a.starts[0] = 0;
     for (int t0 = 0; t0 < a.tables; t0 += N) {
         const int s = t0 + t;
