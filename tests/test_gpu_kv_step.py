@@ -328,3 +328,64 @@ def test_read_four_bits(ops, tables, per, nkv, hd, tpb):
                 blk = int(bt[r // per, p // tpb]) if p // tpb < need else total
                 want = x[blk, :, p % tpb] if blk < total else torch.zeros(nkv, hd)
                 assert _same(got[r], want.float().to(dt))
+
+
+# ---- codes half way between two, and heads whose norm is out of the ordinary ---------------
+
+
+def _halfway(steps, s, rng):
+    """f32 numbers at and next to (k + 1 / 2) s, k below `steps`, by up to 300 steps of f32."""
+    k = rng.integers(0, steps, 4096) + 0.5
+    x = (k * np.float64(s)).astype(np.float32)
+    d = rng.choice([0, 0, 1, 1, 2, 3, 10, 40, 100, 300], x.size) * rng.choice([-1, 1], x.size)
+    return (x.view(np.int32) + d).astype(np.int32).view(np.float32)
+
+
+@pytest.mark.parametrize("fmt", ["q8", "q4"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_codes_between_two(ops, fmt, hd):
+    """Codes are the rounded quotient's, however near it lies to a tie."""
+    rng = np.random.default_rng(hd)
+    rows, nkv = 40, 4
+    x = []
+    for _ in range(2 * rows * nkv):
+        if fmt == "q8":  # the scale is the largest over 127
+            top = np.float32(np.exp(rng.uniform(-20, 20)))
+            v = rng.choice(_halfway(126, top / np.float32(127), rng), hd) * rng.choice([-1, 1], hd).astype(np.float32)
+            v[rng.integers(hd)] = top
+        else:  # base 0 or one that f16 holds, and the scale one too
+            s, v = np.float16(np.exp(rng.uniform(-6, 4))).astype(np.float32), np.zeros(hd, np.float32)
+            for g in range(0, hd, 32):
+                base = rng.choice([np.float32(0), np.float32(-8) * s])
+                v[g:g + 32] = base + rng.choice(_halfway(14, s, rng), 32)
+                v[g], v[g + 1] = base, base + np.float32(15) * s
+        x.append(np.clip(v, -top, top) if fmt == "q8" else v)
+    k, v = (torch.from_numpy(np.stack(y).reshape(rows, nkv, hd)) for y in (x[:rows * nkv], x[rows * nkv:]))
+    q = torch.zeros(rows, nkv, hd, device="cuda")
+    cache = _pages(fmt, 6, 1, nkv, 8, hd, 3)
+    slots = list(range(rows))
+    got = _write(ops, q, k, v, q, None, None, 0.0, [0] * rows, None, slots, cache, fmt, 0)
+    for a, b in zip(got, _expect(fmt, cache, slots, 0, 8, k.numpy(), v.numpy())):
+        assert _same(a, b)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("eps", [0.0, 1e-6, 1e30])
+def test_norms_of_every_size(ops, hd, eps):
+    """Heads of zeros, of f32's smallest and largest numbers, and with infinities and NaN, to f16 pages and to q_out."""
+    g = torch.Generator().manual_seed(hd)
+    sizes = [0.0, 1e-45, 1e-42, 1e-38, 1e-20, 1.0, 1e18, 1e30, 3e37]
+    q = torch.stack([torch.randn(2, hd, generator=g).clamp(-4, 4) * n for n in sizes] * 2)
+    for r, bad in ((-1, float("inf")), (-2, float("-inf")), (-3, float("nan"))):
+        q[r, 0, 5] = bad
+    k = q.flip(0).contiguous()
+    rows = q.shape[0]
+    w = 1 + 0.3 * torch.randn(hd, generator=g)
+    cache = _pages("f16", 3, 1, 2, 16, hd, 3)
+    slots = list(range(rows))
+    out = torch.zeros_like(q).cuda()
+    got = _write(ops, q.cuda(), k, k, out, w, w, eps, [0] * rows, None, slots, cache, "f16", 0)
+    assert _same(out.cpu(), torch.from_numpy(S.normed(q.numpy(), w.numpy(), eps)))
+    with np.errstate(over="ignore"):
+        for a, b in zip(got, _expect("f16", cache, slots, 0, 16, S.normed(k.numpy(), w.numpy(), eps), k.numpy())):
+            assert _same(a, b)
