@@ -196,3 +196,75 @@ def test_the_same_bits_every_time(ops):
     first = _attend(ops, q, cache, bt, pos)
     for _ in range(5):
         assert torch.equal(_attend(ops, q, cache, bt, pos), first)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("ctx", [70, 1500, 6000])
+@pytest.mark.parametrize("per,nh,ragged", [(1, 1, False), (1, 4, False), (2, 2, False), (4, 1, False), (1, 4, True)])
+def test_nan_groups_of_few_columns(ops, hd, ctx, per, nh, ragged):
+    """As above for sets of up to 4 columns: NaN where it is seen, in K of all dims, in V of its own 32, and none from
+    positions behind the row's own or before its window."""
+    g = torch.Generator().manual_seed(hd + ctx)
+    bt, total = _table(g, 1, -(-(ctx + 3) // 16))
+    cache = S.cache_q4(total, 1, 1, 16, hd, 5)
+    window = ctx // 2
+    pos = torch.arange(ctx - per, ctx)
+    q = torch.randn(per, nh, hd, generator=g)
+    clean = S.attention(q, cache, bt, pos, 0, [0, per], window=window)
+    for i in (1, 3):
+        for p in (0, ctx - window - per - 1, ctx, ctx + 2):
+            cache[i][int(bt[0, p // 16]), 0, :, p % 16] = math.nan
+    kw = dict(starts=[0, per]) if ragged else dict(per=per)
+    _check(_attend(ops, q, cache, bt, pos, window=window, **kw), clean)
+    at = ctx - window // 2
+    cache[3][int(bt[0, at // 16]), 0, :, at % 16, 1] = math.nan
+    got = _attend(ops, q, cache, bt, pos, window=window, **kw)
+    rest = torch.arange(hd) // 32 != 1
+    assert bool(torch.isnan(got[..., ~rest]).all()) and P.rel(got[..., rest], clean[..., rest]) <= TOL
+    cache[1][int(bt[0, at // 16]), 0, :, at % 16, 0] = math.nan
+    assert bool(torch.isnan(_attend(ops, q, cache, bt, pos, window=window, **kw)).all())
+
+
+def test_queries_of_any_size(ops):
+    """Queries whose scores are far past 1, up to what f32 holds, and rows with an infinity or a NaN beside others."""
+    g = torch.Generator().manual_seed(3)
+    bt, total = _table(g, 4, 80)
+    cache = S.cache_q4(total, 1, 1, 16, 128, 5)
+    pos = torch.tensor([1200, 900, 40, 1100])
+    q = torch.randn(4, 4, 128, generator=g)
+    q[0] *= 1e-30
+    q[1, 0] *= 3e4
+    q[2, 1, 7], q[3, 2, 100] = math.inf, math.nan
+    ref = S.attention(q, cache, bt, pos, 0, range(5))
+    got = _attend(ops, q, cache, bt, pos)
+    bad = torch.zeros(4, 4, dtype=torch.bool)
+    bad[2, 1] = bad[3, 2] = True
+    assert bool(torch.isnan(got[bad]).all())
+    # the scores of row 1, head 0 reach 8e4, off by 5e-3 each, and the largest stands 370 above the next: its weight is 1
+    assert P.rel(got[~bad], ref[~bad]) <= TOL
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("per,nh", [(2, 2), (3, 6), (20, 4)])
+@pytest.mark.parametrize("tiny_first", [True, False])
+def test_tiny_pages_beside_others(ops, hd, per, nh, tiny_first):
+    """Pages of subnormal f16 values and of ordinary ones in one context; row 0 sees the tiny ones alone and has queries
+    that make up for them, the last row sees all, and the others what their window leaves."""
+    g = torch.Generator().manual_seed(hd + per)
+    bt, total = _table(g, 1, 96)
+    size = torch.ones(96)
+    size[slice(0, 48) if tiny_first else slice(48, 96)] = 1e-6
+    x = [torch.randn(total, 1, 1, 16, hd, generator=g) for _ in range(2)]
+    cache = []
+    for y in x:
+        y[bt[0]] *= size.view(-1, 1, 1, 1, 1)
+        cache += [torch.from_numpy(z) for z in S.quantise4(y.numpy())]
+    pos = torch.randint(0, 1536, (per,), generator=g)
+    pos[0], pos[-1], window = (700, 1535, 0) if tiny_first else (1535, 1530, 700)
+    q = torch.randn(per, nh, hd, generator=g)
+    q[0] *= 1e6
+    ref = S.attention(q, cache, bt, pos, 0, [0, per], window=window)
+    for kw in (dict(per=per), dict(starts=[0, per])):
+        got = _attend(ops, q, cache, bt, pos, window=window, **kw)
+        for r in range(per):
+            assert P.rel(got[r], ref[r]) <= TOL
