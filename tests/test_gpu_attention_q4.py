@@ -268,3 +268,23 @@ def test_tiny_pages_beside_others(ops, hd, per, nh, tiny_first):
         got = _attend(ops, q, cache, bt, pos, window=window, **kw)
         for r in range(per):
             assert P.rel(got[r], ref[r]) <= TOL
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("end", [1, 20, 31])
+def test_tiny_values_among_others_of_a_chunk(ops, hd, end):
+    """A row that sees subnormal f16 values alone, in 64 positions of which other rows see ordinary ones: products of
+    the matrix unit keep 2^-24 of 2^-14 each, so the mean's error is 2^-38 for each of the two sums of 32 positions."""
+    g = torch.Generator().manual_seed(hd + end)
+    bt, total = _table(g, 1, 4)
+    x = [torch.randn(total, 1, 2, 16, hd, generator=g) for _ in range(2)]
+    x[1][bt[0, :2]] *= 2e-6
+    cache = []
+    for y in x:
+        cache += [torch.from_numpy(z) for z in S.quantise4(y.numpy())]
+    pos = torch.tensor([end - 1, 63, 40])
+    q = torch.randn(3, 6, hd, generator=g)
+    ref = S.attention(q, cache, bt, pos, 0, [0, 3])
+    got = _attend(ops, q, cache, bt, pos, per=3)
+    assert float((got[0] - ref[0]).abs().max()) <= 2.0 ** -37
+    _check(got[1:], ref[1:])
