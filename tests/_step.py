@@ -85,7 +85,7 @@ def normed(x, w, eps):
     if w is None:
         return np.asarray(x, np.float32)
     x = np.asarray(x, np.float32)
-    with np.errstate(invalid="ignore", over="ignore"):
+    with np.errstate(divide="ignore", invalid="ignore", over="ignore"):
         d = x.astype(np.float64)
         inv = (1.0 / np.sqrt((d * d).sum(-1, keepdims=True) / x.shape[-1] + float(np.float32(eps)))).astype(np.float32)
         return (x * inv) * np.asarray(w, np.float32)

@@ -87,6 +87,17 @@ def test_plan(ops, n, per, tpb, what, scarce):
     _check_plan(_plan(ops, ctx, new, bt, total, tpb, free, count, rows, in_place=True), want)
 
 
+@pytest.mark.parametrize("n,per,tpb,what", [(5000, 2, 16, "mixed"), (4096, 3, 8, "prompts"), (4097, 3, 8, "prompts"),
+                                            (20000, 1, 4, "decode"), (3, 1 << 16, 8, "prompts"), (2, 1 << 20, 1, "prompts")])
+def test_plan_of_many(ops, n, per, tpb, what):
+    """More sessions than the row starts in LDS, and more rows and pages than a block deals with at once."""
+    rng = np.random.default_rng(n)
+    ctx, new, bt, total, free, count = _sessions(rng, n, per, tpb, 5, what)
+    rows = min(int(np.maximum(new, 0).sum()) + 9, 1 << 20)
+    want = S.plan(ctx, new, bt, total, tpb, free, count, rows)
+    _check_plan(_plan(ops, ctx, new, bt, total, tpb, free, count, rows), want)
+
+
 def test_plan_at_its_limits(ops):
     """A first session that does not fit lets nobody pass, one that no table holds does; all pages gone to the last; no
     rows, no sessions; entries that are no page; a free list too short for what comes back, a count out of its range."""

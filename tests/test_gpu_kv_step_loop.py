@@ -172,10 +172,10 @@ def test_decoding_over_each_cache(ops, fmt):
         s.check(s.expect(new, x))
 
 
-@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 64), (8, 1, 128)])
-def test_steps_in_one_graph(ops, nh, nkv, hd):
+@pytest.mark.parametrize("nh,nkv,hd,rows", [(4, 2, 64, 48), (8, 1, 128, 48), (4, 2, 64, 2100)])
+def test_steps_in_one_graph(ops, nh, nkv, hd, rows):
     """A captured step, replayed with the lengths that the device has by then, eager calls of the same context between."""
-    s, other = (_Server(i, nh=nh, nkv=nkv, hd=hd) for i in (11, 12))
+    s, other = (_Server(i, nh=nh, nkv=nkv, hd=hd, rows=rows, per=9 * rows // 48, n=5 if rows < 100 else 3) for i in (11, 12))
     cap, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     torch.cuda.synchronize()
     with torch.cuda.graph(graph, stream=cap):
