@@ -723,10 +723,11 @@ class HipOps:
         """Norm of each head of q and k, RoPE, and K and V into the pages by slot (cellm_hip_norm_rope_kv_write_*); q_out
         may be q.  Weights [head_dim] or None (not normed), cos_sin or None (not rotated).  Pages by their type: float16
         (or its bits), int8 codes or, for 4 bits, uint8 codes, these two with their scales."""
+        ptr, f32, i32 = self._ptr, _DT.f32, _DT.i32
         rows, vectors = positions_i32.numel(), total_blocks * n_layers * n_kv_heads * tokens_per_block
         n, nq = rows * n_kv_heads * head_dim, rows * n_heads * head_dim
-        weights = [w for w in (q_weight, k_weight) if w is not None]
-        if len(weights) == 2 and q_weight.dtype != k_weight.dtype:
+        weight = k_weight if q_weight is None else q_weight
+        if k_weight is not None and k_weight.dtype != weight.dtype:
             raise TypeError("q_weight and k_weight must share a dtype")
         if kscale is None or kcache.dtype not in _DT.u8:
             cache = self._pages(kcache, vcache, kscale, vscale, head_dim, vectors)
@@ -736,16 +737,15 @@ class HipOps:
                 raise ValueError("kscale and vscale go together")
             cache = self._q4_ptrs(kcache, kscale, vcache, vscale, head_dim, vectors)
             fn = self._lib.cellm_hip_norm_rope_kv_write_q4
+        table = 0 if cos_sin is None else cos_sin.shape[0]
         check(fn(
-            self._h, self._ptr("q", q, _DT.f32, nq), self._ptr("k", k, _DT.f32, n), self._ptr("v", v, _DT.f32, n),
-            self._ptr("q_out", q_out, _DT.f32, nq),
-            None if q_weight is None else self._ptr("q_weight", q_weight, _DT.floats, head_dim),
-            None if k_weight is None else self._ptr("k_weight", k_weight, _DT.floats, head_dim),
-            _torch_dtype_code(weights[0]) if weights else DTYPE_F32, eps, rows, n_heads, n_kv_heads, head_dim,
-            self._ptr("positions", positions_i32, _DT.i32, rows),
-            None if cos_sin is None else self._ptr("cos_sin", cos_sin, _DT.f32, cos_sin.shape[0] * head_dim),
-            0 if cos_sin is None else cos_sin.shape[0], self._ptr("slots", slots_i32, _DT.i32, rows), *cache, total_blocks,
-            n_layers, tokens_per_block, layer, _stream_ptr(stream)))
+            self._h, ptr("q", q, f32, nq), ptr("k", k, f32, n), ptr("v", v, f32, n), ptr("q_out", q_out, f32, nq),
+            None if q_weight is None else ptr("q_weight", q_weight, _DT.floats, head_dim),
+            None if k_weight is None else ptr("k_weight", k_weight, _DT.floats, head_dim),
+            DTYPE_F32 if weight is None else _torch_dtype_code(weight), eps, rows, n_heads, n_kv_heads, head_dim,
+            ptr("positions", positions_i32, i32, rows),
+            None if cos_sin is None else ptr("cos_sin", cos_sin, f32, table * head_dim), table,
+            ptr("slots", slots_i32, i32, rows), *cache, total_blocks, n_layers, tokens_per_block, layer, _stream_ptr(stream)))
 
     def encode_kv_read_q4(self, kcodes, kscale, vcodes, vscale, block_tables, positions_i32, k_out, v_out,
                           n_kv_heads: int, head_dim: int, total_blocks: int, n_layers: int, tokens_per_block: int,
