@@ -40,12 +40,13 @@ __device__ __forceinline__ uint32_t over(uint32_t n, Divisor d)
 //
 // Latency bounds it: one block goes over the sessions, a thread each, and what differs in size from session to
 // session (a finished one's pages, a prompt's) is shared out flat, an entry a thread, by a search in the running
-// sums (four entries a thread: 11.3 us for 11.8 where 13 sessions give 1600 pages back, but 6.9 for 5.8 where few do).
+// sums (four entries a thread of 256: 11.3 us for 11.8 where 13 sessions give 1600 pages back, but 6.9 for 5.8 where few do).
 // The rows' positions and slots are filled by the same block where they are few, else by a second launch over
-// the whole chip (kFillRows).  8 sessions that take a token each 4.4 us, 256 with 24 prompts 11.8, 64 prompts of 64 thousand
-// rows 8.4 (one thread per session for all of its pages, and one block for all rows: 6.6, 22 and 73).
-constexpr int kFillRows = 2048;      // 256 sessions: 1024 rows 6.7 us in one launch and 8.2 in two, 4096 9.4 and 8.4, 8192 20.1 and 11.9
-constexpr int kPlanSmall = 256;      // sessions for which a block of 256 threads is launched, not of 1024: 5.8 us at 256, 8.0
+// the whole chip (kFillRows).  8 sessions that take a token each 4.4 us, 256 with 24 prompts 10.6, 64 prompts of 64 thousand
+// rows 7.8 (one thread per session for all of its pages, and one block for all rows: 6.6, 22 and 73).
+constexpr int kFillRows = 2048;      // 256 sessions: 1024 rows 6.7 us in one launch and 8.2 in two, 4096 9.4 and 8.9, 8192 20.1 and 10.6
+constexpr int kPlanSmall = 256;      // sessions for which a block has so many threads, not 1024: 5.7 us at 256, 8.0 (512 threads: 6.2)
+constexpr int kPlanMany = 512;       // and where rows are many, with as many pages: 256 sessions with 24 prompts 10.6, 256 threads 11.8, 1024 11.5
 constexpr int kFillThreads = 256;
 constexpr int kFillSessions = 4096;  // of which the filling blocks hold the row starts in LDS
 
@@ -473,14 +474,14 @@ hipError_t launch_kv_plan(const KvPlanArgs& a, hipStream_t st)
         constexpr int N = decltype(n)::value;
         hipLaunchKernelGGL((kv_plan_kernel<N, decltype(fill)::value>), dim3(1), dim3(N), 0, st, a);
     };
-    const auto by_size = [&](auto fill) {
-        if (a.tables <= kPlanSmall) go(std::integral_constant<int, 256>{}, fill);
+    const auto by_size = [&](auto few, auto fill) {
+        if (a.tables <= decltype(few)::value) go(few, fill);
         else go(std::integral_constant<int, 1024>{}, fill);
     };
     if (a.rows <= kFillRows) {
-        by_size(std::true_type{});
+        by_size(std::integral_constant<int, kPlanSmall>{}, std::true_type{});
     } else {
-        by_size(std::false_type{});
+        by_size(std::integral_constant<int, kPlanMany>{}, std::false_type{});
         hipLaunchKernelGGL(kv_fill_kernel, dim3((unsigned)((a.rows + kFillThreads - 1) / kFillThreads)), dim3(kFillThreads), 0, st, a);
     }
     return hipGetLastError();
