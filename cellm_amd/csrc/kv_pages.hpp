@@ -140,8 +140,8 @@ __device__ __forceinline__ void values4x8(uint32_t w, h2_t s, h2_t z, uint32_t (
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = as_u32(__builtin_elementwise_fma(c[i], s, z));
 }
-// The lower or upper half of a word in both of them
-__device__ __forceinline__ uint32_t both_low(uint32_t m) { return __builtin_amdgcn_perm(m, m, 0x01000100u); }
-__device__ __forceinline__ uint32_t both_high(uint32_t m) { return __builtin_amdgcn_perm(m, m, 0x03020302u); }
+// The lower or upper half of a word in both of them: as an operand of packed f16 arithmetic it takes no instruction
+__device__ __forceinline__ uint32_t both_low(uint32_t m) { return as_u32(__builtin_shufflevector(as_h2(m), as_h2(m), 0, 0)); }
+__device__ __forceinline__ uint32_t both_high(uint32_t m) { return as_u32(__builtin_shufflevector(as_h2(m), as_h2(m), 1, 1)); }
 
 }  // namespace cellm
