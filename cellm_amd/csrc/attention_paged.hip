@@ -38,7 +38,7 @@
 // operands are unpacked to those values, exactly, and both products are f16's with q (its scale and log2(e) inside) and the
 // weights in two parts each.  Unpacking bounds it where reads do not: 11 instructions for 8 values, 350 of the 560
 // vector instructions of 64 positions beside 16 columns and their 64 products.  131072 positions of one session with
-// 32/8 heads of 128 (168 MB) 41.5 us, 4.0 TB/s; 8 sessions of 4096 to 8192 22.6; a prompt of 1024 behind 1024 73;
+// 32/8 heads of 128 (168 MB) 41.5 us, 4.0 TB/s; 8 sessions of 4096 to 8192 22.6; a prompt of 1024 behind 1024 71;
 // 20 sessions, 3 of them with prompts of 200, window 1024 and a cap 43.8; 701 positions of 14/2 heads of 64 8.2.
 // Rows need not be the same number of each table: a set finds its table in the rows' starts (span_of()).
 //
