@@ -231,7 +231,8 @@ __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table,
 #pragma unroll
             for (int j = 0; j < 8; ++j) d = d + qr[8 * i + j] * (float)w[j];
         }
-        return capped(a, d * a.scale);
+        const float s = capped(a, d * a.scale);
+        return fabsf(s) * kLog2e < INFINITY ? s : s * kLog2e;  // infinite where its exponent is
     };
     const auto reduce = [&](float v, auto op) {
         __syncthreads();
@@ -389,6 +390,13 @@ struct Work {
     Span span;
     int set, lo, hi, step;      // units of positions lo, lo + step, ... below hi (-1: below the columns' ends)
     int split, splits, slot0;   // slot0: work number of the set's split 0
+    // whether a row without drafted nodes sees one of their positions
+    template <int UNIT>
+    __device__ __forceinline__ bool seen_by(const Sight& s) const
+    {
+        const int late = s.start - lo - UNIT;  // the first unit to end behind `start` begins more than this behind lo
+        return s.start < s.ctx && lo + (late >= 0 ? (late / step + 1) * step : 0) < s.ctx;
+    }
 };
 
 // 4-bit pages: the smallest share, in units, with which the sets have no more splits together than `want`, one block on
@@ -821,8 +829,9 @@ __device__ __forceinline__ uint32_t seen_of(const Sight& s, int p0, int g4)
     return below(s.ctx) & ~below(s.start);
 }
 
-// The reference of a column that has seen nothing: below any score, and finite, so that what is not seen (-inf) weighs 0
-constexpr float kNoScore = -0x1p120f;
+// The reference of a column that has seen nothing: no score is below it but -inf, and it is finite, so that what is not
+// seen (-inf) weighs 0.  A sum of weights of 0 then says that the column saw nothing, or scores of -inf alone.
+constexpr float kNoScore = -0x1.fffffep127f;
 
 // The value of the lane N further round in its row of 16
 template <int N>
@@ -1601,7 +1610,9 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
                 for (int r = 0; r < NR / 4; r += 4)
                     fine[u] &= res.put(col, at[u], g4 * (HD / 4) + rd * NR + wave * (NR / 4) + r,
                                        f4_t{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]}, ll);
-                if (kSplits && k.splits > 1 && rd == 0 && wave == 0 && g4 == 0) res.put_sums(col, mm, ll);
+                const bool empty = Q4 && ll == 0.0f;
+                if (empty && rd == 0 && k.seen_by<kWaves * CH>(si[u])) fine[u] = false;  // scores of -inf: NaN, or nothing beside other splits
+                if (kSplits && k.splits > 1 && rd == 0 && wave == 0 && g4 == 0) res.put_sums(col, empty ? -INFINITY : mm, ll);
             }
         }
     }

@@ -772,9 +772,11 @@ int32_t cellm_hip_kv_read_q4(cellm_hip_ctx_t* ctx, const uint8_t* kcodes, const 
  * row_starts[tables] on are left as they were; rows_per_table is 1 then.  Without row_starts
  * `tables` is ignored.  What is multiplied are the f16 values that the codes stand for, with q
  * as two f16 parts (23 bits of an element, 2^-38 of its head's largest); scores and sums are
- * f32, and of values below 2^-14 that a row sees beside larger ones of other rows, in the same
- * 64 positions, its mean keeps 2^-37.  A group of scale NaN makes NaN of the rows that attend to
- * it: of a key of all dims, of a value of its 32.  Everything else is as
+ * f32.  A score past f32's range, itself or times log2(e), weighs nothing beside others where it
+ * is negative; a row with a positive one, or with no others, is NaN.  Of values below 2^-14
+ * that a row sees beside larger ones of other rows, in the same 64 positions, its mean keeps
+ * 2^-37.  A group of scale NaN makes NaN of the rows that attend to it: of a key of all dims, of
+ * a value of its 32.  Everything else is as
  * cellm_hip_attention_gqa_q8kv's. */
 int32_t cellm_hip_attention_gqa_q4kv(cellm_hip_ctx_t* ctx, const float* q, const uint8_t* kcodes, const uint16_t* kscales,
                                      const uint8_t* vcodes, const uint16_t* vscales, const uint32_t* block_tables,
