@@ -933,11 +933,10 @@ __device__ __forceinline__ float score_of(int hi, int mid, int lo, float ks)
 
 // ---- a block's results: its sums where the set is split, else the quotients; the sums of splits added by the last ----
 // COLS columns of a set from column col0 of the table on; a split's sums: [COLS][HD], then R and l, [COLS] each.  Sets of
-// 32 columns are taken where they leave kWideBlocks blocks, and split where there are fewer than kPlanBlocks: never.
+// 32 columns are not split (layout_of()): they are taken where they leave kWideBlocks blocks, one for each CU and more.
 template <int F, int HD, int COLS>
 struct Results {
     static constexpr bool kSplits = COLS == kCols;
-    static_assert(kSplits || kWideBlocks >= kPlanBlocks);
     static constexpr uint32_t kPart = COLS * (HD + 2);
     const MmaArgs& A;
     const Work& k;
@@ -1671,11 +1670,12 @@ Layout layout_of(const PagedAttnArgs& a)
              });
     const long long cap = (long long)a.g.max_blocks * a.g.tpb, units = (cap + unit - 1) / unit;
     const long long blocks = (long long)y.sets * a.g.n_kv;
+    const bool splits = y.ct == 1 && units > kWholeUnits;
     if (a.fmt == KV_Q4) {  // share_of(): up to twice as many splits as wanted, or sets
-        if (blocks < 2 * kPlanBlocks && y.sets <= kPlanSets && units > kWholeUnits) y.want = std::max(1, kPlanBlocks / a.g.n_kv);
+        if (splits && blocks < 2 * kPlanBlocks && y.sets <= kPlanSets) y.want = std::max(1, kPlanBlocks / a.g.n_kv);
         y.works = y.want ? std::min<long long>(std::max<long long>(2 * y.want, y.sets), y.sets * std::min<long long>(kMaxSplits, units)) : y.sets;
     } else {
-        if (blocks < kPlanBlocks && units > kWholeUnits) y.want = std::max(1, kPlanBlocks / a.g.n_kv - y.sets);
+        if (splits && blocks < kPlanBlocks) y.want = std::max(1, kPlanBlocks / a.g.n_kv - y.sets);
         // each set's last split may be short
         y.works = y.want ? std::min<long long>(y.want + y.sets, y.sets * std::min<long long>(kMaxSplits, units)) : y.sets;
     }

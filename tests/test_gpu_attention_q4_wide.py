@@ -197,3 +197,43 @@ def test_codes_past_32_bit_offsets(ops, hd):
     ref = _dense(q, small, torch.arange(pages)[None], pos, starts)
     for ragged in (False, True):
         _check(_attend(ops, q, cache, bt, pos, starts, ragged, layers - 1), ref, pos)
+
+
+def test_they_take_no_scratch():
+    """Sets of 32 columns are not split: no call of theirs takes scratch, on a stream or in a graph."""
+    from cellm_amd import HipOps
+
+    q, cache, bt, pos, starts = _case([40] * 16, 16, 4, 128, 16, 1500)
+    q, cache, bt, pos, out = q.cuda(), [c.cuda() for c in cache], _i32(bt), _i32(pos), torch.zeros(640, 16, 128, device="cuda")
+    starts = _i32(starts)
+    total = len(cache[0])
+
+    def call(ops, stream, ragged):
+        kw = dict(row_starts_i32=starts) if ragged else dict(rows_per_table=40)
+        ops.encode_attention_q4(q, *cache, bt, pos, out, 16, 4, 128, total, 1, 16, 0, stream=stream, **kw)
+
+    def held(f):
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        f()
+        torch.cuda.synchronize()
+        return before - torch.cuda.mem_get_info()[0]
+
+    stream = torch.cuda.Stream()
+    for ops in (HipOps(0), HipOps(0)):  # what the runtime loads with the kernels comes with the first
+        most = 0
+        for ragged in (False, True):
+            eager = held(lambda: call(ops, stream, ragged))
+            graph = torch.cuda.CUDAGraph()
+
+            def capture():
+                with torch.cuda.graph(graph, stream=stream):
+                    call(ops, stream, ragged)
+
+            captured = held(capture)
+            graph.replay()
+            torch.cuda.synchronize()
+            del graph
+            most = max(most, eager, captured)
+        ops.close()
+    assert most <= 2**22  # scratch of splits would be 8 MiB
