@@ -36,10 +36,11 @@
 //
 // 4-bit pages: a code stands for the f16 value f16(c s + z) of its group of 32 dims (kv_pages.hpp), so K's and V's
 // operands are unpacked to those values, exactly, and both products are f16's with q (its scale and log2(e) inside) and the
-// weights in two parts each.  Unpacking bounds it where reads do not: 11 instructions for 8 values, 350 of the 560
-// vector instructions of 64 positions beside 16 columns and their 64 products.  131072 positions of one session with
-// 32/8 heads of 128 (168 MB) 41.5 us, 4.0 TB/s; 8 sessions of 4096 to 8192 22.6; a prompt of 1024 behind 1024 71;
-// 20 sessions, 3 of them with prompts of 200, window 1024 and a cap 43.8; 701 positions of 14/2 heads of 64 8.2.
+// weights in two parts each.  Unpacking bounds it where reads do not: 11 instructions for 8 values and permutes of
+// V's codes and scale words, 384 of the 560 vector instructions of 64 positions beside 16 columns and their 64 products.
+// 131072 positions of one session with 32/8 heads of 128 (168 MB) 42 to 46 us, 3.6 to 4.0 TB/s; 8 sessions of 4096 to 8192
+// 22.8; a prompt of 1024 behind 1024 73; 20 sessions, 3 of them with prompts of 200, window 1024 and a cap 43.8; 701
+// positions of 14/2 heads of 64 8.2.
 // Rows need not be the same number of each table: a set finds its table in the rows' starts (span_of()).
 //
 // The positions of a set of columns are split over blocks by a rule on the device (plan()),
@@ -212,7 +213,8 @@ __device__ __forceinline__ h8_t eight_dims(const void* pages, const void* scales
 // The units of positions lo, lo + step, ... below up of one (row, head) over f16 or 4-bit pages by plain f32 sums, the whole block:
 // reference R, log2(e) times the largest score, sum l of the weights and, in threads below HD, the weighted sum of V
 // (returned).  A unit at a time: a score per thread, then HD threads per position.  For columns whose sums in f16 parts are not finite: inf * lo may be NaN where
-// inf * v is not, and so is the 0 * inf of a position that the column does not see.
+// inf * v is not, and so is the 0 * inf of a position that the column does not see; and for those of 4-bit pages without a
+// weight, whose scores are all -inf.
 template <int F, int HD, int UNIT>
 __device__ float plain_range(const PagedAttnArgs& a, const Sight& si, int table, int row, int head, int lo, int up, int step,
                              bool part, unsigned char* lds, float& R, float& l)
@@ -401,9 +403,12 @@ struct Work {
 
 // 4-bit pages: the smallest share, in units, with which the sets have no more splits together than `want`, one block on
 // each CU; it is looked for between the mean and the share whose short last splits fit too.  Where long ones come out
-// well above the mean, twice as many splits, two blocks on a CU: 16 sessions of 8000 to 16000 positions, 32/8 heads of 128,
-// 61.5 us, 82 with the share of want less the sets; 24 of 4096 to 8192 50 and 60; 32 of lengths apart 19.6 and 23.3, 32
-// of the same 2048 (whole, but now planned) 21.1 and 19.9; with two blocks everywhere one session at 131072 had 46 and not 41.5.
+// well above the mean, twice as many splits, two blocks on a CU.  In turn on one card, 32/8 heads of 128: 16 sessions of 8000
+// to 16000 positions 61.5 us, 66.3 with one block on a CU, 82.5 with the share of want less the sets; 24 of 4096 to
+// 8192 50.6, 53.6 and 58.1; 8 of those 22.8, 22.7 and 24.3; 32 of the same 2048 22.3, 22.1 and 21.7; one at 131072
+// 42.1, 41.7 and 40.9, and 45.7 with two blocks always.  2 want are all the splits there are, one a set at least, and from
+// 2 kPlanBlocks blocks or kPlanSets sets on none: one session at 131072 among 50 at 500 takes 74 us, among 62 400 and
+// among 63 and more 770; by starts, whose set numbers count, among 50 86 and from 51 on 900.
 // Splits of one set meet one after the other, 16 of them in the time that a unit takes: 8192 positions of 8 kv heads in
 // 16 splits of two units 14.9 us, in 32 of one 16.4.
 constexpr int kLongShare = 8;   // units from which two blocks on a CU are looked at
@@ -616,7 +621,8 @@ __device__ __forceinline__ void drop_missing(unsigned long long miss, uint32_t (
 
 // BYTES bytes at off of vector `vector` (VB bytes each) of a 4-bit page's codes or scales.  Offsets of 32 bits where the
 // array has no more (BIG: false): one sum beside a base in scalar registers, where an address of 64 bits takes four times
-// that (131072 positions 44 us, 63 with those; both in one kernel behind a branch, which parts what the loads run beside, 55).
+// that (131072 positions in sets of 16 columns 44.6 us, 47.3 with those; both in one kernel behind a branch, which parts
+// what the loads run beside, a quarter more).
 template <bool BIG, int VB, int BYTES>
 __device__ __forceinline__ void load_bytes(const void* base, uint32_t vector, uint32_t off, uint32_t (&to)[(BYTES + 3) / 4])
 {
@@ -1078,9 +1084,11 @@ struct Results {
 // 4-bit pages, FEW: sets of up to 4 columns, of which an operand's 16 columns have each four times: columns c and c + 8 are
 // the high and the low parts of q and of the weights, so that both take one product and meet at its end (those of the
 // scores at once), and c + 4 is column c again, with the weights of the other half of the chunk's positions: each lane
-// makes half as many.  131072 positions, 32/8 heads of 128: 41.5 us, 45 without; 24 sessions of 4096 to 8192 60 and 63.5;
-// 4 at 1000, where it has more to begin and to end with, 11.9 and 11.5.  (Parts side by side for up to 8 columns: 14/2 heads
-// of 64 at 65536 20.1, 19.7 without.)
+// makes half as many.  131072 positions, 32/8 heads of 128: 42.1 us, 44.6 without; 24 sessions of 4096 to 8192 50.6
+// and 51.4; 32 at 2048 22.3 and 23.7; 4 at 1000, where it has more to begin and to end with, 12.3 and 12.0.  (Parts side by
+// side for up to 8 columns: 14/2 heads of 64 at 65536 20.1, 19.7 without.)
+//
+// Heads of 256 fill the 256 registers: sets of 16 columns spill 2 to 6 of them over 4-bit pages and 45 to 49 over f16 ones.
 template <int F, int HD, int CT, bool CAP, bool BIG = false, bool FEW = false>
 __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A)
 {
@@ -1094,8 +1102,9 @@ __global__ __launch_bounds__(kThreads, 2) void attn_paged_kernel(const MmaArgs A
     constexpr bool kQInLds = (HD > 128 && !FEW) || CT > 1;            // q's parts in LDS, for want of registers
     static_assert(!FEW || (Q4 && CT == 1));
     // Of two waves on a SIMD the one that has products to issue goes first, beside the other's weights: 20 sessions, 3 of 200
-    // rows, 16/4 heads of 128 72.3 us, 76.1 without; a prompt of 1024 with 32/8 72.9 and 74; those three beside them 128.6
-    // and 125.8; heads of 256 at 700 rows 31.9 and 33.6; heads of 64 lose (701 positions 8.6 and 8.3).
+    // rows, 16/4 heads of 128 71.6 us, 75.6 without; with a window and a cap 43.8 and 45.4; heads of 256 at 700 rows 32.4
+    // and 33.6; a prompt of 1024 with 32/8 heads of 128 73.5 both; the 20 sessions with 32/8 129.5 and 125.4; heads of 64
+    // lose (701 positions 8.5 and 8.3).
     constexpr bool kPrio = Q4 && HD >= 128;
     constexpr int COLS = kCols * CT;
     constexpr bool kSplits = Results<F, HD, COLS>::kSplits;

@@ -290,11 +290,12 @@ struct NormWriteArgs {
 // 4 l .. 4 l + 3 and HD / 2 + 4 l .. HD / 2 + 4 l + 3: the pairs of the rotate-half layout, two pairs of each run of
 // the interleaved one, and 8 lanes hold two groups of 4-bit codes.
 //
-// Bytes bound it at many rows, latency at few.  2048 rows of 32/8/8 heads of 128 to 8-bit pages (88 MB) 17.1 us,
-// 5.1 TB/s where a copy of that kind reaches 5.3; 7996 rows of 4/1/1 heads of 256 to 4-bit pages (84 MB) 18.7; one row
-// 2.4.  A vector's loads are all on their way before its position and slot are looked at, the sum goes round by lane
+// Bytes bound it at many rows, latency at few.  Back to back, 2048 rows of 32/8/8 heads of 128 to 8-bit pages (89 MB)
+// take 18.4 us, 4.9 TB/s where a copy of 256 MiB reaches 5.4 (15.9 called one by one, when half of the reads come out of
+// the cache); to 4-bit pages 17.4, to f16 ones 19.7; 7996 rows of 4/1/1 heads of 256 to 4-bit pages (93 MB) 18.3, to f16
+// ones 17.7; one row 2.4.  A vector's loads are all on their way before its position and slot are looked at, the sum goes round by lane
 // moves, quotients by integers are products, codes take no division, and of 4-bit codes two lanes share out their two
-// words (shuffles, divisions and 2-byte stores: 18.6, 21.1 and 2.7 us); rows in order within each XCD read the table
+// words (shuffles, divisions and 2-byte stores took 9 % more, 13 % of 4-bit pages and of one row); rows in order within each XCD read the table
 // of cosines from its own L2 (7996 rows written and read back 25.5 us, 26.1 with blocks dealt out in turn).
 template <int HD, int FMT, int WDT>
 __global__ __launch_bounds__(kThreads) void norm_rope_write_kernel(const NormWriteArgs A)

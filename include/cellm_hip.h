@@ -681,8 +681,10 @@ int32_t cellm_hip_kv_accept_q8(cellm_hip_ctx_t* ctx, int8_t* kcodes, float* ksca
 /* ---- a serving step over a paged cache whose lengths only the device knows ----------
  * cellm_hip_kv_plan makes a step's pages and rows from the sessions' lengths,
  * cellm_hip_norm_rope_kv_write_* puts the rows' K and V into the pages by its slots, and
- * cellm_hip_attention_gqa_q4kv takes its rows as they are: the host needs to know no length,
- * so that a step (and a graph of it) is the same launches whatever the sessions hold. */
+ * cellm_hip_attention_gqa_q4kv takes its rows as they are: over 4-bit pages the host needs to know
+ * no length, so that a step (and a graph of it) is the same launches whatever the sessions
+ * hold.  The attention calls of f16 and 8-bit pages take no row_starts: a planned step is theirs
+ * where every session has rows_per_table rows of it, none idle, waiting or finished. */
 
 /* The pages and rows of a step (the counterpart of the reference's BlockAllocator and
  * PageTable, crates/cellm-cache/src/allocator.rs:11-93, pagetable.rs:8-120, which run on
@@ -774,9 +776,8 @@ int32_t cellm_hip_kv_read_q4(cellm_hip_ctx_t* ctx, const uint8_t* kcodes, const 
  * as two f16 parts (23 bits of an element, 2^-38 of its head's largest); scores and sums are
  * f32.  A score past f32's range, itself or times log2(e), weighs nothing beside others where it
  * is negative; a row with a positive one, or with no others, is NaN.  Of values below 2^-14
- * that a row sees beside larger ones of other rows, in the same 64 positions, its mean keeps
- * 2^-37.  A group of scale NaN makes NaN of the rows that attend to it: of a key of all dims, of
- * a value of its 32.  Everything else is as
+ * a mean keeps 2^-37 where its table holds larger ones, too.  A group of scale NaN makes NaN of
+ * the rows that attend to it: of a key of all dims, of a value of its 32.  Everything else is as
  * cellm_hip_attention_gqa_q8kv's. */
 int32_t cellm_hip_attention_gqa_q4kv(cellm_hip_ctx_t* ctx, const float* q, const uint8_t* kcodes, const uint16_t* kscales,
                                      const uint8_t* vcodes, const uint16_t* vscales, const uint32_t* block_tables,
